@@ -1,0 +1,766 @@
+// Decay attention (include/atlas_decay.h): entry points, the state recurrence over chunks,
+// the float32 CUDA-core kernels for the calls outside the tensor path, and the recurrent
+// single-token form.
+//
+// A sequence is cut into chunks of CH = 128 tokens.  With L tokens in a chunk, local
+// positions t, s and l = exp(log_decay):
+//
+//   forward   dS[c]     = sum_s l^(L-1-s) k_s v_s^T                   every chunk by itself
+//             S[c+1]    = l^L S[c] + dS[c]                            recurrence over chunks
+//             y_t       = scale [ sum_{s<=t} l^(t-s) (q_t.k_s) v_s + l^(t+1) q_t^T S[c] ]
+//   backward  (o = scale dy)  QO[c] = sum_t l^(t+1) q_t o_t^T,  R[c-1] = l^L R[c] + QO[c]
+//             (R[c]: cotangent of the state leaving chunk c)
+//             dq_t = sum_{s<=t} l^(t-s) (o_t.v_s) k_s + l^(t+1) S[c] o_t
+//             dk_s = sum_{t>=s} l^(t-s) (o_t.v_s) q_t + l^(L-1-s) R[c] v_s
+//             dv_s = sum_{t>=s} l^(t-s) (q_t.k_s) o_t + l^(L-1-s) R[c]^T k_s
+//             dlog_decay = sum_{s<=t} (t-s) l^(t-s) (q_t.k_s)(o_t.v_s) + sum_t (t+1) q_t.dq_t^inter
+//                          + sum_s (L-1-s) k_s.dk_s^inter + L l^L <R[c], S[c]>, over all chunks
+//             (the terms of dq and dk that go through S and R are "inter").
+//
+// Every power of l has an exponent >= 0, so no decay, however strong, overflows.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "decay_internal.h"
+#include "scan_internal.h"
+
+namespace atlas {
+namespace decay {
+
+// l^n for n >= 0 (l^0 = 1 also for log_decay = -infinity)
+__device__ __forceinline__ float pow_decay(float g, int n) { return n == 0 ? 1.f : expf((float)n * g); }
+
+// ---------------------------------------------------------------------------
+// recurrence over chunks
+// ---------------------------------------------------------------------------
+// One thread per 4 (VEC) state elements walks the chunks (backward: from the last one) and
+// replaces each chunk's sum by the running state in front of it.  Pure streaming: the loads
+// of UN chunks are in flight together, since only the add depends on the previous chunk.
+// The per-chunk factor l^L is applied as a float pair (its rounding error would otherwise
+// be multiplied in again at every chunk).
+template <int VEC>
+__global__ void __launch_bounds__(256) scan_kernel(Args a, const float* in, float* out, float* buf, bool bwd) {
+  constexpr int UN = 8;
+  const AtlasDecayParams& P = a.p;
+  const int nc = chunks(P), DD = P.D * P.D, per = DD / VEC;
+  const int64_t total = chains(P) * per;
+  const int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (u >= total) return;
+  const int64_t chain = u / per;
+  const int e = (int)(u - chain * per) * VEC;
+  const double g = (double)a.log_decay[chain % P.H];
+  const double f64 = exp(g * CH), fl64 = exp(g * chunk_len(P, nc - 1));
+  float S[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) S[j] = in ? in[chain * DD + e + j] : 0.f;
+  float* base = buf + chain * nc * DD + e;
+  for (int c0 = 0; c0 < nc; c0 += UN) {
+    float x[UN][VEC];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const int c = bwd ? nc - 1 - (c0 + i) : c0 + i;
+      if (c0 + i < nc) {
+        if constexpr (VEC == 4)
+          *(float4*)x[i] = *(const float4*)(base + (int64_t)c * DD);
+        else
+          x[i][0] = base[(int64_t)c * DD];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      if (c0 + i >= nc) break;
+      const int c = bwd ? nc - 1 - (c0 + i) : c0 + i;
+      const double f = c == nc - 1 ? fl64 : f64;
+      const float fh = (float)f, fl = (float)(f - (double)fh);
+      if constexpr (VEC == 4)
+        *(float4*)(base + (int64_t)c * DD) = *(const float4*)S;
+      else
+        base[(int64_t)c * DD] = S[0];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) S[j] = fmaf(S[j], fh, fmaf(S[j], fl, x[i][j]));
+    }
+  }
+  if (out) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) out[chain * DD + e + j] = S[j];
+  }
+}
+
+// dlog_decay[h] = sum over batches and parts, in a fixed order
+__global__ void __launch_bounds__(256) dg_kernel(Args a, float* dg) {
+  const AtlasDecayParams& P = a.p;
+  const int h = blockIdx.x;
+  const int64_t n = (int64_t)P.B * a.dg_parts;
+  double acc = 0;
+  for (int64_t i = threadIdx.x; i < n; i += 256) {
+    const int64_t b = i / a.dg_parts, c = i - b * a.dg_parts;
+    acc += (double)a.dg_part[(b * P.H + h) * a.dg_parts + c];
+  }
+  __shared__ double red[256];
+  red[threadIdx.x] = acc;
+  __syncthreads();
+  for (int k = 128; k > 0; k >>= 1) {
+    if (threadIdx.x < k) red[threadIdx.x] += red[threadIdx.x + k];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) dg[h] = (float)red[0];
+}
+
+// ---------------------------------------------------------------------------
+// float32 CUDA-core kernels (any D <= 128, strides and alignment; float32 activations)
+// ---------------------------------------------------------------------------
+// 256 threads as 16 x 16; thread (ty, tx) owns rows ty + 16 i and columns tx + 16 j of a
+// product, so its operands come from shared memory as broadcasts (rows) and consecutive
+// words (columns).  Token tiles are TT = 32 rows; NI = ceil(D / 16).
+constexpr int TT = 32;
+constexpr int LD = 129;  // row pitch of the token tiles (odd: rows of one column differ in bank)
+
+struct View {
+  const void* p;
+  int64_t sb, st, sh;
+};
+__device__ __forceinline__ View view(const void* p, const int64_t* s) { return View{p, s[0], s[1], s[2]}; }
+__device__ __forceinline__ View flat(const void* p, const AtlasDecayParams& P) {
+  return View{p, (int64_t)P.T * P.H * P.D, (int64_t)P.H * P.D, (int64_t)P.D};
+}
+
+// rows [t0, t0 + TT) of head (b, h) into a tile; rows from t_end on and columns from D on are 0
+template <typename TA>
+__device__ void load_rows(float (*tile)[LD], const View& x, int b, int h, int t0, int t_end, int D, int cols) {
+  const TA* base = (const TA*)x.p + b * x.sb + h * x.sh;
+  for (int u = threadIdx.x; u < TT * cols; u += 256) {
+    const int r = u / cols, c = u - r * cols, t = t0 + r;
+    tile[r][c] = (t < t_end && c < D) ? ld_act(base + (int64_t)t * x.st, (size_t)c) : 0.f;
+  }
+}
+
+// per-chunk sums of weight * X^T Y (see launch_chunk_states)
+template <typename TA, int NI>
+__global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd) {
+  __shared__ float X[TT][LD], Y[TT][LD];
+  const AtlasDecayParams& P = a.p;
+  const int nc = chunks(P), D = P.D;
+  const int64_t chain = blockIdx.x / nc;
+  const int c = (int)(blockIdx.x % nc), b = (int)(chain / P.H), h = (int)(chain % P.H);
+  const int L = chunk_len(P, c), tc = c * CH;
+  const float g = a.log_decay[h];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const View xv = bwd ? view(a.q, P.q_stride) : view(a.k, P.k_stride);
+  const View yv = bwd ? flat(a.dy, P) : view(a.v, P.v_stride);
+  float acc[NI][NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) acc[i][j] = 0.f;
+  for (int s0 = 0; s0 < L; s0 += TT) {
+    __syncthreads();
+    load_rows<TA>(X, xv, b, h, tc + s0, tc + L, D, 16 * NI);
+    load_rows<TA>(Y, yv, b, h, tc + s0, tc + L, D, 16 * NI);
+    __syncthreads();
+    const int n = min(TT, L - s0);
+    for (int r = 0; r < n; ++r) {
+      const float w = bwd ? P.scale * pow_decay(g, s0 + r + 1) : pow_decay(g, L - 1 - s0 - r);
+      float xr[NI], yr[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) xr[i] = w * X[r][ty + 16 * i];
+#pragma unroll
+      for (int j = 0; j < NI; ++j) yr[j] = Y[r][tx + 16 * j];
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = fmaf(xr[i], yr[j], acc[i][j]);
+    }
+  }
+  float* out = (bwd ? a.dstates : a.states) + (chain * nc + c) * (int64_t)D * D;
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int d = ty + 16 * i, e = tx + 16 * j;
+      if (d < D && e < D) out[d * D + e] = acc[i][j];
+    }
+}
+
+// out[r][j] (rows ty, ty + 16; columns tx + 16 j) += w_r * sum_m A[r][m] M(m, column) over a
+// D x D matrix in global memory; transposed: M(m, c) = M[c][m].  `stage` is a free tile.
+template <int NI>
+__device__ void times_state(float (*acc)[NI], const float (*A)[LD], const float* M, bool transposed, int D,
+                            const float* w, float (*stage)[LD]) {
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  for (int m0 = 0; m0 < D; m0 += TT) {
+    __syncthreads();
+    for (int u = threadIdx.x; u < TT * 16 * NI; u += 256) {
+      int m, c;
+      if (transposed) {  // consecutive threads along m, the contiguous axis of M[c][m]
+        c = u / TT, m = u - c * TT;
+      } else {
+        m = u / (16 * NI), c = u - m * (16 * NI);
+      }
+      float x = 0.f;
+      if (m0 + m < D && c < D) x = transposed ? M[(int64_t)c * D + m0 + m] : M[(int64_t)(m0 + m) * D + c];
+      stage[m][c] = x;
+    }
+    __syncthreads();
+    const int n = min(TT, D - m0);
+    for (int m = 0; m < n; ++m) {
+      const float a0 = w[0] * A[ty][m0 + m], a1 = w[1] * A[ty + 16][m0 + m];
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const float x = stage[m][tx + 16 * j];
+        acc[0][j] = fmaf(a0, x, acc[0][j]);
+        acc[1][j] = fmaf(a1, x, acc[1][j]);
+      }
+    }
+  }
+}
+
+// (row ty + 16 i) . (row tx + 16 j) for i, j < 2, of two tiles
+__device__ __forceinline__ void dots(float (*p)[2], const float (*A)[LD], const float (*B)[LD], int D) {
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  p[0][0] = p[0][1] = p[1][0] = p[1][1] = 0.f;
+  for (int m = 0; m < D; ++m) {
+    const float a0 = A[ty][m], a1 = A[ty + 16][m], b0 = B[tx][m], b1 = B[tx + 16][m];
+    p[0][0] = fmaf(a0, b0, p[0][0]);
+    p[0][1] = fmaf(a0, b1, p[0][1]);
+    p[1][0] = fmaf(a1, b0, p[1][0]);
+    p[1][1] = fmaf(a1, b1, p[1][1]);
+  }
+}
+template <int NI>
+__device__ __forceinline__ void times_tile(float (*acc)[NI], const float (*Pm)[TT + 1], const float (*B)[LD]) {
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll 4
+  for (int m = 0; m < TT; ++m) {
+    const float p0 = Pm[ty][m], p1 = Pm[ty + 16][m];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const float x = B[m][tx + 16 * j];
+      acc[0][j] = fmaf(p0, x, acc[0][j]);
+      acc[1][j] = fmaf(p1, x, acc[1][j]);
+    }
+  }
+}
+template <typename TA, int NI>
+__device__ void store_rows(void* x, const float (*acc)[NI], const AtlasDecayParams& P, int b, int h, int t0,
+                           int t_end, float scale) {
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = t0 + ty + 16 * i;
+    if (t >= t_end) continue;
+    TA* row = (TA*)x + (((int64_t)b * P.T + t) * P.H + h) * P.D;
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+      if (tx + 16 * j < P.D) st_act(row, (size_t)(tx + 16 * j), scale * acc[i][j]);
+  }
+}
+
+__device__ __forceinline__ float cta_sum(float v) {  // every thread gets the sum
+  __shared__ float red[8];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += red[i];
+  return s;
+}
+
+struct TilePos {
+  int64_t chain;
+  int tile, b, h, c, L, tc, r0;  // r0: first row of the tile within its chunk
+};
+__device__ __forceinline__ TilePos tile_pos(const AtlasDecayParams& P, int tiles) {
+  TilePos t;
+  t.chain = blockIdx.x / tiles;
+  t.tile = (int)(blockIdx.x % tiles);
+  t.b = (int)(t.chain / P.H);
+  t.h = (int)(t.chain % P.H);
+  t.c = t.tile / (CH / TT);
+  t.L = chunk_len(P, t.c);
+  t.tc = t.c * CH;
+  t.r0 = (t.tile % (CH / TT)) * TT;
+  return t;
+}
+
+// y of one tile of 32 tokens
+template <typename TA, int NI>
+__global__ void __launch_bounds__(256) out_kernel(Args a, int tiles) {
+  extern __shared__ float sm[];
+  float(*A)[LD] = (float(*)[LD])sm;
+  float(*K)[LD] = A + TT;
+  float(*V)[LD] = K + TT;
+  float(*Pm)[TT + 1] = (float(*)[TT + 1])(V + TT);
+  const AtlasDecayParams& P = a.p;
+  const TilePos z = tile_pos(P, tiles);
+  const int D = P.D, cols = 16 * NI, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
+  const float g = a.log_decay[z.h];
+  load_rows<TA>(A, view(a.q, P.q_stride), z.b, z.h, z.tc + z.r0, tend, D, cols);
+  float acc[2][NI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) acc[0][j] = acc[1][j] = 0.f;
+  const float w[2] = {pow_decay(g, z.r0 + ty + 1), pow_decay(g, z.r0 + ty + 17)};
+  times_state<NI>(acc, A, a.states + (z.chain * chunks(P) + z.c) * (int64_t)D * D, false, D, w, K);
+  for (int s0 = 0; s0 <= z.r0; s0 += TT) {
+    __syncthreads();
+    load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, cols);
+    load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + s0, tend, D, cols);
+    __syncthreads();
+    float p[2][2];
+    dots(p, A, K, D);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int lag = z.r0 + ty + 16 * i - (s0 + tx + 16 * j);
+        Pm[ty + 16 * i][tx + 16 * j] = lag >= 0 ? p[i][j] * pow_decay(g, lag) : 0.f;
+      }
+    __syncthreads();
+    times_tile<NI>(acc, Pm, V);
+  }
+  store_rows<TA, NI>(a.y, acc, P, z.b, z.h, z.tc + z.r0, tend, P.scale);
+}
+
+// dq of one tile of 32 tokens, and its part of dlog_decay (terms with q)
+template <typename TA, int NI>
+__global__ void __launch_bounds__(256) dq_kernel(Args a, int tiles) {
+  extern __shared__ float sm[];
+  float(*Q)[LD] = (float(*)[LD])sm;
+  float(*O)[LD] = Q + TT;
+  float(*K)[LD] = O + TT;
+  float(*V)[LD] = K + TT;
+  float(*Pm)[TT + 1] = (float(*)[TT + 1])(V + TT);
+  const AtlasDecayParams& P = a.p;
+  const TilePos z = tile_pos(P, tiles);
+  const int D = P.D, cols = 16 * NI, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
+  const float g = a.log_decay[z.h];
+  load_rows<TA>(Q, view(a.q, P.q_stride), z.b, z.h, z.tc + z.r0, tend, D, cols);
+  load_rows<TA>(O, flat(a.dy, P), z.b, z.h, z.tc + z.r0, tend, D, cols);
+  float acc[2][NI], dg = 0.f;
+#pragma unroll
+  for (int j = 0; j < NI; ++j) acc[0][j] = acc[1][j] = 0.f;
+  const float w[2] = {P.scale * pow_decay(g, z.r0 + ty + 1), P.scale * pow_decay(g, z.r0 + ty + 17)};
+  const int64_t so = (z.chain * chunks(P) + z.c) * (int64_t)D * D;
+  times_state<NI>(acc, O, a.states + so, true, D, w, K);
+#pragma unroll
+  for (int j = 0; j < NI; ++j)  // columns from D on are 0 in Q
+    dg += (float)(z.r0 + ty + 1) * Q[ty][tx + 16 * j] * acc[0][j] +
+          (float)(z.r0 + ty + 17) * Q[ty + 16][tx + 16 * j] * acc[1][j];
+  for (int s0 = 0; s0 <= z.r0; s0 += TT) {
+    __syncthreads();
+    load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, cols);
+    load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + s0, tend, D, cols);
+    __syncthreads();
+    float p[2][2], x[2][2];
+    dots(p, Q, K, D);
+    dots(x, O, V, D);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int lag = z.r0 + ty + 16 * i - (s0 + tx + 16 * j);
+        const float da = lag >= 0 ? P.scale * pow_decay(g, lag) * x[i][j] : 0.f;
+        if (lag > 0) dg += (float)lag * p[i][j] * da;
+        Pm[ty + 16 * i][tx + 16 * j] = da;
+      }
+    __syncthreads();
+    times_tile<NI>(acc, Pm, K);
+  }
+  store_rows<TA, NI>(a.dq, acc, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
+  dg = cta_sum(dg);
+  if (threadIdx.x == 0) a.dg_part[z.chain * a.dg_parts + z.tile] = dg;
+}
+
+// dk and dv of one tile of 32 tokens, and the terms of dlog_decay with k, R and S
+template <typename TA, int NI>
+__global__ void __launch_bounds__(256) dkv_kernel(Args a, int tiles) {
+  extern __shared__ float sm[];
+  float(*K)[LD] = (float(*)[LD])sm;
+  float(*V)[LD] = K + TT;
+  float(*Q)[LD] = V + TT;
+  float(*O)[LD] = Q + TT;
+  float(*Pm)[TT + 1] = (float(*)[TT + 1])(O + TT);
+  float(*Am)[TT + 1] = Pm + TT;
+  const AtlasDecayParams& P = a.p;
+  const TilePos z = tile_pos(P, tiles);
+  const int D = P.D, cols = 16 * NI, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
+  const float g = a.log_decay[z.h];
+  load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + z.r0, tend, D, cols);
+  load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + z.r0, tend, D, cols);
+  float dk[2][NI], dv[2][NI], dg = 0.f;
+#pragma unroll
+  for (int j = 0; j < NI; ++j) dk[0][j] = dk[1][j] = dv[0][j] = dv[1][j] = 0.f;
+  const int n0 = z.L - 1 - z.r0 - ty, n1 = n0 - 16;  // steps from the row to the chunk's end
+  const float w[2] = {n0 >= 0 ? pow_decay(g, n0) : 0.f, n1 >= 0 ? pow_decay(g, n1) : 0.f};
+  const int64_t so = (z.chain * chunks(P) + z.c) * (int64_t)D * D;
+  const float *R = a.dstates + so, *S = a.states + so;
+  times_state<NI>(dk, V, R, true, D, w, Q);
+  times_state<NI>(dv, K, R, false, D, w, Q);
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    if (n0 > 0) dg += (float)n0 * K[ty][tx + 16 * j] * dk[0][j];
+    if (n1 > 0) dg += (float)n1 * K[ty + 16][tx + 16 * j] * dk[1][j];
+  }
+  if (z.r0 == 0) {  // once for each chunk
+    float rs = 0.f;
+    for (int u = threadIdx.x; u < D * D; u += 256) rs = fmaf(R[u], S[u], rs);
+    dg += (float)z.L * pow_decay(g, z.L) * rs;
+  }
+  for (int t0 = z.r0; t0 < z.L; t0 += TT) {
+    __syncthreads();
+    load_rows<TA>(Q, view(a.q, P.q_stride), z.b, z.h, z.tc + t0, tend, D, cols);
+    load_rows<TA>(O, flat(a.dy, P), z.b, z.h, z.tc + t0, tend, D, cols);
+    __syncthreads();
+    float p[2][2], x[2][2];
+    dots(p, K, Q, D);
+    dots(x, V, O, D);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int lag = t0 + tx + 16 * j - (z.r0 + ty + 16 * i);
+        const float f = lag >= 0 ? P.scale * pow_decay(g, lag) : 0.f;
+        Pm[ty + 16 * i][tx + 16 * j] = lag >= 0 ? f * p[i][j] : 0.f;
+        Am[ty + 16 * i][tx + 16 * j] = lag >= 0 ? f * x[i][j] : 0.f;
+      }
+    __syncthreads();
+    times_tile<NI>(dk, Am, Q);
+    times_tile<NI>(dv, Pm, O);
+  }
+  store_rows<TA, NI>(a.dk, dk, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
+  store_rows<TA, NI>(a.dv, dv, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
+  dg = cta_sum(dg);
+  if (threadIdx.x == 0) a.dg_part[z.chain * a.dg_parts + tiles + z.tile] = dg;
+}
+
+// ---------------------------------------------------------------------------
+// recurrent form
+// ---------------------------------------------------------------------------
+// One CTA per (sequence, head, slice of 32 value columns): the columns of the state are
+// independent, so a slice needs no exchange with the others.  Thread (row group rg, column
+// group cg) keeps rows rg, rg + 256 / CG, ... of VEC consecutive columns in registers from
+// the first token to the last; y's sum over rows goes through shared memory.
+template <typename TA, int VEC>
+__global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, const int32_t* slots, int32_t n_slots,
+                                                   float* out) {
+  constexpr int CG = 32 / VEC, RG = 256 / CG, NR = 128 / RG;  // column groups, row groups, rows a thread
+  __shared__ float red[RG / (32 / CG)][32 + 1], qs[128], ks[128];
+  const AtlasDecayParams& P = a.p;
+  const int D = P.D, slices = (D + 31) / 32;
+  const int64_t chain = blockIdx.x / slices;
+  const int sl = (int)(blockIdx.x % slices), b = (int)(chain / P.H), h = (int)(chain % P.H);
+  const int cg = threadIdx.x % CG, rg = threadIdx.x / CG, e0 = 32 * sl + cg * VEC;
+  const int32_t row = slots ? slots[b] : b;
+  const bool idle = slots && (row < 0 || row >= n_slots);
+  TA* y = (TA*)a.y + ((int64_t)b * P.T * P.H + h) * D;
+  if (idle) {
+    for (int u = threadIdx.x; u < P.T * 32; u += 256) {
+      const int t = u / 32, e = 32 * sl + u % 32;
+      if (e < D) st_act(y + (int64_t)t * P.H * D, (size_t)e, 0.f);
+    }
+    return;
+  }
+  const int64_t off = ((int64_t)row * P.H + h) * D * D;
+  const float l = pow_decay(a.log_decay[h], 1);
+  const TA* q = (const TA*)a.q + b * P.q_stride[0] + h * P.q_stride[2];
+  const TA* k = (const TA*)a.k + b * P.k_stride[0] + h * P.k_stride[2];
+  const TA* v = (const TA*)a.v + b * P.v_stride[0] + h * P.v_stride[2];
+  float S[NR][VEC];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int d = rg + i * RG;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) S[i][j] = 0.f;
+    if (in && d < D && e0 < D) {
+      if constexpr (VEC == 4)
+        *(float4*)S[i] = *(const float4*)(in + off + (int64_t)d * D + e0);
+      else
+        S[i][0] = in[off + (int64_t)d * D + e0];
+    }
+  }
+  for (int t = 0; t < P.T; ++t) {
+    if (threadIdx.x < 128) {
+      qs[threadIdx.x] = threadIdx.x < D ? ld_act(q + t * P.q_stride[1], (size_t)threadIdx.x) : 0.f;
+    } else {
+      const int d = threadIdx.x - 128;
+      ks[d] = d < D ? ld_act(k + t * P.k_stride[1], (size_t)d) : 0.f;
+    }
+    float vv[VEC], acc[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      vv[j] = e0 + j < D ? ld_act(v + t * P.v_stride[1], (size_t)(e0 + j)) : 0.f;
+      acc[j] = 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int d = rg + i * RG;
+      if (d < D) {
+        const float kd = ks[d], qd = qs[d];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          S[i][j] = fmaf(l, S[i][j], kd * vv[j]);
+          acc[j] = fmaf(qd, S[i][j], acc[j]);
+        }
+      }
+    }
+    // rows of this warp (lanes CG apart), then warps through shared memory
+#pragma unroll
+    for (int o = CG; o < 32; o <<= 1)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+    if ((threadIdx.x & 31) < CG) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) red[threadIdx.x >> 5][cg * VEC + j] = acc[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
+      const int e = 32 * sl + threadIdx.x;
+      if (e < D) st_act(y + (int64_t)t * P.H * D, (size_t)e, P.scale * s);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int d = rg + i * RG;
+    if (d < D && e0 < D) {
+      if constexpr (VEC == 4)
+        *(float4*)(out + off + (int64_t)d * D + e0) = *(const float4*)S[i];
+      else
+        out[off + (int64_t)d * D + e0] = S[i][0];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+static int check(const AtlasDecayParams* p) {
+  if (!p) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (p->abi_version != ATLAS_ABI_VERSION) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "abi_version mismatch");
+  if (p->B < 0 || p->T < 0 || p->H < 0 || p->D < 1)
+    return report_error(ATLAS_ERR_INVALID_ARGUMENT, "B, T and H must not be negative and D must be positive");
+  if (p->D > 128) return report_error(ATLAS_ERR_UNSUPPORTED, "decay attention: head_dim D must be at most 128");
+  if (p->act_dtype != ATLAS_F32 && p->act_dtype != ATLAS_BF16)
+    return report_error(ATLAS_ERR_INVALID_ARGUMENT, "act_dtype must be ATLAS_F32 or ATLAS_BF16");
+  if (!std::isfinite(p->scale)) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "scale must be finite");
+  for (const int64_t* s : {p->q_stride, p->k_stride, p->v_stride})
+    if (s[0] < 0 || s[1] < 0 || s[2] < 0)
+      return report_error(ATLAS_ERR_INVALID_ARGUMENT, "strides must not be negative");
+  if (p->T > 1 << 30) return report_error(ATLAS_ERR_UNSUPPORTED, "decay attention: T must be at most 2^30");
+  // grids are one-dimensional: (batch, head, 32-token tile) and (batch, head, state element / 256)
+  const int64_t n = chains(*p);
+  if (n * std::max(4 * chunks(*p), 64) >= (int64_t)1 << 31)
+    return report_error(ATLAS_ERR_UNSUPPORTED, "decay attention: B * H * T is too large for one call");
+  clear_error();
+  return ATLAS_OK;
+}
+
+static size_t state_bytes(const AtlasDecayParams& p) {
+  return (size_t)chains(p) * chunks(p) * p.D * p.D * sizeof(float);
+}
+static int parts(const AtlasDecayParams& p) { return 2 * chunks(p) * (CH / TT); }  // of dlog_decay per chain
+static size_t ws_bytes(const AtlasDecayParams& p) {
+  return state_bytes(p) + (size_t)chains(p) * parts(p) * sizeof(float);
+}
+static int status_of(cudaError_t e) {
+  return e == cudaSuccess ? ATLAS_OK : report_error(ATLAS_ERR_CUDA, cudaGetErrorString(e));
+}
+static bool empty(const AtlasDecayParams& p) { return chains(p) == 0; }
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+static bool strides8(const int64_t* s) { return s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0; }
+// The tensor path moves 16-byte groups of 8 channels.
+static bool tensor_path(const Args& a) {
+  const AtlasDecayParams& p = a.p;
+  return p.act_dtype == ATLAS_BF16 && p.D % 8 == 0 && strides8(p.q_stride) && strides8(p.k_stride) &&
+         strides8(p.v_stride) && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.dy) &&
+         aligned16(a.y) && aligned16(a.dq) && aligned16(a.dk) && aligned16(a.dv) && aligned16(a.states) &&
+         aligned16(a.dstates);
+}
+
+static cudaError_t scan(const Args& a, const float* in, float* out, bool bwd, cudaStream_t s) {
+  float* buf = bwd ? a.dstates : a.states;
+  const bool v4 = a.p.D % 2 == 0 && aligned16(in) && aligned16(out) && aligned16(buf);  // D * D % 4 == 0
+  const int64_t n = chains(a.p) * a.p.D * a.p.D / (v4 ? 4 : 1);
+  const unsigned grid = (unsigned)((n + 255) / 256);
+  if (v4)
+    scan_kernel<4><<<grid, 256, 0, s>>>(a, in, out, buf, bwd);
+  else
+    scan_kernel<1><<<grid, 256, 0, s>>>(a, in, out, buf, bwd);
+  return cudaGetLastError();
+}
+
+// the CUDA-core kernels for one activation type and NI = ceil(D / 16), rounded up to 2, 4 or 8
+template <typename TA, int NI>
+struct Plain {
+  static size_t smem(int tiles, int squares) {
+    return ((size_t)tiles * TT * LD + (size_t)squares * TT * (TT + 1)) * sizeof(float);
+  }
+  static cudaError_t sums(const Args& a, bool bwd, cudaStream_t s) {
+    sums_kernel<TA, NI><<<(unsigned)(chains(a.p) * chunks(a.p)), 256, 0, s>>>(a, bwd);
+    return cudaGetLastError();
+  }
+  static cudaError_t out(const Args& a, cudaStream_t s) {
+    const int tiles = (a.p.T + TT - 1) / TT;
+    const size_t sm = smem(3, 1);
+    cudaError_t e = cudaFuncSetAttribute(out_kernel<TA, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+    if (e != cudaSuccess) return e;
+    out_kernel<TA, NI><<<(unsigned)(chains(a.p) * tiles), 256, sm, s>>>(a, tiles);
+    return cudaGetLastError();
+  }
+  static cudaError_t grads(const Args& a, cudaStream_t s) {
+    const int tiles = (a.p.T + TT - 1) / TT;
+    const unsigned grid = (unsigned)(chains(a.p) * tiles);
+    size_t sm = smem(4, 1);
+    cudaError_t e = cudaFuncSetAttribute(dq_kernel<TA, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+    if (e != cudaSuccess) return e;
+    dq_kernel<TA, NI><<<grid, 256, sm, s>>>(a, tiles);
+    sm = smem(4, 2);
+    e = cudaFuncSetAttribute(dkv_kernel<TA, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+    if (e != cudaSuccess) return e;
+    dkv_kernel<TA, NI><<<grid, 256, sm, s>>>(a, tiles);
+    return cudaGetLastError();
+  }
+};
+enum Phase { SUMS_FWD, SUMS_BWD, OUT, GRADS };
+template <typename TA, int NI>
+static cudaError_t plain_ni(const Args& a, Phase f, cudaStream_t s) {
+  using K = Plain<TA, NI>;
+  return f == OUT ? K::out(a, s) : f == GRADS ? K::grads(a, s) : K::sums(a, f == SUMS_BWD, s);
+}
+template <typename TA>
+static cudaError_t plain_t(const Args& a, Phase f, cudaStream_t s) {
+  return a.p.D <= 32 ? plain_ni<TA, 2>(a, f, s) : a.p.D <= 64 ? plain_ni<TA, 4>(a, f, s) : plain_ni<TA, 8>(a, f, s);
+}
+static cudaError_t run(const Args& a, Phase f, bool tensor, cudaStream_t s) {
+  if (tensor)
+    return f == OUT ? tc::launch_out(a, s) : f == GRADS ? tc::launch_grads(a, s)
+                                                        : tc::launch_chunk_states(a, f == SUMS_BWD, s);
+  return a.p.act_dtype == ATLAS_BF16 ? plain_t<__nv_bfloat16>(a, f, s) : plain_t<float>(a, f, s);
+}
+
+// out = in (or zeros): what an empty sequence leaves
+static cudaError_t pass_state(const AtlasDecayParams& p, const float* in, float* out, cudaStream_t s) {
+  if (!out || in == out) return cudaSuccess;
+  const size_t n = (size_t)chains(p) * p.D * p.D * sizeof(float);
+  return in ? cudaMemcpyAsync(out, in, n, cudaMemcpyDeviceToDevice, s) : cudaMemsetAsync(out, 0, n, s);
+}
+
+template <typename TA>
+static cudaError_t step_t(const Args& a, const float* in, const int32_t* slots, int32_t n, float* out, cudaStream_t s) {
+  const unsigned grid = (unsigned)(chains(a.p) * ((a.p.D + 31) / 32));
+  if (a.p.D % 4 == 0 && aligned16(in) && aligned16(out))
+    step_kernel<TA, 4><<<grid, 256, 0, s>>>(a, in, slots, n, out);
+  else
+    step_kernel<TA, 1><<<grid, 256, 0, s>>>(a, in, slots, n, out);
+  return cudaGetLastError();
+}
+
+}  // namespace decay
+}  // namespace atlas
+
+using namespace atlas;
+using namespace atlas::decay;
+
+extern "C" size_t atlas_decay_saved_bytes(const AtlasDecayParams* p) {
+  if (check(p) != ATLAS_OK) return 0;
+  return state_bytes(*p);
+}
+
+extern "C" size_t atlas_decay_workspace_bytes(const AtlasDecayParams* p) {
+  if (check(p) != ATLAS_OK) return 0;
+  return ws_bytes(*p);
+}
+
+extern "C" int atlas_decay_fwd(const AtlasDecayParams* p, const void* q, const void* k, const void* v,
+                               const float* log_decay, const float* state_in, void* y, float* state_out, void* saved,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check(p);
+  if (rc) return rc;
+  if (empty(*p)) return ATLAS_OK;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (!state_out || !log_decay) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
+  if (p->T == 0) return status_of(pass_state(*p, state_in, state_out, s));
+  if (!q || !k || !v || !y) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
+  if (!saved && (!workspace || workspace_bytes < state_bytes(*p)))
+    return report_error(ATLAS_ERR_WORKSPACE, "workspace smaller than atlas_decay_workspace_bytes()");
+  Args a{};
+  a.p = *p;
+  a.q = q, a.k = k, a.v = v;
+  a.log_decay = log_decay;
+  a.y = y;
+  a.states = (float*)(saved ? saved : workspace);
+  a.status = device_status_ptr();
+  const bool tensor = tensor_path(a);
+  cudaError_t e = run(a, SUMS_FWD, tensor, s);
+  if (e == cudaSuccess) e = scan(a, state_in, state_out, false, s);
+  if (e == cudaSuccess) e = run(a, OUT, tensor, s);
+  return status_of(e);
+}
+
+extern "C" int atlas_decay_bwd(const AtlasDecayParams* p, const void* q, const void* k, const void* v,
+                               const float* log_decay, const void* saved, const void* dy, const float* dstate_out,
+                               void* dq, void* dk, void* dv, float* dlog_decay, float* dstate_in, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  int rc = check(p);
+  if (rc) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (empty(*p) || p->T == 0) {
+    if (p->H > 0 && dlog_decay) {
+      // an empty sequence passes the state through: no decay is applied
+      cudaError_t e = cudaMemsetAsync(dlog_decay, 0, (size_t)p->H * sizeof(float), s);
+      if (e != cudaSuccess) return status_of(e);
+    }
+    return empty(*p) ? ATLAS_OK : status_of(pass_state(*p, dstate_out, dstate_in, s));
+  }
+  if (!q || !k || !v || !log_decay || !saved || !dy || !dq || !dk || !dv)
+    return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
+  if (!workspace || workspace_bytes < ws_bytes(*p))
+    return report_error(ATLAS_ERR_WORKSPACE, "workspace smaller than atlas_decay_workspace_bytes()");
+  Args a{};
+  a.p = *p;
+  a.q = q, a.k = k, a.v = v, a.dy = dy;
+  a.log_decay = log_decay;
+  a.dq = dq, a.dk = dk, a.dv = dv;
+  a.states = (float*)const_cast<void*>(saved);
+  a.dstates = (float*)workspace;
+  a.dg_part = (float*)((uint8_t*)workspace + state_bytes(*p));
+  a.status = device_status_ptr();
+  const bool tensor = tensor_path(a);
+  a.dg_parts = tensor ? chunks(*p) : 2 * ((p->T + TT - 1) / TT);
+  cudaError_t e = run(a, SUMS_BWD, tensor, s);
+  if (e == cudaSuccess) e = scan(a, dstate_out, dstate_in, true, s);
+  if (e == cudaSuccess) e = run(a, GRADS, tensor, s);
+  if (e == cudaSuccess && dlog_decay) {
+    dg_kernel<<<p->H, 256, 0, s>>>(a, dlog_decay);
+    e = cudaGetLastError();
+  }
+  return status_of(e);
+}
+
+extern "C" int atlas_decay_step(const AtlasDecayParams* p, const void* q, const void* k, const void* v,
+                                const float* log_decay, const float* state_in, const int32_t* slots, int32_t n_slots,
+                                void* y, float* state_out, void* stream) {
+  int rc = check(p);
+  if (rc) return rc;
+  if (empty(*p)) return ATLAS_OK;
+  if (!state_in || !state_out || !log_decay)
+    return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
+  if (slots && n_slots < 0) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "n_slots must not be negative");
+  if (p->T > 0 && (!q || !k || !v || !y)) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
+  Args a{};
+  a.p = *p;
+  a.q = q, a.k = k, a.v = v, a.y = y;
+  a.log_decay = log_decay;
+  cudaStream_t s = (cudaStream_t)stream;
+  return status_of(p->act_dtype == ATLAS_BF16 ? step_t<__nv_bfloat16>(a, state_in, slots, n_slots, state_out, s)
+                                              : step_t<float>(a, state_in, slots, n_slots, state_out, s));
+}
