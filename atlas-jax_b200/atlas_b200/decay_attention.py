@@ -9,11 +9,12 @@ states by one or a few tokens (generation).  Every computation runs in libatlas_
 """
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib as L
-from .scan import _WS, _ptr, _stream
+from .scan import _WS, addr, empty_like, on_device, stream_of
 
 
 class AtlasDecayParams(ctypes.Structure):
@@ -44,81 +45,93 @@ def _lib():
     return lib
 
 
-def _check(q, k, v, log_decay):
-    """Shapes, types and devices; returns q, k, v with contiguous channels."""
-    if q.dim() != 4:
-        raise ValueError(f"q: expected (B, T, H, D), got {tuple(q.shape)}")
-    if q.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"q: expected float32 or bfloat16, got {q.dtype}")
-    for n, x in (("q", q), ("k", k), ("v", v)):
-        if x.dtype != q.dtype or x.shape != q.shape or not x.is_cuda or x.device != q.device:
-            raise ValueError(f"{n}: expected CUDA {q.dtype} {tuple(q.shape)}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    _need(log_decay, (q.shape[2],), "log_decay", q.device)
-    return [x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous() for x in (q, k, v)]
+class _Plan:
+    """What a call needs that depends on shapes, strides and types alone."""
+
+    def __init__(self, q, k, v, g, scale):
+        (shape, st, dtype, dev) = q
+        if len(shape) != 4:
+            raise ValueError(f"q: expected (B, T, H, D), got {tuple(shape)}")
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"q: expected float32 or bfloat16, got {dtype}")
+        for n, x in (("q", q), ("k", k), ("v", v)):
+            if x[0] != shape or x[2] != dtype or x[3] != dev or dev < 0:
+                raise ValueError(f"{n}: expected CUDA {dtype} {tuple(shape)} on the device of q, got {x[2]} {tuple(x[0])}")
+        B, T, H, D = shape
+        if g[0] != (H,) or g[2] != torch.float32 or g[3] != dev or (g[1] != (1,) and H > 1):
+            raise ValueError(f"log_decay: expected contiguous CUDA float32 {(H,)}, got {g[2]} {tuple(g[0])}")
+        self.packed = D == 1 or all(x[1][3] == 1 for x in (q, k, v))  # channels contiguous
+        strides = [(ctypes.c_int64 * 3)(*x[1][:3]) for x in (q, k, v)]
+        self.params = AtlasDecayParams(L.ATLAS_ABI_VERSION, B, T, H, D,
+                                       L.ATLAS_BF16 if dtype == torch.bfloat16 else L.ATLAS_F32,
+                                       D ** -0.5 if scale is None else scale, 0, *strides)
+        self.ref = ctypes.byref(self.params)
+        self.shape, self.dtype = tuple(shape), dtype
+        self.B, self.state_shape = B, (B, H, D, D)
+        self.saved_bytes = self._size(_lib().atlas_decay_saved_bytes)
+        self.workspace_bytes = self._size(_lib().atlas_decay_workspace_bytes)
+
+    def _size(self, query):
+        """A size query's answer; 0 is an error only when it left a message."""
+        n = query(self.ref)
+        if n == 0 and L.load().atlas_last_error_string():
+            raise L.AtlasError(L.ATLAS_ERR_INVALID_ARGUMENT, L.load().atlas_last_error_string().decode())
+        return n
 
 
-def _need(x, shape, name, device):
-    if x.dtype != torch.float32 or tuple(x.shape) != tuple(shape) or not x.is_contiguous() or x.device != device:
-        raise ValueError(f"{name}: expected contiguous CUDA float32 {tuple(shape)}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+_plans = functools.lru_cache(maxsize=512)(_Plan)
 
 
-def _params(q, k, v, scale):
-    B, T, H, D = q.shape
-    s = [(ctypes.c_int64 * 3)(*x.stride()[:3]) for x in (q, k, v)]
-    return AtlasDecayParams(L.ATLAS_ABI_VERSION, B, T, H, D, L.ATLAS_BF16 if q.dtype == torch.bfloat16 else L.ATLAS_F32,
-                            D ** -0.5 if scale is None else scale, 0, *s)
+def _plan(q, k, v, log_decay, scale):
+    """Checks the inputs; returns their plan and q, k, v with contiguous channels."""
+    p = _plans(*[(x.shape, x.stride(), x.dtype, x.get_device()) for x in (q, k, v, log_decay)], scale)
+    if not p.packed:
+        return _plan(q.contiguous(), k.contiguous(), v.contiguous(), log_decay, scale)
+    return p, q, k, v
 
 
-def _size(n):
-    """A size query's answer; 0 is an error only when it left a message."""
-    if n == 0 and L.load().atlas_last_error_string():
-        raise L.AtlasError(L.ATLAS_ERR_INVALID_ARGUMENT, L.load().atlas_last_error_string().decode())
-    return n
+def _need(x, shape, name, q):
+    if x.dtype != torch.float32 or x.shape != shape or not x.is_contiguous() or x.get_device() != q.get_device():
+        raise ValueError(f"{name}: expected contiguous float32 {tuple(shape)} on {q.device}, "
+                         f"got {x.dtype} {tuple(x.shape)} on {x.device}")
 
 
 def decay_attention_forward(q, k, v, log_decay, state=None, scale=None, need_saved=True, workspace=None):
     """q, k, v: (B, T, H, D) float32 or bf16, any strides with contiguous channels; log_decay
     (H,) float32; state (B, H, D, D) float32 or None (zeros); scale defaults to D^-0.5.
     Returns (y, state after the last token, saved for the backward or None)."""
-    lib = _lib()
-    q, k, v = _check(q, k, v, log_decay)
-    B, T, H, D = q.shape
+    p, q, k, v = _plan(q, k, v, log_decay, scale)
     dev = q.device
     if state is not None:
-        _need(state, (B, H, D, D), "state", dev)
-    with torch.cuda.device(dev):
-        p = _params(q, k, v, scale)
-        y = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
-        out = torch.empty(B, H, D, D, device=dev)
-        nbytes = _size(lib.atlas_decay_saved_bytes(ctypes.byref(p)))
-        saved = torch.empty(nbytes, dtype=torch.uint8, device=dev) if need_saved else None
-        ws, wsb = (None, 0) if need_saved else (workspace or _WS).get(nbytes, dev)
-        L.check(lib.atlas_decay_fwd(ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state), _ptr(y),
-                                    _ptr(out), _ptr(saved), _ptr(ws), wsb, _stream(dev)))
+        _need(state, p.state_shape, "state", q)
+    with on_device(dev):
+        y = empty_like(q)
+        out = torch.empty(p.state_shape, device=dev) if state is None else empty_like(state)
+        saved = torch.empty(p.saved_bytes, dtype=torch.uint8, device=dev) if need_saved else None
+        ws, wsb = (None, 0) if need_saved else (workspace or _WS).get(p.saved_bytes, dev)
+        L.check(_lib().atlas_decay_fwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), addr(state),
+                                       y.data_ptr(), out.data_ptr(), addr(saved), addr(ws), wsb, stream_of(dev)))
     return y, out, saved
 
 
 def decay_attention_backward(q, k, v, log_decay, saved, dy, dstate=None, scale=None, workspace=None):
     """VJP of ``decay_attention_forward``: (dq, dk, dv, dlog_decay, dstate_in)."""
-    lib = _lib()
-    q, k, v = _check(q, k, v, log_decay)
-    B, T, H, D = q.shape
+    p, q, k, v = _plan(q, k, v, log_decay, scale)
     dev = q.device
-    if dy.dtype != q.dtype or dy.shape != q.shape or dy.device != dev:
-        raise ValueError(f"dy: expected CUDA {q.dtype} {tuple(q.shape)}, got {dy.dtype} {tuple(dy.shape)} on {dy.device}")
+    if dy.dtype != p.dtype or dy.shape != p.shape or dy.get_device() != q.get_device():
+        raise ValueError(f"dy: expected {p.dtype} {p.shape} on {dev}, got {dy.dtype} {tuple(dy.shape)} on {dy.device}")
     dy = dy.contiguous()
     if dstate is not None:
-        _need(dstate, (B, H, D, D), "dstate", dev)
-    with torch.cuda.device(dev):
-        p = _params(q, k, v, scale)
-        if saved.numel() * saved.element_size() < _size(lib.atlas_decay_saved_bytes(ctypes.byref(p))):
-            raise ValueError("saved: not what decay_attention_forward saved for these inputs")
-        dq, dk, dv = (torch.empty(B, T, H, D, dtype=q.dtype, device=dev) for _ in range(3))
-        dg, dstate_in = torch.empty(H, device=dev), torch.empty(B, H, D, D, device=dev)
-        ws, wsb = (workspace or _WS).get(_size(lib.atlas_decay_workspace_bytes(ctypes.byref(p))), dev)
-        L.check(lib.atlas_decay_bwd(ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(saved), _ptr(dy),
-                                    _ptr(dstate), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dg), _ptr(dstate_in), _ptr(ws), wsb,
-                                    _stream(dev)))
+        _need(dstate, p.state_shape, "dstate", q)
+    if saved.numel() * saved.element_size() != p.saved_bytes or saved.get_device() != q.get_device():
+        raise ValueError("saved: not what decay_attention_forward saved for these inputs")
+    with on_device(dev):
+        dq, dk, dv = empty_like(q), empty_like(q), empty_like(q)
+        dg, dstate_in = torch.empty(p.shape[2], device=dev), torch.empty(p.state_shape, device=dev)
+        ws, wsb = (workspace or _WS).get(p.workspace_bytes, dev)
+        L.check(_lib().atlas_decay_bwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+                                       saved.data_ptr(), dy.data_ptr(), addr(dstate), dq.data_ptr(), dk.data_ptr(),
+                                       dv.data_ptr(), dg.data_ptr(), dstate_in.data_ptr(), addr(ws), wsb, stream_of(dev)))
     return dq, dk, dv, dg, dstate_in
 
 
@@ -130,22 +143,22 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None, out=
     sequence a row of its own; a slot outside the pool marks an idle sequence, whose y is
     0).  The new states are written to ``out`` (a buffer like ``state``; default: in place).
     Returns (y, out)."""
-    lib = _lib()
-    q, k, v = _check(q, k, v, log_decay)
-    B, T, H, D = q.shape
+    p, q, k, v = _plan(q, k, v, log_decay, scale)
     dev = q.device
-    n = B if slots is None else state.shape[0]
-    _need(state, (n, H, D, D), "state", dev)
-    out = state if out is None else out
-    _need(out, (n, H, D, D), "out", dev)
-    if slots is not None and (slots.dtype != torch.int32 or tuple(slots.shape) != (B,) or not slots.is_contiguous()
-                              or slots.device != dev):
-        raise ValueError(f"slots: expected contiguous CUDA int32 ({B},), got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
-    with torch.cuda.device(dev):
-        p = _params(q, k, v, scale)
-        y = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
-        L.check(lib.atlas_decay_step(ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state), _ptr(slots),
-                                     n, _ptr(y), _ptr(out), _stream(dev)))
+    n = p.B if slots is None else state.shape[0]
+    shape = (n,) + p.state_shape[1:]
+    _need(state, shape, "state", q)
+    if out is None:
+        out = state
+    else:
+        _need(out, shape, "out", q)
+    if slots is not None and (slots.dtype != torch.int32 or slots.shape != (p.B,) or not slots.is_contiguous()
+                              or slots.get_device() != q.get_device()):
+        raise ValueError(f"slots: expected contiguous int32 ({p.B},) on {dev}, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
+    with on_device(dev):
+        y = empty_like(q)
+        L.check(_lib().atlas_decay_step(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+                                        state.data_ptr(), addr(slots), n, y.data_ptr(), out.data_ptr(), stream_of(dev)))
     return y, out
 
 

@@ -6,11 +6,12 @@ x is (..., N) with weight and bias (N,), or (..., G, N) with weight and bias (G,
 for each group (the heads of an attention output)."""
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib as L
-from .scan import _WS, _ptr, _stream
+from .scan import _WS, addr, on_device, stream_of
 
 
 class AtlasNormParams(ctypes.Structure):
@@ -37,49 +38,66 @@ def _lib():
     return lib
 
 
-def _group(x, weight, bias):
-    """(G, N) of the parameters, checked against x."""
-    if x.dtype not in (torch.float32, torch.bfloat16) or not x.is_cuda or x.dim() < 1:
-        raise ValueError(f"x: expected a CUDA float32 or bfloat16 (..., N) tensor, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    shape = None
-    for n, w in (("weight", weight), ("bias", bias)):
-        if w is None:
-            continue
-        if shape is None:
-            shape = tuple(w.shape)
-            if len(shape) not in (1, 2) or x.dim() < len(shape) or tuple(x.shape[-len(shape):]) != shape:
-                raise ValueError(f"{n}: {shape} are not the last one or two axes of x {tuple(x.shape)}")
-        if w.dtype != torch.float32 or tuple(w.shape) != shape or not w.is_contiguous() or w.device != x.device:
-            raise ValueError(f"{n}: expected contiguous float32 {shape} on {x.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
-    return (1, x.shape[-1]) if shape is None or len(shape) == 1 else shape
+class _Plan:
+    """What a call needs that depends on shapes and types alone.  x: (shape, type, device);
+    params: the same with contiguity for weight and bias, or None."""
+
+    def __init__(self, x, weight, bias, eps):
+        shape, dtype, dev = x
+        if dtype not in (torch.float32, torch.bfloat16) or dev < 0 or len(shape) < 1:
+            raise ValueError(f"x: expected a CUDA float32 or bfloat16 (..., N) tensor, got {dtype} {tuple(shape)}")
+        p = None
+        for n, w in (("weight", weight), ("bias", bias)):
+            if w is None:
+                continue
+            if p is None:
+                p = tuple(w[0])
+                if len(p) not in (1, 2) or len(shape) < len(p) or tuple(shape[-len(p):]) != p:
+                    raise ValueError(f"{n}: {p} are not the last one or two axes of x {tuple(shape)}")
+            if w[1] != torch.float32 or tuple(w[0]) != p or w[2] != dev or not w[3]:
+                raise ValueError(f"{n}: expected contiguous float32 {p} on the device of x, got {w[1]} {tuple(w[0])}")
+        self.param_shape = p or (shape[-1],)
+        G, N = (1, shape[-1]) if len(self.param_shape) == 1 else self.param_shape
+        rows = shape.numel() // (G * N) if G * N else 0
+        self.params = AtlasNormParams(L.ATLAS_ABI_VERSION, L.ATLAS_BF16 if dtype == torch.bfloat16 else L.ATLAS_F32,
+                                      rows, G, N, eps, 0)
+        self.ref, self.vecs = ctypes.byref(self.params), rows * G
+        self.workspace_bytes = _lib().atlas_layernorm_workspace_bytes(self.ref)
+        if self.workspace_bytes == 0:
+            raise L.AtlasError(L.ATLAS_ERR_INVALID_ARGUMENT, L.load().atlas_last_error_string().decode())
 
 
-def _params(x, G, N, eps):
-    rows = x.numel() // (G * N) if G * N else 0
-    return AtlasNormParams(L.ATLAS_ABI_VERSION, L.ATLAS_BF16 if x.dtype == torch.bfloat16 else L.ATLAS_F32, rows, G, N,
-                           eps, 0)
+_plans = functools.lru_cache(maxsize=512)(_Plan)
+
+
+def _key(w):
+    return None if w is None else (w.shape, w.dtype, w.get_device(), w.is_contiguous())
+
+
+def _plan(x, weight, bias, eps):
+    return _plans((x.shape, x.dtype, x.get_device()), _key(weight), _key(bias), eps)
 
 
 def _like(x, ref, name):
-    if x.dtype != ref.dtype or x.shape != ref.shape or x.device != ref.device:
+    if x.dtype != ref.dtype or x.shape != ref.shape or x.get_device() != ref.get_device():
         raise ValueError(f"{name}: expected {ref.dtype} {tuple(ref.shape)} on {ref.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
     return x.contiguous()
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None):
     """Returns (y, h, stats): h = x + residual (x itself without a residual), y its layer
-    norm, stats (vectors, 2) float32 the means and reciprocal deviations of h."""
-    lib = _lib()
-    G, N = _group(x, weight, bias)
+    norm, stats (vectors, 2) float32 what the backward needs of the statistics of h."""
+    p = _plan(x, weight, bias, eps)
     x = x.contiguous()
-    residual = None if residual is None else _like(residual, x, "residual")
-    with torch.cuda.device(x.device):
-        p = _params(x, G, N, eps)
+    dev = x.device
+    with on_device(dev):
         y = torch.empty_like(x)
-        h = x if residual is None else torch.empty_like(x)
-        stats = torch.empty(p.rows * G, 2, device=x.device)
-        L.check(lib.atlas_layernorm_fwd(ctypes.byref(p), _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(y),
-                                        None if residual is None else _ptr(h), _ptr(stats), _stream(x.device)))
+        h = x
+        if residual is not None:
+            residual, h = _like(residual, x, "residual"), torch.empty_like(x)
+        stats = torch.empty((p.vecs, 2), device=dev)
+        L.check(_lib().atlas_layernorm_fwd(p.ref, x.data_ptr(), addr(residual), addr(weight), addr(bias), y.data_ptr(),
+                                           None if residual is None else h.data_ptr(), stats.data_ptr(), stream_of(dev)))
     return y, h, stats
 
 
@@ -88,25 +106,28 @@ def layer_norm_backward(dy, h, weight, stats, dh=None, need_params=True, shape=N
     residual; dh the cotangent of h (None: zeros); the parameter gradients have the shape
     of ``weight`` (or ``shape``, for a norm with a bias alone) and are None with
     need_params=False."""
-    lib = _lib()
-    G, N = _group(h, weight, None)
-    shape = tuple(weight.shape) if weight is not None else (h.shape[-1],) if shape is None else tuple(shape)
-    if weight is None and len(shape) == 2:
-        G = shape[0]
+    if weight is None and shape is not None:  # a plan for parameters of that shape
+        p = _plans((h.shape, h.dtype, h.get_device()), (tuple(shape), torch.float32, h.get_device(), True), None, 0.0)
+    else:
+        p = _plan(h, weight, None, 0.0)
     h = h.contiguous()
     dy = _like(dy, h, "dy")
-    dh = None if dh is None else _like(dh, h, "dh")
+    if dh is not None:
+        dh = _like(dh, h, "dh")
     dev = h.device
-    with torch.cuda.device(dev):
-        p = _params(h, G, N, 0.0)
-        if stats.dtype != torch.float32 or tuple(stats.shape) != (p.rows * G, 2) or not stats.is_contiguous() \
-                or stats.device != dev:
-            raise ValueError(f"stats: expected contiguous float32 {(p.rows * G, 2)} on {dev}, got {stats.dtype} {tuple(stats.shape)}")
+    if stats.dtype != torch.float32 or stats.shape != (p.vecs, 2) or not stats.is_contiguous() \
+            or stats.get_device() != h.get_device():
+        raise ValueError(f"stats: expected contiguous float32 {(p.vecs, 2)} on {dev}, got {stats.dtype} {tuple(stats.shape)}")
+    with on_device(dev):
         dx = torch.empty_like(h)
-        dw, db = (torch.empty(shape, device=dev), torch.empty(shape, device=dev)) if need_params else (None, None)
-        ws, wsb = (workspace or _WS).get(lib.atlas_layernorm_workspace_bytes(ctypes.byref(p)), dev)
-        L.check(lib.atlas_layernorm_bwd(ctypes.byref(p), _ptr(dy), _ptr(h), _ptr(weight), _ptr(stats), _ptr(dh), _ptr(dx),
-                                        _ptr(dw), _ptr(db), _ptr(ws), wsb, _stream(dev)))
+        dw = db = ws = None
+        wsb = 0
+        if need_params:
+            dw = torch.empty(p.param_shape, device=dev) if weight is None else torch.empty_like(weight)
+            db = torch.empty_like(dw)
+            ws, wsb = (workspace or _WS).get(p.workspace_bytes, dev)
+        L.check(_lib().atlas_layernorm_bwd(p.ref, dy.data_ptr(), h.data_ptr(), addr(weight), stats.data_ptr(), addr(dh),
+                                           dx.data_ptr(), addr(dw), addr(db), addr(ws), wsb, stream_of(dev)))
     return dx, dw, db
 
 

@@ -7,6 +7,7 @@ for the custom-VJP pair): ``scan_forward`` / ``scan_backward`` are the two halve
 of the custom VJP and ``AtlasScan`` glues them into autograd.
 """
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -39,6 +40,30 @@ def _stream(dev):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+# The same for short calls, whose launch overhead counts: plain integers (a ctypes
+# prototype takes them as pointers), the current stream without a Stream object around it
+# (2 us of a call of 10), and no device switch where none is needed.
+def addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def stream_of(dev):
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
+
+
+def empty_like(x):
+    """An uninitialised contiguous tensor of x's shape, type and device."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def on_device(dev):
+    """Context in which ``dev`` is the current device."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+_HERE = contextlib.nullcontext()
+
+
 def _check_act(x, name, dtype, shape):
     if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous() or not x.is_cuda:
         raise ValueError(f"{name}: expected contiguous CUDA {dtype} {shape}, got {x.dtype} {tuple(x.shape)}")
@@ -57,7 +82,7 @@ class Workspace:
     def get(self, nbytes, device):
         if nbytes == 0:
             return None, 0
-        key = (device, torch.cuda.current_stream(device).cuda_stream)
+        key = (device, stream_of(device))
         buf = self.bufs.get(key)
         if buf is None or buf.numel() < nbytes:
             buf = self.bufs[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)

@@ -611,7 +611,7 @@ struct Plain {
   static cudaError_t out(const Args& a, cudaStream_t s) {
     const int tiles = (a.p.T + TT - 1) / TT;
     const size_t sm = smem(3, 1);
-    cudaError_t e = cudaFuncSetAttribute(out_kernel<TA, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+    cudaError_t e = allow_smem<out_kernel<TA, NI>>(sm);
     if (e != cudaSuccess) return e;
     out_kernel<TA, NI><<<(unsigned)(chains(a.p) * tiles), 256, sm, s>>>(a, tiles);
     return cudaGetLastError();
@@ -620,11 +620,11 @@ struct Plain {
     const int tiles = (a.p.T + TT - 1) / TT;
     const unsigned grid = (unsigned)(chains(a.p) * tiles);
     size_t sm = smem(4, 1);
-    cudaError_t e = cudaFuncSetAttribute(dq_kernel<TA, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+    cudaError_t e = allow_smem<dq_kernel<TA, NI>>(sm);
     if (e != cudaSuccess) return e;
     dq_kernel<TA, NI><<<grid, 256, sm, s>>>(a, tiles);
     sm = smem(4, 2);
-    e = cudaFuncSetAttribute(dkv_kernel<TA, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+    e = allow_smem<dkv_kernel<TA, NI>>(sm);
     if (e != cudaSuccess) return e;
     dkv_kernel<TA, NI><<<grid, 256, sm, s>>>(a, tiles);
     return cudaGetLastError();

@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "atlas_decay.h"
+#include "scan_internal.h"
 
 namespace atlas {
 namespace decay {
@@ -27,6 +28,18 @@ __host__ __device__ inline int64_t chains(const AtlasDecayParams& p) { return (i
 __host__ __device__ inline int chunk_len(const AtlasDecayParams& p, int c) {
   const int left = p.T - c * CH;
   return left < CH ? left : CH;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory; asked of the driver once per device.
+template <auto Kernel>
+cudaError_t allow_smem(size_t bytes) {
+  static DeviceCache done;
+  cudaError_t e = cudaSuccess;
+  done.get([&] {
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e == cudaSuccess ? 0 : -1;
+  });
+  return e;
 }
 
 // tcgen05 path (decay_tc.cu): bf16, D a multiple of 8, 16-byte aligned rows.

@@ -497,7 +497,7 @@ static unsigned grid(const Args& a) { return (unsigned)(chains(a.p) * chunks(a.p
 template <int DP>
 static cudaError_t sums(const Args& a, bool bwd, cudaStream_t s) {
   const size_t sm = 4 * TILE<DP> + sizeof(Ctl) + 128;
-  cudaError_t e = cudaFuncSetAttribute(sums_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+  cudaError_t e = allow_smem<sums_kernel<DP>>(sm);
   if (e != cudaSuccess) return e;
   sums_kernel<DP><<<grid(a), 256, sm, s>>>(a, bwd);
   return cudaGetLastError();
@@ -505,7 +505,7 @@ static cudaError_t sums(const Args& a, bool bwd, cudaStream_t s) {
 template <int DP>
 static cudaError_t out(const Args& a, cudaStream_t s) {
   const size_t sm = 3 * TILE<DP> + std::max(2 * STILE<DP>, PTILE) + sizeof(Ctl) + 128;
-  cudaError_t e = cudaFuncSetAttribute(out_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+  cudaError_t e = allow_smem<out_kernel<DP>>(sm);
   if (e != cudaSuccess) return e;
   out_kernel<DP><<<grid(a), 256, sm, s>>>(a);
   return cudaGetLastError();
@@ -513,7 +513,7 @@ static cudaError_t out(const Args& a, cudaStream_t s) {
 template <int DP>
 static cudaError_t grads(const Args& a, cudaStream_t s) {
   const size_t sm = 4 * TILE<DP> + std::max(3 * STILE<DP>, 2 * PTILE) + sizeof(Ctl) + 128;
-  cudaError_t e = cudaFuncSetAttribute(grads_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+  cudaError_t e = allow_smem<grads_kernel<DP>>(sm);
   if (e != cudaSuccess) return e;
   grads_kernel<DP><<<grid(a), 512, sm, s>>>(a);
   return cudaGetLastError();

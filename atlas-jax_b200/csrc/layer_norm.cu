@@ -9,8 +9,8 @@
 //   SUB    a power of two of lanes (4 .. 32) inside a warp, one group each: short vectors
 //          (heads).  The weights repeat every G * N channels, so a thread whose position
 //          advances by whole rows keeps its channels: the weight gradients stay in registers.
-//   WARP   one warp, CHN groups: up to 32 * VEC * CHN channels
-//   BLOCK  all warps of a block: longer vectors
+//   WARPS  1 to 16 whole warps; several teams share a block while they fit 8 warps, each with
+//          a named barrier of its own for its sums
 //   BIG    vectors beyond that: the block reads the vector once for each sum
 //   TINY   up to 8 channels: one thread in float64.  The gradient of so short a vector
 //          cancels (for two channels it is of the order eps / var: the normalised pair is
@@ -50,17 +50,92 @@ struct alignas(sizeof(TA) * VEC) Pack {
   TA v[VEC];
 };
 template <typename TA, int VEC>
-__device__ __forceinline__ void load(float* f, const TA* p) {
-  const Pack<TA, VEC> k = *(const Pack<TA, VEC>*)p;
+__device__ __forceinline__ void unpack(float* f, const Pack<TA, VEC>& k) {
+  if constexpr (sizeof(TA) == 2 && VEC > 1) {
+    const __nv_bfloat162* h = (const __nv_bfloat162*)&k;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) f[j] = ld_act(k.v, (size_t)j);
+    for (int j = 0; j < VEC / 2; ++j) {
+      const float2 t = __bfloat1622float2(h[j]);
+      f[2 * j] = t.x;
+      f[2 * j + 1] = t.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = ld_act(k.v, (size_t)j);
+  }
+}
+template <typename TA, int VEC>
+__device__ __forceinline__ void load(float* f, const TA* p) {
+  unpack<TA, VEC>(f, *(const Pack<TA, VEC>*)p);
 }
 template <typename TA, int VEC>
 __device__ __forceinline__ void store(TA* p, const float* f) {
   Pack<TA, VEC> k;
+  if constexpr (sizeof(TA) == 2 && VEC > 1) {
+    __nv_bfloat162* h = (__nv_bfloat162*)&k;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) st_act(k.v, (size_t)j, f[j]);
+    for (int j = 0; j < VEC / 2; ++j) h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) st_act(k.v, (size_t)j, f[j]);
+  }
   *(Pack<TA, VEC>*)p = k;
+}
+// Two lanes of float32 in one instruction (same rounding as the scalar ones): the backward is
+// as near to the issue limit as to the memory's.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 f2_get(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// A group as pairs; a single channel is a pair with a zero.
+template <int VEC>
+constexpr int PAIRS = (VEC + 1) / 2;
+template <typename TA, int VEC>
+__device__ __forceinline__ void unpack2(F2* f, const Pack<TA, VEC>& k) {
+  float t[VEC];
+  unpack<TA, VEC>(t, k);
+#pragma unroll
+  for (int j = 0; j < PAIRS<VEC>; ++j) f[j] = f2(t[2 * j], 2 * j + 1 < VEC ? t[2 * j + 1] : 0.f);
+}
+template <typename TA, int VEC>
+__device__ __forceinline__ void store2(TA* p, const F2* f) {
+  float t[2 * PAIRS<VEC>];
+#pragma unroll
+  for (int j = 0; j < PAIRS<VEC>; ++j) {
+    const float2 x = f2_get(f[j]);
+    t[2 * j] = x.x;
+    t[2 * j + 1] = x.y;
+  }
+  store<TA, VEC>(p, t);
+}
+// 16 bytes from global to this thread's own slot in shared memory, without registers
+__device__ __forceinline__ void copy16(void* slot, const void* g) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slot)), "l"(g)
+               : "memory");
 }
 template <typename TA>
 __device__ __forceinline__ float round_to(float x) {
@@ -83,28 +158,28 @@ __device__ __forceinline__ void load_param(float* f, const float* p, float missi
   }
 }
 
-enum Team { SUB, WARP, BLOCK };
+enum Team { SUB, ONE, MANY };  // MANY: WARPS teams of more than one warp
 
-// Sums of K values over a team; every lane gets them.  BLOCK: `red` holds 2 x 32 x K floats,
-// used alternately so that one barrier per call is enough.
+// Sums of K values over a team; every lane gets them.  MANY: `red` holds 2 x 16 x K floats of
+// the team, used alternately so that one barrier per call is enough.
 template <Team TEAM, int LANES, int K>
-__device__ __forceinline__ void team_sum(float* v, float* red, int& turn) {
+__device__ __forceinline__ void team_sum(float* v, float* red, int& turn, int warps, int barrier) {
   constexpr int W = TEAM == SUB ? LANES : 32;
 #pragma unroll
   for (int o = W / 2; o > 0; o >>= 1)
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-  if constexpr (TEAM == BLOCK) {
-    float* r = red + turn * 32 * K;
+  if constexpr (TEAM == MANY) {
+    float* r = red + turn * 16 * K;
     turn ^= 1;
-    const int w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const int w = (threadIdx.x >> 5) % warps;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
       for (int k = 0; k < K; ++k) r[w * K + k] = v[k];
-    __syncthreads();
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] = 0.f;
-    for (int i = 0; i < nw; ++i)
+    for (int i = 0; i < warps; ++i)
 #pragma unroll
       for (int k = 0; k < K; ++k) v[k] += r[i * K + k];
   }
@@ -112,29 +187,33 @@ __device__ __forceinline__ void team_sum(float* v, float* red, int& turn) {
 
 // Where this thread's team works: its vectors are first, first + stride, ... and lane /
 // lanes place it in the team.  SUB: the position inside a row is fixed, rows advance.
+// WARPS: `per_block` teams of a block take consecutive vectors.
 template <Team TEAM, int LANES>
 struct Place {
   int64_t first, stride;
-  int lane, lanes;
-  __device__ __forceinline__ Place(const Args& a, int rows_per_block) {
+  int lane, lanes, team, warps;
+  __device__ __forceinline__ Place(const Args& a, int per_block) {
     if constexpr (TEAM == SUB) {
       const int per_row = a.G * LANES, slot = threadIdx.x / per_row, in_row = threadIdx.x % per_row;
       lane = in_row % LANES;
       lanes = LANES;
-      first = ((int64_t)blockIdx.x * rows_per_block + slot) * a.G + in_row / LANES;
-      if (slot >= rows_per_block) first = a.vecs;  // spare threads of the last warp
-      stride = (int64_t)gridDim.x * rows_per_block * a.G;
-    } else if constexpr (TEAM == WARP) {
-      lane = threadIdx.x & 31;
-      lanes = 32;
-      first = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-      stride = (int64_t)gridDim.x * (blockDim.x >> 5);
+      warps = 1;
+      team = slot;
+      first = ((int64_t)blockIdx.x * per_block + slot) * a.G + in_row / LANES;
+      if (slot >= per_block) first = a.vecs;  // spare threads of the last warp
+      stride = (int64_t)gridDim.x * per_block * a.G;
     } else {
-      lane = threadIdx.x;
-      lanes = blockDim.x;
-      first = blockIdx.x;
-      stride = gridDim.x;
+      lanes = TEAM == ONE ? 32 : blockDim.x / per_block;
+      warps = lanes >> 5;
+      team = threadIdx.x / lanes;
+      lane = threadIdx.x % lanes;
+      first = (int64_t)blockIdx.x * per_block + team;
+      stride = (int64_t)gridDim.x * per_block;
     }
+  }
+  // every lane of a warp (SUB) or team runs the same number of rounds
+  __device__ __forceinline__ bool done(int64_t v, int64_t vecs) const {
+    return TEAM == SUB ? !__any_sync(0xffffffffu, v < vecs) : v >= vecs;
   }
 };
 
@@ -142,16 +221,15 @@ struct Place {
 // forward
 // ---------------------------------------------------------------------------
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
-__global__ void __launch_bounds__(TEAM == BLOCK ? 512 : 256) fwd_kernel(Args a, int rows_per_block) {
-  __shared__ float red[2 * 32];
+__global__ void __launch_bounds__(TEAM == MANY ? 512 : 256) fwd_kernel(Args a, int per_block) {
+  __shared__ float red_all[8][2 * 16];
   int turn = 0;
-  const Place<TEAM, LANES> z(a, rows_per_block);
+  const Place<TEAM, LANES> z(a, per_block);
+  float* red = red_all[TEAM == MANY ? z.team : 0];
   const TA *x = (const TA*)a.x, *res = (const TA*)a.res;
   const float inv = 1.f / (float)a.N;
-  // every lane of a warp runs the same number of rounds (the shuffles need them all)
-  for (int64_t v0 = z.first;; v0 += z.stride) {
+  for (int64_t v0 = z.first; !z.done(v0, a.vecs); v0 += z.stride) {
     const bool on = v0 < a.vecs;
-    if (TEAM == BLOCK ? !on : !__any_sync(0xffffffffu, on)) break;
     const int64_t base = v0 * a.N;
     float f[CHN][VEC], s[1] = {0.f};
 #pragma unroll
@@ -178,7 +256,7 @@ __global__ void __launch_bounds__(TEAM == BLOCK ? 512 : 256) fwd_kernel(Args a, 
     for (int c = 0; c < CHN; ++c)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) s[0] += f[c][j];
-    team_sum<TEAM, LANES, 1>(s, red, turn);
+    team_sum<TEAM, LANES, 1>(s, red, turn, z.warps, 1 + z.team);
     const float mean = s[0] * inv;
     s[0] = 0.f;
 #pragma unroll
@@ -190,7 +268,7 @@ __global__ void __launch_bounds__(TEAM == BLOCK ? 512 : 256) fwd_kernel(Args a, 
         if (n < a.N) s[0] = fmaf(f[c][j], f[c][j], s[0]);
       }
     }
-    team_sum<TEAM, LANES, 1>(s, red, turn);
+    team_sum<TEAM, LANES, 1>(s, red, turn, z.warps, 1 + z.team);
     const float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps));
     if (on && z.lane == 0 && a.stats) *(float2*)(a.stats + 2 * v0) = make_float2(mean, rstd);
     const int g = a.G == 1 ? 0 : (int)(v0 % a.G);
@@ -214,129 +292,164 @@ __global__ void __launch_bounds__(TEAM == BLOCK ? 512 : 256) fwd_kernel(Args a, 
 // ---------------------------------------------------------------------------
 // With z = (h - mean) rstd and u = dy w:  dx = rstd (u - mean(u) - z mean(u z)) + dh,
 // dw += dy z, db += dy.
+// The vectors to come are copied into a ring in shared memory, `stages` - 1 of them ahead;
+// every thread copies the groups that it will work on itself, so the ring needs no barrier
+// and holds no registers (a register prefetch spilled, which made every copy wait for its
+// load: 325 us at 65536 x 768 bf16 with dh).  Single channels (VEC = 1) are loaded directly.
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
-__global__ void __launch_bounds__(TEAM == BLOCK ? 512 : 256) bwd_kernel(Args a, int rows_per_block) {
-  extern __shared__ float acc_sm[];  // WARP, SUB: 2 x width
-  __shared__ float red[2 * 32 * 2];
+__global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : TEAM == SUB ? 4 : VEC * CHN <= 8 ? 3 : 2)
+    bwd_kernel(Args a, int per_block, int stages) {
+  extern __shared__ __align__(16) uint8_t dyn[];  // the ring, then 2 x width sums where teams share channels
+  __shared__ float red_all[8][2 * 16 * 2];
+  constexpr bool RING = VEC > 1;
+  constexpr int NP = PAIRS<VEC>;
+  typedef Pack<TA, VEC> Raw;
   int turn = 0;
-  const Place<TEAM, LANES> z(a, rows_per_block);
-  const TA *h = (const TA*)a.h, *dy = (const TA*)a.dy, *dh = (const TA*)a.dh;
+  const Place<TEAM, LANES> z(a, per_block);
+  float* red = red_all[TEAM == MANY ? z.team : 0];
   const float inv = 1.f / (float)a.N;
   const int g = a.G == 1 ? 0 : (int)(z.first % a.G);  // the stride is a multiple of G
-  float w[CHN][VEC], dw[CHN][VEC], db[CHN][VEC];
+  const int n0 = z.lane * VEC, dn = z.lanes * VEC;    // this thread's groups start at n0 + c * dn
+  const float* wg = a.w ? a.w + (int64_t)g * a.N + n0 : nullptr;
+  const TA *h = (const TA*)a.h + n0, *dy = (const TA*)a.dy + n0, *dh = a.dh ? (const TA*)a.dh + n0 : nullptr;
+  F2 dw[CHN][NP], db[CHN][NP];
 #pragma unroll
-  for (int c = 0; c < CHN; ++c) {
-    const int n = (c * z.lanes + z.lane) * VEC;
+  for (int c = 0; c < CHN; ++c)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) w[c][j] = dw[c][j] = db[c][j] = 0.f;
-    if (n < a.N) load_param<VEC>(w[c], a.w ? a.w + (int64_t)g * a.N + n : nullptr, 1.f);
-  }
-  for (int64_t v0 = z.first;; v0 += z.stride) {
+    for (int j = 0; j < NP; ++j) dw[c][j] = db[c][j] = f2(0.f, 0.f);
+  Raw* ring = (Raw*)dyn + threadIdx.x;  // slot (stage, stream, c): 3 streams
+  const int pitch = blockDim.x;
+  auto fetch = [&](int64_t v, int st) {
+    if constexpr (RING) {
+      if (v < a.vecs) {
+        const int64_t o = v * a.N;
+        Raw* r = ring + st * 3 * CHN * pitch;
+#pragma unroll
+        for (int c = 0; c < CHN; ++c)
+          if (n0 + c * dn < a.N) {
+            copy16(r + c * pitch, h + o + c * dn);
+            copy16(r + (CHN + c) * pitch, dy + o + c * dn);
+            if (dh) copy16(r + (2 * CHN + c) * pitch, dh + o + c * dn);
+          }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  int at = 0;  // stage of the current vector
+  for (int i = 0; i < 3; ++i) fetch(i < stages - 1 ? z.first + i * z.stride : a.vecs, i);  // 3 groups always
+  float2 nst = z.first < a.vecs ? *(const float2*)(a.cstats + 2 * z.first) : make_float2(0.f, 0.f);
+  for (int64_t v0 = z.first; !z.done(v0, a.vecs); v0 += z.stride) {
     const bool on = v0 < a.vecs;
-    if (TEAM == BLOCK ? !on : !__any_sync(0xffffffffu, on)) break;
-    const int64_t base = v0 * a.N;
-    float f[CHN][VEC], d[CHN][VEC];
-#pragma unroll
-    for (int c = 0; c < CHN; ++c) {
-      const int n = (c * z.lanes + z.lane) * VEC;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[c][j] = d[c][j] = 0.f;
-      if (on && n < a.N) {
-        load<TA, VEC>(f[c], h + base + n);
-        load<TA, VEC>(d[c], dy + base + n);
-      }
+    const float2 st = nst;
+    if (v0 + z.stride < a.vecs) nst = *(const float2*)(a.cstats + 2 * (v0 + z.stride));
+    if constexpr (RING) {
+      // the group of this vector is the (stages - 1)-th newest
+      if (stages == 4)
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    float2 st = on ? *(const float2*)(a.cstats + 2 * v0) : make_float2(0.f, 0.f);
-    float s[2] = {0.f, 0.f};
+    F2 f[CHN][NP], d[CHN][NP], s0 = f2(0.f, 0.f), s1 = f2(0.f, 0.f);
+    const F2 nmean = f2(-st.x, -st.x), rstd = f2(st.y, st.y);
+    const Raw* slot = ring + at * 3 * CHN * pitch;
+    const int64_t o = v0 * a.N;
 #pragma unroll
     for (int c = 0; c < CHN; ++c) {
-      const int n = (c * z.lanes + z.lane) * VEC;
-      if (n < a.N) {
+      if (on && n0 + c * dn < a.N) {
+        if constexpr (RING) {
+          unpack2<TA, VEC>(f[c], slot[c * pitch]);
+          unpack2<TA, VEC>(d[c], slot[(CHN + c) * pitch]);
+        } else {
+          unpack2<TA, VEC>(f[c], *(const Raw*)(h + o + c * dn));
+          unpack2<TA, VEC>(d[c], *(const Raw*)(dy + o + c * dn));
+        }
+        float w[2 * NP];
+        w[2 * NP - 1] = 0.f;
+        load_param<VEC>(w, wg ? wg + c * dn : nullptr, 1.f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float zz = (f[c][j] - st.x) * st.y;
-          dw[c][j] = fmaf(d[c][j], zz, dw[c][j]);
-          db[c][j] += d[c][j];
-          const float u = d[c][j] * w[c][j];
-          s[0] += u;
-          s[1] = fmaf(u, zz, s[1]);
-          f[c][j] = zz;
-          d[c][j] = u;
+        for (int j = 0; j < NP; ++j) {
+          f[c][j] = (f[c][j] + nmean) * rstd;
+          dw[c][j] = fma2(d[c][j], f[c][j], dw[c][j]);
+          db[c][j] = db[c][j] + d[c][j];
+          d[c][j] = d[c][j] * f2(w[2 * j], w[2 * j + 1]);
+          s0 = s0 + d[c][j];
+          s1 = fma2(d[c][j], f[c][j], s1);
         }
       }
     }
-    team_sum<TEAM, LANES, 2>(s, red, turn);
-    const float m1 = s[0] * inv, m2 = s[1] * inv;
+    if constexpr (RING) {  // into the slot of the vector before
+      const int to = at == 0 ? stages - 1 : at - 1;
+      fetch(v0 + (stages - 1) * z.stride, to);
+      at = at + 1 == stages ? 0 : at + 1;
+    }
+    const float2 t0 = f2_get(s0), t1 = f2_get(s1);
+    float s[2] = {t0.x + t0.y, t1.x + t1.y};
+    team_sum<TEAM, LANES, 2>(s, red, turn, z.warps, 1 + z.team);
+    const float m1 = -st.y * (s[0] * inv), m2 = -st.y * (s[1] * inv);
+    const F2 c1 = f2(m1, m1), c2 = f2(m2, m2);
 #pragma unroll
     for (int c = 0; c < CHN; ++c) {
-      const int n = (c * z.lanes + z.lane) * VEC;
-      if (on && n < a.N) {
+      if (on && n0 + c * dn < a.N) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) d[c][j] = st.y * (d[c][j] - m1 - f[c][j] * m2);
+        for (int j = 0; j < NP; ++j) d[c][j] = fma2(rstd, d[c][j], fma2(f[c][j], c2, c1));
         if (dh) {
-          load<TA, VEC>(f[c], dh + base + n);
+          if constexpr (RING)
+            unpack2<TA, VEC>(f[c], slot[(2 * CHN + c) * pitch]);
+          else
+            unpack2<TA, VEC>(f[c], *(const Raw*)(dh + o + c * dn));
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) d[c][j] += f[c][j];
+          for (int j = 0; j < NP; ++j) d[c][j] = d[c][j] + f[c][j];
         }
-        store<TA, VEC>((TA*)a.dx + base + n, d[c]);
+        store2<TA, VEC>((TA*)a.dx + o + n0 + c * dn, d[c]);
       }
     }
   }
   if (!a.part) return;
   float* pw = a.part + (int64_t)blockIdx.x * 2 * a.width;
   float* pb = pw + a.width;
-  if constexpr (TEAM == BLOCK) {
+  // teams of one block with the same channels add up in turn
+  float* aw = (float*)(dyn + (RING ? stages * 3 * CHN * pitch * (int)sizeof(Raw) : 0));
+  if (TEAM != SUB && per_block == 1) aw = pw;  // one team: straight to its partial row
+  float* ab = aw + a.width;
+  const int off = (TEAM == SUB ? g * a.N : 0) + n0;
+  for (int i = 0; i < per_block; ++i) {
+    if (i == z.team) {
 #pragma unroll
-    for (int c = 0; c < CHN; ++c) {
-      const int n = (c * z.lanes + z.lane) * VEC;
-      if (n < a.N) {
+      for (int c = 0; c < CHN; ++c) {
+        if (n0 + c * dn < a.N) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          pw[n + j] = dw[c][j];
-          pb[n + j] = db[c][j];
-        }
-      }
-    }
-  } else {
-    // teams of one block with the same channels add up in turn
-    float *aw = acc_sm, *ab = acc_sm + a.width;
-    const int turns = TEAM == SUB ? rows_per_block : blockDim.x >> 5;
-    const int mine = TEAM == SUB ? threadIdx.x / (a.G * LANES) : threadIdx.x >> 5;
-    const int off = TEAM == SUB ? g * a.N : 0;
-    for (int i = 0; i < turns; ++i) {
-      if (i == mine) {
-#pragma unroll
-        for (int c = 0; c < CHN; ++c) {
-          const int n = (c * z.lanes + z.lane) * VEC;
-          if (n < a.N) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              const int o = off + n + j;
-              aw[o] = i == 0 ? dw[c][j] : aw[o] + dw[c][j];
-              ab[o] = i == 0 ? db[c][j] : ab[o] + db[c][j];
-            }
+          for (int j = 0; j < VEC; ++j) {
+            const int k = off + c * dn + j;
+            const float2 x = f2_get(dw[c][j / 2]), y = f2_get(db[c][j / 2]);
+            const float xw = j & 1 ? x.y : x.x, xb = j & 1 ? y.y : y.x;
+            aw[k] = i == 0 ? xw : aw[k] + xw;
+            ab[k] = i == 0 ? xb : ab[k] + xb;
           }
         }
       }
-      __syncthreads();
     }
-    for (int o = threadIdx.x; o < a.width; o += blockDim.x) {
-      pw[o] = aw[o];
-      pb[o] = ab[o];
-    }
+    __syncthreads();
+  }
+  if (aw == pw) return;
+  for (int k = threadIdx.x; k < a.width; k += blockDim.x) {
+    pw[k] = aw[k];
+    pb[k] = ab[k];
   }
 }
 
 // dw, db (G, N) from the partial rows: channel (g, n) is column (g * N + n) % width of the
 // rows p with p % groups == group, groups = G * N / width.
-__global__ void __launch_bounds__(1024) param_kernel(Args a, int parts, float* dw, float* db) {
-  __shared__ float red[2][32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = blockIdx.x * 32 + tx, total = a.G * a.N;
+// A block adds up 8 channels (a 32-byte sector of each row), 64 rows side by side.
+constexpr int PCOL = 8, PROW = 64;
+__global__ void __launch_bounds__(PCOL * PROW) param_kernel(Args a, int parts, float* dw, float* db) {
+  __shared__ float red[2][PROW][PCOL];
+  const int tx = threadIdx.x % PCOL, ty = threadIdx.x / PCOL, col = blockIdx.x * PCOL + tx, total = a.G * a.N;
   const int groups = total / a.width;
   float sw = 0.f, sb = 0.f;
   if (col < total) {
     const int grp = col / a.width, n = col % a.width;
-    for (int p = grp + ty * groups; p < parts; p += 32 * groups) {
+#pragma unroll 4
+    for (int p = grp + ty * groups; p < parts; p += PROW * groups) {
       const float* r = a.part + (int64_t)p * 2 * a.width + n;
       sw += r[0];
       sb += r[a.width];
@@ -345,9 +458,17 @@ __global__ void __launch_bounds__(1024) param_kernel(Args a, int parts, float* d
   red[0][ty][tx] = sw;
   red[1][ty][tx] = sb;
   __syncthreads();
+  if (ty < 16) {
+    const int which = ty >> 3, part = ty & 7;  // 8 threads a sum, neighbours 8 lanes apart in one warp
+    float s = 0.f;
+    for (int i = part; i < PROW; i += 8) s += red[which][i][tx];
+    __syncwarp();
+    red[which][part][tx] = s;
+  }
+  __syncthreads();
   if (ty < 2) {
     float s = 0.f;
-    for (int i = 0; i < 32; ++i) s += red[ty][i][tx];
+    for (int i = 0; i < 8; ++i) s += red[ty][i][tx];
     float* out = ty ? db : dw;
     if (col < total && out) out[col] = s;
   }
@@ -375,14 +496,14 @@ __global__ void __launch_bounds__(512) big_fwd_kernel(Args a) {
       s[0] += f;
     }
     const TA* h = res ? hh : x;
-    team_sum<BLOCK, 32, 1>(s, red, turn);
+    team_sum<MANY, 32, 1>(s, red, turn, 16, 1);
     const float mean = s[0] * inv;
     s[0] = 0.f;
     for (int n = threadIdx.x; n < a.N; n += 512) {
       const float f = ld_act(h, (size_t)n) - mean;
       s[0] = fmaf(f, f, s[0]);
     }
-    team_sum<BLOCK, 32, 1>(s, red, turn);
+    team_sum<MANY, 32, 1>(s, red, turn, 16, 1);
     const float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps));
     if (threadIdx.x == 0 && a.stats) *(float2*)(a.stats + 2 * v) = make_float2(mean, rstd);
     for (int n = threadIdx.x; n < a.N; n += 512) {
@@ -410,7 +531,7 @@ __global__ void __launch_bounds__(512) big_bwd_kernel(Args a) {
       s[0] += u;
       s[1] = fmaf(u, (ld_act(h, (size_t)n) - st.x) * st.y, s[1]);
     }
-    team_sum<BLOCK, 32, 2>(s, red, turn);
+    team_sum<MANY, 32, 2>(s, red, turn, 16, 1);
     for (int n = threadIdx.x; n < a.N; n += 512) {
       const float u = ld_act(dy, (size_t)n) * (w ? w[n] : 1.f), zz = (ld_act(h, (size_t)n) - st.x) * st.y;
       const float d = st.y * (u - s[0] * inv - zz * (s[1] * inv));
@@ -523,7 +644,8 @@ __global__ void __launch_bounds__(256) tiny_param_kernel(Args a) {
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-constexpr int PARTS = 592;  // most blocks of the backward (and partial rows): 4 per SM
+constexpr int SMS = 148;
+constexpr int MAX_SMEM = 208 << 10;  // dynamic, of a backward block: 2 stages of 512 threads x 4 groups x 3 streams + sums
 constexpr int BIG_PARTS = 64;
 constexpr int MAX_GN = 1 << 20;
 
@@ -549,23 +671,25 @@ static int status_of(cudaError_t e) {
   return e == cudaSuccess ? ATLAS_OK : report_error(ATLAS_ERR_CUDA, cudaGetErrorString(e));
 }
 
-// How a problem runs.  VEC: channels per load; SUB for vectors of 2 to 32 aligned groups,
-// a power of two, where the row of G vectors fits a block; TINY for up to 8 channels; else WARP up to 4 groups (16
-// bytes) or 8 single channels a lane; else BLOCK up to 2 bf16 groups, 4 float32 groups or 8
-// single channels a thread (what the backward holds without spilling); else BIG.
+// How a problem runs.  VEC: channels per load.  SUB for vectors of 4 to 32 aligned groups, a
+// power of two, where the row of G vectors fits a block; TINY for up to 8 channels; WARPS
+// while a thread holds at most 3 groups of 8 bf16, 4 groups of 4 float32 or 8 single
+// channels (what the backward keeps in 128 registers); else BIG.  As few warps as hold the
+// vector: the shuffles and address arithmetic of a vector are paid once for each warp.
 struct Plan {
   bool big, tiny;
   Team team;
-  int vec, lanes, chn, threads, rows_per_block, width, parts;
+  int vec, lanes, chn, threads, per_block, width, parts;
   int64_t grid;
 };
 static Plan plan(const Args& a, int act_dtype, bool vec_ok, bool bwd) {
   Plan z{};
   const int full = act_dtype == ATLAS_BF16 ? 8 : 4;
   z.vec = vec_ok && a.N % full == 0 ? full : 1;
-  const int groups = (a.N + z.vec - 1) / z.vec;
+  const int groups = (a.N + z.vec - 1) / z.vec, most = z.vec == 8 ? 3 : z.vec == 4 ? 4 : 8;  // groups a thread
   const bool pow2 = (groups & (groups - 1)) == 0;
-  z.rows_per_block = 1;
+  z.per_block = 1;
+  z.threads = 256;
   int64_t units;  // blocks' worth of work
   if (a.N <= TINY) {
     z.tiny = true;
@@ -575,38 +699,34 @@ static Plan plan(const Args& a, int act_dtype, bool vec_ok, bool bwd) {
     z.team = SUB;
     z.lanes = groups;
     z.chn = 1;
-    z.rows_per_block = 256 / (a.G * groups);
-    z.threads = (z.rows_per_block * a.G * groups + 31) / 32 * 32;
+    z.per_block = 256 / (a.G * groups);
+    z.threads = (z.per_block * a.G * groups + 31) / 32 * 32;
     z.width = a.G * a.N;
-    units = (a.rows + z.rows_per_block - 1) / z.rows_per_block;
-  } else if (groups <= (z.vec > 1 ? 128 : 256) && (a.G == 1 || !bwd)) {
-    z.team = WARP;
-    z.lanes = 32;
-    z.chn = (groups + 31) / 32;
-    z.threads = 256;
+    units = (a.rows + z.per_block - 1) / z.per_block;
+  } else if (groups <= 512 * most) {
+    const int per_lane = z.vec == 8 ? 3 : 4;
+    const int warps = std::min(16, (groups + 32 * per_lane - 1) / (32 * per_lane));
+    z.team = warps == 1 ? ONE : MANY;
+    z.chn = (groups + 32 * warps - 1) / (32 * warps);
+    if (z.vec == 1) z.chn = z.chn <= 4 ? 4 : 8;
+    // a block's teams share channels; with weights for each group that needs one team
+    z.per_block = bwd && a.G > 1 ? 1 : std::max(1, 8 / warps);
+    z.threads = 32 * warps * z.per_block;
     z.width = a.N;
-    units = (a.vecs + 7) / 8;
-  } else if (groups <= 512 * (z.vec == 8 ? 2 : z.vec == 4 ? 4 : 8)) {
-    z.team = BLOCK;
-    z.lanes = 0;
-    z.chn = (groups + 511) / 512;
-    z.width = a.N;
-    units = a.vecs;
+    units = (a.vecs + z.per_block - 1) / z.per_block;
   } else {
     z.big = true;
+    z.threads = 512;
     z.width = a.G * a.N;
     units = a.vecs;
   }
-  if (!z.big && !z.tiny) {
-    if (z.vec == 1) z.chn = z.chn <= 4 ? 4 : 8;
-    if (z.team == BLOCK) z.threads = ((groups + z.chn - 1) / z.chn + 31) / 32 * 32;
-  }
-  const int64_t most = bwd ? PARTS : 148 * 16;
-  z.grid = std::max<int64_t>(1, std::min(units, most));
-  if (bwd && !z.big && !z.tiny && z.team == BLOCK) {  // a multiple of G: each block keeps one group's weights
+  // the backward's blocks are what an SM holds at its register use, the forward's many more
+  const int64_t blocks = SMS * (bwd ? (z.threads * z.chn * z.vec <= 2048 ? 4 : 2) : 16);
+  z.grid = std::max<int64_t>(1, std::min(units, blocks));
+  if (bwd && !z.big && !z.tiny && z.team != SUB && a.G > 1)  // a multiple of G: a block keeps one group's weights
     z.grid = std::min<int64_t>(units, std::max<int64_t>(a.G, z.grid / a.G * a.G));
-  }
-  z.parts = (int)(z.big || z.tiny ? std::min<int64_t>(z.big ? BIG_PARTS : PARTS, std::max<int64_t>(1, a.rows)) : z.grid);
+  z.parts = (int)(z.big ? std::min<int64_t>(BIG_PARTS, std::max<int64_t>(1, a.rows))
+                  : z.tiny ? std::min<int64_t>(4 * SMS, std::max<int64_t>(1, a.rows)) : z.grid);
   return z;
 }
 
@@ -622,13 +742,30 @@ static size_t ws_bytes(const AtlasNormParams& p) {
   return n;
 }
 
+// A kernel's dynamic shared memory above 48 KB, asked of the driver once per device.
+template <auto Kernel>
+static cudaError_t allow_smem() {
+  static DeviceCache done;
+  cudaError_t e = cudaSuccess;
+  done.get([&] {
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
+    return e == cudaSuccess ? 0 : -1;
+  });
+  return e;
+}
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
 static cudaError_t go(const Args& a, const Plan& z, bool bwd, cudaStream_t s) {
+  
   if (bwd) {
-    const size_t sm = TEAM == BLOCK ? 0 : (size_t)2 * z.width * sizeof(float);
-    bwd_kernel<TA, TEAM, LANES, VEC, CHN><<<(unsigned)z.grid, z.threads, sm, s>>>(a, z.rows_per_block);
+      // 4 stages while the blocks that an SM's registers hold have room for them, else 2
+      const size_t stage = VEC > 1 ? (size_t)3 * CHN * z.threads * 16 : 0;
+      const int stages = 4 * stage <= 50 << 10 ? 4 : 2;
+      const size_t sm = stages * stage + (TEAM == SUB || z.per_block > 1 ? (size_t)2 * z.width * sizeof(float) : 0);
+      cudaError_t e = allow_smem<bwd_kernel<TA, TEAM, LANES, VEC, CHN>>();
+      if (e != cudaSuccess) return e;
+      bwd_kernel<TA, TEAM, LANES, VEC, CHN><<<(unsigned)z.grid, z.threads, sm, s>>>(a, z.per_block, stages);
   } else {
-    fwd_kernel<TA, TEAM, LANES, VEC, CHN><<<(unsigned)z.grid, z.threads, 0, s>>>(a, z.rows_per_block);
+    fwd_kernel<TA, TEAM, LANES, VEC, CHN><<<(unsigned)z.grid, z.threads, 0, s>>>(a, z.per_block);
   }
   return cudaGetLastError();
 }
@@ -636,12 +773,11 @@ template <typename TA, Team TEAM, int VEC>
 static cudaError_t by_chn(const Args& a, const Plan& z, bool bwd, cudaStream_t s) {
   if constexpr (VEC > 1) {
     if (z.chn == 1) return go<TA, TEAM, 32, VEC, 1>(a, z, bwd, s);
-    if constexpr (TEAM == BLOCK && VEC == 8) {
-      return go<TA, TEAM, 32, VEC, 2>(a, z, bwd, s);
+    if (z.chn == 2) return go<TA, TEAM, 32, VEC, 2>(a, z, bwd, s);
+    if constexpr (VEC == 8) {
+      return go<TA, TEAM, 32, VEC, 3>(a, z, bwd, s);
     } else {
-      if (z.chn == 2) return go<TA, TEAM, 32, VEC, 2>(a, z, bwd, s);
-      if (z.chn == 3) return go<TA, TEAM, 32, VEC, 3>(a, z, bwd, s);
-      return go<TA, TEAM, 32, VEC, 4>(a, z, bwd, s);
+      return z.chn == 3 ? go<TA, TEAM, 32, VEC, 3>(a, z, bwd, s) : go<TA, TEAM, 32, VEC, 4>(a, z, bwd, s);
     }
   } else {
     return z.chn == 4 ? go<TA, TEAM, 32, 1, 4>(a, z, bwd, s) : go<TA, TEAM, 32, 1, 8>(a, z, bwd, s);
@@ -683,9 +819,9 @@ static cudaError_t run(const Args& a, const Plan& z, bool bwd, cudaStream_t s) {
       default: return go<TA, SUB, 32, FULL, 1>(a, z, bwd, s);
     }
   }
-  if (z.team == WARP)
-    return z.vec > 1 ? by_chn<TA, WARP, FULL>(a, z, bwd, s) : by_chn<TA, WARP, 1>(a, z, bwd, s);
-  return z.vec > 1 ? by_chn<TA, BLOCK, FULL>(a, z, bwd, s) : by_chn<TA, BLOCK, 1>(a, z, bwd, s);
+  if (z.team == ONE)
+    return z.vec > 1 ? by_chn<TA, ONE, FULL>(a, z, bwd, s) : by_chn<TA, ONE, 1>(a, z, bwd, s);
+  return z.vec > 1 ? by_chn<TA, MANY, FULL>(a, z, bwd, s) : by_chn<TA, MANY, 1>(a, z, bwd, s);
 }
 static cudaError_t launch(const Args& a, const AtlasNormParams& p, const Plan& z, bool bwd, cudaStream_t s) {
   return p.act_dtype == ATLAS_BF16 ? run<bf16, 8>(a, z, bwd, s) : run<float, 4>(a, z, bwd, s);
@@ -752,7 +888,7 @@ extern "C" int atlas_layernorm_bwd(const AtlasNormParams* p, const void* dy, con
   a.width = z.width;
   cudaError_t e = launch(a, *p, z, true, s);
   if (e == cudaSuccess && params) {
-    param_kernel<<<(unsigned)((p->G * p->N + 31) / 32), 1024, 0, s>>>(a, z.parts, dweight, dbias);
+    param_kernel<<<(unsigned)((p->G * p->N + PCOL - 1) / PCOL), PCOL * PROW, 0, s>>>(a, z.parts, dweight, dbias);
     e = cudaGetLastError();
   }
   return status_of(e);
