@@ -19,7 +19,7 @@ from .scan import _WS, addr, empty_like, on_device, stream_of
 
 class AtlasDecayParams(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_int32) for n in ("abi_version", "B", "T", "H", "D", "act_dtype")] +
-                [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)] +
+                [("scale", ctypes.c_float), ("aligned16", ctypes.c_int32)] +
                 [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")])
 
 
@@ -32,7 +32,7 @@ def _lib():
     lib = L.load()
     if not _bound:
         pp = ctypes.POINTER(AtlasDecayParams)
-        for n in ("atlas_decay_saved_bytes", "atlas_decay_workspace_bytes"):
+        for n in ("atlas_decay_saved_bytes", "atlas_decay_fwd_workspace_bytes", "atlas_decay_bwd_workspace_bytes"):
             getattr(lib, n).restype = ctypes.c_size_t
             getattr(lib, n).argtypes = [pp]
         lib.atlas_decay_fwd.restype = ctypes.c_int
@@ -48,7 +48,7 @@ def _lib():
 class _Plan:
     """What a call needs that depends on shapes, strides and types alone."""
 
-    def __init__(self, q, k, v, g, scale):
+    def __init__(self, q, k, v, g, scale, aligned):
         (shape, st, dtype, dev) = q
         if len(shape) != 4:
             raise ValueError(f"q: expected (B, T, H, D), got {tuple(shape)}")
@@ -60,16 +60,20 @@ class _Plan:
         B, T, H, D = shape
         if g[0] != (H,) or g[2] != torch.float32 or g[3] != dev or (g[1] != (1,) and H > 1):
             raise ValueError(f"log_decay: expected contiguous CUDA float32 {(H,)}, got {g[2]} {tuple(g[0])}")
-        self.packed = D == 1 or all(x[1][3] == 1 for x in (q, k, v))  # channels contiguous
+        # contiguous channels; bf16 on the tensor cores also has no broadcast (stride 0) axes
+        fast = dtype == torch.bfloat16 and D % 8 == 0
+        self.packed = all((x[1][3] == 1 or D == 1) and not (fast and any(s == 0 and n > 1 for s, n in zip(x[1], shape)))
+                          for x in (q, k, v))
         strides = [(ctypes.c_int64 * 3)(*x[1][:3]) for x in (q, k, v)]
         self.params = AtlasDecayParams(L.ATLAS_ABI_VERSION, B, T, H, D,
                                        L.ATLAS_BF16 if dtype == torch.bfloat16 else L.ATLAS_F32,
-                                       D ** -0.5 if scale is None else scale, 0, *strides)
+                                       D ** -0.5 if scale is None else scale, int(aligned), *strides)
         self.ref = ctypes.byref(self.params)
         self.shape, self.dtype = tuple(shape), dtype
         self.B, self.state_shape = B, (B, H, D, D)
         self.saved_bytes = self._size(_lib().atlas_decay_saved_bytes)
-        self.workspace_bytes = self._size(_lib().atlas_decay_workspace_bytes)
+        self.fwd_workspace_bytes = self._size(_lib().atlas_decay_fwd_workspace_bytes)
+        self.bwd_workspace_bytes = self._size(_lib().atlas_decay_bwd_workspace_bytes)
 
     def _size(self, query):
         """A size query's answer; 0 is an error only when it left a message."""
@@ -84,10 +88,16 @@ _plans = functools.lru_cache(maxsize=512)(_Plan)
 
 def _plan(q, k, v, log_decay, scale):
     """Checks the inputs; returns their plan and q, k, v with contiguous channels."""
-    p = _plans(*[(x.shape, x.stride(), x.dtype, x.get_device()) for x in (q, k, v, log_decay)], scale)
+    aligned = (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 == 0
+    p = _plans(*[(x.shape, x.stride(), x.dtype, x.get_device()) for x in (q, k, v, log_decay)], scale, aligned)
     if not p.packed:
         return _plan(q.contiguous(), k.contiguous(), v.contiguous(), log_decay, scale)
     return p, q, k, v
+
+
+def _aligned(x):
+    """x, or a copy of it where it starts off the 16-byte grid."""
+    return x if x is None or x.data_ptr() & 15 == 0 else x.clone()
 
 
 def _need(x, shape, name, q):
@@ -104,11 +114,12 @@ def decay_attention_forward(q, k, v, log_decay, state=None, scale=None, need_sav
     dev = q.device
     if state is not None:
         _need(state, p.state_shape, "state", q)
+        state = _aligned(state)
     with on_device(dev):
         y = empty_like(q)
         out = torch.empty(p.state_shape, device=dev) if state is None else empty_like(state)
         saved = torch.empty(p.saved_bytes, dtype=torch.uint8, device=dev) if need_saved else None
-        ws, wsb = (None, 0) if need_saved else (workspace or _WS).get(p.saved_bytes, dev)
+        ws, wsb = (None, 0) if need_saved else (workspace or _WS).get(p.fwd_workspace_bytes, dev)
         L.check(_lib().atlas_decay_fwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), addr(state),
                                        y.data_ptr(), out.data_ptr(), addr(saved), addr(ws), wsb, stream_of(dev)))
     return y, out, saved
@@ -120,15 +131,16 @@ def decay_attention_backward(q, k, v, log_decay, saved, dy, dstate=None, scale=N
     dev = q.device
     if dy.dtype != p.dtype or dy.shape != p.shape or dy.get_device() != q.get_device():
         raise ValueError(f"dy: expected {p.dtype} {p.shape} on {dev}, got {dy.dtype} {tuple(dy.shape)} on {dy.device}")
-    dy = dy.contiguous()
+    dy = _aligned(dy.contiguous())
     if dstate is not None:
         _need(dstate, p.state_shape, "dstate", q)
+        dstate = _aligned(dstate)
     if saved.numel() * saved.element_size() != p.saved_bytes or saved.get_device() != q.get_device():
         raise ValueError("saved: not what decay_attention_forward saved for these inputs")
     with on_device(dev):
         dq, dk, dv = empty_like(q), empty_like(q), empty_like(q)
         dg, dstate_in = torch.empty(p.shape[2], device=dev), torch.empty(p.state_shape, device=dev)
-        ws, wsb = (workspace or _WS).get(p.workspace_bytes, dev)
+        ws, wsb = (workspace or _WS).get(p.bwd_workspace_bytes, dev)
         L.check(_lib().atlas_decay_bwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
                                        saved.data_ptr(), dy.data_ptr(), addr(dstate), dq.data_ptr(), dk.data_ptr(),
                                        dv.data_ptr(), dg.data_ptr(), dstate_in.data_ptr(), addr(ws), wsb, stream_of(dev)))

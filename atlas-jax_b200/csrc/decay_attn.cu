@@ -1,5 +1,5 @@
-// Decay attention (include/atlas_decay.h): entry points, the state recurrence over chunks,
-// the float32 CUDA-core kernels for the calls outside the tensor path, and the recurrent
+// Decay attention (include/atlas_decay.h): entry points, the float32 CUDA-core kernels for
+// the calls outside the tensor path (decay_scan.cu, decay_tc.cu), and the recurrent
 // single-token form.
 //
 // A sequence is cut into chunks of CH = 128 tokens.  With L tokens in a chunk, local
@@ -137,7 +137,7 @@ __device__ void load_rows(float (*tile)[LD], const View& x, int b, int h, int t0
   }
 }
 
-// per-chunk sums of weight * X^T Y (see launch_chunk_states)
+// per-chunk sums of weight * X^T Y (forward: k, v, l^(L-1-s); bwd: q, scale dy, l^(t+1))
 template <typename TA, int NI>
 __global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd) {
   __shared__ float X[TT][LD], Y[TT][LD];
@@ -576,14 +576,20 @@ static int status_of(cudaError_t e) {
 static bool empty(const AtlasDecayParams& p) { return chains(p) == 0; }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-static bool strides8(const int64_t* s) { return s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0; }
-// The tensor path moves 16-byte groups of 8 channels.
-static bool tensor_path(const Args& a) {
-  const AtlasDecayParams& p = a.p;
-  return p.act_dtype == ATLAS_BF16 && p.D % 8 == 0 && strides8(p.q_stride) && strides8(p.k_stride) &&
-         strides8(p.v_stride) && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.dy) &&
-         aligned16(a.y) && aligned16(a.dq) && aligned16(a.dk) && aligned16(a.dv) && aligned16(a.states) &&
-         aligned16(a.dstates);
+// The tensor path moves 16-byte groups of 8 channels by TMA.  Params alone decide.
+static bool tensor_path(const AtlasDecayParams& p) {
+  return p.act_dtype == ATLAS_BF16 && p.D % 8 == 0 && p.aligned16 && tcore::mappable(p, p.q_stride) &&
+         tcore::mappable(p, p.k_stride) && tcore::mappable(p, p.v_stride);
+}
+// what the forward needs where it keeps no states
+static size_t fwd_bytes(const AtlasDecayParams& p) { return tensor_path(p) ? tcore::mid_bytes(p) : state_bytes(p); }
+// the pointers that a call promises to be 16-byte aligned
+template <class... T>
+static int check_aligned(const AtlasDecayParams& p, T... ptr) {
+  if (!p.aligned16) return ATLAS_OK;
+  for (const void* x : {(const void*)ptr...})
+    if (!aligned16(x)) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "aligned16 is set, but a buffer is not 16-byte aligned");
+  return ATLAS_OK;
 }
 
 static cudaError_t scan(const Args& a, const float* in, float* out, bool bwd, cudaStream_t s) {
@@ -640,11 +646,13 @@ template <typename TA>
 static cudaError_t plain_t(const Args& a, Phase f, cudaStream_t s) {
   return a.p.D <= 32 ? plain_ni<TA, 2>(a, f, s) : a.p.D <= 64 ? plain_ni<TA, 4>(a, f, s) : plain_ni<TA, 8>(a, f, s);
 }
-static cudaError_t run(const Args& a, Phase f, bool tensor, cudaStream_t s) {
-  if (tensor)
-    return f == OUT ? tc::launch_out(a, s) : f == GRADS ? tc::launch_grads(a, s)
-                                                        : tc::launch_chunk_states(a, f == SUMS_BWD, s);
+static cudaError_t plain(const Args& a, Phase f, cudaStream_t s) {
   return a.p.act_dtype == ATLAS_BF16 ? plain_t<__nv_bfloat16>(a, f, s) : plain_t<float>(a, f, s);
+}
+// the states entering every chunk (bwd: leaving), from the chunks' sums
+static cudaError_t plain_states(const Args& a, const float* in, float* out, bool bwd, cudaStream_t s) {
+  const cudaError_t e = plain(a, bwd ? SUMS_BWD : SUMS_FWD, s);
+  return e == cudaSuccess ? scan(a, in, out, bwd, s) : e;
 }
 
 // out = in (or zeros): what an empty sequence leaves
@@ -675,7 +683,12 @@ extern "C" size_t atlas_decay_saved_bytes(const AtlasDecayParams* p) {
   return state_bytes(*p);
 }
 
-extern "C" size_t atlas_decay_workspace_bytes(const AtlasDecayParams* p) {
+extern "C" size_t atlas_decay_fwd_workspace_bytes(const AtlasDecayParams* p) {
+  if (check(p) != ATLAS_OK) return 0;
+  return fwd_bytes(*p);
+}
+
+extern "C" size_t atlas_decay_bwd_workspace_bytes(const AtlasDecayParams* p) {
   if (check(p) != ATLAS_OK) return 0;
   return ws_bytes(*p);
 }
@@ -690,8 +703,11 @@ extern "C" int atlas_decay_fwd(const AtlasDecayParams* p, const void* q, const v
   if (!state_out || !log_decay) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
   if (p->T == 0) return status_of(pass_state(*p, state_in, state_out, s));
   if (!q || !k || !v || !y) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
-  if (!saved && (!workspace || workspace_bytes < state_bytes(*p)))
-    return report_error(ATLAS_ERR_WORKSPACE, "workspace smaller than atlas_decay_workspace_bytes()");
+  const size_t need = saved ? 0 : fwd_bytes(*p);
+  if (need && (!workspace || workspace_bytes < need))
+    return report_error(ATLAS_ERR_WORKSPACE, "workspace smaller than atlas_decay_fwd_workspace_bytes()");
+  rc = check_aligned(*p, q, k, v, y, state_in, state_out, saved, saved ? nullptr : workspace);
+  if (rc) return rc;
   Args a{};
   a.p = *p;
   a.q = q, a.k = k, a.v = v;
@@ -699,10 +715,9 @@ extern "C" int atlas_decay_fwd(const AtlasDecayParams* p, const void* q, const v
   a.y = y;
   a.states = (float*)(saved ? saved : workspace);
   a.status = device_status_ptr();
-  const bool tensor = tensor_path(a);
-  cudaError_t e = run(a, SUMS_FWD, tensor, s);
-  if (e == cudaSuccess) e = scan(a, state_in, state_out, false, s);
-  if (e == cudaSuccess) e = run(a, OUT, tensor, s);
+  if (tensor_path(*p)) return status_of(tcore::launch_seq(a, false, state_in, state_out, (float*)saved, (float*)workspace, s));
+  cudaError_t e = plain_states(a, state_in, state_out, false, s);
+  if (e == cudaSuccess) e = plain(a, OUT, s);
   return status_of(e);
 }
 
@@ -724,7 +739,9 @@ extern "C" int atlas_decay_bwd(const AtlasDecayParams* p, const void* q, const v
   if (!q || !k || !v || !log_decay || !saved || !dy || !dq || !dk || !dv)
     return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
   if (!workspace || workspace_bytes < ws_bytes(*p))
-    return report_error(ATLAS_ERR_WORKSPACE, "workspace smaller than atlas_decay_workspace_bytes()");
+    return report_error(ATLAS_ERR_WORKSPACE, "workspace smaller than atlas_decay_bwd_workspace_bytes()");
+  rc = check_aligned(*p, q, k, v, dy, dq, dk, dv, saved, dstate_out, dstate_in, workspace);
+  if (rc) return rc;
   Args a{};
   a.p = *p;
   a.q = q, a.k = k, a.v = v, a.dy = dy;
@@ -734,11 +751,11 @@ extern "C" int atlas_decay_bwd(const AtlasDecayParams* p, const void* q, const v
   a.dstates = (float*)workspace;
   a.dg_part = (float*)((uint8_t*)workspace + state_bytes(*p));
   a.status = device_status_ptr();
-  const bool tensor = tensor_path(a);
+  const bool tensor = tensor_path(*p);
   a.dg_parts = tensor ? chunks(*p) : 2 * ((p->T + TT - 1) / TT);
-  cudaError_t e = run(a, SUMS_BWD, tensor, s);
-  if (e == cudaSuccess) e = scan(a, dstate_out, dstate_in, true, s);
-  if (e == cudaSuccess) e = run(a, GRADS, tensor, s);
+  cudaError_t e = tensor ? tcore::launch_seq(a, true, dstate_out, dstate_in, a.dstates, nullptr, s)
+                         : plain_states(a, dstate_out, dstate_in, true, s);
+  if (e == cudaSuccess) e = tensor ? tcore::launch_grads(a, s) : plain(a, GRADS, s);
   if (e == cudaSuccess && dlog_decay) {
     dg_kernel<<<p->H, 256, 0, s>>>(a, dlog_decay);
     e = cudaGetLastError();

@@ -42,14 +42,18 @@ cudaError_t allow_smem(size_t bytes) {
   return e;
 }
 
-// tcgen05 path (decay_tc.cu): bf16, D a multiple of 8, 16-byte aligned rows.
-namespace tc {
-// Per-chunk state sums into a.states (fwd: sum l^(L-1-s) k_s v_s^T) or a.dstates
-// (bwd: scale * sum l^(t+1) q_t dy_t^T).
-cudaError_t launch_chunk_states(const Args& a, bool bwd, cudaStream_t s);
-cudaError_t launch_out(const Args& a, cudaStream_t s);
+// tcgen05 path: bf16, D a multiple of 8, 16-byte aligned rows.
+namespace tcore {
+bool mappable(const AtlasDecayParams& p, const int64_t* strides);  // whether TMA can address such a tensor
+// The walk along the sequences (decay_scan.cu): forward y and states, or (bwd) the cotangent
+// states.  saves: (chains, chunks, D, D), the state entering every chunk in the order of the
+// walk, or NULL with mid_bytes() of scratch in `mid`.
+size_t mid_bytes(const AtlasDecayParams& p);
+cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, float* saves, float* mid,
+                       cudaStream_t s);
+// dq, dk, dv and the parts of dlog_decay, chunk by chunk, from a.states and a.dstates (decay_tc.cu)
 cudaError_t launch_grads(const Args& a, cudaStream_t s);
-}  // namespace tc
+}  // namespace tcore
 
 }  // namespace decay
 }  // namespace atlas

@@ -1,0 +1,732 @@
+// Decay attention (include/atlas_decay.h), the pass along the sequence on the tcgen05
+// tensor cores: outputs and states of the forward, and the cotangent states of the backward.
+//
+// One CTA walks a segment of one (batch, head) in blocks of C = 64 tokens with the state
+// S in registers (float32).  Per block of L tokens, l = exp(log_decay):
+//
+//     A  = Q K^T               dS = K'^T V,  k'_s = l^(L-1-s) k_s       QS = Q S
+//     P  = l^(t-s) o A         S <- l^L S + dS                          O  = P V
+//     y_t = scale (O_t + l^(t+1) QS_t)
+//
+// Only QS and the update of S depend on the block before, so the CTA is a pipeline of
+// groups that hand blocks on through mbarriers:
+//
+//     8 (4) warps   k' split into three bf16 parts (float32 accuracy of the state)
+//     4 warps       scores: A from TMEM, decayed, masked, rounded to bf16
+//     4 warps       outputs: O and QS from TMEM, y through shared memory and a TMA store
+//     8 (16) warps  the state: dS from TMEM, S in registers, two bf16 parts of S for QS
+//     one warp      issues the MMAs;  one warp issues the TMA loads of q, k, v
+//
+// The same kernel without q's side gives the states alone: the sums of a segment (first
+// pass of a split sequence), and with (q, scale dy, l^(t+1)) for (k, v, l^(L-1-s)) and the blocks
+// taken from the last to the first, the cotangent states of the backward.
+//
+// A sequence is split into segments where there are fewer (batch, head) pairs than SMs: the
+// segments' sums first, then the recurrence over segments, then every segment from the
+// state that enters it.
+//
+// Layout: q, k, v, y tiles as TMA writes them (rows of 128 bytes, 128-byte swizzle, a box per
+// 64 channels); k', scores and S in the core-matrix layout of tc_ops.cuh.  All M = 64
+// accumulators sit in 16 lanes of each TMEM lane quadrant and are read with 16x256b loads,
+// which spread them over all 32 lanes of a warp: lane holds rows lane / 4 and lane / 4 + 8,
+// columns 8 j + 2 (lane % 4) and the next one.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "common.cuh"
+#include "decay_internal.h"
+#include "f32x2.cuh"
+#include "tc_ops.cuh"
+
+namespace atlas {
+namespace decay {
+namespace tcore {
+
+using namespace tcx;
+typedef __nv_bfloat16 bf16;
+
+constexpr int C = 64;  // tokens of a block
+constexpr int BOX = C * 128;  // bytes of a TMA box: 64 tokens x 64 channels
+
+template <int DP>
+struct Cfg {
+  static constexpr int NB = DP / 64;                    // boxes of a tile
+  static constexpr int TILE = NB * BOX;                 // 64 tokens x DP channels
+  static constexpr int STAGES = DP == 64 ? 3 : 2;       // of q, k, v
+  static constexpr int DBL = DP == 64 ? 2 : 1;          // buffers of k', scores, S and the accumulators
+  static constexpr int KWARPS = DP == 64 ? 8 : 4;       // warps of the k' group
+  static constexpr int SWARPS = DP == 64 ? 8 : 16;      // warps of the state group
+  static constexpr int NT = 32 * (KWARPS + 10 + SWARPS);
+  static constexpr int W_P = KWARPS, W_Y = W_P + 4, W_S = W_Y + 4, W_MMA = W_S + SWARPS;  // first warps of the groups
+  static constexpr int PT = C * C * 2;                  // a tile of scores
+  static constexpr int ST = DP * DP * 2;                // one part of a state
+  static constexpr int OFF_KP = STAGES * 3 * TILE;
+  static constexpr int OFF_P = OFF_KP + DBL * 3 * TILE;
+  static constexpr int OFF_S = OFF_P + DBL * PT;
+  static constexpr int OFF_Y = OFF_S + DBL * 2 * ST;
+  static constexpr int OFF_CTL = OFF_Y + (DP == 64 ? 2 : 1) * BOX;
+  // TMEM columns
+  static constexpr uint32_t T_A = 0, T_DS = DBL * 64, T_QS = T_DS + DBL * DP, T_O = T_QS + DBL * DP;
+  static_assert(T_O + DBL * DP <= 512, "TMEM");
+};
+
+struct Ctl {
+  uint64_t full[3], empty[3];        // stages
+  uint64_t a_full[2], a_free[2];     // A in TMEM
+  uint64_t kp_full[2], kp_free[2];   // k' parts
+  uint64_t ds_full[2], ds_free[2];   // dS in TMEM
+  uint64_t s_full[2], s_free[2];     // parts of S
+  uint64_t p_full[2], p_free[2];     // scores
+  uint64_t o_full[2], o_free[2];     // O and QS in TMEM
+  uint64_t fin;
+  uint32_t tmem;
+  volatile int bad;
+};
+template <int DP>
+constexpr size_t SMEM = Cfg<DP>::OFF_CTL + sizeof(Ctl) + 1024;
+
+struct SeqArgs {
+  AtlasDecayParams p;
+  const float* log_decay;
+  const float* in;  // (chains, D, D) entering the first segment of the walk, or NULL: zeros
+  float* out;       // leaving the last one
+  // The states entering segments 1, 2, .. of the walk: segment s of a chain at
+  // (chain * mid_pitch + mid_first + s * mid_step) * D * D.  The sums' pass writes the sum of
+  // segment s to the place of segment s + 1.
+  float* mid;
+  int64_t mid_pitch, mid_first, mid_step;
+  float* saves;  // state entering every 128-token chunk, in the order of the walk; or NULL
+  int segs;        // segments of a sequence
+  int seg_blocks;  // blocks of a segment (even)
+  int sums;        // the sums' pass: segments 0 .. segs - 2, each from zeros
+  int* status;
+};
+__device__ __forceinline__ float* mid_state(const SeqArgs& a, int64_t chain, int s) {
+  return a.mid + (chain * a.mid_pitch + a.mid_first + s * a.mid_step) * a.p.D * a.p.D;
+}
+
+// ---- PTX ----
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int h, int t, int b, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(h), "r"(t), "r"(b), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int h, int t, int b, const void* src) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(map),
+               "r"(x), "r"(h), "r"(t), "r"(b), "r"(smem_u32(src))
+               : "memory");
+}
+// 16 lanes x 64 columns: v[4 j + 2 i + k] = row lane / 4 + 8 i, column 8 j + 2 (lane % 4) + k
+__device__ __forceinline__ void tmem_frag64(uint32_t addr, float* v) {
+  uint32_t* r = (uint32_t*)v;
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+// the same for 32 columns
+__device__ __forceinline__ void tmem_frag32(uint32_t addr, float* v) {
+  uint32_t* r = (uint32_t*)v;
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+// K-major operand of a TMA tile (64 channels of K a box); 16 channels on: +32 bytes
+__device__ __forceinline__ uint64_t desc_tile(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+// MN-major operand of a TMA tile (tokens are K, a box per 64 channels of N); 16 tokens on: +2048 bytes
+__device__ __forceinline__ uint64_t desc_tile_mn(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(BOX >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// Waits for completion number n (from 0) of a barrier.  Bounded; a timeout anywhere in the
+// CTA is recorded and lets every group leave its loop.
+__device__ __forceinline__ bool wait(Ctl& c, uint64_t* bar, int n, int* status) {
+  for (uint32_t i = 0; i < 4000000u; ++i) {
+    if (mbar_try_wait(bar, (uint32_t)n & 1)) return true;
+    if ((i & 15) == 15 && c.bad) return false;
+  }
+  c.bad = 1;
+  set_status(status, ATLAS_ERR_DEVICE_TIMEOUT);
+  return false;
+}
+// one arrival for a whole warp, after its shared-memory writes / TMEM reads
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) arrive(bar);
+}
+
+// Barrier of the four output warps; whether all of them say yes.
+__device__ __forceinline__ bool group_all(bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)yes)
+      : "memory");
+  return r != 0;
+}
+
+// Eight float32 values as three bf16 parts whose sum holds 24 bits, 16-byte groups `stride` apart.
+__device__ __forceinline__ void put_parts3(uint8_t* dst, uint32_t stride, F2* v) {
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    uint4 pk;
+    uint32_t* h = (uint32_t*)&pk;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h[j] = bf2_pack(v[j]);
+      if (p < 2) v[j] = v[j] - bf2_unpack(h[j]);
+    }
+    *(uint4*)(dst + p * stride) = pk;
+  }
+}
+__device__ __forceinline__ float powd(float g, int n) { return n == 0 ? 1.f : expf((float)n * g); }
+
+struct Walk {  // one CTA's blocks: first, first + step, ..., n of them
+  int64_t chain;
+  int b, h, seg, first, step, n;
+};
+
+template <int DP, bool FWD>
+__global__ void __launch_bounds__(Cfg<DP>::NT, 1)
+    seq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_x,
+               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_o, const SeqArgs a,
+               bool reversed) {
+  using K = Cfg<DP>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  Ctl& ctl = *(Ctl*)(sm + K::OFF_CTL);
+  const AtlasDecayParams& P = a.p;
+  // the warp's number as a uniform value: each role's branch is then known not to diverge
+  const int w = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int D = P.D, nblk = (P.T + C - 1) / C;
+  Walk z;
+  const int per_chain = a.segs - a.sums;
+  z.chain = blockIdx.x / per_chain;
+  z.seg = (int)(blockIdx.x % per_chain);  // in the order of the walk
+  z.b = (int)(z.chain / P.H);
+  z.h = (int)(z.chain % P.H);
+  {
+    const int at = reversed ? a.segs - 1 - z.seg : z.seg;
+    const int lo = at * a.seg_blocks, hi = min(nblk, lo + a.seg_blocks);
+    z.n = hi - lo;
+    z.first = reversed ? hi - 1 : lo;
+    z.step = reversed ? -1 : 1;
+  }
+  const float g = a.log_decay[z.h];
+
+  if (w == K::W_MMA) {
+    tmem_alloc(&ctl.tmem, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < K::STAGES; ++i) {
+      mbar_init(&ctl.full[i], 1);
+      mbar_init(&ctl.empty[i], 1 + K::KWARPS);  // the last MMA, and the warps that read k
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl.a_full[i], 1);
+      mbar_init(&ctl.a_free[i], 4);
+      mbar_init(&ctl.kp_full[i], K::KWARPS);
+      mbar_init(&ctl.kp_free[i], 1);
+      mbar_init(&ctl.p_full[i], 4);
+      mbar_init(&ctl.p_free[i], 1);
+      mbar_init(&ctl.o_full[i], 1);
+      mbar_init(&ctl.o_free[i], 4);
+      mbar_init(&ctl.ds_full[i], 1);
+      mbar_init(&ctl.ds_free[i], K::SWARPS);
+      mbar_init(&ctl.s_full[i], K::SWARPS);
+      mbar_init(&ctl.s_free[i], 1);
+    }
+    mbar_init(&ctl.fin, 1);
+    ctl.bad = 0;
+    fence_mbar_init();
+  }
+  if (FWD)  // score blocks above the diagonal are written here once and never again
+    for (int u = threadIdx.x; u < K::DBL * K::PT / 16; u += K::NT) *(uint4*)(sm + K::OFF_P + u * 16) = make_uint4(0, 0, 0, 0);
+  fence_async_smem();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tm = ctl.tmem;
+
+  if (w < K::KWARPS) {
+    // ---- k' : thread (token row, every KP-th 16-byte group) ----
+    constexpr int KP = K::KWARPS / 2;
+    const int r = threadIdx.x & 63, first = threadIdx.x >> 6;
+    const float wfull = reversed ? powd(g, r + 1) : powd(g, C - 1 - r);
+    for (int i = 0; i < z.n; ++i) {
+      const int st = i % K::STAGES, b = i % K::DBL, blk = z.first + i * z.step;
+      const int L = min(C, P.T - blk * C);
+      if (!wait(ctl, &ctl.full[st], i / K::STAGES, a.status)) break;
+      if (i >= K::DBL && !wait(ctl, &ctl.kp_free[b], i / K::DBL - 1, a.status)) break;
+      const float wr = reversed || L == C ? wfull : r < L ? powd(g, L - 1 - r) : 0.f;
+      const F2 w2 = f2(wr, wr);
+      const uint8_t* x = sm + (st * 3 + 1) * K::TILE + r * 128;
+      uint8_t* kp = sm + K::OFF_KP + b * 3 * K::TILE + cm_off(r, 0, DP);
+#pragma unroll 2
+      for (int jj = 0; jj < DP / 8 / KP; ++jj) {
+        const int j = first + KP * jj;
+        const uint4 pk = *(const uint4*)(x + (j >> 3) * BOX + (((j & 7) ^ (r & 7)) << 4));
+        F2 v[4] = {w2 * bf2_unpack(pk.x), w2 * bf2_unpack(pk.y), w2 * bf2_unpack(pk.z), w2 * bf2_unpack(pk.w)};
+        put_parts3(kp + j * 128, K::TILE, v);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        arrive(&ctl.kp_full[b]);
+        arrive(&ctl.empty[st]);
+      }
+    }
+  } else if (w < K::W_Y) {
+    // ---- scores ----
+    if (FWD) {
+      const int q = w & 3, r = lane >> 2, c2 = 2 * (lane & 3), t0 = 16 * q + r;
+      // l^(t - s) of this thread's entries: row t0 at the column pair of block j, which is row
+      // t0 + 8 at that of block j + 1
+      F2 W[9];
+#pragma unroll
+      for (int j = 0; j < 9; ++j) W[j] = f2(powd(g, max(0, t0 - (8 * (j - 1) + c2))), powd(g, max(0, t0 - (8 * (j - 1) + c2 + 1))));
+      uint8_t* prow = sm + K::OFF_P + cm_off(t0, c2, C);
+      for (int i = 0; i < z.n; ++i) {
+        const int b = i % K::DBL, n = i / K::DBL;
+        if (!wait(ctl, &ctl.a_full[b], n, a.status)) break;
+        fence_after();
+        float v[32];
+        tmem_frag64(tm + K::T_A + 64 * b + ((uint32_t)(32 * q) << 16), v);
+        tmem_wait_ld();
+        fence_before();
+        warp_arrive(&ctl.a_free[b]);
+        if (i >= K::DBL && !wait(ctl, &ctl.p_free[b], n - 1, a.status)) break;
+        uint8_t* p = prow + b * K::PT;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j <= 2 * q + 1) {  // 8-column blocks that reach the diagonal or lie below it
+            F2 e = f2(v[4 * j], v[4 * j + 1]) * W[j + 1], f = f2(v[4 * j + 2], v[4 * j + 3]) * W[j];
+            if (j >= 2 * q) {  // the two diagonal blocks: keep s <= t
+              const int d0 = t0 - (8 * j + c2), d1 = d0 + 8;
+              const float2 x = f2_get(e), y = f2_get(f);
+              e = f2(d0 >= 0 ? x.x : 0.f, d0 >= 1 ? x.y : 0.f);
+              f = f2(d1 >= 0 ? y.x : 0.f, d1 >= 1 ? y.y : 0.f);
+            }
+            *(uint32_t*)(p + j * 128) = bf2_pack(e);
+            *(uint32_t*)(p + C * 16 + j * 128) = bf2_pack(f);  // 8 rows on
+          }
+        }
+        fence_async_smem();
+        warp_arrive(&ctl.p_full[b]);
+      }
+    }
+  } else if (w < K::W_S) {
+    // ---- outputs ----
+    if (FWD) {
+      const int q = w & 3, r = lane >> 2, c2 = 2 * (lane & 3), t0 = 16 * q + r;
+      const float i0 = P.scale * powd(g, t0 + 1), i1 = P.scale * powd(g, t0 + 9);
+      const bool lead = threadIdx.x == K::W_Y * 32;
+      const F2 i02 = f2(i0, i0), i12 = f2(i1, i1), sc2 = f2(P.scale, P.scale);
+      for (int i = 0; i < z.n; ++i) {
+        const int b = i % K::DBL, blk = z.first + i * z.step;
+        bool ok = wait(ctl, &ctl.o_full[b], i / K::DBL, a.status);
+        fence_after();
+#pragma unroll
+        for (int hb = 0; hb < K::NB; ++hb) {
+          // the staging buffer of the store before last (DP = 128: of the last) has been read
+          if (lead) {
+            if (DP == 64)
+              asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            else
+              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          }
+          if (!group_all(ok)) {  // the same verdict in all four warps
+            ok = false;
+            break;
+          }
+          uint8_t* y = sm + K::OFF_Y + (DP == 64 ? (i & 1) * BOX : 0) + t0 * 128 + 2 * c2;
+          const uint32_t at = tm + ((uint32_t)(32 * q) << 16) + b * DP + 64 * hb;
+#pragma unroll
+          for (int hc = 0; hc < 2; ++hc) {  // 32 columns
+            float v[16], x[16];
+            tmem_frag32(at + K::T_O + 32 * hc, v);
+            tmem_frag32(at + K::T_QS + 32 * hc, x);
+            tmem_wait_ld();
+            if (hb == K::NB - 1 && hc == 1) {
+              fence_before();
+              warp_arrive(&ctl.o_free[b]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const F2 e = fma2(i02, f2(x[4 * j], x[4 * j + 1]), sc2 * f2(v[4 * j], v[4 * j + 1]));
+              const F2 f = fma2(i12, f2(x[4 * j + 2], x[4 * j + 3]), sc2 * f2(v[4 * j + 2], v[4 * j + 3]));
+              uint8_t* d = y + (((4 * hc + j) ^ r) << 4);  // t0 % 8 = r
+              *(uint32_t*)d = bf2_pack(e);
+              *(uint32_t*)(d + 8 * 128) = bf2_pack(f);
+            }
+          }
+          fence_async_smem();
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (lead) {
+            if (64 * hb < D) tma_store(&map_o, 64 * hb, z.h, blk * C, z.b, y - (t0 * 128 + 2 * c2));
+            bulk_commit();
+          }
+        }
+        if (!ok) break;
+      }
+      if (lead) bulk_wait0();
+    }
+  } else if (w < K::W_MMA) {
+    // ---- the state ----
+    // DP = 64: 16 rows in lanes 0-15 of the quadrant.  DP = 128: rows are lanes.  A warp has 16 rows and
+    // half of the columns.
+    const int sub = (w - K::W_S) >> 2, q = w & 3, r = lane >> 2, c2 = 2 * (lane & 3);
+    const int hf = DP == 64 ? 0 : sub & 1, e0 = (DP == 64 ? sub : sub >> 1) * (DP / 2);
+    const int d0 = DP == 64 ? 16 * q + r : 32 * q + 16 * hf + r;
+    const uint32_t at = tm + K::T_DS + e0 + ((uint32_t)(32 * q + 16 * hf) << 16);
+    constexpr int NJ = DP / 16;  // 8-column blocks of a warp
+    F2 S[2 * NJ];                // [2 j]: row d0, columns e0 + 8 j + c2 and the next; [2 j + 1]: row d0 + 8
+    const int64_t DD = (int64_t)D * D;
+    const bool in0 = d0 < D, in1 = d0 + 8 < D;
+    {
+      const float* s = a.sums ? nullptr : z.seg > 0 ? mid_state(a, z.chain, z.seg) : a.in ? a.in + z.chain * DD : nullptr;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int e = e0 + 8 * j + c2;
+        float2 x = make_float2(0.f, 0.f), y = x;
+        if (s && e < D) {
+          if (in0) x = *(const float2*)(s + (int64_t)d0 * D + e);
+          if (in1) y = *(const float2*)(s + (int64_t)(d0 + 8) * D + e);
+        }
+        S[2 * j] = f2(x.x, x.y), S[2 * j + 1] = f2(y.x, y.y);
+      }
+    }
+    auto put_state = [&](float* out) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int e = e0 + 8 * j + c2;
+        if (e < D) {
+          if (in0) *(float2*)(out + (int64_t)d0 * D + e) = f2_get(S[2 * j]);
+          if (in1) *(float2*)(out + (int64_t)(d0 + 8) * D + e) = f2_get(S[2 * j + 1]);
+        }
+      }
+    };
+    // decay over a block as a float pair: its rounding would be multiplied in again every block
+    const double fd = exp((double)g * C);
+    const float fh = (float)fd, fl = (float)(fd - (double)fh), sc = reversed ? P.scale : 1.f;
+    for (int i = 0; i < z.n; ++i) {
+      const int blk = z.first + i * z.step, b = i % K::DBL, n = i / K::DBL;
+      if (a.saves && (reversed ? (blk & 1) || blk == nblk - 1 : !(blk & 1)))
+        put_state(a.saves + (z.chain * chunks(P) + blk / 2) * DD);
+      if (FWD) {
+        if (i >= K::DBL && !wait(ctl, &ctl.s_free[b], n - 1, a.status)) break;
+        uint8_t* s = sm + K::OFF_S + b * 2 * K::ST + cm_off(d0, e0 + c2, DP);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const F2 x = S[2 * j + k];
+            const uint32_t hi = bf2_pack(x);
+            uint8_t* d = s + j * 128 + k * DP * 16;  // 8 rows on
+            *(uint32_t*)d = hi;
+            *(uint32_t*)(d + K::ST) = bf2_pack(x - bf2_unpack(hi));
+          }
+        fence_async_smem();
+        warp_arrive(&ctl.s_full[b]);
+      }
+      float fbh = fh, fbl = fl;
+      if ((blk + 1) * C > P.T) {
+        const double f = exp((double)g * (P.T - blk * C));
+        fbh = (float)f, fbl = (float)(f - (double)fbh);
+      }
+      if (!wait(ctl, &ctl.ds_full[b], n, a.status)) break;
+      fence_after();
+      float v[4 * NJ];
+      if constexpr (DP == 64)
+        tmem_frag32(at + b * DP, v);
+      else
+        tmem_frag64(at + b * DP, v);
+      tmem_wait_ld();
+      fence_before();
+      warp_arrive(&ctl.ds_free[b]);
+      const F2 h2 = f2(fbh, fbh), l2 = f2(fbl, fbl), c = f2(sc, sc);
+#pragma unroll
+      for (int j = 0; j < 2 * NJ; ++j) {
+        F2 x = f2(v[2 * j], v[2 * j + 1]);
+        if (!FWD) x = x * c;
+        S[j] = fma2(S[j], h2, fma2(S[j], l2, x));
+      }
+    }
+    if (a.sums)
+      put_state(mid_state(a, z.chain, z.seg + 1));
+    else if (a.out && z.seg == a.segs - 1)
+      put_state(a.out + z.chain * DD);
+  } else if (w == K::W_MMA) {
+    // ---- MMAs ----
+    // Descriptors step through a tile by adding to their start address (bytes / 16).
+    const uint32_t base = smem_u32(sm);
+    const uint32_t tmu = __shfl_sync(0xffffffffu, tm, 0);
+    auto tile = [&](int i, int which) { return base + ((i % K::STAGES) * 3 + which) * K::TILE; };
+    auto scores = [&](int i) {  // A = Q K^T
+      const uint32_t id = idesc_bf16(64, 64, false, false), d = tmu + K::T_A + 64 * (i % K::DBL);
+      const uint64_t q = desc_tile(tile(i, 0)), k = desc_tile(tile(i, 1));
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const uint64_t o = ((ks >> 2) * BOX + (ks & 3) * 32) / 16;
+        mma_kf16(d, q + o, k + o, id, ks > 0);
+      }
+      mma_commit(&ctl.a_full[i % K::DBL]);
+    };
+    auto sums = [&](int i) {  // dS = K'^T V
+      const uint32_t id = idesc_bf16(DP, DP, true, true);
+      const uint64_t v = desc_tile_mn(tile(i, 2));
+      const uint64_t kp = desc_mnmajor(base + K::OFF_KP + (i % K::DBL) * 3 * K::TILE, DP);
+#pragma unroll
+      for (int p = 2; p >= 0; --p)  // small parts first: each step truncates to the accumulator's exponent
+#pragma unroll
+        for (int ks = 0; ks < C / 16; ++ks)
+          mma_kf16(tmu + K::T_DS + (i % K::DBL) * DP, kp + (p * K::TILE + ks * DP * 32) / 16, v + ks * (2048 / 16), id, p < 2 || ks > 0);
+      mma_commit(&ctl.kp_free[i % K::DBL]);
+      mma_commit(&ctl.ds_full[i % K::DBL]);
+    };
+    bool ok = true;
+    if (FWD) {
+      ok = wait(ctl, &ctl.full[0], 0, a.status);
+      if (ok) scores(0);
+    }
+    for (int i = 0; i < z.n && ok; ++i) {
+      const int b = i % K::DBL, n = i / K::DBL;
+      if (FWD && i + 1 < z.n) {
+        const int b1 = (i + 1) % K::DBL;
+        ok = wait(ctl, &ctl.full[(i + 1) % K::STAGES], (i + 1) / K::STAGES, a.status) &&
+             (i + 1 < K::DBL || wait(ctl, &ctl.a_free[b1], (i + 1) / K::DBL - 1, a.status));
+        if (!ok) break;
+        fence_after();
+        scores(i + 1);
+      }
+      ok = (FWD || wait(ctl, &ctl.full[i % K::STAGES], i / K::STAGES, a.status)) &&
+           wait(ctl, &ctl.kp_full[b], n, a.status) && (i < K::DBL || wait(ctl, &ctl.ds_free[b], n - 1, a.status));
+      if (!ok) break;
+      fence_after();
+      sums(i);
+      if (FWD) {
+        ok = wait(ctl, &ctl.s_full[b], n, a.status) && (i < K::DBL || wait(ctl, &ctl.o_free[b], n - 1, a.status));
+        if (!ok) break;
+        fence_after();
+        const uint32_t id = idesc_bf16(64, DP, false, true);
+        const uint64_t q = desc_tile(tile(i, 0)), S = desc_mnmajor(base + K::OFF_S + b * 2 * K::ST, DP);
+#pragma unroll
+        for (int p = 1; p >= 0; --p)
+#pragma unroll
+          for (int ks = 0; ks < DP / 16; ++ks)
+            mma_kf16(tmu + K::T_QS + b * DP, q + ((ks >> 2) * BOX + (ks & 3) * 32) / 16,
+                     S + (p * K::ST + ks * DP * 32) / 16, id, p < 1 || ks > 0);
+        mma_commit(&ctl.s_free[b]);
+        ok = wait(ctl, &ctl.p_full[b], n, a.status);
+        if (!ok) break;
+        fence_after();
+        const uint64_t v = desc_tile_mn(tile(i, 2)), pt = desc_kmajor(base + K::OFF_P + b * K::PT, C);
+#pragma unroll
+        for (int ks = 0; ks < C / 16; ++ks)
+          mma_kf16(tmu + K::T_O + b * DP, pt + ks * (256 / 16), v + ks * (2048 / 16), id, ks > 0);
+        mma_commit(&ctl.p_free[b]);
+        mma_commit(&ctl.o_full[b]);
+      }
+      mma_commit(&ctl.empty[i % K::STAGES]);
+    }
+    mma_commit(&ctl.fin);  // nothing of this CTA is in flight on the tensor core when its TMEM is freed
+    wait(ctl, &ctl.fin, 0, a.status);
+  } else if (lane == 0) {
+    // ---- loads ----
+    int i = 0;
+    for (; i < z.n; ++i) {
+      const int st = i % K::STAGES, blk = z.first + i * z.step;
+      if (i >= K::STAGES && !wait(ctl, &ctl.empty[st], i / K::STAGES - 1, a.status)) break;
+      const int nbox = D > 64 ? 2 : 1;
+      mbar_expect_tx(&ctl.full[st], (uint32_t)((FWD ? 3 : 2) * nbox * BOX));
+      uint8_t* t = sm + st * 3 * K::TILE;
+      for (int hb = 0; hb < nbox; ++hb) {
+        if (FWD) tma_load(t + hb * BOX, &map_q, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
+        tma_load(t + K::TILE + hb * BOX, &map_x, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
+        tma_load(t + 2 * K::TILE + hb * BOX, &map_y, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
+      }
+    }
+    if (ctl.bad)  // let the copies land before the CTA goes
+      for (int k = max(0, i - K::STAGES); k < i; ++k)
+        for (int n = 0; n < 1000000 && !mbar_try_wait(&ctl.full[k % K::STAGES], (uint32_t)(k / K::STAGES) & 1); ++n) {
+        }
+  }
+  fence_before();
+  __syncthreads();
+  if (w == K::W_MMA) tmem_dealloc(tm, 512);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// (B, T, H, D) activations with element strides s (batch, token, head) as boxes of 64 tokens x
+// 64 channels of one head, 128-byte swizzle; elements outside read as zero and are not written.
+// An axis of length 1 takes the row size as its stride (its own is never used).
+static bool make_map(CUtensorMap* m, const void* x, const AtlasDecayParams& p, const int64_t* s) {
+  auto enc = encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.D, (cuuint64_t)p.H, (cuuint64_t)p.T, (cuuint64_t)p.B};
+  const cuuint64_t row = (cuuint64_t)p.D * 2;
+  const cuuint64_t strides[3] = {p.H > 1 ? (cuuint64_t)s[2] * 2 : row, p.T > 1 ? (cuuint64_t)s[1] * 2 : row,
+                                 p.B > 1 ? (cuuint64_t)s[0] * 2 : row};
+  const cuuint32_t box[4] = {64, 1, C, 1}, es[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(x), dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The strides that a tensor map holds: multiples of 16 bytes below 2^40, none of them 0.
+bool mappable(const AtlasDecayParams& p, const int64_t* s) {
+  const int64_t n[3] = {p.B, p.T, p.H};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 != 0 || s[i] >= (int64_t)1 << 39)) return false;
+  return encode_fn() != nullptr;
+}
+
+template <int DP, bool FWD>
+static cudaError_t launch(const CUtensorMap& q, const CUtensorMap& x, const CUtensorMap& y, const CUtensorMap& o,
+                          const SeqArgs& a, bool reversed, cudaStream_t s) {
+  cudaError_t e = allow_smem<seq_kernel<DP, FWD>>(SMEM<DP>);
+  if (e != cudaSuccess) return e;
+  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums)), Cfg<DP>::NT, SMEM<DP>, s>>>(q, x, y, o, a, reversed);
+  return cudaGetLastError();
+}
+
+// How many segments to cut a sequence into, and their blocks (even: a multiple of a saved
+// chunk).  In block times: a CTA an SM, `waves` of them; a split adds the sums' pass, at
+// about 0.6 of a full block's time, and two launches (about 8 blocks' time).
+struct Split {
+  int segs, blocks;
+};
+static Split split(const AtlasDecayParams& p) {
+  const int nblk = (p.T + C - 1) / C;
+  const int64_t n = chains(p), sms = 148;
+  Split best{1, (nblk + 1) / 2 * 2};
+  double cost = (double)((n + sms - 1) / sms) * nblk;
+  for (int k = 2; k <= 64 && k <= nblk / 2; ++k) {
+    const int len = ((nblk + k - 1) / k + 1) / 2 * 2, segs = (nblk + len - 1) / len;
+    if (segs != k) continue;
+    const double c = (double)((n * k + sms - 1) / sms) * len + 0.6 * (double)((n * (k - 1) + sms - 1) / sms) * len + 8;
+    if (c < 0.95 * cost) cost = c, best = Split{k, len};
+  }
+  return best;
+}
+
+// The states entering segments 1, 2, ..: S <- l^len S + sum, in place.  One thread per 4
+// elements of a chain's state; len: of segment 0, and of the others.
+__global__ void __launch_bounds__(256) mid_kernel(SeqArgs a, int len0, int len) {
+  const int per = a.p.D * a.p.D / 4;
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= chains(a.p) * per) return;
+  const int64_t chain = u / per;
+  const int e = (int)(u - chain * per) * 4;
+  const double g = (double)a.log_decay[chain % a.p.H], f = exp(g * len);
+  float4 S = a.in ? *(const float4*)(a.in + chain * per * 4 + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 x = *(const float4*)(mid_state(a, chain, 1) + e);
+  for (int s = 1; s < a.segs; ++s) {
+    float* m = mid_state(a, chain, s) + e;
+    const float4 y = s + 1 < a.segs ? *(const float4*)(mid_state(a, chain, s + 1) + e) : x;  // the next load early
+    const double fs = s == 1 ? exp(g * len0) : f;
+    const float fh = (float)fs, fl = (float)(fs - (double)fh);
+    S.x = fmaf(S.x, fh, fmaf(S.x, fl, x.x));
+    S.y = fmaf(S.y, fh, fmaf(S.y, fl, x.y));
+    S.z = fmaf(S.z, fh, fmaf(S.z, fl, x.z));
+    S.w = fmaf(S.w, fh, fmaf(S.w, fl, x.w));
+    *(float4*)m = S;
+    x = y;
+  }
+}
+
+size_t mid_bytes(const AtlasDecayParams& p) {
+  return (size_t)chains(p) * (split(p).segs - 1) * p.D * p.D * sizeof(float);
+}
+
+cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, float* saves, float* mid,
+                       cudaStream_t s) {
+  const AtlasDecayParams& p = a.p;
+  const int64_t flat[3] = {(int64_t)p.T * p.H * p.D, (int64_t)p.H * p.D, p.D};
+  CUtensorMap mq{}, mx{}, my{}, mo{};
+  bool ok;
+  if (bwd)
+    ok = make_map(&mx, a.q, p, p.q_stride) && make_map(&my, a.dy, p, flat);
+  else
+    ok = make_map(&mq, a.q, p, p.q_stride) && make_map(&mx, a.k, p, p.k_stride) && make_map(&my, a.v, p, p.v_stride) &&
+         make_map(&mo, a.y, p, flat);
+  if (!ok) return cudaErrorInvalidValue;
+  const Split z = split(p);
+  const bool wide = p.D > 64;
+  SeqArgs q{};
+  q.p = p;
+  q.log_decay = a.log_decay;
+  q.in = in;
+  q.out = out;
+  q.saves = nullptr;
+  q.segs = z.segs;
+  q.seg_blocks = z.blocks;
+  q.status = a.status;
+  if (saves) {  // a segment's entering state is that of its first chunk in the walk
+    const int per = z.blocks / 2;
+    q.mid = saves;
+    q.mid_pitch = chunks(p);
+    q.mid_first = bwd ? (int64_t)z.segs * per - 1 : 0;
+    q.mid_step = bwd ? -per : per;
+  } else {
+    q.mid = mid;
+    q.mid_pitch = z.segs - 1;
+    q.mid_first = -1;
+    q.mid_step = 1;
+  }
+  if (z.segs > 1) {
+    q.sums = 1;
+    cudaError_t e = wide ? launch<128, false>(mq, mx, my, mo, q, bwd, s) : launch<64, false>(mq, mx, my, mo, q, bwd, s);
+    if (e != cudaSuccess) return e;
+    const int full = z.blocks * C, last = p.T - (z.segs - 1) * full;
+    const int64_t n = chains(p) * p.D * p.D / 4;
+    mid_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(q, bwd ? last : full, full);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    q.sums = 0;
+  }
+  q.saves = saves;
+  if (bwd) return wide ? launch<128, false>(mq, mx, my, mo, q, true, s) : launch<64, false>(mq, mx, my, mo, q, true, s);
+  return wide ? launch<128, true>(mq, mx, my, mo, q, false, s) : launch<64, true>(mq, mx, my, mo, q, false, s);
+}
+
+}  // namespace tcore
+}  // namespace decay
+}  // namespace atlas

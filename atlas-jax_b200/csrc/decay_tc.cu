@@ -1,9 +1,9 @@
-// Decay attention (include/atlas_decay.h) on the tcgen05 tensor cores: bf16 activations,
-// D a multiple of 8 up to 128 (zero-padded to DP = 64 or 128 channels in shared memory).
+// Decay attention (include/atlas_decay.h): the gradients of q, k and v on the tcgen05 tensor
+// cores.  bf16 activations, D a multiple of 8 up to 128 (zero-padded to DP = 64 or 128
+// channels in shared memory).
 //
 // One CTA owns one 128-token chunk of one (batch, head); the states between chunks come
-// from the chunk sums and the recurrence over chunks (decay_attn.cu), so chunks are
-// independent here.  Operand tiles are bf16 in the core-matrix layout of tc_ops.cuh, which
+// from the walks along the sequence (decay_scan.cu), so chunks are independent here.  Operand tiles are bf16 in the core-matrix layout of tc_ops.cuh, which
 // serves as K-major and as MN-major operand, so no tile is transposed; accumulators are
 // float32 in TMEM.
 //
@@ -24,7 +24,7 @@
 
 namespace atlas {
 namespace decay {
-namespace tc {
+namespace tcore {
 
 using namespace tcx;
 typedef __nv_bfloat16 bf16;
@@ -199,140 +199,6 @@ __device__ __forceinline__ void store8(uint8_t* dst, const float* v) {
 }
 
 // ---------------------------------------------------------------------------
-// chunk sums: sum_r w_r x_r y_r^T, (x, y, w) = (k, v, l^(L-1-r)) or (q, scale dy, l^(r+1))
-// ---------------------------------------------------------------------------
-// 8 warps.  w x is split into three bf16 parts, the first over x's own tile.
-template <int DP>
-__global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd) {
-  extern __shared__ uint8_t raw[];
-  uint8_t* X = align128(raw);
-  uint8_t* Y = X + 3 * TILE<DP>;
-  Ctl& ctl = *(Ctl*)(Y + TILE<DP>);
-  const AtlasDecayParams& P = a.p;
-  const Pos z = position(P);
-  const int D = P.D, w = threadIdx.x >> 5;
-  if (bwd) {
-    load_tile<DP>(X, head(a.q, P.q_stride, z), P.q_stride[1], z.L, D);
-    load_tile<DP>(Y, (const bf16*)a.dy + flat_row(P, z, 0), (int64_t)P.H * D, z.L, D);
-  } else {
-    load_tile<DP>(X, head(a.k, P.k_stride, z), P.k_stride[1], z.L, D);
-    load_tile<DP>(Y, head(a.v, P.v_stride, z), P.v_stride[1], z.L, D);
-  }
-  setup(ctl, DP, a.log_decay[z.h]);
-  cp_async_wait_all();
-  cta_sync();
-  for (int u = threadIdx.x; u < CH * DP / 8; u += 256) {
-    const int r = (u & 7) | (u / DP << 3);
-    const float wr = bwd ? ctl.pw[r + 1] : r < z.L ? ctl.pw[z.L - 1 - r] : 0.f;
-    const uint4 pk = *(const uint4*)(X + u * 16);
-    const __nv_bfloat162* h = (const __nv_bfloat162*)&pk;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = __bfloat1622float2(h[j]);
-      v[2 * j] = wr * f.x;
-      v[2 * j + 1] = wr * f.y;
-    }
-    store_parts<3>(X + u * 16, TILE<DP>, v);
-  }
-  fence_async_smem();
-  cta_sync();
-  if (w == 0) {
-    for (int p = 2; p >= 0; --p)
-      mma(ctl.tmem, X + p * TILE<DP>, DP, true, Y, DP, true, DP, DP, CH, p < 2);
-    mma_commit(&ctl.bar);
-  }
-  __syncwarp();
-  uint32_t phase = 0;
-  if (wait_mma(ctl, phase, a.status)) {
-    // M = 128: row = lane of the quadrant; M = 64: lanes 0-15 of each quadrant hold 16 rows
-    const int qd = w & 3, l = threadIdx.x & 31, c0 = (w >> 2) * (DP / 2);
-    const int d = DP == 128 ? 32 * qd + l : 16 * qd + l;
-    const float f = bwd ? P.scale : 1.f;
-    float v[DP / 2];
-    tmem_ld<DP / 2>(ctl.tmem + ((uint32_t)(32 * qd) << 16) + c0, v);
-    if ((DP == 128 || l < 16) && d < D) {
-      float* out = (bwd ? a.dstates : a.states) + z.chunk_index * (int64_t)D * D + (int64_t)d * D;
-#pragma unroll
-      for (int j = 0; j < DP / 2; j += 4)
-        if (c0 + j < D) *(float4*)(out + c0 + j) = make_float4(f * v[j], f * v[j + 1], f * v[j + 2], f * v[j + 3]);
-    }
-  }
-  cta_sync();
-  if (w == 0) tmem_dealloc(ctl.tmem, DP);
-}
-
-// ---------------------------------------------------------------------------
-// outputs
-// ---------------------------------------------------------------------------
-// 8 warps: warp w reads lane quadrant w % 4 (rows), column half w / 4.  TMEM: scores (128
-// columns, later P V), Q S behind them.  The region R holds the two parts of S, then P.
-template <int DP>
-__global__ void __launch_bounds__(256) out_kernel(Args a) {
-  extern __shared__ uint8_t raw[];
-  constexpr int RB = 2 * STILE<DP> > PTILE ? 2 * STILE<DP> : PTILE;
-  uint8_t* Q = align128(raw);
-  uint8_t* K = Q + TILE<DP>;
-  uint8_t* V = K + TILE<DP>;
-  uint8_t* R = V + TILE<DP>;
-  Ctl& ctl = *(Ctl*)(R + RB);
-  const AtlasDecayParams& P = a.p;
-  const Pos z = position(P);
-  const int D = P.D, w = threadIdx.x >> 5, qd = w & 3, ch = w >> 2, t = 32 * qd + (threadIdx.x & 31);
-  load_tile<DP>(Q, head(a.q, P.q_stride, z), P.q_stride[1], z.L, D);
-  load_tile<DP>(K, head(a.k, P.k_stride, z), P.k_stride[1], z.L, D);
-  load_tile<DP>(V, head(a.v, P.v_stride, z), P.v_stride[1], z.L, D);
-  load_state<DP, 2>(R, a.states + z.chunk_index * (int64_t)D * D, D);
-  setup(ctl, 256, a.log_decay[z.h]);
-  cp_async_wait_all();
-  fence_async_smem();
-  cta_sync();
-  const uint32_t tm = ctl.tmem, lane = (uint32_t)(32 * qd) << 16;
-  uint32_t phase = 0;
-  if (w == 0) {
-    mma(tm, Q, DP, false, K, DP, false, CH, CH, DP, false);
-    for (int p = 1; p >= 0; --p)
-      mma(tm + 128, Q, DP, false, R + p * STILE<DP>, DP, true, CH, DP, DP, p < 1);
-    mma_commit(&ctl.bar);
-  }
-  __syncwarp();
-  if (wait_mma(ctl, phase, a.status)) {
-#pragma unroll
-    for (int cb = 0; cb < 64; cb += 16) {
-      const int s0 = 64 * ch + cb;
-      float v[16];
-      tmem_ld<16>(tm + lane + s0, v);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = t >= s0 + j ? v[j] * ctl.pw[max(t - s0 - j, 0)] : 0.f;
-      store8(R + cm_off(t, s0, CH), v);
-      store8(R + cm_off(t, s0 + 8, CH), v + 8);
-    }
-    fence_async_smem();
-    cta_sync();
-    if (w == 0) {
-      mma(tm, R, CH, false, V, DP, true, CH, DP, CH, false);
-      mma_commit(&ctl.bar);
-    }
-    __syncwarp();
-    if (wait_mma(ctl, phase, a.status)) {
-      const float wi = ctl.pw[t + 1];
-#pragma unroll
-      for (int cb = 0; cb < DP / 2; cb += 16) {
-        const int c0 = ch * (DP / 2) + cb;
-        float v[16], x[16];
-        tmem_ld<16>(tm + lane + c0, v);
-        tmem_ld<16>(tm + lane + 128 + c0, x);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = P.scale * fmaf(wi, x[j], v[j]);
-        if (t < z.L) store_row<16>((bf16*)a.y + flat_row(P, z, t), c0, D, v);
-      }
-    }
-  }
-  cta_sync();
-  if (w == 0) tmem_dealloc(tm, 256);
-}
-
-// ---------------------------------------------------------------------------
 // gradients
 // ---------------------------------------------------------------------------
 // 16 warps: warp w reads lane quadrant w % 4, column quarter w / 4.  TMEM: A = Q K^T in
@@ -495,22 +361,6 @@ __global__ void __launch_bounds__(512, 1) grads_kernel(Args a) {
 static unsigned grid(const Args& a) { return (unsigned)(chains(a.p) * chunks(a.p)); }
 
 template <int DP>
-static cudaError_t sums(const Args& a, bool bwd, cudaStream_t s) {
-  const size_t sm = 4 * TILE<DP> + sizeof(Ctl) + 128;
-  cudaError_t e = allow_smem<sums_kernel<DP>>(sm);
-  if (e != cudaSuccess) return e;
-  sums_kernel<DP><<<grid(a), 256, sm, s>>>(a, bwd);
-  return cudaGetLastError();
-}
-template <int DP>
-static cudaError_t out(const Args& a, cudaStream_t s) {
-  const size_t sm = 3 * TILE<DP> + std::max(2 * STILE<DP>, PTILE) + sizeof(Ctl) + 128;
-  cudaError_t e = allow_smem<out_kernel<DP>>(sm);
-  if (e != cudaSuccess) return e;
-  out_kernel<DP><<<grid(a), 256, sm, s>>>(a);
-  return cudaGetLastError();
-}
-template <int DP>
 static cudaError_t grads(const Args& a, cudaStream_t s) {
   const size_t sm = 4 * TILE<DP> + std::max(3 * STILE<DP>, 2 * PTILE) + sizeof(Ctl) + 128;
   cudaError_t e = allow_smem<grads_kernel<DP>>(sm);
@@ -519,12 +369,8 @@ static cudaError_t grads(const Args& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_chunk_states(const Args& a, bool bwd, cudaStream_t s) {
-  return a.p.D <= 64 ? sums<64>(a, bwd, s) : sums<128>(a, bwd, s);
-}
-cudaError_t launch_out(const Args& a, cudaStream_t s) { return a.p.D <= 64 ? out<64>(a, s) : out<128>(a, s); }
 cudaError_t launch_grads(const Args& a, cudaStream_t s) { return a.p.D <= 64 ? grads<64>(a, s) : grads<128>(a, s); }
 
-}  // namespace tc
+}  // namespace tcore
 }  // namespace decay
 }  // namespace atlas

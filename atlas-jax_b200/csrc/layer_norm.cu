@@ -24,6 +24,7 @@
 
 #include "atlas_norm.h"
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "scan_internal.h"
 
 namespace atlas {
@@ -81,37 +82,8 @@ __device__ __forceinline__ void store(TA* p, const float* f) {
   }
   *(Pack<TA, VEC>*)p = k;
 }
-// Two lanes of float32 in one instruction (same rounding as the scalar ones): the backward is
-// as near to the issue limit as to the memory's.
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 f2_get(F2 a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
-  return r;
-}
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-// A group as pairs; a single channel is a pair with a zero.
+// A group as pairs (the backward is as near to the issue limit as to the memory's); a single
+// channel is a pair with a zero.
 template <int VEC>
 constexpr int PAIRS = (VEC + 1) / 2;
 template <typename TA, int VEC>

@@ -50,7 +50,9 @@ typedef struct {
   int32_t B, T, H, D;
   int32_t act_dtype; /* ATLAS_F32 or ATLAS_BF16 */
   float scale;       /* of the read-out */
-  int32_t reserved;  /* 0 */
+  int32_t aligned16; /* 1: every buffer of the calls is 16-byte aligned (then checked); what the
+                      * tensor cores need, beside bf16, D % 8 == 0 and strides of the axes longer
+                      * than 1 that are positive multiples of 8 */
   /* elements between batches, tokens and heads of q, k and v */
   int64_t q_stride[3], k_stride[3], v_stride[3];
 } AtlasDecayParams;
@@ -59,8 +61,10 @@ typedef struct {
  * (0 on invalid params, with the message set, and for empty problems). */
 size_t atlas_decay_saved_bytes(const AtlasDecayParams* p);
 
-/* Bytes of workspace that covers both directions (0 as above). */
-size_t atlas_decay_workspace_bytes(const AtlasDecayParams* p);
+/* Bytes of workspace of a forward without `saved`, and of the backward (0 on invalid params,
+ * and where none is needed). */
+size_t atlas_decay_fwd_workspace_bytes(const AtlasDecayParams* p);
+size_t atlas_decay_bwd_workspace_bytes(const AtlasDecayParams* p);
 
 /* Forward.  state_in may be NULL (zeros); state_out = S after token T - 1 and may be the same
  * buffer as state_in; saved may be NULL when no backward follows. */

@@ -9,10 +9,10 @@ from atlas_b200 import _lib as L
 
 def _decay(**kw):
     from atlas_b200.decay_attention import AtlasDecayParams
-    b = dict(abi=L.ATLAS_ABI_VERSION, B=2, T=300, H=3, D=64, dt=L.ATLAS_BF16, scale=0.125, stride=(300 * 192, 192, 64))
+    b = dict(abi=L.ATLAS_ABI_VERSION, B=2, T=300, H=3, D=64, dt=L.ATLAS_BF16, scale=0.125, aligned=1, stride=(300 * 192, 192, 64))
     b.update(kw)
     s = [(ctypes.c_int64 * 3)(*b["stride"]) for _ in range(3)]
-    return AtlasDecayParams(b["abi"], b["B"], b["T"], b["H"], b["D"], b["dt"], b["scale"], 0, *s)
+    return AtlasDecayParams(b["abi"], b["B"], b["T"], b["H"], b["D"], b["dt"], b["scale"], b["aligned"], *s)
 
 
 def _norm(**kw):
@@ -39,7 +39,9 @@ def test_decay_sizes():
     p = _decay()
     # the state entering each of ceil(300 / 128) chunks
     assert lib.atlas_decay_saved_bytes(ctypes.byref(p)) == 2 * 3 * 3 * 64 * 64 * 4
-    assert lib.atlas_decay_workspace_bytes(ctypes.byref(p)) >= 2 * 3 * 3 * 64 * 64 * 4
+    assert lib.atlas_decay_bwd_workspace_bytes(ctypes.byref(p)) >= 2 * 3 * 3 * 64 * 64 * 4
+    # without 16-byte alignment the forward keeps every chunk's state
+    assert lib.atlas_decay_fwd_workspace_bytes(ctypes.byref(_decay(aligned=0))) == 2 * 3 * 3 * 64 * 64 * 4
     assert lib.atlas_decay_saved_bytes(ctypes.byref(_decay(T=0))) == 0 and lib.atlas_last_error_string() == b""
 
 
@@ -62,7 +64,10 @@ def test_decay_refusals():
     p = _decay()
     x = ctypes.c_void_p(16)
     assert lib.atlas_decay_fwd(ctypes.byref(p), *[None] * 9, 0, None) == L.ATLAS_ERR_INVALID_ARGUMENT
-    assert lib.atlas_decay_fwd(ctypes.byref(p), *[x] * 7, None, x, 16, None) == L.ATLAS_ERR_WORKSPACE
+    assert lib.atlas_decay_fwd(ctypes.byref(_decay(aligned=0)), *[x] * 7, None, x, 16, None) == L.ATLAS_ERR_WORKSPACE
+    odd = ctypes.c_void_p(20)
+    assert lib.atlas_decay_fwd(ctypes.byref(p), x, odd, *[x] * 5, x, None, 0, None) == L.ATLAS_ERR_INVALID_ARGUMENT
+    assert b"aligned" in lib.atlas_last_error_string()
     assert lib.atlas_decay_bwd(ctypes.byref(p), *[x] * 13, 16, None) == L.ATLAS_ERR_WORKSPACE
     assert lib.atlas_decay_step(ctypes.byref(p), *[x] * 6, -1, x, x, None) == L.ATLAS_ERR_INVALID_ARGUMENT
     assert lib.atlas_decay_fwd(None, *[None] * 9, 0, None) == L.ATLAS_ERR_INVALID_ARGUMENT
