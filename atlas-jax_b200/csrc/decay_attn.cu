@@ -1,8 +1,8 @@
 // Decay attention (include/atlas_decay.h): entry points, the float32 CUDA-core kernels for
-// the calls outside the tensor path (decay_scan.cu, decay_tc.cu), and the recurrent
+// the calls outside the tensor path (decay_scan.cu, decay_grad.cu), and the recurrent
 // single-token form.
 //
-// A sequence is cut into chunks of CH = 128 tokens.  With L tokens in a chunk, local
+// A sequence is cut into chunks of CH = 64 tokens.  With L tokens in a chunk, local
 // positions t, s and l = exp(log_decay):
 //
 //   forward   dS[c]     = sum_s l^(L-1-s) k_s v_s^T                   every chunk by itself

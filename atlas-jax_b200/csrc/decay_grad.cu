@@ -1,0 +1,367 @@
+// Decay attention (include/atlas_decay.h): the gradients of q, k and v and the parts of
+// dlog_decay on the tcgen05 tensor cores, from the states that the walks along the sequence
+// keep in front of every block (decay_scan.cu).  With O = dy, S the state entering a block
+// of L <= 64 tokens, R the cotangent of the state leaving it, M_ts = l^(t-s) for s <= t:
+//
+//     A = Q K^T,  P = M o A,  B = O V^T,  dA = M o B
+//     dq = scale (dA K + l^(t+1) O S^T)
+//     dk = scale dA^T Q + l^(L-1-s) V R^T
+//     dv = scale P^T O + l^(L-1-s) K R
+//     dlog_decay += scale sum (t-s) A dA + sum (t+1) q . dq_S + sum (L-1-s) k . dk_R + L l^L <R, S>
+//     (dq_S, dk_R: the terms with S and R)
+//
+// Blocks are independent: one CTA each.  q, k, v, dy arrive by TMA and leave as dq, dk, dv
+// through the same tiles; S and R are split into three bf16 parts (dlog_decay is a float32
+// output; dv needs two of R's).  All accumulators have M = 64 (decay_tc.cuh); warp w reads
+// lane quadrant w % 4 and the column half w / 4.
+//
+// D <= 64: two rounds of MMAs (A, B, O S^T, V R^T, then K R, dA K, dA^T Q, P^T O in the same
+// 256 TMEM columns), 97 KB of shared memory: two CTAs share an SM, and one's loads and
+// float32 work run during the other's MMAs.  D <= 128: the parts of S and R take turns in one
+// region and K R has columns of its own; one CTA an SM.
+#include <algorithm>
+
+#include "decay_tc.cuh"
+
+namespace atlas {
+namespace decay {
+namespace tcore {
+
+template <int DP>
+struct GCfg {
+  static constexpr int NB = DP / 64, TILE = NB * BOX, ST = DP * DP * 2, PT = C * C * 2;
+  static constexpr int OFF_PARTS = 4 * TILE;
+  static constexpr int OFF_P = OFF_PARTS + (DP == 64 ? 6 : 3) * ST;
+  static constexpr int OFF_CTL = OFF_P + 2 * PT;
+  // TMEM columns of the first round and of the second
+  static constexpr uint32_t COLS = DP == 64 ? 256 : 512;
+  static constexpr uint32_t T_A = 0, T_B = 64, T_OS = 128, T_VR = 128 + DP;
+  static constexpr uint32_t T_KR = DP == 64 ? 0 : 384, T_DQ = DP == 64 ? 64 : 128, T_DK = DP == 64 ? 128 : 256,
+                            T_DV = DP == 64 ? 192 : 0;
+};
+struct GCtl {
+  float pw[C + 1];
+  float red[8];
+  uint64_t loaded, done;
+  uint32_t tmem;
+  volatile int bad;
+};
+template <int DP>
+constexpr size_t GRAD_SMEM = GCfg<DP>::OFF_CTL + sizeof(GCtl) + 1024;
+
+struct Maps {
+  CUtensorMap q, k, v, o, dq, dk, dv;
+};
+
+__device__ __forceinline__ void cta_sync() {
+  fence_before();
+  __syncthreads();
+  fence_after();
+}
+// every thread waits (bounded); false after a timeout, uniformly
+__device__ __forceinline__ bool wait_all(GCtl& c, uint64_t* bar, uint32_t parity, int* status) {
+  const bool ok = c.bad || mbar_wait(bar, parity, 4000000u);
+  if (!ok) {
+    set_status(status, ATLAS_ERR_DEVICE_TIMEOUT);
+    c.bad = 1;
+  }
+  cta_sync();
+  return !c.bad;
+}
+// one warp: D (+)= A B, descriptors stepping by sa and sb per 16 of K
+template <int N>
+__device__ __forceinline__ void mma_steps(uint32_t d, uint64_t A, uint64_t sa, uint64_t B, uint64_t sb, uint32_t id,
+                                          bool accumulate) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) mma_kf16(d, A + k * sa, B + k * sb, id, accumulate || k > 0);
+}
+template <int NV>
+__device__ __forceinline__ void frag(uint32_t addr, float* v) {
+  if constexpr (NV == 16)
+    tmem_frag32(addr, v);
+  else
+    tmem_frag64(addr, v);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __grid_constant__ Maps maps, const Args a) {
+  using G = GCfg<DP>;
+  constexpr int NV = DP / 4;  // values of an output fragment: 2 rows x DP / 8 columns of a thread
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  GCtl& ctl = *(GCtl*)(sm + G::OFF_CTL);
+  const AtlasDecayParams& P = a.p;
+  const int tid = threadIdx.x, w = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, D = P.D;
+  const int nc = chunks(P);
+  const int64_t chain = blockIdx.x / nc;
+  const int c = (int)(blockIdx.x % nc), b = (int)(chain / P.H), h = (int)(chain % P.H), L = chunk_len(P, c);
+  const int q = w & 3, hf = w >> 2, r = lane >> 2, c2 = 2 * (lane & 3), t0 = 16 * q + r;
+  const float g = a.log_decay[h];
+  const uint32_t base = smem_u32(sm);
+  if (tid == 0) {
+    mbar_init(&ctl.loaded, 1);
+    mbar_init(&ctl.done, 1);
+    fence_mbar_init();
+    ctl.bad = 0;
+    const int nbox = D > 64 ? 2 : 1;
+    mbar_expect_tx(&ctl.loaded, (uint32_t)(4 * nbox * BOX));
+    for (int i = 0; i < nbox; ++i) {
+      tma_load(sm + i * BOX, &maps.q, 64 * i, h, c * C, b, &ctl.loaded);
+      tma_load(sm + G::TILE + i * BOX, &maps.k, 64 * i, h, c * C, b, &ctl.loaded);
+      tma_load(sm + 2 * G::TILE + i * BOX, &maps.v, 64 * i, h, c * C, b, &ctl.loaded);
+      tma_load(sm + 3 * G::TILE + i * BOX, &maps.o, 64 * i, h, c * C, b, &ctl.loaded);
+    }
+  }
+  if (w == 1) {
+    tmem_alloc(&ctl.tmem, G::COLS);
+    tmem_relinquish();
+  }
+  if (tid >= 64 && tid <= 64 + C) ctl.pw[tid - 64] = powd(g, tid - 64);
+
+  // S and R (float32, D x D) -> three parts each; <R, S>
+  const float* Sg = a.states + (int64_t)blockIdx.x * D * D;
+  const float* Rg = a.dstates + (int64_t)blockIdx.x * D * D;
+  float rs = 0.f;
+  auto load8 = [&](const float* M, int u, F2* v) {
+    const int d = (u & 7) | (u / DP << 3), e = ((u >> 3) % (DP / 8)) * 8;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+    if (d < D && e < D) {
+      x = *(const float4*)(M + d * D + e);
+      y = *(const float4*)(M + d * D + e + 4);
+    }
+    v[0] = f2(x.x, x.y), v[1] = f2(x.z, x.w), v[2] = f2(y.x, y.y), v[3] = f2(y.z, y.w);
+  };
+  auto dot8 = [&](const F2* x, const F2* y) {
+    const F2 s = fma2(x[0], y[0], fma2(x[1], y[1], fma2(x[2], y[2], x[3] * y[3])));
+    const float2 t = f2_get(s);
+    rs += t.x + t.y;
+  };
+  uint8_t* parts = sm + G::OFF_PARTS;
+  if constexpr (DP == 64) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int u = tid + 256 * i;
+      F2 x[4], y[4];
+      load8(Sg, u, x);
+      load8(Rg, u, y);
+      dot8(x, y);
+      put_parts3(parts + u * 16, G::ST, x);
+      put_parts3(parts + 3 * G::ST + u * 16, G::ST, y);
+    }
+  } else {
+#pragma unroll 2
+    for (int i = 0; i < DP * DP / 8 / 256; ++i) {
+      const int u = tid + 256 * i;
+      F2 x[4];
+      load8(Sg, u, x);
+      put_parts3(parts + u * 16, G::ST, x);
+    }
+  }
+  fence_async_smem();
+  cta_sync();
+  bool ok = wait_all(ctl, &ctl.loaded, 0, a.status);
+  const uint32_t tm = ctl.tmem, tmu = __shfl_sync(0xffffffffu, tm, 0), at = tm + ((uint32_t)(32 * q) << 16);
+  const uint64_t pd = desc_mnmajor(base + G::OFF_PARTS, DP), pk = desc_kmajor(base + G::OFF_PARTS, DP);
+  constexpr uint64_t STEP_K = 256 / 16, STEP_MN = DP * 32 / 16, PART = G::ST / 16, TSTEP_MN = 2048 / 16;
+  const uint32_t id_ss = idesc_bf16(64, 64, false, false), id_kk = idesc_bf16(64, DP, false, false),
+                 id_kn = idesc_bf16(64, DP, false, true), id_nn = idesc_bf16(64, DP, true, true);
+  // X times a state's part: K-major X tile (boxes of 64 channels) and K- or MN-major part
+  auto times_parts = [&](uint32_t d, uint32_t tile, uint64_t part0, bool mn, int np) {
+    const uint64_t x = desc_tile(tile);
+    for (int p = np - 1; p >= 0; --p) {
+#pragma unroll
+      for (int bx = 0; bx < G::NB; ++bx)
+        mma_steps<4>(d, x + bx * (BOX / 16), 2, part0 + p * PART + bx * 4 * (mn ? STEP_MN : STEP_K), mn ? STEP_MN : STEP_K,
+                     mn ? id_kn : id_kk, p < np - 1 || bx > 0);
+    }
+  };
+  uint32_t phase = 0;
+  if (ok) {
+    if (w == 0) {
+      const uint64_t dq_ = desc_tile(base), dk_ = desc_tile(base + G::TILE), dv_ = desc_tile(base + 2 * G::TILE),
+                     do_ = desc_tile(base + 3 * G::TILE);
+#pragma unroll
+      for (int bx = 0; bx < G::NB; ++bx) {
+        mma_steps<4>(tmu + G::T_A, dq_ + bx * (BOX / 16), 2, dk_ + bx * (BOX / 16), 2, id_ss, bx > 0);
+        mma_steps<4>(tmu + G::T_B, do_ + bx * (BOX / 16), 2, dv_ + bx * (BOX / 16), 2, id_ss, bx > 0);
+      }
+      times_parts(tmu + G::T_OS, base + 3 * G::TILE, pk, false, 3);  // O S^T
+      if (DP == 64) times_parts(tmu + G::T_VR, base + 2 * G::TILE, pk + 3 * PART, false, 3);  // V R^T
+      mma_commit(&ctl.done);
+    }
+    __syncwarp();
+    ok = wait_all(ctl, &ctl.done, phase, a.status);
+    phase ^= 1;
+  }
+  if (DP != 64 && ok) {  // the parts of R in the place of S's
+#pragma unroll 2
+    for (int i = 0; i < DP * DP / 8 / 256; ++i) {
+      const int u = tid + 256 * i;
+      F2 x[4], y[4];
+      load8(Sg, u, x);
+      load8(Rg, u, y);
+      dot8(x, y);
+      put_parts3(parts + u * 16, G::ST, y);
+    }
+    fence_async_smem();
+    cta_sync();
+    if (w == 0) {
+      times_parts(tmu + G::T_VR, base + 2 * G::TILE, pk, false, 3);
+      times_parts(tmu + G::T_KR, base + G::TILE, pd, true, 2);
+      mma_commit(&ctl.done);
+    }
+    __syncwarp();
+    ok = wait_all(ctl, &ctl.done, phase, a.status);
+    phase ^= 1;
+  }
+  float dg = 0.f;
+  F2 dq[NV / 2], dk[NV / 2];  // [2 j]: row t0, columns 8 j + c2 and the next of this half; [2 j + 1]: row t0 + 8
+  const float wo0 = t0 < L ? ctl.pw[L - 1 - t0] : 0.f, wo1 = t0 + 8 < L ? ctl.pw[L - 9 - t0] : 0.f;
+  if (ok) {
+    // 8-byte-per-pair dot of rows t0 and t0 + 8 of a tile with a fragment
+    auto dot_rows = [&](int which, const F2* v, float f0, float f1) {
+      F2 s0 = f2(0.f, 0.f), s1 = s0;
+#pragma unroll
+      for (int j = 0; j < NV / 4; ++j) {
+        const int col = hf * (DP / 2) + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
+        const uint8_t* x = sm + which * G::TILE + bx * BOX + t0 * 128 + ((jj ^ r) << 4) + 2 * c2;
+        s0 = fma2(bf2_unpack(*(const uint32_t*)x), v[2 * j], s0);
+        s1 = fma2(bf2_unpack(*(const uint32_t*)(x + 8 * 128)), v[2 * j + 1], s1);
+      }
+      const float2 x = f2_get(s0), y = f2_get(s1);
+      return f0 * (x.x + x.y) + f1 * (y.x + y.y);
+    };
+    float v[NV];
+    frag<NV>(at + G::T_OS + hf * (DP / 2), v);
+    tmem_wait_ld();
+    const F2 i0 = f2(ctl.pw[t0 + 1], ctl.pw[t0 + 1]), i1 = f2(ctl.pw[t0 + 9], ctl.pw[t0 + 9]);
+#pragma unroll
+    for (int j = 0; j < NV / 4; ++j) {
+      dq[2 * j] = i0 * f2(v[4 * j], v[4 * j + 1]);
+      dq[2 * j + 1] = i1 * f2(v[4 * j + 2], v[4 * j + 3]);
+    }
+    dg += P.scale * dot_rows(0, dq, (float)(t0 + 1), (float)(t0 + 9));
+    frag<NV>(at + G::T_VR + hf * (DP / 2), v);
+    tmem_wait_ld();
+    const F2 o0 = f2(wo0, wo0), o1 = f2(wo1, wo1);
+#pragma unroll
+    for (int j = 0; j < NV / 4; ++j) {
+      dk[2 * j] = o0 * f2(v[4 * j], v[4 * j + 1]);
+      dk[2 * j + 1] = o1 * f2(v[4 * j + 2], v[4 * j + 3]);
+    }
+    dg += dot_rows(1, dk, (float)max(L - 1 - t0, 0), (float)max(L - 9 - t0, 0));
+    if (L > 0) dg += (float)L * ctl.pw[L] * rs;
+    // scores
+    float x[16], y[16];
+    tmem_frag32(at + G::T_A + 32 * hf, x);
+    tmem_frag32(at + G::T_B + 32 * hf, y);
+    tmem_wait_ld();
+    F2 gl = f2(0.f, 0.f);
+    uint8_t* pt = sm + G::OFF_P + cm_off(t0, 32 * hf + c2, C);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int lag = t0 + 8 * k - (32 * hf + 8 * j + c2);  // of the pair's first column
+        const float m0 = lag >= 0 ? ctl.pw[lag] : 0.f, m1 = lag >= 1 ? ctl.pw[lag - 1] : 0.f;
+        // masked scores are dropped, not multiplied by 0
+        const F2 A = f2(lag >= 0 ? x[4 * j + 2 * k] : 0.f, lag >= 1 ? x[4 * j + 2 * k + 1] : 0.f);
+        const F2 B = f2(lag >= 0 ? y[4 * j + 2 * k] : 0.f, lag >= 1 ? y[4 * j + 2 * k + 1] : 0.f);
+        const F2 M = f2(m0, m1), dA = M * B;
+        gl = fma2(f2((float)lag, (float)(lag - 1)) * A, dA, gl);
+        *(uint32_t*)(pt + k * C * 16 + j * 128) = bf2_pack(M * A);
+        *(uint32_t*)(pt + G::PT + k * C * 16 + j * 128) = bf2_pack(dA);
+      }
+    const float2 gg = f2_get(gl);
+    dg += P.scale * (gg.x + gg.y);
+    fence_async_smem();
+    cta_sync();
+    if (w == 0) {
+      const uint32_t p0 = base + G::OFF_P, p1 = p0 + G::PT;
+      mma_steps<4>(tmu + G::T_DQ, desc_kmajor(p1, C), 256 / 16, desc_tile_mn(base + G::TILE), TSTEP_MN, id_kn, false);
+      mma_steps<4>(tmu + G::T_DK, desc_mnmajor(p1, C), C * 32 / 16, desc_tile_mn(base), TSTEP_MN, id_nn, false);
+      mma_steps<4>(tmu + G::T_DV, desc_mnmajor(p0, C), C * 32 / 16, desc_tile_mn(base + 3 * G::TILE), TSTEP_MN, id_nn, false);
+      if (DP == 64) times_parts(tmu + G::T_KR, base + G::TILE, pd + 3 * PART, true, 2);  // K R
+      mma_commit(&ctl.done);
+    }
+    __syncwarp();
+    ok = wait_all(ctl, &ctl.done, phase, a.status);
+    phase ^= 1;
+  }
+  if (ok) {
+    // outputs through the tiles of q, k and v, which nothing reads any more
+    const F2 sc = f2(P.scale, P.scale);
+    auto put = [&](int which, const F2* v) {
+#pragma unroll
+      for (int j = 0; j < NV / 4; ++j) {
+        const int col = hf * (DP / 2) + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
+        uint8_t* y = sm + which * G::TILE + bx * BOX + t0 * 128 + ((jj ^ r) << 4) + 2 * c2;
+        *(uint32_t*)y = bf2_pack(v[2 * j]);
+        *(uint32_t*)(y + 8 * 128) = bf2_pack(v[2 * j + 1]);
+      }
+    };
+    float v[NV];
+    frag<NV>(at + G::T_DQ + hf * (DP / 2), v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < NV / 2; ++j) dq[j] = sc * (dq[j] + f2(v[2 * j], v[2 * j + 1]));
+    put(0, dq);
+    frag<NV>(at + G::T_DK + hf * (DP / 2), v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < NV / 2; ++j) dk[j] = fma2(sc, f2(v[2 * j], v[2 * j + 1]), dk[j]);
+    put(1, dk);
+    frag<NV>(at + G::T_KR + hf * (DP / 2), v);
+    tmem_wait_ld();
+    const F2 o0 = f2(wo0, wo0), o1 = f2(wo1, wo1);
+#pragma unroll
+    for (int j = 0; j < NV / 2; ++j) dk[j] = (j & 1 ? o1 : o0) * f2(v[2 * j], v[2 * j + 1]);
+    frag<NV>(at + G::T_DV + hf * (DP / 2), v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < NV / 2; ++j) dk[j] = fma2(sc, f2(v[2 * j], v[2 * j + 1]), dk[j]);
+    put(2, dk);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dg += __shfl_xor_sync(0xffffffffu, dg, o);
+    if (lane == 0) ctl.red[w] = dg;
+    fence_async_smem();
+    cta_sync();
+    if (tid == 0) {
+      for (int i = 0; i < (D > 64 ? 2 : 1); ++i) {
+        tma_store(&maps.dq, 64 * i, h, c * C, b, sm + i * BOX);
+        tma_store(&maps.dk, 64 * i, h, c * C, b, sm + G::TILE + i * BOX);
+        tma_store(&maps.dv, 64 * i, h, c * C, b, sm + 2 * G::TILE + i * BOX);
+      }
+      bulk_commit();
+      float s = 0.f;
+      for (int i = 0; i < 8; ++i) s += ctl.red[i];
+      a.dg_part[blockIdx.x] = s;
+      bulk_wait_read0();
+    }
+  }
+  cta_sync();
+  if (w == 1) tmem_dealloc(tm, G::COLS);
+}
+
+template <int DP>
+static cudaError_t launch(const Maps& m, const Args& a, cudaStream_t s) {
+  cudaError_t e = allow_smem<grads_kernel<DP>>(GRAD_SMEM<DP>);
+  if (e != cudaSuccess) return e;
+  grads_kernel<DP><<<(unsigned)(chains(a.p) * chunks(a.p)), 256, GRAD_SMEM<DP>, s>>>(m, a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_grads(const Args& a, cudaStream_t s) {
+  const AtlasDecayParams& p = a.p;
+  const int64_t flat[3] = {(int64_t)p.T * p.H * p.D, (int64_t)p.H * p.D, p.D};
+  Maps m;
+  if (!make_map(&m.q, a.q, p, p.q_stride) || !make_map(&m.k, a.k, p, p.k_stride) || !make_map(&m.v, a.v, p, p.v_stride) ||
+      !make_map(&m.o, a.dy, p, flat) || !make_map(&m.dq, a.dq, p, flat) || !make_map(&m.dk, a.dk, p, flat) ||
+      !make_map(&m.dv, a.dv, p, flat))
+    return cudaErrorInvalidValue;
+  return p.D <= 64 ? launch<64>(m, a, s) : launch<128>(m, a, s);
+}
+
+}  // namespace tcore
+}  // namespace decay
+}  // namespace atlas

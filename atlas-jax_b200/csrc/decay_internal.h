@@ -1,4 +1,4 @@
-// Shared by the decay attention kernels (decay_attn.cu, decay_tc.cu).
+// Shared by the decay attention kernels (decay_attn.cu, decay_scan.cu, decay_grad.cu).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -9,7 +9,7 @@
 namespace atlas {
 namespace decay {
 
-constexpr int CH = 128;  // tokens of a chunk: a state is kept for each, on every path
+constexpr int CH = 64;  // tokens of a chunk: a state is kept for each, on every path
 
 struct Args {
   AtlasDecayParams p;
@@ -51,7 +51,7 @@ bool mappable(const AtlasDecayParams& p, const int64_t* strides);  // whether TM
 size_t mid_bytes(const AtlasDecayParams& p);
 cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, float* saves, float* mid,
                        cudaStream_t s);
-// dq, dk, dv and the parts of dlog_decay, chunk by chunk, from a.states and a.dstates (decay_tc.cu)
+// dq, dk, dv and the parts of dlog_decay, chunk by chunk, from a.states and a.dstates (decay_grad.cu)
 cudaError_t launch_grads(const Args& a, cudaStream_t s);
 }  // namespace tcore
 

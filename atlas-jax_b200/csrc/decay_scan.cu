@@ -30,27 +30,14 @@
 // accumulators sit in 16 lanes of each TMEM lane quadrant and are read with 16x256b loads,
 // which spread them over all 32 lanes of a warp: lane holds rows lane / 4 and lane / 4 + 8,
 // columns 8 j + 2 (lane % 4) and the next one.
-#include <cuda.h>
-#include <cuda_bf16.h>
-#include <cudaTypedefs.h>
-
 #include <algorithm>
 #include <mutex>
 
-#include "common.cuh"
-#include "decay_internal.h"
-#include "f32x2.cuh"
-#include "tc_ops.cuh"
+#include "decay_tc.cuh"
 
 namespace atlas {
 namespace decay {
 namespace tcore {
-
-using namespace tcx;
-typedef __nv_bfloat16 bf16;
-
-constexpr int C = 64;  // tokens of a block
-constexpr int BOX = C * 128;  // bytes of a TMA box: 64 tokens x 64 channels
 
 template <int DP>
 struct Cfg {
@@ -87,7 +74,7 @@ struct Ctl {
   volatile int bad;
 };
 template <int DP>
-constexpr size_t SMEM = Cfg<DP>::OFF_CTL + sizeof(Ctl) + 1024;
+constexpr size_t SEQ_SMEM = Cfg<DP>::OFF_CTL + sizeof(Ctl) + 1024;
 
 struct SeqArgs {
   AtlasDecayParams p;
@@ -99,62 +86,14 @@ struct SeqArgs {
   // segment s to the place of segment s + 1.
   float* mid;
   int64_t mid_pitch, mid_first, mid_step;
-  float* saves;  // state entering every 128-token chunk, in the order of the walk; or NULL
+  float* saves;    // state entering every block, in the order of the walk; or NULL
   int segs;        // segments of a sequence
-  int seg_blocks;  // blocks of a segment (even)
+  int seg_blocks;  // blocks of a segment
   int sums;        // the sums' pass: segments 0 .. segs - 2, each from zeros
   int* status;
 };
 __device__ __forceinline__ float* mid_state(const SeqArgs& a, int64_t chain, int s) {
   return a.mid + (chain * a.mid_pitch + a.mid_first + s * a.mid_step) * a.p.D * a.p.D;
-}
-
-// ---- PTX ----
-__device__ __forceinline__ void arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int h, int t, int b, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(x), "r"(h), "r"(t), "r"(b), "r"(smem_u32(bar))
-      : "memory");
-}
-__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int h, int t, int b, const void* src) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(map),
-               "r"(x), "r"(h), "r"(t), "r"(b), "r"(smem_u32(src))
-               : "memory");
-}
-// 16 lanes x 64 columns: v[4 j + 2 i + k] = row lane / 4 + 8 i, column 8 j + 2 (lane % 4) + k
-__device__ __forceinline__ void tmem_frag64(uint32_t addr, float* v) {
-  uint32_t* r = (uint32_t*)v;
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
-}
-// the same for 32 columns
-__device__ __forceinline__ void tmem_frag32(uint32_t addr, float* v) {
-  uint32_t* r = (uint32_t*)v;
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
-}
-// K-major operand of a TMA tile (64 channels of K a box); 16 channels on: +32 bytes
-__device__ __forceinline__ uint64_t desc_tile(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-         (uint64_t)2 << 61;
-}
-// MN-major operand of a TMA tile (tokens are K, a box per 64 channels of N); 16 tokens on: +2048 bytes
-__device__ __forceinline__ uint64_t desc_tile_mn(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(BOX >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
 // Waits for completion number n (from 0) of a barrier.  Bounded; a timeout anywhere in the
@@ -185,22 +124,6 @@ __device__ __forceinline__ bool group_all(bool yes) {
       : "memory");
   return r != 0;
 }
-
-// Eight float32 values as three bf16 parts whose sum holds 24 bits, 16-byte groups `stride` apart.
-__device__ __forceinline__ void put_parts3(uint8_t* dst, uint32_t stride, F2* v) {
-#pragma unroll
-  for (int p = 0; p < 3; ++p) {
-    uint4 pk;
-    uint32_t* h = (uint32_t*)&pk;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      h[j] = bf2_pack(v[j]);
-      if (p < 2) v[j] = v[j] - bf2_unpack(h[j]);
-    }
-    *(uint4*)(dst + p * stride) = pk;
-  }
-}
-__device__ __forceinline__ float powd(float g, int n) { return n == 0 ? 1.f : expf((float)n * g); }
 
 struct Walk {  // one CTA's blocks: first, first + step, ..., n of them
   int64_t chain;
@@ -433,8 +356,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
     const float fh = (float)fd, fl = (float)(fd - (double)fh), sc = reversed ? P.scale : 1.f;
     for (int i = 0; i < z.n; ++i) {
       const int blk = z.first + i * z.step, b = i % K::DBL, n = i / K::DBL;
-      if (a.saves && (reversed ? (blk & 1) || blk == nblk - 1 : !(blk & 1)))
-        put_state(a.saves + (z.chain * chunks(P) + blk / 2) * DD);
+      if (a.saves) put_state(a.saves + (z.chain * nblk + blk) * DD);
       if (FWD) {
         if (i >= K::DBL && !wait(ctl, &ctl.s_free[b], n - 1, a.status)) break;
         uint8_t* s = sm + K::OFF_S + b * 2 * K::ST + cm_off(d0, e0 + c2, DP);
@@ -597,7 +519,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 // (B, T, H, D) activations with element strides s (batch, token, head) as boxes of 64 tokens x
 // 64 channels of one head, 128-byte swizzle; elements outside read as zero and are not written.
 // An axis of length 1 takes the row size as its stride (its own is never used).
-static bool make_map(CUtensorMap* m, const void* x, const AtlasDecayParams& p, const int64_t* s) {
+bool make_map(CUtensorMap* m, const void* x, const AtlasDecayParams& p, const int64_t* s) {
   auto enc = encode_fn();
   if (!enc) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)p.D, (cuuint64_t)p.H, (cuuint64_t)p.T, (cuuint64_t)p.B};
@@ -621,27 +543,27 @@ bool mappable(const AtlasDecayParams& p, const int64_t* s) {
 template <int DP, bool FWD>
 static cudaError_t launch(const CUtensorMap& q, const CUtensorMap& x, const CUtensorMap& y, const CUtensorMap& o,
                           const SeqArgs& a, bool reversed, cudaStream_t s) {
-  cudaError_t e = allow_smem<seq_kernel<DP, FWD>>(SMEM<DP>);
+  cudaError_t e = allow_smem<seq_kernel<DP, FWD>>(SEQ_SMEM<DP>);
   if (e != cudaSuccess) return e;
-  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums)), Cfg<DP>::NT, SMEM<DP>, s>>>(q, x, y, o, a, reversed);
+  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums)), Cfg<DP>::NT, SEQ_SMEM<DP>, s>>>(q, x, y, o, a, reversed);
   return cudaGetLastError();
 }
 
-// How many segments to cut a sequence into, and their blocks (even: a multiple of a saved
-// chunk).  In block times: a CTA an SM, `waves` of them; a split adds the sums' pass, at
-// about 0.6 of a full block's time, and two launches (about 8 blocks' time).
+// How many segments to cut a sequence into, and their blocks.  In block times: a CTA an SM,
+// rounds of them; a split adds the sums' pass, at about 0.5 of a full block's time, and two
+// launches (about 4 blocks' time).
 struct Split {
   int segs, blocks;
 };
 static Split split(const AtlasDecayParams& p) {
   const int nblk = (p.T + C - 1) / C;
   const int64_t n = chains(p), sms = 148;
-  Split best{1, (nblk + 1) / 2 * 2};
+  Split best{1, nblk};
   double cost = (double)((n + sms - 1) / sms) * nblk;
-  for (int k = 2; k <= 64 && k <= nblk / 2; ++k) {
-    const int len = ((nblk + k - 1) / k + 1) / 2 * 2, segs = (nblk + len - 1) / len;
+  for (int k = 2; k <= 64 && k <= nblk; ++k) {
+    const int len = (nblk + k - 1) / k, segs = (nblk + len - 1) / len;
     if (segs != k) continue;
-    const double c = (double)((n * k + sms - 1) / sms) * len + 0.6 * (double)((n * (k - 1) + sms - 1) / sms) * len + 8;
+    const double c = (double)((n * k + sms - 1) / sms) * len + 0.5 * (double)((n * (k - 1) + sms - 1) / sms) * len + 4;
     if (c < 0.95 * cost) cost = c, best = Split{k, len};
   }
   return best;
@@ -699,12 +621,11 @@ cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, flo
   q.segs = z.segs;
   q.seg_blocks = z.blocks;
   q.status = a.status;
-  if (saves) {  // a segment's entering state is that of its first chunk in the walk
-    const int per = z.blocks / 2;
+  if (saves) {  // a segment's entering state is that of its first block in the walk
     q.mid = saves;
     q.mid_pitch = chunks(p);
-    q.mid_first = bwd ? (int64_t)z.segs * per - 1 : 0;
-    q.mid_step = bwd ? -per : per;
+    q.mid_first = bwd ? (int64_t)z.segs * z.blocks - 1 : 0;
+    q.mid_step = bwd ? -z.blocks : z.blocks;
   } else {
     q.mid = mid;
     q.mid_pitch = z.segs - 1;

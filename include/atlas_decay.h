@@ -28,7 +28,7 @@
  * (states, dlog_decay) is kept to float32 accuracy by splitting float32 operands into three
  * bf16 parts.
  * Causality holds for finite inputs; an infinity or NaN in v or k of a token reaches the
- * outputs of its own 128-token chunk as well as those after it.
+ * outputs of its own 64-token chunk as well as those after it.
  *
  * Conventions (status codes, thread-local error string, stream as void*, caller-owned
  * device buffers) are those of atlas_scan.h.
@@ -57,7 +57,7 @@ typedef struct {
   int64_t q_stride[3], k_stride[3], v_stride[3];
 } AtlasDecayParams;
 
-/* Bytes of the forward's `saved` buffer: the state entering every 128-token chunk
+/* Bytes of the forward's `saved` buffer: the state entering every 64-token chunk
  * (0 on invalid params, with the message set, and for empty problems). */
 size_t atlas_decay_saved_bytes(const AtlasDecayParams* p);
 

@@ -37,11 +37,11 @@ def test_decay_sizes():
     from atlas_b200.decay_attention import _lib
     lib = _lib()
     p = _decay()
-    # the state entering each of ceil(300 / 128) chunks
-    assert lib.atlas_decay_saved_bytes(ctypes.byref(p)) == 2 * 3 * 3 * 64 * 64 * 4
-    assert lib.atlas_decay_bwd_workspace_bytes(ctypes.byref(p)) >= 2 * 3 * 3 * 64 * 64 * 4
+    # the state entering each of ceil(300 / 64) chunks
+    assert lib.atlas_decay_saved_bytes(ctypes.byref(p)) == 2 * 3 * 5 * 64 * 64 * 4
+    assert lib.atlas_decay_bwd_workspace_bytes(ctypes.byref(p)) >= 2 * 3 * 5 * 64 * 64 * 4
     # without 16-byte alignment the forward keeps every chunk's state
-    assert lib.atlas_decay_fwd_workspace_bytes(ctypes.byref(_decay(aligned=0))) == 2 * 3 * 3 * 64 * 64 * 4
+    assert lib.atlas_decay_fwd_workspace_bytes(ctypes.byref(_decay(aligned=0))) == 2 * 3 * 5 * 64 * 64 * 4
     assert lib.atlas_decay_saved_bytes(ctypes.byref(_decay(T=0))) == 0 and lib.atlas_last_error_string() == b""
 
 
