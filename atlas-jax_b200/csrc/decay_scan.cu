@@ -15,7 +15,7 @@
 //     4 warps       scores: A from TMEM, decayed, masked, rounded to bf16
 //     4 warps       outputs: O and QS from TMEM, y through shared memory and a TMA store
 //     8 (16) warps  the state: dS from TMEM, S in registers, two bf16 parts of S for QS
-//     one warp      issues the MMAs;  one warp issues the TMA loads of q, k, v
+//     3 warps       issue the MMAs;  one warp issues the TMA loads of q, k, v
 //
 // The same kernel without q's side gives the states alone: the sums of a segment (first
 // pass of a split sequence), and with (q, scale dy, l^(t+1)) for (k, v, l^(L-1-s)) and the blocks
@@ -47,8 +47,8 @@ struct Cfg {
   static constexpr int DBL = DP == 64 ? 2 : 1;          // buffers of k', scores, S and the accumulators
   static constexpr int KWARPS = DP == 64 ? 8 : 4;       // warps of the k' group
   static constexpr int SWARPS = DP == 64 ? 8 : 16;      // warps of the state group
-  static constexpr int NT = 32 * (KWARPS + 10 + SWARPS);
-  static constexpr int W_P = KWARPS, W_Y = W_P + 4, W_S = W_Y + 4, W_MMA = W_S + SWARPS;  // first warps of the groups
+  static constexpr int NT = 32 * (KWARPS + 12 + SWARPS);
+  static constexpr int W_P = KWARPS, W_Y = W_P + 4, W_S = W_Y + 4, W_MMA = W_S + SWARPS;  // first warps of the groups (MMA: three)
   static constexpr int PT = C * C * 2;                  // a tile of scores
   static constexpr int ST = DP * DP * 2;                // one part of a state
   static constexpr int OFF_KP = STAGES * 3 * TILE;
@@ -62,6 +62,7 @@ struct Cfg {
 };
 
 struct Ctl {
+  F2 w[2 * C];                       // w[C + lag] = (l^lag, l^(lag - 1)), clamped at exponent 0
   uint64_t full[3], empty[3];        // stages
   uint64_t a_full[2], a_free[2];     // A in TMEM
   uint64_t kp_full[2], kp_free[2];   // k' parts
@@ -97,15 +98,20 @@ __device__ __forceinline__ float* mid_state(const SeqArgs& a, int64_t chain, int
 }
 
 // Waits for completion number n (from 0) of a barrier.  Bounded; a timeout anywhere in the
-// CTA is recorded and lets every group leave its loop.
-__device__ __forceinline__ bool wait(Ctl& c, uint64_t* bar, int n, int* status) {
+// CTA is recorded and lets every group leave its loop.  Only the first poll is inline: the
+// groups share the schedulers' instruction caches, and their loops together are about as
+// large as those (unrolled further, the kernel ran 20 to 40 % longer).
+__device__ __noinline__ bool wait_on(Ctl& c, uint64_t* bar, uint32_t parity, int* status) {
   for (uint32_t i = 0; i < 4000000u; ++i) {
-    if (mbar_try_wait(bar, (uint32_t)n & 1)) return true;
+    if (mbar_try_wait(bar, parity)) return true;
     if ((i & 15) == 15 && c.bad) return false;
   }
   c.bad = 1;
   set_status(status, ATLAS_ERR_DEVICE_TIMEOUT);
   return false;
+}
+__device__ __forceinline__ bool wait(Ctl& c, uint64_t* bar, int n, int* status) {
+  return mbar_try_wait(bar, (uint32_t)n & 1) || wait_on(c, bar, (uint32_t)n & 1, status);
 }
 // one arrival for a whole warp, after its shared-memory writes / TMEM reads
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
@@ -165,7 +171,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < K::STAGES; ++i) {
       mbar_init(&ctl.full[i], 1);
-      mbar_init(&ctl.empty[i], 1 + K::KWARPS);  // the last MMA, and the warps that read k
+      mbar_init(&ctl.empty[i], (FWD ? 3 : 1) + K::KWARPS);  // the issuing warps' last MMAs, and the warps that read k
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.a_full[i], 1);
@@ -174,17 +180,18 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
       mbar_init(&ctl.kp_free[i], 1);
       mbar_init(&ctl.p_full[i], 4);
       mbar_init(&ctl.p_free[i], 1);
-      mbar_init(&ctl.o_full[i], 1);
+      mbar_init(&ctl.o_full[i], 2);  // O and QS
       mbar_init(&ctl.o_free[i], 4);
       mbar_init(&ctl.ds_full[i], 1);
       mbar_init(&ctl.ds_free[i], K::SWARPS);
       mbar_init(&ctl.s_full[i], K::SWARPS);
       mbar_init(&ctl.s_free[i], 1);
     }
-    mbar_init(&ctl.fin, 1);
+    mbar_init(&ctl.fin, FWD ? 3 : 1);
     ctl.bad = 0;
     fence_mbar_init();
   }
+  for (int u = threadIdx.x; u < 2 * C; u += K::NT) ctl.w[u] = f2(powd(g, max(u - C, 0)), powd(g, max(u - C - 1, 0)));
   if (FWD)  // score blocks above the diagonal are written here once and never again
     for (int u = threadIdx.x; u < K::DBL * K::PT / 16; u += K::NT) *(uint4*)(sm + K::OFF_P + u * 16) = make_uint4(0, 0, 0, 0);
   fence_async_smem();
@@ -207,7 +214,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
       const F2 w2 = f2(wr, wr);
       const uint8_t* x = sm + (st * 3 + 1) * K::TILE + r * 128;
       uint8_t* kp = sm + K::OFF_KP + b * 3 * K::TILE + cm_off(r, 0, DP);
-#pragma unroll 2
+#pragma unroll 1
       for (int jj = 0; jj < DP / 8 / KP; ++jj) {
         const int j = first + KP * jj;
         const uint4 pk = *(const uint4*)(x + (j >> 3) * BOX + (((j & 7) ^ (r & 7)) << 4));
@@ -225,39 +232,38 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
     // ---- scores ----
     if (FWD) {
       const int q = w & 3, r = lane >> 2, c2 = 2 * (lane & 3), t0 = 16 * q + r;
-      // l^(t - s) of this thread's entries: row t0 at the column pair of block j, which is row
-      // t0 + 8 at that of block j + 1
-      F2 W[9];
-#pragma unroll
-      for (int j = 0; j < 9; ++j) W[j] = f2(powd(g, max(0, t0 - (8 * (j - 1) + c2))), powd(g, max(0, t0 - (8 * (j - 1) + c2 + 1))));
       uint8_t* prow = sm + K::OFF_P + cm_off(t0, c2, C);
       for (int i = 0; i < z.n; ++i) {
         const int b = i % K::DBL, n = i / K::DBL;
         if (!wait(ctl, &ctl.a_full[b], n, a.status)) break;
-        fence_after();
-        float v[32];
-        tmem_frag64(tm + K::T_A + 64 * b + ((uint32_t)(32 * q) << 16), v);
-        tmem_wait_ld();
-        fence_before();
-        warp_arrive(&ctl.a_free[b]);
         if (i >= K::DBL && !wait(ctl, &ctl.p_free[b], n - 1, a.status)) break;
-        uint8_t* p = prow + b * K::PT;
+        fence_after();
+#pragma unroll 1
+        for (int hc = 0; hc < 2; ++hc) {  // 32 columns; those beyond the warp's diagonal stay zero
+          if (2 * hc <= q) {
+            float v[16];
+            tmem_frag32(tm + K::T_A + 64 * b + 32 * hc + ((uint32_t)(32 * q) << 16), v);
+            tmem_wait_ld();
+            uint8_t* p = prow + b * K::PT + hc * 512;
+            int lag = t0 - (32 * hc + c2);  // of the first column of block j = 0, row t0
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j <= 2 * q + 1) {  // 8-column blocks that reach the diagonal or lie below it
-            F2 e = f2(v[4 * j], v[4 * j + 1]) * W[j + 1], f = f2(v[4 * j + 2], v[4 * j + 3]) * W[j];
-            if (j >= 2 * q) {  // the two diagonal blocks: keep s <= t
-              const int d0 = t0 - (8 * j + c2), d1 = d0 + 8;
-              const float2 x = f2_get(e), y = f2_get(f);
-              e = f2(d0 >= 0 ? x.x : 0.f, d0 >= 1 ? x.y : 0.f);
-              f = f2(d1 >= 0 ? y.x : 0.f, d1 >= 1 ? y.y : 0.f);
+            for (int j = 0; j < 4; ++j, lag -= 8) {
+              // masked entries are dropped, not multiplied by 0
+              const F2 m = f2(lag >= 0 ? v[4 * j] : 0.f, lag >= 1 ? v[4 * j + 1] : 0.f);
+              const F2 o = f2(lag >= -8 ? v[4 * j + 2] : 0.f, lag >= -7 ? v[4 * j + 3] : 0.f);
+              const F2* wt = ctl.w + lag + C;
+              *(uint32_t*)(p + j * 128) = bf2_pack(m * wt[0]);
+              *(uint32_t*)(p + C * 16 + j * 128) = bf2_pack(o * wt[8]);  // 8 rows on
             }
-            *(uint32_t*)(p + j * 128) = bf2_pack(e);
-            *(uint32_t*)(p + C * 16 + j * 128) = bf2_pack(f);  // 8 rows on
           }
         }
+        fence_before();
         fence_async_smem();
-        warp_arrive(&ctl.p_full[b]);
+        __syncwarp();
+        if (lane == 0) {
+          arrive(&ctl.a_free[b]);
+          arrive(&ctl.p_full[b]);
+        }
       }
     }
   } else if (w < K::W_S) {
@@ -286,7 +292,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
           }
           uint8_t* y = sm + K::OFF_Y + (DP == 64 ? (i & 1) * BOX : 0) + t0 * 128 + 2 * c2;
           const uint32_t at = tm + ((uint32_t)(32 * q) << 16) + b * DP + 64 * hb;
-#pragma unroll
+#pragma unroll 1
           for (int hc = 0; hc < 2; ++hc) {  // 32 columns
             float v[16], x[16];
             tmem_frag32(at + K::T_O + 32 * hc, v);
@@ -400,81 +406,91 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
       put_state(mid_state(a, z.chain, z.seg + 1));
     else if (a.out && z.seg == a.segs - 1)
       put_state(a.out + z.chain * DD);
-  } else if (w == K::W_MMA) {
+  } else if (w < K::W_MMA + 3) {
     // ---- MMAs ----
+    // Issuing blocks while the tensor pipe is busy, and a wait costs its latency even when it
+    // is over at once; with one warp for all of them the pipe idled through every wait.
     // Descriptors step through a tile by adding to their start address (bytes / 16).
     const uint32_t base = smem_u32(sm);
     const uint32_t tmu = __shfl_sync(0xffffffffu, tm, 0);
     auto tile = [&](int i, int which) { return base + ((i % K::STAGES) * 3 + which) * K::TILE; };
-    auto scores = [&](int i) {  // A = Q K^T
-      const uint32_t id = idesc_bf16(64, 64, false, false), d = tmu + K::T_A + 64 * (i % K::DBL);
-      const uint64_t q = desc_tile(tile(i, 0)), k = desc_tile(tile(i, 1));
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        const uint64_t o = ((ks >> 2) * BOX + (ks & 3) * 32) / 16;
-        mma_kf16(d, q + o, k + o, id, ks > 0);
-      }
-      mma_commit(&ctl.a_full[i % K::DBL]);
-    };
-    auto sums = [&](int i) {  // dS = K'^T V
+    if (w == K::W_MMA) {  // dS = K'^T V
       const uint32_t id = idesc_bf16(DP, DP, true, true);
-      const uint64_t v = desc_tile_mn(tile(i, 2));
-      const uint64_t kp = desc_mnmajor(base + K::OFF_KP + (i % K::DBL) * 3 * K::TILE, DP);
+      for (int i = 0; i < z.n; ++i) {
+        const int b = i % K::DBL, n = i / K::DBL;
+        if (!(wait(ctl, &ctl.full[i % K::STAGES], i / K::STAGES, a.status) && wait(ctl, &ctl.kp_full[b], n, a.status) &&
+              (i < K::DBL || wait(ctl, &ctl.ds_free[b], n - 1, a.status))))
+          break;
+        fence_after();
+        const uint64_t v = desc_tile_mn(tile(i, 2)), kp = desc_mnmajor(base + K::OFF_KP + b * 3 * K::TILE, DP);
+#pragma unroll 1
+        for (int p = 2; p >= 0; --p)  // small parts first: each step truncates to the accumulator's exponent
 #pragma unroll
-      for (int p = 2; p >= 0; --p)  // small parts first: each step truncates to the accumulator's exponent
+          for (int ks = 0; ks < C / 16; ++ks)
+            mma_kf16(tmu + K::T_DS + b * DP, kp + (p * K::TILE + ks * DP * 32) / 16, v + ks * (2048 / 16), id,
+                     p < 2 || ks > 0);
+        mma_commit(&ctl.kp_free[b]);
+        mma_commit(&ctl.ds_full[b]);
+        mma_commit(&ctl.empty[i % K::STAGES]);
+      }
+    } else if (FWD && w == K::W_MMA + 1) {  // A = Q K^T of the next block, O = P V
+      const uint32_t id = idesc_bf16(64, 64, false, false), ido = idesc_bf16(64, DP, false, true);
+      auto scores = [&](int i) {
+        const uint64_t q = desc_tile(tile(i, 0)), k = desc_tile(tile(i, 1));
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          const uint64_t o = ((ks >> 2) * BOX + (ks & 3) * 32) / 16;
+          mma_kf16(tmu + K::T_A + 64 * (i % K::DBL), q + o, k + o, id, ks > 0);
+        }
+        mma_commit(&ctl.a_full[i % K::DBL]);
+      };
+      bool ok = wait(ctl, &ctl.full[0], 0, a.status);
+      if (ok) scores(0);
+      for (int i = 0; i < z.n && ok; ++i) {
+        const int b = i % K::DBL, n = i / K::DBL;
+        if (i + 1 < z.n) {
+          const int b1 = (i + 1) % K::DBL;
+          ok = wait(ctl, &ctl.full[(i + 1) % K::STAGES], (i + 1) / K::STAGES, a.status) &&
+               (i + 1 < K::DBL || wait(ctl, &ctl.a_free[b1], (i + 1) / K::DBL - 1, a.status));
+          if (!ok) break;
+          fence_after();
+          scores(i + 1);
+        }
+        ok = wait(ctl, &ctl.p_full[b], n, a.status) && (i < K::DBL || wait(ctl, &ctl.o_free[b], n - 1, a.status));
+        if (!ok) break;
+        fence_after();
+        const uint64_t v = desc_tile_mn(tile(i, 2)), pt = desc_kmajor(base + K::OFF_P + b * K::PT, C);
 #pragma unroll
         for (int ks = 0; ks < C / 16; ++ks)
-          mma_kf16(tmu + K::T_DS + (i % K::DBL) * DP, kp + (p * K::TILE + ks * DP * 32) / 16, v + ks * (2048 / 16), id, p < 2 || ks > 0);
-      mma_commit(&ctl.kp_free[i % K::DBL]);
-      mma_commit(&ctl.ds_full[i % K::DBL]);
-    };
-    bool ok = true;
-    if (FWD) {
-      ok = wait(ctl, &ctl.full[0], 0, a.status);
-      if (ok) scores(0);
-    }
-    for (int i = 0; i < z.n && ok; ++i) {
-      const int b = i % K::DBL, n = i / K::DBL;
-      if (FWD && i + 1 < z.n) {
-        const int b1 = (i + 1) % K::DBL;
-        ok = wait(ctl, &ctl.full[(i + 1) % K::STAGES], (i + 1) / K::STAGES, a.status) &&
-             (i + 1 < K::DBL || wait(ctl, &ctl.a_free[b1], (i + 1) / K::DBL - 1, a.status));
-        if (!ok) break;
-        fence_after();
-        scores(i + 1);
+          mma_kf16(tmu + K::T_O + b * DP, pt + ks * (256 / 16), v + ks * (2048 / 16), ido, ks > 0);
+        mma_commit(&ctl.p_free[b]);
+        mma_commit(&ctl.o_full[b]);
+        mma_commit(&ctl.empty[i % K::STAGES]);
       }
-      ok = (FWD || wait(ctl, &ctl.full[i % K::STAGES], i / K::STAGES, a.status)) &&
-           wait(ctl, &ctl.kp_full[b], n, a.status) && (i < K::DBL || wait(ctl, &ctl.ds_free[b], n - 1, a.status));
-      if (!ok) break;
-      fence_after();
-      sums(i);
-      if (FWD) {
-        ok = wait(ctl, &ctl.s_full[b], n, a.status) && (i < K::DBL || wait(ctl, &ctl.o_free[b], n - 1, a.status));
-        if (!ok) break;
+    } else if (FWD) {  // QS
+      const uint32_t id = idesc_bf16(64, DP, false, true);
+      for (int i = 0; i < z.n; ++i) {
+        const int b = i % K::DBL, n = i / K::DBL;
+        if (!(wait(ctl, &ctl.full[i % K::STAGES], i / K::STAGES, a.status) && wait(ctl, &ctl.s_full[b], n, a.status) &&
+              (i < K::DBL || wait(ctl, &ctl.o_free[b], n - 1, a.status))))
+          break;
         fence_after();
-        const uint32_t id = idesc_bf16(64, DP, false, true);
         const uint64_t q = desc_tile(tile(i, 0)), S = desc_mnmajor(base + K::OFF_S + b * 2 * K::ST, DP);
-#pragma unroll
+#pragma unroll 1
         for (int p = 1; p >= 0; --p)
 #pragma unroll
           for (int ks = 0; ks < DP / 16; ++ks)
             mma_kf16(tmu + K::T_QS + b * DP, q + ((ks >> 2) * BOX + (ks & 3) * 32) / 16,
                      S + (p * K::ST + ks * DP * 32) / 16, id, p < 1 || ks > 0);
         mma_commit(&ctl.s_free[b]);
-        ok = wait(ctl, &ctl.p_full[b], n, a.status);
-        if (!ok) break;
-        fence_after();
-        const uint64_t v = desc_tile_mn(tile(i, 2)), pt = desc_kmajor(base + K::OFF_P + b * K::PT, C);
-#pragma unroll
-        for (int ks = 0; ks < C / 16; ++ks)
-          mma_kf16(tmu + K::T_O + b * DP, pt + ks * (256 / 16), v + ks * (2048 / 16), id, ks > 0);
-        mma_commit(&ctl.p_free[b]);
         mma_commit(&ctl.o_full[b]);
+        mma_commit(&ctl.empty[i % K::STAGES]);
       }
-      mma_commit(&ctl.empty[i % K::STAGES]);
     }
-    mma_commit(&ctl.fin);  // nothing of this CTA is in flight on the tensor core when its TMEM is freed
-    wait(ctl, &ctl.fin, 0, a.status);
+    if (FWD || w == K::W_MMA) {
+      mma_commit(&ctl.fin);  // nothing of this CTA is in flight on the tensor core when its TMEM is freed
+      wait(ctl, &ctl.fin, 0, a.status);
+    }
   } else if (lane == 0) {
     // ---- loads ----
     int i = 0;
