@@ -12,8 +12,8 @@
 //
 // Blocks are independent: one CTA each.  q, k, v, dy arrive by TMA and leave as dq, dk, dv
 // through the same tiles; S and R are split into three bf16 parts (dlog_decay is a float32
-// output; dv needs two of R's).  All accumulators have M = 64 (decay_tc.cuh); warp w reads
-// lane quadrant w % 4 and the column half w / 4.
+// output; dv needs two of R's).  All accumulators have M = 64 (decay_tc.cuh); warp w of
+// 16 reads lane quadrant w % 4 and the column quarter w / 4.
 //
 // D <= 64: two rounds of MMAs (A, B, O S^T, V R^T, then K R, dA K, dA^T Q, P^T O in the same
 // 256 TMEM columns), 97 KB of shared memory: two CTAs share an SM, and one's loads and
@@ -26,6 +26,8 @@
 namespace atlas {
 namespace decay {
 namespace tcore {
+
+constexpr int NT = 512;
 
 template <int DP>
 struct GCfg {
@@ -41,7 +43,7 @@ struct GCfg {
 };
 struct GCtl {
   float pw[C + 1];
-  float red[8];
+  float red[NT / 32];
   uint64_t loaded, done;
   uint32_t tmem;
   volatile int bad;
@@ -77,16 +79,16 @@ __device__ __forceinline__ void mma_steps(uint32_t d, uint64_t A, uint64_t sa, u
 }
 template <int NV>
 __device__ __forceinline__ void frag(uint32_t addr, float* v) {
-  if constexpr (NV == 16)
-    tmem_frag32(addr, v);
+  if constexpr (NV == 8)
+    tmem_frag16(addr, v);
   else
-    tmem_frag64(addr, v);
+    tmem_frag32(addr, v);
 }
 
 template <int DP>
-__global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __grid_constant__ Maps maps, const Args a) {
+__global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __grid_constant__ Maps maps, const Args a) {
   using G = GCfg<DP>;
-  constexpr int NV = DP / 4;  // values of an output fragment: 2 rows x DP / 8 columns of a thread
+  constexpr int CW = DP / 4, NV = CW / 2;  // columns of a warp; values of a thread's fragment: 2 rows x CW / 4 columns
   extern __shared__ uint8_t raw[];
   uint8_t* sm = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   GCtl& ctl = *(GCtl*)(sm + G::OFF_CTL);
@@ -137,24 +139,22 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __gr
     rs += t.x + t.y;
   };
   uint8_t* parts = sm + G::OFF_PARTS;
+  constexpr int NU = DP * DP / 8 / NT;  // groups of 8 of a state a thread
+  F2 x[NU][4];
   if constexpr (DP == 64) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int u = tid + 256 * i;
-      F2 x[4], y[4];
-      load8(Sg, u, x);
-      load8(Rg, u, y);
-      dot8(x, y);
-      put_parts3(parts + u * 16, G::ST, x);
-      put_parts3(parts + 3 * G::ST + u * 16, G::ST, y);
-    }
+    F2 y[4];
+    load8(Sg, tid, x[0]);
+    load8(Rg, tid, y);
+    dot8(x[0], y);
+    put_parts3(parts + tid * 16, G::ST, x[0]);
+    put_parts3(parts + 3 * G::ST + tid * 16, G::ST, y);
   } else {
-#pragma unroll 2
-    for (int i = 0; i < DP * DP / 8 / 256; ++i) {
-      const int u = tid + 256 * i;
-      F2 x[4];
-      load8(Sg, u, x);
-      put_parts3(parts + u * 16, G::ST, x);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) load8(Sg, tid + NT * i, x[i]);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      F2 y[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
+      put_parts3(parts + (tid + NT * i) * 16, G::ST, y);
     }
   }
   fence_async_smem();
@@ -190,19 +190,22 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __gr
       mma_commit(&ctl.done);
     }
     __syncwarp();
+    if constexpr (DP != 64) {  // R, while the products with S run
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        F2 y[4];
+        load8(Rg, tid + NT * i, y);
+        dot8(x[i], y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][j] = y[j];
+      }
+    }
     ok = wait_all(ctl, &ctl.done, phase, a.status);
     phase ^= 1;
   }
   if (DP != 64 && ok) {  // the parts of R in the place of S's
-#pragma unroll 2
-    for (int i = 0; i < DP * DP / 8 / 256; ++i) {
-      const int u = tid + 256 * i;
-      F2 x[4], y[4];
-      load8(Sg, u, x);
-      load8(Rg, u, y);
-      dot8(x, y);
-      put_parts3(parts + u * 16, G::ST, y);
-    }
+#pragma unroll
+    for (int i = 0; i < NU; ++i) put_parts3(parts + (tid + NT * i) * 16, G::ST, x[i]);
     fence_async_smem();
     cta_sync();
     if (w == 0) {
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __gr
       F2 s0 = f2(0.f, 0.f), s1 = s0;
 #pragma unroll
       for (int j = 0; j < NV / 4; ++j) {
-        const int col = hf * (DP / 2) + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
+        const int col = hf * CW + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
         const uint8_t* x = sm + which * G::TILE + bx * BOX + t0 * 128 + ((jj ^ r) << 4) + 2 * c2;
         s0 = fma2(bf2_unpack(*(const uint32_t*)x), v[2 * j], s0);
         s1 = fma2(bf2_unpack(*(const uint32_t*)(x + 8 * 128)), v[2 * j + 1], s1);
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __gr
       return f0 * (x.x + x.y) + f1 * (y.x + y.y);
     };
     float v[NV];
-    frag<NV>(at + G::T_OS + hf * (DP / 2), v);
+    frag<NV>(at + G::T_OS + hf * CW, v);
     tmem_wait_ld();
     const F2 i0 = f2(ctl.pw[t0 + 1], ctl.pw[t0 + 1]), i1 = f2(ctl.pw[t0 + 9], ctl.pw[t0 + 9]);
 #pragma unroll
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __gr
       dq[2 * j + 1] = i1 * f2(v[4 * j + 2], v[4 * j + 3]);
     }
     dg += P.scale * dot_rows(0, dq, (float)(t0 + 1), (float)(t0 + 9));
-    frag<NV>(at + G::T_VR + hf * (DP / 2), v);
+    frag<NV>(at + G::T_VR + hf * CW, v);
     tmem_wait_ld();
     const F2 o0 = f2(wo0, wo0), o1 = f2(wo1, wo1);
 #pragma unroll
@@ -252,21 +255,21 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __gr
     dg += dot_rows(1, dk, (float)max(L - 1 - t0, 0), (float)max(L - 9 - t0, 0));
     if (L > 0) dg += (float)L * ctl.pw[L] * rs;
     // scores
-    float x[16], y[16];
-    tmem_frag32(at + G::T_A + 32 * hf, x);
-    tmem_frag32(at + G::T_B + 32 * hf, y);
+    float xa[8], xb[8];
+    tmem_frag16(at + G::T_A + 16 * hf, xa);
+    tmem_frag16(at + G::T_B + 16 * hf, xb);
     tmem_wait_ld();
     F2 gl = f2(0.f, 0.f);
-    uint8_t* pt = sm + G::OFF_P + cm_off(t0, 32 * hf + c2, C);
+    uint8_t* pt = sm + G::OFF_P + cm_off(t0, 16 * hf + c2, C);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int lag = t0 + 8 * k - (32 * hf + 8 * j + c2);  // of the pair's first column
+        const int lag = t0 + 8 * k - (16 * hf + 8 * j + c2);  // of the pair's first column
         const float m0 = lag >= 0 ? ctl.pw[lag] : 0.f, m1 = lag >= 1 ? ctl.pw[lag - 1] : 0.f;
         // masked scores are dropped, not multiplied by 0
-        const F2 A = f2(lag >= 0 ? x[4 * j + 2 * k] : 0.f, lag >= 1 ? x[4 * j + 2 * k + 1] : 0.f);
-        const F2 B = f2(lag >= 0 ? y[4 * j + 2 * k] : 0.f, lag >= 1 ? y[4 * j + 2 * k + 1] : 0.f);
+        const F2 A = f2(lag >= 0 ? xa[4 * j + 2 * k] : 0.f, lag >= 1 ? xa[4 * j + 2 * k + 1] : 0.f);
+        const F2 B = f2(lag >= 0 ? xb[4 * j + 2 * k] : 0.f, lag >= 1 ? xb[4 * j + 2 * k + 1] : 0.f);
         const F2 M = f2(m0, m1), dA = M * B;
         gl = fma2(f2((float)lag, (float)(lag - 1)) * A, dA, gl);
         *(uint32_t*)(pt + k * C * 16 + j * 128) = bf2_pack(M * A);
@@ -294,29 +297,29 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __gr
     auto put = [&](int which, const F2* v) {
 #pragma unroll
       for (int j = 0; j < NV / 4; ++j) {
-        const int col = hf * (DP / 2) + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
+        const int col = hf * CW + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
         uint8_t* y = sm + which * G::TILE + bx * BOX + t0 * 128 + ((jj ^ r) << 4) + 2 * c2;
         *(uint32_t*)y = bf2_pack(v[2 * j]);
         *(uint32_t*)(y + 8 * 128) = bf2_pack(v[2 * j + 1]);
       }
     };
     float v[NV];
-    frag<NV>(at + G::T_DQ + hf * (DP / 2), v);
+    frag<NV>(at + G::T_DQ + hf * CW, v);
     tmem_wait_ld();
 #pragma unroll
     for (int j = 0; j < NV / 2; ++j) dq[j] = sc * (dq[j] + f2(v[2 * j], v[2 * j + 1]));
     put(0, dq);
-    frag<NV>(at + G::T_DK + hf * (DP / 2), v);
+    frag<NV>(at + G::T_DK + hf * CW, v);
     tmem_wait_ld();
 #pragma unroll
     for (int j = 0; j < NV / 2; ++j) dk[j] = fma2(sc, f2(v[2 * j], v[2 * j + 1]), dk[j]);
     put(1, dk);
-    frag<NV>(at + G::T_KR + hf * (DP / 2), v);
+    frag<NV>(at + G::T_KR + hf * CW, v);
     tmem_wait_ld();
     const F2 o0 = f2(wo0, wo0), o1 = f2(wo1, wo1);
 #pragma unroll
     for (int j = 0; j < NV / 2; ++j) dk[j] = (j & 1 ? o1 : o0) * f2(v[2 * j], v[2 * j + 1]);
-    frag<NV>(at + G::T_DV + hf * (DP / 2), v);
+    frag<NV>(at + G::T_DV + hf * CW, v);
     tmem_wait_ld();
 #pragma unroll
     for (int j = 0; j < NV / 2; ++j) dk[j] = fma2(sc, f2(v[2 * j], v[2 * j + 1]), dk[j]);
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) grads_kernel(const __gr
       }
       bulk_commit();
       float s = 0.f;
-      for (int i = 0; i < 8; ++i) s += ctl.red[i];
+      for (int i = 0; i < NT / 32; ++i) s += ctl.red[i];
       a.dg_part[blockIdx.x] = s;
       bulk_wait_read0();
     }
@@ -347,7 +350,7 @@ template <int DP>
 static cudaError_t launch(const Maps& m, const Args& a, cudaStream_t s) {
   cudaError_t e = allow_smem<grads_kernel<DP>>(GRAD_SMEM<DP>);
   if (e != cudaSuccess) return e;
-  grads_kernel<DP><<<(unsigned)(chains(a.p) * chunks(a.p)), 256, GRAD_SMEM<DP>, s>>>(m, a);
+  grads_kernel<DP><<<(unsigned)(chains(a.p) * chunks(a.p)), NT, GRAD_SMEM<DP>, s>>>(m, a);
   return cudaGetLastError();
 }
 

@@ -47,7 +47,13 @@ __device__ __forceinline__ void tmem_frag64(uint32_t addr, float* v) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
-// the same for 32 columns
+// the same for 16 and 32 columns
+__device__ __forceinline__ void tmem_frag16(uint32_t addr, float* v) {
+  uint32_t* r = (uint32_t*)v;
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
+}
 __device__ __forceinline__ void tmem_frag32(uint32_t addr, float* v) {
   uint32_t* r = (uint32_t*)v;
   asm volatile(
