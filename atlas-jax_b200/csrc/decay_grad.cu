@@ -15,10 +15,10 @@
 // output; dv needs two of R's).  All accumulators have M = 64 (decay_tc.cuh); warp w of
 // 16 reads lane quadrant w % 4 and the column quarter w / 4.
 //
-// D <= 64: two rounds of MMAs (A, B, O S^T, V R^T, then K R, dA K, dA^T Q, P^T O in the same
-// 256 TMEM columns), 97 KB of shared memory: two CTAs share an SM, and one's loads and
-// float32 work run during the other's MMAs.  D <= 128: the parts of S and R take turns in one
-// region and K R has columns of its own; one CTA an SM.
+// D <= 64: 256 TMEM columns (dA K, P^T O, dA^T Q and K R take the places of A, B, O S^T and
+// V R^T), 97 KB of shared memory: two CTAs share an SM, and one's loads and float32 work
+// run during the other's MMAs.  D <= 128: the parts of S and R take turns in one region and
+// K R has columns of its own; one CTA an SM.
 #include <algorithm>
 
 #include "decay_tc.cuh"
@@ -35,16 +35,16 @@ struct GCfg {
   static constexpr int OFF_PARTS = 4 * TILE;
   static constexpr int OFF_P = OFF_PARTS + (DP == 64 ? 6 : 3) * ST;
   static constexpr int OFF_CTL = OFF_P + 2 * PT;
-  // TMEM columns of the first round and of the second
+  // TMEM columns of A, B and the products with S and R, and of those that take their places
   static constexpr uint32_t COLS = DP == 64 ? 256 : 512;
   static constexpr uint32_t T_A = 0, T_B = 64, T_OS = 128, T_VR = 128 + DP;
-  static constexpr uint32_t T_KR = DP == 64 ? 0 : 384, T_DQ = DP == 64 ? 64 : 128, T_DK = DP == 64 ? 128 : 256,
-                            T_DV = DP == 64 ? 192 : 0;
+  static constexpr uint32_t T_DQ = DP == 64 ? 0 : 128, T_DV = DP == 64 ? 64 : 0, T_DK = DP == 64 ? 128 : 256,
+                            T_KR = DP == 64 ? 192 : 384;
 };
 struct GCtl {
   float pw[C + 1];
   float red[NT / 32];
-  uint64_t loaded, done;
+  uint64_t loaded, done[5];
   uint32_t tmem;
   volatile int bad;
 };
@@ -60,15 +60,14 @@ __device__ __forceinline__ void cta_sync() {
   __syncthreads();
   fence_after();
 }
-// every thread waits (bounded); false after a timeout, uniformly
-__device__ __forceinline__ bool wait_all(GCtl& c, uint64_t* bar, uint32_t parity, int* status) {
-  const bool ok = c.bad || mbar_wait(bar, parity, 4000000u);
-  if (!ok) {
+// Waits (bounded).  After a timeout the CTA goes through its remaining steps without waiting
+// and stores nothing.
+__device__ __forceinline__ void wait_for(GCtl& c, uint64_t* bar, int* status) {
+  if (!c.bad && !mbar_wait(bar, 0, 4000000u)) {
     set_status(status, ATLAS_ERR_DEVICE_TIMEOUT);
     c.bad = 1;
   }
-  cta_sync();
-  return !c.bad;
+  fence_after();
 }
 // one warp: D (+)= A B, descriptors stepping by sa and sb per 16 of K
 template <int N>
@@ -100,27 +99,7 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   const int q = w & 3, hf = w >> 2, r = lane >> 2, c2 = 2 * (lane & 3), t0 = 16 * q + r;
   const float g = a.log_decay[h];
   const uint32_t base = smem_u32(sm);
-  if (tid == 0) {
-    mbar_init(&ctl.loaded, 1);
-    mbar_init(&ctl.done, 1);
-    fence_mbar_init();
-    ctl.bad = 0;
-    const int nbox = D > 64 ? 2 : 1;
-    mbar_expect_tx(&ctl.loaded, (uint32_t)(4 * nbox * BOX));
-    for (int i = 0; i < nbox; ++i) {
-      tma_load(sm + i * BOX, &maps.q, 64 * i, h, c * C, b, &ctl.loaded);
-      tma_load(sm + G::TILE + i * BOX, &maps.k, 64 * i, h, c * C, b, &ctl.loaded);
-      tma_load(sm + 2 * G::TILE + i * BOX, &maps.v, 64 * i, h, c * C, b, &ctl.loaded);
-      tma_load(sm + 3 * G::TILE + i * BOX, &maps.o, 64 * i, h, c * C, b, &ctl.loaded);
-    }
-  }
-  if (w == 1) {
-    tmem_alloc(&ctl.tmem, G::COLS);
-    tmem_relinquish();
-  }
-  if (tid >= 64 && tid <= 64 + C) ctl.pw[tid - 64] = powd(g, tid - 64);
-
-  // S and R (float32, D x D) -> three parts each; <R, S>
+  // S and R (float32, D x D) -> three parts each; <R, S>.  Their loads go out first.
   const float* Sg = a.states + (int64_t)blockIdx.x * D * D;
   const float* Rg = a.dstates + (int64_t)blockIdx.x * D * D;
   float rs = 0.f;
@@ -141,16 +120,50 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   uint8_t* parts = sm + G::OFF_PARTS;
   constexpr int NU = DP * DP / 8 / NT;  // groups of 8 of a state a thread
   F2 x[NU][4];
-  if constexpr (DP == 64) {
-    F2 y[4];
-    load8(Sg, tid, x[0]);
-    load8(Rg, tid, y);
-    dot8(x[0], y);
-    put_parts3(parts + tid * 16, G::ST, x[0]);
-    put_parts3(parts + 3 * G::ST + tid * 16, G::ST, y);
-  } else {
+  F2 y0[4];
 #pragma unroll
-    for (int i = 0; i < NU; ++i) load8(Sg, tid + NT * i, x[i]);
+  for (int i = 0; i < NU; ++i) load8(Sg, tid + NT * i, x[i]);
+  if (DP == 64) load8(Rg, tid, y0);
+  if (tid == 0) {
+    mbar_init(&ctl.loaded, 1);
+    for (int i = 0; i < 5; ++i) mbar_init(&ctl.done[i], 1);
+    fence_mbar_init();
+    ctl.bad = 0;
+    const int nbox = D > 64 ? 2 : 1;
+    mbar_expect_tx(&ctl.loaded, (uint32_t)(4 * nbox * BOX));
+    for (int i = 0; i < nbox; ++i) {
+      tma_load(sm + i * BOX, &maps.q, 64 * i, h, c * C, b, &ctl.loaded);
+      tma_load(sm + G::TILE + i * BOX, &maps.k, 64 * i, h, c * C, b, &ctl.loaded);
+      tma_load(sm + 2 * G::TILE + i * BOX, &maps.v, 64 * i, h, c * C, b, &ctl.loaded);
+      tma_load(sm + 3 * G::TILE + i * BOX, &maps.o, 64 * i, h, c * C, b, &ctl.loaded);
+    }
+  }
+  // Into L2 for the CTA that will run here next: with its data on the way already, a CTA's first
+  // phase is short (two CTAs an SM hide only part of it).
+  const int64_t nb = (int64_t)blockIdx.x + (DP == 64 ? 2 : 1) * 148;
+  if (tid == 64 && nb < gridDim.x) {
+    const int64_t nchain = nb / nc;
+    const int nt = (int)(nb % nc) * C, nbat = (int)(nchain / P.H), nh = (int)(nchain % P.H);
+    for (int i = 0; i < (D > 64 ? 2 : 1); ++i) {
+      tma_prefetch(&maps.q, 64 * i, nh, nt, nbat);
+      tma_prefetch(&maps.k, 64 * i, nh, nt, nbat);
+      tma_prefetch(&maps.v, 64 * i, nh, nt, nbat);
+      tma_prefetch(&maps.o, 64 * i, nh, nt, nbat);
+    }
+    bulk_prefetch_l2(a.states + nb * D * D, D * D * 4);
+    bulk_prefetch_l2(a.dstates + nb * D * D, D * D * 4);
+  }
+  if (w == 1) {
+    tmem_alloc(&ctl.tmem, G::COLS);
+    tmem_relinquish();
+  }
+  if (tid >= 64 && tid <= 64 + C) ctl.pw[tid - 64] = powd(g, tid - 64);
+
+  if constexpr (DP == 64) {
+    dot8(x[0], y0);
+    put_parts3(parts + tid * 16, G::ST, x[0]);
+    put_parts3(parts + 3 * G::ST + tid * 16, G::ST, y0);
+  } else {
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       F2 y[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
@@ -159,15 +172,17 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   }
   fence_async_smem();
   cta_sync();
-  bool ok = wait_all(ctl, &ctl.loaded, 0, a.status);
   const uint32_t tm = ctl.tmem, tmu = __shfl_sync(0xffffffffu, tm, 0), at = tm + ((uint32_t)(32 * q) << 16);
   const uint64_t pd = desc_mnmajor(base + G::OFF_PARTS, DP), pk = desc_kmajor(base + G::OFF_PARTS, DP);
   constexpr uint64_t STEP_K = 256 / 16, STEP_MN = DP * 32 / 16, PART = G::ST / 16, TSTEP_MN = 2048 / 16;
   const uint32_t id_ss = idesc_bf16(64, 64, false, false), id_kk = idesc_bf16(64, DP, false, false),
                  id_kn = idesc_bf16(64, DP, false, true), id_nn = idesc_bf16(64, DP, true, true);
-  // X times a state's part: K-major X tile (boxes of 64 channels) and K- or MN-major part
+  const uint32_t tq = base, tk = base + G::TILE, tv = base + 2 * G::TILE, to = base + 3 * G::TILE;  // tiles
+  const uint32_t sp = base + G::OFF_P, sa = sp + G::PT;                                             // P, dA
+  // a tile (K-major, boxes of 64 channels) times a state's parts, K- or MN-major
   auto times_parts = [&](uint32_t d, uint32_t tile, uint64_t part0, bool mn, int np) {
     const uint64_t x = desc_tile(tile);
+#pragma unroll 1
     for (int p = np - 1; p >= 0; --p) {
 #pragma unroll
       for (int bx = 0; bx < G::NB; ++bx)
@@ -175,86 +190,40 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
                      mn ? id_kn : id_kk, p < np - 1 || bx > 0);
     }
   };
-  uint32_t phase = 0;
-  if (ok) {
-    if (w == 0) {
-      const uint64_t dq_ = desc_tile(base), dk_ = desc_tile(base + G::TILE), dv_ = desc_tile(base + 2 * G::TILE),
-                     do_ = desc_tile(base + 3 * G::TILE);
+  auto issue_dq = [&] { mma_steps<4>(tmu + G::T_DQ, desc_kmajor(sa, C), 256 / 16, desc_tile_mn(tk), TSTEP_MN, id_kn, false); };
+  auto issue_dk = [&] { mma_steps<4>(tmu + G::T_DK, desc_mnmajor(sa, C), C * 32 / 16, desc_tile_mn(tq), TSTEP_MN, id_nn, false); };
+  auto issue_dv = [&] { mma_steps<4>(tmu + G::T_DV, desc_mnmajor(sp, C), C * 32 / 16, desc_tile_mn(to), TSTEP_MN, id_nn, false); };
+
+  // The products are issued in the order in which their operands come, each step's float32 work
+  // running during the next one's MMAs:
+  //   A, B | products with S (and R) | scores | P and dA products that have room | the rest
+  if (w == 0) {
+    wait_for(ctl, &ctl.loaded, a.status);
 #pragma unroll
-      for (int bx = 0; bx < G::NB; ++bx) {
-        mma_steps<4>(tmu + G::T_A, dq_ + bx * (BOX / 16), 2, dk_ + bx * (BOX / 16), 2, id_ss, bx > 0);
-        mma_steps<4>(tmu + G::T_B, do_ + bx * (BOX / 16), 2, dv_ + bx * (BOX / 16), 2, id_ss, bx > 0);
-      }
-      times_parts(tmu + G::T_OS, base + 3 * G::TILE, pk, false, 3);  // O S^T
-      if (DP == 64) times_parts(tmu + G::T_VR, base + 2 * G::TILE, pk + 3 * PART, false, 3);  // V R^T
-      mma_commit(&ctl.done);
+    for (int bx = 0; bx < G::NB; ++bx) {
+      mma_steps<4>(tmu + G::T_A, desc_tile(tq + bx * BOX), 2, desc_tile(tk + bx * BOX), 2, id_ss, bx > 0);
+      mma_steps<4>(tmu + G::T_B, desc_tile(to + bx * BOX), 2, desc_tile(tv + bx * BOX), 2, id_ss, bx > 0);
     }
-    __syncwarp();
-    if constexpr (DP != 64) {  // R, while the products with S run
-#pragma unroll
-      for (int i = 0; i < NU; ++i) {
-        F2 y[4];
-        load8(Rg, tid + NT * i, y);
-        dot8(x[i], y);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] = y[j];
-      }
-    }
-    ok = wait_all(ctl, &ctl.done, phase, a.status);
-    phase ^= 1;
+    mma_commit(&ctl.done[0]);
+    times_parts(tmu + G::T_OS, to, pk, false, 3);                               // O S^T
+    if (DP == 64) times_parts(tmu + G::T_VR, tv, pk + 3 * PART, false, 3);      // V R^T
+    mma_commit(&ctl.done[1]);
   }
-  if (DP != 64 && ok) {  // the parts of R in the place of S's
+  __syncwarp();
+  if constexpr (DP != 64) {  // R, while the products with S run
 #pragma unroll
-    for (int i = 0; i < NU; ++i) put_parts3(parts + (tid + NT * i) * 16, G::ST, x[i]);
-    fence_async_smem();
-    cta_sync();
-    if (w == 0) {
-      times_parts(tmu + G::T_VR, base + 2 * G::TILE, pk, false, 3);
-      times_parts(tmu + G::T_KR, base + G::TILE, pd, true, 2);
-      mma_commit(&ctl.done);
+    for (int i = 0; i < NU; ++i) {
+      F2 y[4];
+      load8(Rg, tid + NT * i, y);
+      dot8(x[i], y);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i][j] = y[j];
     }
-    __syncwarp();
-    ok = wait_all(ctl, &ctl.done, phase, a.status);
-    phase ^= 1;
   }
   float dg = 0.f;
-  F2 dq[NV / 2], dk[NV / 2];  // [2 j]: row t0, columns 8 j + c2 and the next of this half; [2 j + 1]: row t0 + 8
-  const float wo0 = t0 < L ? ctl.pw[L - 1 - t0] : 0.f, wo1 = t0 + 8 < L ? ctl.pw[L - 9 - t0] : 0.f;
-  if (ok) {
-    // 8-byte-per-pair dot of rows t0 and t0 + 8 of a tile with a fragment
-    auto dot_rows = [&](int which, const F2* v, float f0, float f1) {
-      F2 s0 = f2(0.f, 0.f), s1 = s0;
-#pragma unroll
-      for (int j = 0; j < NV / 4; ++j) {
-        const int col = hf * CW + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
-        const uint8_t* x = sm + which * G::TILE + bx * BOX + t0 * 128 + ((jj ^ r) << 4) + 2 * c2;
-        s0 = fma2(bf2_unpack(*(const uint32_t*)x), v[2 * j], s0);
-        s1 = fma2(bf2_unpack(*(const uint32_t*)(x + 8 * 128)), v[2 * j + 1], s1);
-      }
-      const float2 x = f2_get(s0), y = f2_get(s1);
-      return f0 * (x.x + x.y) + f1 * (y.x + y.y);
-    };
-    float v[NV];
-    frag<NV>(at + G::T_OS + hf * CW, v);
-    tmem_wait_ld();
-    const F2 i0 = f2(ctl.pw[t0 + 1], ctl.pw[t0 + 1]), i1 = f2(ctl.pw[t0 + 9], ctl.pw[t0 + 9]);
-#pragma unroll
-    for (int j = 0; j < NV / 4; ++j) {
-      dq[2 * j] = i0 * f2(v[4 * j], v[4 * j + 1]);
-      dq[2 * j + 1] = i1 * f2(v[4 * j + 2], v[4 * j + 3]);
-    }
-    dg += P.scale * dot_rows(0, dq, (float)(t0 + 1), (float)(t0 + 9));
-    frag<NV>(at + G::T_VR + hf * CW, v);
-    tmem_wait_ld();
-    const F2 o0 = f2(wo0, wo0), o1 = f2(wo1, wo1);
-#pragma unroll
-    for (int j = 0; j < NV / 4; ++j) {
-      dk[2 * j] = o0 * f2(v[4 * j], v[4 * j + 1]);
-      dk[2 * j + 1] = o1 * f2(v[4 * j + 2], v[4 * j + 3]);
-    }
-    dg += dot_rows(1, dk, (float)max(L - 1 - t0, 0), (float)max(L - 9 - t0, 0));
-    if (L > 0) dg += (float)L * ctl.pw[L] * rs;
-    // scores
+  // ---- scores ----
+  wait_for(ctl, &ctl.done[0], a.status);
+  {
     float xa[8], xb[8];
     tmem_frag16(at + G::T_A + 16 * hf, xa);
     tmem_frag16(at + G::T_B + 16 * hf, xb);
@@ -266,83 +235,140 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int lag = t0 + 8 * k - (16 * hf + 8 * j + c2);  // of the pair's first column
-        const float m0 = lag >= 0 ? ctl.pw[lag] : 0.f, m1 = lag >= 1 ? ctl.pw[lag - 1] : 0.f;
+        const F2 M = f2(lag >= 0 ? ctl.pw[lag] : 0.f, lag >= 1 ? ctl.pw[lag - 1] : 0.f);
         // masked scores are dropped, not multiplied by 0
         const F2 A = f2(lag >= 0 ? xa[4 * j + 2 * k] : 0.f, lag >= 1 ? xa[4 * j + 2 * k + 1] : 0.f);
         const F2 B = f2(lag >= 0 ? xb[4 * j + 2 * k] : 0.f, lag >= 1 ? xb[4 * j + 2 * k + 1] : 0.f);
-        const F2 M = f2(m0, m1), dA = M * B;
+        const F2 dA = M * B;
         gl = fma2(f2((float)lag, (float)(lag - 1)) * A, dA, gl);
         *(uint32_t*)(pt + k * C * 16 + j * 128) = bf2_pack(M * A);
         *(uint32_t*)(pt + G::PT + k * C * 16 + j * 128) = bf2_pack(dA);
       }
     const float2 gg = f2_get(gl);
-    dg += P.scale * (gg.x + gg.y);
-    fence_async_smem();
+    dg = P.scale * (gg.x + gg.y);
+  }
+  if constexpr (DP != 64) {  // the parts of R in the place of S's
+    wait_for(ctl, &ctl.done[1], a.status);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) put_parts3(parts + (tid + NT * i) * 16, G::ST, x[i]);
+  }
+  fence_async_smem();
+  cta_sync();
+  if (w == 0) {
+    if (DP == 64) {
+      issue_dq();
+      issue_dv();
+    } else {
+      times_parts(tmu + G::T_VR, tv, pk, false, 3);
+      times_parts(tmu + G::T_KR, tk, pd, true, 2);
+      issue_dv();
+    }
+    mma_commit(&ctl.done[2]);
+  }
+  __syncwarp();
+  // ---- the terms with S and R ----
+  F2 dq[NV / 2], dk[NV / 2];  // [2 j]: row t0, columns 8 j + c2 and the next of this quarter; [2 j + 1]: row t0 + 8
+  const float wo0 = t0 < L ? ctl.pw[L - 1 - t0] : 0.f, wo1 = t0 + 8 < L ? ctl.pw[L - 9 - t0] : 0.f;
+  const F2 o0 = f2(wo0, wo0), o1 = f2(wo1, wo1);
+  // rows t0 and t0 + 8 of a tile . a fragment
+  auto dot_rows = [&](int which, const F2* v, float f0, float f1) {
+    F2 s0 = f2(0.f, 0.f), s1 = s0;
+#pragma unroll
+    for (int j = 0; j < NV / 4; ++j) {
+      const int col = hf * CW + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
+      const uint8_t* y = sm + which * G::TILE + bx * BOX + t0 * 128 + ((jj ^ r) << 4) + 2 * c2;
+      s0 = fma2(bf2_unpack(*(const uint32_t*)y), v[2 * j], s0);
+      s1 = fma2(bf2_unpack(*(const uint32_t*)(y + 8 * 128)), v[2 * j + 1], s1);
+    }
+    const float2 u = f2_get(s0), v1 = f2_get(s1);
+    return f0 * (u.x + u.y) + f1 * (v1.x + v1.y);
+  };
+  // fragment of columns `col` on, row t0 times f0, row t0 + 8 times f1
+  auto scaled = [&](uint32_t col, F2 f0, F2 f1, F2* v) {
+    float t[NV];
+    frag<NV>(at + col + hf * CW, t);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < NV / 2; ++j) v[j] = (j & 1 ? f1 : f0) * f2(t[2 * j], t[2 * j + 1]);
+  };
+  auto scaled_dk = [&] {
+    scaled(G::T_VR, o0, o1, dk);
+    dg += dot_rows(1, dk, (float)max(L - 1 - t0, 0), (float)max(L - 9 - t0, 0)) + (float)L * ctl.pw[L] * rs;
+  };
+  wait_for(ctl, &ctl.loaded, a.status);  // (long over: this thread is about to read the tiles itself)
+  wait_for(ctl, &ctl.done[1], a.status);
+  scaled(G::T_OS, f2(ctl.pw[t0 + 1], ctl.pw[t0 + 1]), f2(ctl.pw[t0 + 9], ctl.pw[t0 + 9]), dq);
+  dg += P.scale * dot_rows(0, dq, (float)(t0 + 1), (float)(t0 + 9));
+  if (DP == 64) scaled_dk();
+  cta_sync();
+  if (w == 0) {
+    if (DP == 64) {
+      issue_dk();
+      times_parts(tmu + G::T_KR, tk, pd + 3 * PART, true, 2);
+    } else {
+      issue_dq();
+    }
+    mma_commit(&ctl.done[3]);
+  }
+  __syncwarp();
+  wait_for(ctl, &ctl.done[2], a.status);
+  if (DP != 64) {
+    scaled_dk();
     cta_sync();
     if (w == 0) {
-      const uint32_t p0 = base + G::OFF_P, p1 = p0 + G::PT;
-      mma_steps<4>(tmu + G::T_DQ, desc_kmajor(p1, C), 256 / 16, desc_tile_mn(base + G::TILE), TSTEP_MN, id_kn, false);
-      mma_steps<4>(tmu + G::T_DK, desc_mnmajor(p1, C), C * 32 / 16, desc_tile_mn(base), TSTEP_MN, id_nn, false);
-      mma_steps<4>(tmu + G::T_DV, desc_mnmajor(p0, C), C * 32 / 16, desc_tile_mn(base + 3 * G::TILE), TSTEP_MN, id_nn, false);
-      if (DP == 64) times_parts(tmu + G::T_KR, base + G::TILE, pd + 3 * PART, true, 2);  // K R
-      mma_commit(&ctl.done);
+      issue_dk();
+      mma_commit(&ctl.done[4]);
     }
     __syncwarp();
-    ok = wait_all(ctl, &ctl.done, phase, a.status);
-    phase ^= 1;
+    wait_for(ctl, &ctl.done[3], a.status);
   }
-  if (ok) {
-    // outputs through the tiles of q, k and v, which nothing reads any more
-    const F2 sc = f2(P.scale, P.scale);
-    auto put = [&](int which, const F2* v) {
+  // ---- outputs, through tiles that no product reads any more ----
+  const F2 sc = f2(P.scale, P.scale);
+  auto put = [&](int which, const F2* v) {
 #pragma unroll
-      for (int j = 0; j < NV / 4; ++j) {
-        const int col = hf * CW + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
-        uint8_t* y = sm + which * G::TILE + bx * BOX + t0 * 128 + ((jj ^ r) << 4) + 2 * c2;
-        *(uint32_t*)y = bf2_pack(v[2 * j]);
-        *(uint32_t*)(y + 8 * 128) = bf2_pack(v[2 * j + 1]);
-      }
-    };
-    float v[NV];
-    frag<NV>(at + G::T_DQ + hf * CW, v);
-    tmem_wait_ld();
-#pragma unroll
-    for (int j = 0; j < NV / 2; ++j) dq[j] = sc * (dq[j] + f2(v[2 * j], v[2 * j + 1]));
-    put(0, dq);
-    frag<NV>(at + G::T_DK + hf * CW, v);
-    tmem_wait_ld();
-#pragma unroll
-    for (int j = 0; j < NV / 2; ++j) dk[j] = fma2(sc, f2(v[2 * j], v[2 * j + 1]), dk[j]);
-    put(1, dk);
-    frag<NV>(at + G::T_KR + hf * CW, v);
-    tmem_wait_ld();
-    const F2 o0 = f2(wo0, wo0), o1 = f2(wo1, wo1);
-#pragma unroll
-    for (int j = 0; j < NV / 2; ++j) dk[j] = (j & 1 ? o1 : o0) * f2(v[2 * j], v[2 * j + 1]);
-    frag<NV>(at + G::T_DV + hf * CW, v);
-    tmem_wait_ld();
-#pragma unroll
-    for (int j = 0; j < NV / 2; ++j) dk[j] = fma2(sc, f2(v[2 * j], v[2 * j + 1]), dk[j]);
-    put(2, dk);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dg += __shfl_xor_sync(0xffffffffu, dg, o);
-    if (lane == 0) ctl.red[w] = dg;
-    fence_async_smem();
-    cta_sync();
-    if (tid == 0) {
-      for (int i = 0; i < (D > 64 ? 2 : 1); ++i) {
-        tma_store(&maps.dq, 64 * i, h, c * C, b, sm + i * BOX);
-        tma_store(&maps.dk, 64 * i, h, c * C, b, sm + G::TILE + i * BOX);
-        tma_store(&maps.dv, 64 * i, h, c * C, b, sm + 2 * G::TILE + i * BOX);
-      }
-      bulk_commit();
-      float s = 0.f;
-      for (int i = 0; i < NT / 32; ++i) s += ctl.red[i];
-      a.dg_part[blockIdx.x] = s;
-      bulk_wait_read0();
+    for (int j = 0; j < NV / 4; ++j) {
+      const int col = hf * CW + 8 * j, bx = col >> 6, jj = (col >> 3) & 7;
+      uint8_t* y = sm + which * G::TILE + bx * BOX + t0 * 128 + ((jj ^ r) << 4) + 2 * c2;
+      *(uint32_t*)y = bf2_pack(v[2 * j]);
+      *(uint32_t*)(y + 8 * 128) = bf2_pack(v[2 * j + 1]);
     }
-  }
+  };
+  float v[NV];
+  frag<NV>(at + G::T_DQ + hf * CW, v);
+  tmem_wait_ld();
+#pragma unroll
+  for (int j = 0; j < NV / 2; ++j) dq[j] = sc * (dq[j] + f2(v[2 * j], v[2 * j + 1]));
+  put(3, dq);  // dy's tile: dV, its last reader, is done (done[2])
+  wait_for(ctl, &ctl.done[DP == 64 ? 3 : 4], a.status);
+  frag<NV>(at + G::T_DK + hf * CW, v);
+  tmem_wait_ld();
+#pragma unroll
+  for (int j = 0; j < NV / 2; ++j) dk[j] = fma2(sc, f2(v[2 * j], v[2 * j + 1]), dk[j]);
+  put(0, dk);
+  F2 dv[NV / 2];
+  scaled(G::T_KR, o0, o1, dv);
+  frag<NV>(at + G::T_DV + hf * CW, v);
+  tmem_wait_ld();
+#pragma unroll
+  for (int j = 0; j < NV / 2; ++j) dv[j] = fma2(sc, f2(v[2 * j], v[2 * j + 1]), dv[j]);
+  put(1, dv);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) dg += __shfl_xor_sync(0xffffffffu, dg, o);
+  if (lane == 0) ctl.red[w] = dg;
+  fence_async_smem();
   cta_sync();
+  if (tid == 0 && !ctl.bad) {
+    for (int i = 0; i < (D > 64 ? 2 : 1); ++i) {
+      tma_store(&maps.dq, 64 * i, h, c * C, b, sm + 3 * G::TILE + i * BOX);
+      tma_store(&maps.dk, 64 * i, h, c * C, b, sm + i * BOX);
+      tma_store(&maps.dv, 64 * i, h, c * C, b, sm + G::TILE + i * BOX);
+    }
+    bulk_commit();
+    float s = 0.f;
+    for (int i = 0; i < NT / 32; ++i) s += ctl.red[i];
+    a.dg_part[blockIdx.x] = s;
+    bulk_wait_read0();
+  }
   if (w == 1) tmem_dealloc(tm, G::COLS);
 }
 

@@ -35,6 +35,12 @@ __device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int h, 
                "r"(x), "r"(h), "r"(t), "r"(b), "r"(smem_u32(src))
                : "memory");
 }
+// a box into L2 ahead of its load
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map, int x, int h, int t, int b) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(x), "r"(h),
+               "r"(t), "r"(b)
+               : "memory");
+}
 // 16 lanes x 64 columns: v[4 j + 2 i + k] = row lane / 4 + 8 i, column 8 j + 2 (lane % 4) + k
 __device__ __forceinline__ void tmem_frag64(uint32_t addr, float* v) {
   uint32_t* r = (uint32_t*)v;
