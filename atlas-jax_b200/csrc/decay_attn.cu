@@ -441,31 +441,32 @@ __global__ void __launch_bounds__(256) dkv_kernel(Args a, int tiles) {
 // ---------------------------------------------------------------------------
 // recurrent form
 // ---------------------------------------------------------------------------
-// One CTA per (sequence, head, slice of 32 value columns): the columns of the state are
+// One CTA per (sequence, head, slice of SL value columns): the columns of the state are
 // independent, so a slice needs no exchange with the others.  Thread (row group rg, column
-// group cg) keeps rows rg, rg + 256 / CG, ... of VEC consecutive columns in registers from
-// the first token to the last; y's sum over rows goes through shared memory.
-template <typename TA, int VEC>
+// group cg) keeps rows rg, rg + RG, ... of VEC consecutive columns in registers from the
+// first token to the last; y's sum over rows goes through shared memory.  Bound by the state's
+// bytes where there are many sequences: SL = 64 then moves four 16-byte groups a thread
+// (DP = 64), 32 twice as many CTAs for few sequences.
+template <typename TA, int DP, int SL, int VEC>
 __global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, const int32_t* slots, int32_t n_slots,
                                                    float* out) {
-  constexpr int CG = 32 / VEC, RG = 256 / CG, NR = 128 / RG;  // column groups, row groups, rows a thread
-  __shared__ float red[RG / (32 / CG)][32 + 1], qs[128], ks[128];
+  constexpr int CG = SL / VEC, RG = 256 / CG, NR = DP / RG;  // column groups, row groups, rows a thread
+  static_assert(CG <= 32 && NR >= 1, "a warp holds whole rows of a slice");
+  __shared__ float red[8][SL + 1], qs[DP], ks[DP];
   const AtlasDecayParams& P = a.p;
-  const int D = P.D, slices = (D + 31) / 32;
-  const int64_t chain = blockIdx.x / slices;
-  const int sl = (int)(blockIdx.x % slices), b = (int)(chain / P.H), h = (int)(chain % P.H);
-  const int cg = threadIdx.x % CG, rg = threadIdx.x / CG, e0 = 32 * sl + cg * VEC;
+  const int D = P.D, slices = (D + SL - 1) / SL;
+  const int chain = blockIdx.x / slices, sl = blockIdx.x % slices, b = chain / P.H, h = chain % P.H;
+  const int cg = threadIdx.x % CG, rg = threadIdx.x / CG, e0 = SL * sl + cg * VEC;
   const int32_t row = slots ? slots[b] : b;
-  const bool idle = slots && (row < 0 || row >= n_slots);
   TA* y = (TA*)a.y + ((int64_t)b * P.T * P.H + h) * D;
-  if (idle) {
-    for (int u = threadIdx.x; u < P.T * 32; u += 256) {
-      const int t = u / 32, e = 32 * sl + u % 32;
+  if (slots && (row < 0 || row >= n_slots)) {  // idle
+    for (int u = threadIdx.x; u < P.T * SL; u += 256) {
+      const int t = u / SL, e = SL * sl + u % SL;
       if (e < D) st_act(y + (int64_t)t * P.H * D, (size_t)e, 0.f);
     }
     return;
   }
-  const int64_t off = ((int64_t)row * P.H + h) * D * D;
+  const int64_t off = ((int64_t)row * P.H + h) * D * D + rg * D + e0;
   const float l = pow_decay(a.log_decay[h], 1);
   const TA* q = (const TA*)a.q + b * P.q_stride[0] + h * P.q_stride[2];
   const TA* k = (const TA*)a.k + b * P.k_stride[0] + h * P.k_stride[2];
@@ -473,23 +474,21 @@ __global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, cons
   float S[NR][VEC];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    const int d = rg + i * RG;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) S[i][j] = 0.f;
-    if (in && d < D && e0 < D) {
+    if (in && rg + i * RG < D && e0 < D) {
       if constexpr (VEC == 4)
-        *(float4*)S[i] = *(const float4*)(in + off + (int64_t)d * D + e0);
+        *(float4*)S[i] = *(const float4*)(in + off + i * RG * D);
       else
-        S[i][0] = in[off + (int64_t)d * D + e0];
+        S[i][0] = in[off + i * RG * D];
     }
   }
   for (int t = 0; t < P.T; ++t) {
-    if (threadIdx.x < 128) {
-      qs[threadIdx.x] = threadIdx.x < D ? ld_act(q + t * P.q_stride[1], (size_t)threadIdx.x) : 0.f;
-    } else {
-      const int d = threadIdx.x - 128;
-      ks[d] = d < D ? ld_act(k + t * P.k_stride[1], (size_t)d) : 0.f;
-    }
+    if (threadIdx.x < DP)
+      qs[threadIdx.x] = (int)threadIdx.x < D ? ld_act(q + t * P.q_stride[1], (size_t)threadIdx.x) : 0.f;
+    else if (threadIdx.x < 2 * DP)
+      ks[threadIdx.x - DP] =
+          (int)threadIdx.x - DP < D ? ld_act(k + t * P.k_stride[1], (size_t)(threadIdx.x - DP)) : 0.f;
     float vv[VEC], acc[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
@@ -498,15 +497,12 @@ __global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, cons
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const int d = rg + i * RG;
-      if (d < D) {
-        const float kd = ks[d], qd = qs[d];
+    for (int i = 0; i < NR; ++i) {  // rows from D on: k = q = 0
+      const float kd = ks[rg + i * RG], qd = qs[rg + i * RG];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          S[i][j] = fmaf(l, S[i][j], kd * vv[j]);
-          acc[j] = fmaf(qd, S[i][j], acc[j]);
-        }
+      for (int j = 0; j < VEC; ++j) {
+        S[i][j] = fmaf(l, S[i][j], kd * vv[j]);
+        acc[j] = fmaf(qd, S[i][j], acc[j]);
       }
     }
     // rows of this warp (lanes CG apart), then warps through shared memory
@@ -519,22 +515,21 @@ __global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, cons
       for (int j = 0; j < VEC; ++j) red[threadIdx.x >> 5][cg * VEC + j] = acc[j];
     }
     __syncthreads();
-    if (threadIdx.x < 32) {
+    if (threadIdx.x < SL) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
-      const int e = 32 * sl + threadIdx.x;
+      const int e = SL * sl + threadIdx.x;
       if (e < D) st_act(y + (int64_t)t * P.H * D, (size_t)e, P.scale * s);
     }
   }
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    const int d = rg + i * RG;
-    if (d < D && e0 < D) {
+    if (rg + i * RG < D && e0 < D) {
       if constexpr (VEC == 4)
-        *(float4*)(out + off + (int64_t)d * D + e0) = *(const float4*)S[i];
+        *(float4*)(out + off + i * RG * D) = *(const float4*)S[i];
       else
-        out[off + (int64_t)d * D + e0] = S[i][0];
+        out[off + i * RG * D] = S[i][0];
     }
   }
 }
@@ -662,14 +657,20 @@ static cudaError_t pass_state(const AtlasDecayParams& p, const float* in, float*
   return in ? cudaMemcpyAsync(out, in, n, cudaMemcpyDeviceToDevice, s) : cudaMemsetAsync(out, 0, n, s);
 }
 
+template <typename TA, int DP, int SL, int VEC>
+static cudaError_t step_go(const Args& a, const float* in, const int32_t* slots, int32_t n, float* out, cudaStream_t s) {
+  step_kernel<TA, DP, SL, VEC><<<(unsigned)(chains(a.p) * ((a.p.D + SL - 1) / SL)), 256, 0, s>>>(a, in, slots, n, out);
+  return cudaGetLastError();
+}
+template <typename TA, int DP>
+static cudaError_t step_dp(const Args& a, const float* in, const int32_t* slots, int32_t n, float* out, cudaStream_t s) {
+  if (a.p.D % 4 != 0 || !aligned16(in) || !aligned16(out)) return step_go<TA, DP, 32, 1>(a, in, slots, n, out, s);
+  return chains(a.p) < 2 * 148 ? step_go<TA, DP, 32, 4>(a, in, slots, n, out, s)
+                               : step_go<TA, DP, 64, 4>(a, in, slots, n, out, s);
+}
 template <typename TA>
 static cudaError_t step_t(const Args& a, const float* in, const int32_t* slots, int32_t n, float* out, cudaStream_t s) {
-  const unsigned grid = (unsigned)(chains(a.p) * ((a.p.D + 31) / 32));
-  if (a.p.D % 4 == 0 && aligned16(in) && aligned16(out))
-    step_kernel<TA, 4><<<grid, 256, 0, s>>>(a, in, slots, n, out);
-  else
-    step_kernel<TA, 1><<<grid, 256, 0, s>>>(a, in, slots, n, out);
-  return cudaGetLastError();
+  return a.p.D <= 64 ? step_dp<TA, 64>(a, in, slots, n, out, s) : step_dp<TA, 128>(a, in, slots, n, out, s);
 }
 
 }  // namespace decay
