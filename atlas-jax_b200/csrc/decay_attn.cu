@@ -112,11 +112,20 @@ __global__ void __launch_bounds__(256) dg_kernel(Args a, float* dg) {
 // ---------------------------------------------------------------------------
 // float32 CUDA-core kernels (any D <= 128, strides and alignment; float32 activations)
 // ---------------------------------------------------------------------------
-// 256 threads as 16 x 16; thread (ty, tx) owns rows ty + 16 i and columns tx + 16 j of a
-// product, so its operands come from shared memory as broadcasts (rows) and consecutive
-// words (columns).  Token tiles are TT = 32 rows; NI = ceil(D / 16).
+// 256 threads as 16 x 16 over token tiles of TT = 32 rows in shared memory, D zero-padded to
+// DP.  Thread (ty, tx) owns rows ty and ty + 16 of a tile's product and NJ groups of VW
+// consecutive columns; it reads its operands as 16-byte groups (rows along the summed axis,
+// columns along the output), so a multiply-add costs a quarter of a shared-memory load or less.
 constexpr int TT = 32;
-constexpr int LD = 129;  // row pitch of the token tiles (odd: rows of one column differ in bank)
+constexpr int LP = TT + 4;  // row pitch of a tile of scores: 16-byte aligned rows
+
+template <int DP>
+struct Tile {
+  static constexpr int LD = DP + 4;  // row pitch: 16-byte aligned, 8 rows apart in different banks
+  static constexpr int VW = DP == 32 ? 2 : 4, NJ = DP / 16 / VW, NC = VW * NJ;  // columns of a thread
+  float x[TT][LD];
+  static __device__ __forceinline__ int col(int tx, int j) { return VW * tx + 16 * VW * j; }
+};
 
 struct View {
   const void* p;
@@ -127,125 +136,193 @@ __device__ __forceinline__ View flat(const void* p, const AtlasDecayParams& P) {
   return View{p, (int64_t)P.T * P.H * P.D, (int64_t)P.H * P.D, (int64_t)P.D};
 }
 
-// rows [t0, t0 + TT) of head (b, h) into a tile; rows from t_end on and columns from D on are 0
-template <typename TA>
-__device__ void load_rows(float (*tile)[LD], const View& x, int b, int h, int t0, int t_end, int D, int cols) {
+// rows [t0, t0 + TT) of head (b, h) into a tile; rows from t_end on and columns from D on are
+// 0.  vec: groups of four channels can be loaded at once.
+template <typename TA, int DP>
+__device__ void load_rows(Tile<DP>& tile, const View& x, int b, int h, int t0, int t_end, int D, bool vec) {
   const TA* base = (const TA*)x.p + b * x.sb + h * x.sh;
-  for (int u = threadIdx.x; u < TT * cols; u += 256) {
-    const int r = u / cols, c = u - r * cols, t = t0 + r;
-    tile[r][c] = (t < t_end && c < D) ? ld_act(base + (int64_t)t * x.st, (size_t)c) : 0.f;
+#pragma unroll
+  for (int i = 0; i < TT * DP / 4 / 256; ++i) {
+    const int u = threadIdx.x + 256 * i, r = u / (DP / 4), c = 4 * (u % (DP / 4)), t = t0 + r;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (t < t_end && c < D) {
+      const TA* p = base + (int64_t)t * x.st + c;
+      if (vec) {
+        if constexpr (sizeof(TA) == 4) {
+          *(float4*)v = *(const float4*)p;
+        } else {
+          const uint2 k = *(const uint2*)p;
+          const __nv_bfloat16* e = (const __nv_bfloat16*)&k;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = __bfloat162float(e[j]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < D) v[j] = ld_act(p, (size_t)j);
+      }
+    }
+    *(float4*)&tile.x[r][c] = *(const float4*)v;
+  }
+}
+// columns tx owns, of row r
+template <int DP>
+__device__ __forceinline__ void row_cols(float* v, const Tile<DP>& t, int r, int tx) {
+  using L = Tile<DP>;
+#pragma unroll
+  for (int j = 0; j < L::NJ; ++j) {
+    if constexpr (L::VW == 4)
+      *(float4*)(v + 4 * j) = *(const float4*)&t.x[r][L::col(tx, j)];
+    else
+      *(float2*)v = *(const float2*)&t.x[r][L::col(tx, j)];
   }
 }
 
-// per-chunk sums of weight * X^T Y (forward: k, v, l^(L-1-s); bwd: q, scale dy, l^(t+1))
-template <typename TA, int NI>
-__global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd) {
-  __shared__ float X[TT][LD], Y[TT][LD];
+// per-chunk sums of weight * X^T Y (forward: k, v, l^(L-1-s); bwd: q, scale dy, l^(t+1)).
+// Thread (ty, tx): rows NR ty + i and its columns.
+template <typename TA, int DP>
+__global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd, bool vec) {
+  using L = Tile<DP>;
+  constexpr int NR = DP / 16;
+  __shared__ L X, Y;
+  __shared__ float w[CH];
   const AtlasDecayParams& P = a.p;
   const int nc = chunks(P), D = P.D;
   const int64_t chain = blockIdx.x / nc;
   const int c = (int)(blockIdx.x % nc), b = (int)(chain / P.H), h = (int)(chain % P.H);
-  const int L = chunk_len(P, c), tc = c * CH;
+  const int len = chunk_len(P, c), tc = c * CH;
   const float g = a.log_decay[h];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const View xv = bwd ? view(a.q, P.q_stride) : view(a.k, P.k_stride);
   const View yv = bwd ? flat(a.dy, P) : view(a.v, P.v_stride);
-  float acc[NI][NI];
+  if (threadIdx.x < CH)
+    w[threadIdx.x] = bwd ? P.scale * pow_decay(g, threadIdx.x + 1)
+                         : (int)threadIdx.x < len ? pow_decay(g, len - 1 - threadIdx.x) : 0.f;
+  float acc[NR][L::NC];
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+  for (int i = 0; i < NR; ++i)
 #pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = 0.f;
-  for (int s0 = 0; s0 < L; s0 += TT) {
+    for (int j = 0; j < L::NC; ++j) acc[i][j] = 0.f;
+  for (int s0 = 0; s0 < len; s0 += TT) {
     __syncthreads();
-    load_rows<TA>(X, xv, b, h, tc + s0, tc + L, D, 16 * NI);
-    load_rows<TA>(Y, yv, b, h, tc + s0, tc + L, D, 16 * NI);
+    load_rows<TA>(X, xv, b, h, tc + s0, tc + len, D, vec);
+    load_rows<TA>(Y, yv, b, h, tc + s0, tc + len, D, vec);
     __syncthreads();
-    const int n = min(TT, L - s0);
-    for (int r = 0; r < n; ++r) {
-      const float w = bwd ? P.scale * pow_decay(g, s0 + r + 1) : pow_decay(g, L - 1 - s0 - r);
-      float xr[NI], yr[NI];
+#pragma unroll 4
+    for (int r = 0; r < TT; ++r) {  // rows beyond the chunk are 0
+      const float wr = w[s0 + r];
+      float xr[NR], yr[L::NC];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) xr[i] = w * X[r][ty + 16 * i];
+      for (int i = 0; i < NR; i += 2) {
+        const float2 t = *(const float2*)&X.x[r][NR * ty + i];
+        xr[i] = wr * t.x;
+        xr[i + 1] = wr * t.y;
+      }
+      row_cols(yr, Y, r, tx);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) yr[j] = Y[r][tx + 16 * j];
+      for (int i = 0; i < NR; ++i)
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = fmaf(xr[i], yr[j], acc[i][j]);
+        for (int j = 0; j < L::NC; ++j) acc[i][j] = fmaf(xr[i], yr[j], acc[i][j]);
     }
   }
   float* out = (bwd ? a.dstates : a.states) + (chain * nc + c) * (int64_t)D * D;
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+  for (int i = 0; i < NR; ++i)
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int d = ty + 16 * i, e = tx + 16 * j;
+    for (int j = 0; j < L::NC; ++j) {
+      const int d = NR * ty + i, e = L::col(tx, j / L::VW) + j % L::VW;
       if (d < D && e < D) out[d * D + e] = acc[i][j];
     }
 }
 
-// out[r][j] (rows ty, ty + 16; columns tx + 16 j) += w_r * sum_m A[r][m] M(m, column) over a
-// D x D matrix in global memory; transposed: M(m, c) = M[c][m].  `stage` is a free tile.
-template <int NI>
-__device__ void times_state(float (*acc)[NI], const float (*A)[LD], const float* M, bool transposed, int D,
-                            const float* w, float (*stage)[LD]) {
+// acc (rows ty, ty + 16; the thread's columns) += w_r * sum_m A[r][m] M(m, column) over a D x D
+// matrix in global memory; transposed: M(m, c) = M[c][m].  `stage` is a free tile.
+template <int DP>
+__device__ void times_state(float (*acc)[Tile<DP>::NC], const Tile<DP>& A, const float* M, bool transposed, int D,
+                            const float* w, Tile<DP>& stage) {
+  using L = Tile<DP>;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float part[2][L::NC];
+#pragma unroll
+  for (int j = 0; j < L::NC; ++j) part[0][j] = part[1][j] = 0.f;
   for (int m0 = 0; m0 < D; m0 += TT) {
     __syncthreads();
-    for (int u = threadIdx.x; u < TT * 16 * NI; u += 256) {
-      int m, c;
-      if (transposed) {  // consecutive threads along m, the contiguous axis of M[c][m]
-        c = u / TT, m = u - c * TT;
-      } else {
-        m = u / (16 * NI), c = u - m * (16 * NI);
-      }
+#pragma unroll
+    for (int i = 0; i < TT * DP / 256; ++i) {
+      const int u = threadIdx.x + 256 * i;
+      // consecutive threads along the contiguous axis of M
+      const int m = transposed ? u % TT : u / DP, c = transposed ? u / TT : u % DP;
       float x = 0.f;
       if (m0 + m < D && c < D) x = transposed ? M[(int64_t)c * D + m0 + m] : M[(int64_t)(m0 + m) * D + c];
-      stage[m][c] = x;
+      stage.x[m][c] = x;
     }
     __syncthreads();
-    const int n = min(TT, D - m0);
-    for (int m = 0; m < n; ++m) {
-      const float a0 = w[0] * A[ty][m0 + m], a1 = w[1] * A[ty + 16][m0 + m];
 #pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const float x = stage[m][tx + 16 * j];
-        acc[0][j] = fmaf(a0, x, acc[0][j]);
-        acc[1][j] = fmaf(a1, x, acc[1][j]);
+    for (int m = 0; m < TT; m += 4) {  // rows of `stage` beyond D are 0
+      const float4 a0 = *(const float4*)&A.x[ty][m0 + m], a1 = *(const float4*)&A.x[ty + 16][m0 + m];
+      const float p0[4] = {a0.x, a0.y, a0.z, a0.w}, p1[4] = {a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float x[L::NC];
+        row_cols(x, stage, m + k, tx);
+#pragma unroll
+        for (int j = 0; j < L::NC; ++j) {
+          part[0][j] = fmaf(p0[k], x[j], part[0][j]);
+          part[1][j] = fmaf(p1[k], x[j], part[1][j]);
+        }
       }
     }
+  }
+#pragma unroll
+  for (int j = 0; j < L::NC; ++j) {
+    acc[0][j] = fmaf(w[0], part[0][j], acc[0][j]);
+    acc[1][j] = fmaf(w[1], part[1][j], acc[1][j]);
   }
 }
 
+__device__ __forceinline__ float dot4(float4 x, float4 y, float s) {
+  return fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s))));
+}
 // (row ty + 16 i) . (row tx + 16 j) for i, j < 2, of two tiles
-__device__ __forceinline__ void dots(float (*p)[2], const float (*A)[LD], const float (*B)[LD], int D) {
+template <int DP>
+__device__ __forceinline__ void dots(float (*p)[2], const Tile<DP>& A, const Tile<DP>& B) {
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   p[0][0] = p[0][1] = p[1][0] = p[1][1] = 0.f;
-  for (int m = 0; m < D; ++m) {
-    const float a0 = A[ty][m], a1 = A[ty + 16][m], b0 = B[tx][m], b1 = B[tx + 16][m];
-    p[0][0] = fmaf(a0, b0, p[0][0]);
-    p[0][1] = fmaf(a0, b1, p[0][1]);
-    p[1][0] = fmaf(a1, b0, p[1][0]);
-    p[1][1] = fmaf(a1, b1, p[1][1]);
+#pragma unroll 8
+  for (int m = 0; m < DP; m += 4) {
+    const float4 a0 = *(const float4*)&A.x[ty][m], a1 = *(const float4*)&A.x[ty + 16][m];
+    const float4 b0 = *(const float4*)&B.x[tx][m], b1 = *(const float4*)&B.x[tx + 16][m];
+    p[0][0] = dot4(a0, b0, p[0][0]);
+    p[0][1] = dot4(a0, b1, p[0][1]);
+    p[1][0] = dot4(a1, b0, p[1][0]);
+    p[1][1] = dot4(a1, b1, p[1][1]);
   }
 }
-template <int NI>
-__device__ __forceinline__ void times_tile(float (*acc)[NI], const float (*Pm)[TT + 1], const float (*B)[LD]) {
+// acc += Pm (32 x 32) B
+template <int DP>
+__device__ __forceinline__ void times_tile(float (*acc)[Tile<DP>::NC], const float (*Pm)[LP], const Tile<DP>& B) {
+  using L = Tile<DP>;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll 4
-  for (int m = 0; m < TT; ++m) {
-    const float p0 = Pm[ty][m], p1 = Pm[ty + 16][m];
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const float x = B[m][tx + 16 * j];
-      acc[0][j] = fmaf(p0, x, acc[0][j]);
-      acc[1][j] = fmaf(p1, x, acc[1][j]);
+  for (int m = 0; m < TT; m += 4) {
+    const float4 a0 = *(const float4*)&Pm[ty][m], a1 = *(const float4*)&Pm[ty + 16][m];
+    const float p0[4] = {a0.x, a0.y, a0.z, a0.w}, p1[4] = {a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float x[L::NC];
+      row_cols(x, B, m + k, tx);
+#pragma unroll
+      for (int j = 0; j < L::NC; ++j) {
+        acc[0][j] = fmaf(p0[k], x[j], acc[0][j]);
+        acc[1][j] = fmaf(p1[k], x[j], acc[1][j]);
+      }
     }
   }
 }
-template <typename TA, int NI>
-__device__ void store_rows(void* x, const float (*acc)[NI], const AtlasDecayParams& P, int b, int h, int t0,
+template <typename TA, int DP>
+__device__ void store_rows(void* x, const float (*acc)[Tile<DP>::NC], const AtlasDecayParams& P, int b, int h, int t0,
                            int t_end, float scale) {
+  using L = Tile<DP>;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -253,8 +330,10 @@ __device__ void store_rows(void* x, const float (*acc)[NI], const AtlasDecayPara
     if (t >= t_end) continue;
     TA* row = (TA*)x + (((int64_t)b * P.T + t) * P.H + h) * P.D;
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
-      if (tx + 16 * j < P.D) st_act(row, (size_t)(tx + 16 * j), scale * acc[i][j]);
+    for (int j = 0; j < L::NC; ++j) {
+      const int e = L::col(tx, j / L::VW) + j % L::VW;
+      if (e < P.D) st_act(row, (size_t)e, scale * acc[i][j]);
+    }
   }
 }
 
@@ -275,10 +354,10 @@ struct TilePos {
   int64_t chain;
   int tile, b, h, c, L, tc, r0;  // r0: first row of the tile within its chunk
 };
-__device__ __forceinline__ TilePos tile_pos(const AtlasDecayParams& P, int tiles) {
+__device__ __forceinline__ TilePos tile_pos(const AtlasDecayParams& P, int64_t index, int tiles) {
   TilePos t;
-  t.chain = blockIdx.x / tiles;
-  t.tile = (int)(blockIdx.x % tiles);
+  t.chain = index / tiles;
+  t.tile = (int)(index % tiles);
   t.b = (int)(t.chain / P.H);
   t.h = (int)(t.chain % P.H);
   t.c = t.tile / (CH / TT);
@@ -289,153 +368,166 @@ __device__ __forceinline__ TilePos tile_pos(const AtlasDecayParams& P, int tiles
 }
 
 // y of one tile of 32 tokens
-template <typename TA, int NI>
-__global__ void __launch_bounds__(256) out_kernel(Args a, int tiles) {
+template <typename TA, int DP>
+__global__ void __launch_bounds__(256) out_kernel(Args a, int tiles, bool vec) {
+  using L = Tile<DP>;
   extern __shared__ float sm[];
-  float(*A)[LD] = (float(*)[LD])sm;
-  float(*K)[LD] = A + TT;
-  float(*V)[LD] = K + TT;
-  float(*Pm)[TT + 1] = (float(*)[TT + 1])(V + TT);
+  L &A = *(L*)sm, &K = *(&A + 1), &V = *(&A + 2);
+  float(*Pm)[LP] = (float(*)[LP])(&A + 3);
+  __shared__ float pw[CH + 1];
   const AtlasDecayParams& P = a.p;
-  const TilePos z = tile_pos(P, tiles);
-  const int D = P.D, cols = 16 * NI, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
-  const float g = a.log_decay[z.h];
-  load_rows<TA>(A, view(a.q, P.q_stride), z.b, z.h, z.tc + z.r0, tend, D, cols);
-  float acc[2][NI];
+  const TilePos z = tile_pos(P, blockIdx.x, tiles);
+  const int D = P.D, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
+  if (threadIdx.x <= CH) pw[threadIdx.x] = pow_decay(a.log_decay[z.h], threadIdx.x);
+  load_rows<TA>(A, view(a.q, P.q_stride), z.b, z.h, z.tc + z.r0, tend, D, vec);
+  float acc[2][L::NC];
 #pragma unroll
-  for (int j = 0; j < NI; ++j) acc[0][j] = acc[1][j] = 0.f;
-  const float w[2] = {pow_decay(g, z.r0 + ty + 1), pow_decay(g, z.r0 + ty + 17)};
-  times_state<NI>(acc, A, a.states + (z.chain * chunks(P) + z.c) * (int64_t)D * D, false, D, w, K);
+  for (int j = 0; j < L::NC; ++j) acc[0][j] = acc[1][j] = 0.f;
+  __syncthreads();
+  const float w[2] = {pw[z.r0 + ty + 1], pw[z.r0 + ty + 17]};
+  times_state<DP>(acc, A, a.states + (z.chain * chunks(P) + z.c) * (int64_t)D * D, false, D, w, K);
   for (int s0 = 0; s0 <= z.r0; s0 += TT) {
     __syncthreads();
-    load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, cols);
-    load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + s0, tend, D, cols);
+    load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, vec);
+    load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + s0, tend, D, vec);
     __syncthreads();
     float p[2][2];
-    dots(p, A, K, D);
+    dots(p, A, K);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int lag = z.r0 + ty + 16 * i - (s0 + tx + 16 * j);
-        Pm[ty + 16 * i][tx + 16 * j] = lag >= 0 ? p[i][j] * pow_decay(g, lag) : 0.f;
+        Pm[ty + 16 * i][tx + 16 * j] = lag >= 0 ? p[i][j] * pw[lag] : 0.f;
       }
     __syncthreads();
-    times_tile<NI>(acc, Pm, V);
+    times_tile<DP>(acc, Pm, V);
   }
-  store_rows<TA, NI>(a.y, acc, P, z.b, z.h, z.tc + z.r0, tend, P.scale);
+  store_rows<TA, DP>(a.y, acc, P, z.b, z.h, z.tc + z.r0, tend, P.scale);
 }
 
 // dq of one tile of 32 tokens, and its part of dlog_decay (terms with q)
-template <typename TA, int NI>
-__global__ void __launch_bounds__(256) dq_kernel(Args a, int tiles) {
-  extern __shared__ float sm[];
-  float(*Q)[LD] = (float(*)[LD])sm;
-  float(*O)[LD] = Q + TT;
-  float(*K)[LD] = O + TT;
-  float(*V)[LD] = K + TT;
-  float(*Pm)[TT + 1] = (float(*)[TT + 1])(V + TT);
+template <typename TA, int DP>
+__device__ void dq_tile(const Args& a, const TilePos& z, int part, bool vec, Tile<DP>* t, const float* pw) {
+  using L = Tile<DP>;
+  L &Q = t[0], &O = t[1], &K = t[2], &V = t[3];
+  float(*Pm)[LP] = (float(*)[LP])(t + 4);
   const AtlasDecayParams& P = a.p;
-  const TilePos z = tile_pos(P, tiles);
-  const int D = P.D, cols = 16 * NI, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
-  const float g = a.log_decay[z.h];
-  load_rows<TA>(Q, view(a.q, P.q_stride), z.b, z.h, z.tc + z.r0, tend, D, cols);
-  load_rows<TA>(O, flat(a.dy, P), z.b, z.h, z.tc + z.r0, tend, D, cols);
-  float acc[2][NI], dg = 0.f;
+  const int D = P.D, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
+  load_rows<TA>(Q, view(a.q, P.q_stride), z.b, z.h, z.tc + z.r0, tend, D, vec);
+  load_rows<TA>(O, flat(a.dy, P), z.b, z.h, z.tc + z.r0, tend, D, vec);
+  float acc[2][L::NC], dg = 0.f;
 #pragma unroll
-  for (int j = 0; j < NI; ++j) acc[0][j] = acc[1][j] = 0.f;
-  const float w[2] = {P.scale * pow_decay(g, z.r0 + ty + 1), P.scale * pow_decay(g, z.r0 + ty + 17)};
-  const int64_t so = (z.chain * chunks(P) + z.c) * (int64_t)D * D;
-  times_state<NI>(acc, O, a.states + so, true, D, w, K);
+  for (int j = 0; j < L::NC; ++j) acc[0][j] = acc[1][j] = 0.f;
+  const float w[2] = {P.scale * pw[z.r0 + ty + 1], P.scale * pw[z.r0 + ty + 17]};
+  times_state<DP>(acc, O, a.states + (z.chain * chunks(P) + z.c) * (int64_t)D * D, true, D, w, K);
+  {  // columns from D on are 0 in Q
+    float q0[L::NC], q1[L::NC];
+    row_cols(q0, Q, ty, tx);
+    row_cols(q1, Q, ty + 16, tx);
 #pragma unroll
-  for (int j = 0; j < NI; ++j)  // columns from D on are 0 in Q
-    dg += (float)(z.r0 + ty + 1) * Q[ty][tx + 16 * j] * acc[0][j] +
-          (float)(z.r0 + ty + 17) * Q[ty + 16][tx + 16 * j] * acc[1][j];
+    for (int j = 0; j < L::NC; ++j)
+      dg += (float)(z.r0 + ty + 1) * q0[j] * acc[0][j] + (float)(z.r0 + ty + 17) * q1[j] * acc[1][j];
+  }
   for (int s0 = 0; s0 <= z.r0; s0 += TT) {
     __syncthreads();
-    load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, cols);
-    load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + s0, tend, D, cols);
+    load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, vec);
+    load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + s0, tend, D, vec);
     __syncthreads();
     float p[2][2], x[2][2];
-    dots(p, Q, K, D);
-    dots(x, O, V, D);
+    dots(p, Q, K);
+    dots(x, O, V);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int lag = z.r0 + ty + 16 * i - (s0 + tx + 16 * j);
-        const float da = lag >= 0 ? P.scale * pow_decay(g, lag) * x[i][j] : 0.f;
+        const float da = lag >= 0 ? P.scale * pw[lag] * x[i][j] : 0.f;
         if (lag > 0) dg += (float)lag * p[i][j] * da;
         Pm[ty + 16 * i][tx + 16 * j] = da;
       }
     __syncthreads();
-    times_tile<NI>(acc, Pm, K);
+    times_tile<DP>(acc, Pm, K);
   }
-  store_rows<TA, NI>(a.dq, acc, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
+  store_rows<TA, DP>(a.dq, acc, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
   dg = cta_sum(dg);
-  if (threadIdx.x == 0) a.dg_part[z.chain * a.dg_parts + z.tile] = dg;
+  if (threadIdx.x == 0) a.dg_part[z.chain * a.dg_parts + part] = dg;
 }
 
 // dk and dv of one tile of 32 tokens, and the terms of dlog_decay with k, R and S
-template <typename TA, int NI>
-__global__ void __launch_bounds__(256) dkv_kernel(Args a, int tiles) {
-  extern __shared__ float sm[];
-  float(*K)[LD] = (float(*)[LD])sm;
-  float(*V)[LD] = K + TT;
-  float(*Q)[LD] = V + TT;
-  float(*O)[LD] = Q + TT;
-  float(*Pm)[TT + 1] = (float(*)[TT + 1])(O + TT);
-  float(*Am)[TT + 1] = Pm + TT;
+template <typename TA, int DP>
+__device__ void dkv_tile(const Args& a, const TilePos& z, int part, bool vec, Tile<DP>* t, const float* pw) {
+  using L = Tile<DP>;
+  L &K = t[0], &V = t[1], &Q = t[2], &O = t[3];
+  float(*Pm)[LP] = (float(*)[LP])(t + 4);
+  float(*Am)[LP] = Pm + TT;
   const AtlasDecayParams& P = a.p;
-  const TilePos z = tile_pos(P, tiles);
-  const int D = P.D, cols = 16 * NI, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
-  const float g = a.log_decay[z.h];
-  load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + z.r0, tend, D, cols);
-  load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + z.r0, tend, D, cols);
-  float dk[2][NI], dv[2][NI], dg = 0.f;
+  const int D = P.D, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
+  load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + z.r0, tend, D, vec);
+  load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + z.r0, tend, D, vec);
+  float dk[2][L::NC], dv[2][L::NC], dg = 0.f;
 #pragma unroll
-  for (int j = 0; j < NI; ++j) dk[0][j] = dk[1][j] = dv[0][j] = dv[1][j] = 0.f;
+  for (int j = 0; j < L::NC; ++j) dk[0][j] = dk[1][j] = dv[0][j] = dv[1][j] = 0.f;
   const int n0 = z.L - 1 - z.r0 - ty, n1 = n0 - 16;  // steps from the row to the chunk's end
-  const float w[2] = {n0 >= 0 ? pow_decay(g, n0) : 0.f, n1 >= 0 ? pow_decay(g, n1) : 0.f};
+  const float w[2] = {n0 >= 0 ? pw[n0] : 0.f, n1 >= 0 ? pw[n1] : 0.f};
   const int64_t so = (z.chain * chunks(P) + z.c) * (int64_t)D * D;
   const float *R = a.dstates + so, *S = a.states + so;
-  times_state<NI>(dk, V, R, true, D, w, Q);
-  times_state<NI>(dv, K, R, false, D, w, Q);
+  times_state<DP>(dk, V, R, true, D, w, Q);
+  times_state<DP>(dv, K, R, false, D, w, Q);
+  {
+    float k0[L::NC], k1[L::NC];
+    row_cols(k0, K, ty, tx);
+    row_cols(k1, K, ty + 16, tx);
 #pragma unroll
-  for (int j = 0; j < NI; ++j) {
-    if (n0 > 0) dg += (float)n0 * K[ty][tx + 16 * j] * dk[0][j];
-    if (n1 > 0) dg += (float)n1 * K[ty + 16][tx + 16 * j] * dk[1][j];
+    for (int j = 0; j < L::NC; ++j) {
+      if (n0 > 0) dg += (float)n0 * k0[j] * dk[0][j];
+      if (n1 > 0) dg += (float)n1 * k1[j] * dk[1][j];
+    }
   }
   if (z.r0 == 0) {  // once for each chunk
     float rs = 0.f;
     for (int u = threadIdx.x; u < D * D; u += 256) rs = fmaf(R[u], S[u], rs);
-    dg += (float)z.L * pow_decay(g, z.L) * rs;
+    dg += (float)z.L * pw[z.L] * rs;
   }
   for (int t0 = z.r0; t0 < z.L; t0 += TT) {
     __syncthreads();
-    load_rows<TA>(Q, view(a.q, P.q_stride), z.b, z.h, z.tc + t0, tend, D, cols);
-    load_rows<TA>(O, flat(a.dy, P), z.b, z.h, z.tc + t0, tend, D, cols);
+    load_rows<TA>(Q, view(a.q, P.q_stride), z.b, z.h, z.tc + t0, tend, D, vec);
+    load_rows<TA>(O, flat(a.dy, P), z.b, z.h, z.tc + t0, tend, D, vec);
     __syncthreads();
     float p[2][2], x[2][2];
-    dots(p, K, Q, D);
-    dots(x, V, O, D);
+    dots(p, K, Q);
+    dots(x, V, O);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int lag = t0 + tx + 16 * j - (z.r0 + ty + 16 * i);
-        const float f = lag >= 0 ? P.scale * pow_decay(g, lag) : 0.f;
+        const float f = lag >= 0 ? P.scale * pw[lag] : 0.f;
         Pm[ty + 16 * i][tx + 16 * j] = lag >= 0 ? f * p[i][j] : 0.f;
         Am[ty + 16 * i][tx + 16 * j] = lag >= 0 ? f * x[i][j] : 0.f;
       }
     __syncthreads();
-    times_tile<NI>(dk, Am, Q);
-    times_tile<NI>(dv, Pm, O);
+    times_tile<DP>(dk, Am, Q);
+    times_tile<DP>(dv, Pm, O);
   }
-  store_rows<TA, NI>(a.dk, dk, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
-  store_rows<TA, NI>(a.dv, dv, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
+  store_rows<TA, DP>(a.dk, dk, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
+  store_rows<TA, DP>(a.dv, dv, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
   dg = cta_sum(dg);
-  if (threadIdx.x == 0) a.dg_part[z.chain * a.dg_parts + tiles + z.tile] = dg;
+  if (threadIdx.x == 0) a.dg_part[z.chain * a.dg_parts + part] = dg;
+}
+
+// even CTAs take dk and dv of a tile (the longer work first), odd ones dq
+template <typename TA, int DP>
+__global__ void __launch_bounds__(256) grads_kernel(Args a, int tiles, bool vec) {
+  extern __shared__ float sm[];
+  __shared__ float pw[CH + 1];
+  const TilePos z = tile_pos(a.p, blockIdx.x >> 1, tiles);
+  if (threadIdx.x <= CH) pw[threadIdx.x] = pow_decay(a.log_decay[z.h], threadIdx.x);
+  __syncthreads();
+  if (blockIdx.x & 1)
+    dq_tile<TA, DP>(a, z, z.tile, vec, (Tile<DP>*)sm, pw);
+  else
+    dkv_tile<TA, DP>(a, z, tiles + z.tile, vec, (Tile<DP>*)sm, pw);
 }
 
 // ---------------------------------------------------------------------------
@@ -599,47 +691,38 @@ static cudaError_t scan(const Args& a, const float* in, float* out, bool bwd, cu
   return cudaGetLastError();
 }
 
-// the CUDA-core kernels for one activation type and NI = ceil(D / 16), rounded up to 2, 4 or 8
-template <typename TA, int NI>
-struct Plain {
-  static size_t smem(int tiles, int squares) {
-    return ((size_t)tiles * TT * LD + (size_t)squares * TT * (TT + 1)) * sizeof(float);
-  }
-  static cudaError_t sums(const Args& a, bool bwd, cudaStream_t s) {
-    sums_kernel<TA, NI><<<(unsigned)(chains(a.p) * chunks(a.p)), 256, 0, s>>>(a, bwd);
-    return cudaGetLastError();
-  }
-  static cudaError_t out(const Args& a, cudaStream_t s) {
-    const int tiles = (a.p.T + TT - 1) / TT;
-    const size_t sm = smem(3, 1);
-    cudaError_t e = allow_smem<out_kernel<TA, NI>>(sm);
-    if (e != cudaSuccess) return e;
-    out_kernel<TA, NI><<<(unsigned)(chains(a.p) * tiles), 256, sm, s>>>(a, tiles);
-    return cudaGetLastError();
-  }
-  static cudaError_t grads(const Args& a, cudaStream_t s) {
-    const int tiles = (a.p.T + TT - 1) / TT;
-    const unsigned grid = (unsigned)(chains(a.p) * tiles);
-    size_t sm = smem(4, 1);
-    cudaError_t e = allow_smem<dq_kernel<TA, NI>>(sm);
-    if (e != cudaSuccess) return e;
-    dq_kernel<TA, NI><<<grid, 256, sm, s>>>(a, tiles);
-    sm = smem(4, 2);
-    e = allow_smem<dkv_kernel<TA, NI>>(sm);
-    if (e != cudaSuccess) return e;
-    dkv_kernel<TA, NI><<<grid, 256, sm, s>>>(a, tiles);
-    return cudaGetLastError();
-  }
-};
+// whether groups of four channels of every tensor can be loaded at once
+static bool vec4(const Args& a) {
+  const AtlasDecayParams& p = a.p;
+  const int64_t bytes = p.act_dtype == ATLAS_BF16 ? 2 : 4;
+  int64_t all = p.D * bytes;
+  for (const int64_t* s : {p.q_stride, p.k_stride, p.v_stride}) all |= s[0] * bytes | s[1] * bytes | s[2] * bytes;
+  for (const void* x : {a.q, a.k, a.v, a.dy}) all |= (int64_t)(uintptr_t)x;
+  return all % (4 * bytes) == 0;
+}
+// the CUDA-core kernels for one activation type and padded head size
 enum Phase { SUMS_FWD, SUMS_BWD, OUT, GRADS };
-template <typename TA, int NI>
-static cudaError_t plain_ni(const Args& a, Phase f, cudaStream_t s) {
-  using K = Plain<TA, NI>;
-  return f == OUT ? K::out(a, s) : f == GRADS ? K::grads(a, s) : K::sums(a, f == SUMS_BWD, s);
+template <typename TA, int DP>
+static cudaError_t plain_dp(const Args& a, Phase f, cudaStream_t s) {
+  const int tiles = (a.p.T + TT - 1) / TT;
+  const bool vec = vec4(a);
+  const auto smem = [](int n, int squares) { return n * sizeof(Tile<DP>) + (size_t)squares * TT * LP * sizeof(float); };
+  if (f == OUT) {
+    const cudaError_t e = allow_smem<out_kernel<TA, DP>>(smem(3, 1));
+    if (e != cudaSuccess) return e;
+    out_kernel<TA, DP><<<(unsigned)(chains(a.p) * tiles), 256, smem(3, 1), s>>>(a, tiles, vec);
+  } else if (f == GRADS) {
+    const cudaError_t e = allow_smem<grads_kernel<TA, DP>>(smem(4, 2));
+    if (e != cudaSuccess) return e;
+    grads_kernel<TA, DP><<<(unsigned)(chains(a.p) * tiles * 2), 256, smem(4, 2), s>>>(a, tiles, vec);
+  } else {
+    sums_kernel<TA, DP><<<(unsigned)(chains(a.p) * chunks(a.p)), 256, 0, s>>>(a, f == SUMS_BWD, vec);
+  }
+  return cudaGetLastError();
 }
 template <typename TA>
 static cudaError_t plain_t(const Args& a, Phase f, cudaStream_t s) {
-  return a.p.D <= 32 ? plain_ni<TA, 2>(a, f, s) : a.p.D <= 64 ? plain_ni<TA, 4>(a, f, s) : plain_ni<TA, 8>(a, f, s);
+  return a.p.D <= 32 ? plain_dp<TA, 32>(a, f, s) : a.p.D <= 64 ? plain_dp<TA, 64>(a, f, s) : plain_dp<TA, 128>(a, f, s);
 }
 static cudaError_t plain(const Args& a, Phase f, cudaStream_t s) {
   return a.p.act_dtype == ATLAS_BF16 ? plain_t<__nv_bfloat16>(a, f, s) : plain_t<float>(a, f, s);
