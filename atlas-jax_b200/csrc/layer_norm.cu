@@ -88,21 +88,33 @@ template <int VEC>
 constexpr int PAIRS = (VEC + 1) / 2;
 template <typename TA, int VEC>
 __device__ __forceinline__ void unpack2(F2* f, const Pack<TA, VEC>& k) {
-  float t[VEC];
-  unpack<TA, VEC>(t, k);
+  if constexpr (sizeof(TA) == 2 && VEC > 1) {
+    const uint32_t* h = (const uint32_t*)&k;
 #pragma unroll
-  for (int j = 0; j < PAIRS<VEC>; ++j) f[j] = f2(t[2 * j], 2 * j + 1 < VEC ? t[2 * j + 1] : 0.f);
+    for (int j = 0; j < PAIRS<VEC>; ++j) f[j] = bf2_unpack(h[j]);
+  } else if constexpr (VEC > 1) {
+    const uint64_t* h = (const uint64_t*)&k;
+#pragma unroll
+    for (int j = 0; j < PAIRS<VEC>; ++j) f[j].v = h[j];
+  } else {
+    f[0] = f2(ld_act(k.v, 0), 0.f);
+  }
 }
 template <typename TA, int VEC>
 __device__ __forceinline__ void store2(TA* p, const F2* f) {
-  float t[2 * PAIRS<VEC>];
+  if constexpr (VEC > 1) {
+    Pack<TA, VEC> k;
 #pragma unroll
-  for (int j = 0; j < PAIRS<VEC>; ++j) {
-    const float2 x = f2_get(f[j]);
-    t[2 * j] = x.x;
-    t[2 * j + 1] = x.y;
+    for (int j = 0; j < PAIRS<VEC>; ++j) {
+      if constexpr (sizeof(TA) == 2)
+        ((uint32_t*)&k)[j] = bf2_pack(f[j]);
+      else
+        ((uint64_t*)&k)[j] = f[j].v;
+    }
+    *(Pack<TA, VEC>*)p = k;
+  } else {
+    st_act(p, 0, f2_get(f[0]).x);
   }
-  store<TA, VEC>(p, t);
 }
 // 16 bytes from global to this thread's own slot in shared memory, without registers
 __device__ __forceinline__ void copy16(void* slot, const void* g) {
@@ -271,7 +283,7 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256) fwd_kernel(Args a, i
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
 __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : TEAM == SUB ? 4 : VEC * CHN <= 8 ? 3 : 2)
     bwd_kernel(Args a, int per_block, int stages) {
-  extern __shared__ __align__(16) uint8_t dyn[];  // the ring, then 2 x width sums where teams share channels
+  extern __shared__ __align__(16) uint8_t dyn[];  // the ring; after it the teams' sums, 2 x width each
   __shared__ float red_all[8][2 * 16 * 2];
   constexpr bool RING = VEC > 1;
   constexpr int NP = PAIRS<VEC>;
@@ -378,34 +390,36 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : T
   }
   if (!a.part) return;
   float* pw = a.part + (int64_t)blockIdx.x * 2 * a.width;
-  float* pb = pw + a.width;
-  // teams of one block with the same channels add up in turn
-  float* aw = (float*)(dyn + (RING ? stages * 3 * CHN * pitch * (int)sizeof(Raw) : 0));
-  if (TEAM != SUB && per_block == 1) aw = pw;  // one team: straight to its partial row
-  float* ab = aw + a.width;
+  // the teams of the block side by side, where the ring was, then added up in order
+  if (RING) asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  const bool alone = TEAM != SUB && per_block == 1;  // one team: straight to its partial row
+  float* aw = alone ? pw : (float*)dyn + z.team * 2 * a.width;
   const int off = (TEAM == SUB ? g * a.N : 0) + n0;
-  for (int i = 0; i < per_block; ++i) {
-    if (i == z.team) {
+  if (z.team < per_block) {
 #pragma unroll
-      for (int c = 0; c < CHN; ++c) {
-        if (n0 + c * dn < a.N) {
+    for (int c = 0; c < CHN; ++c)
+      if (n0 + c * dn < a.N) {
+        float* k = aw + off + c * dn;
+        if constexpr (VEC % 4 == 0) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int k = off + c * dn + j;
-            const float2 x = f2_get(dw[c][j / 2]), y = f2_get(db[c][j / 2]);
-            const float xw = j & 1 ? x.y : x.x, xb = j & 1 ? y.y : y.x;
-            aw[k] = i == 0 ? xw : aw[k] + xw;
-            ab[k] = i == 0 ? xb : ab[k] + xb;
+          for (int j = 0; j < NP; j += 2) {
+            const float2 x = f2_get(dw[c][j]), y = f2_get(dw[c][j + 1]), u = f2_get(db[c][j]), v = f2_get(db[c][j + 1]);
+            *(float4*)(k + 2 * j) = make_float4(x.x, x.y, y.x, y.y);
+            *(float4*)(k + a.width + 2 * j) = make_float4(u.x, u.y, v.x, v.y);
           }
+        } else {
+          k[0] = f2_get(dw[c][0]).x;
+          k[a.width] = f2_get(db[c][0]).x;
         }
       }
-    }
-    __syncthreads();
   }
-  if (aw == pw) return;
-  for (int k = threadIdx.x; k < a.width; k += blockDim.x) {
-    pw[k] = aw[k];
-    pb[k] = ab[k];
+  if (alone) return;
+  __syncthreads();
+  for (int k = threadIdx.x; k < 2 * a.width; k += blockDim.x) {
+    float s = 0.f;
+    for (int i = 0; i < per_block; ++i) s += ((const float*)dyn)[i * 2 * a.width + k];
+    pw[k] = s;
   }
 }
 
@@ -692,9 +706,12 @@ static Plan plan(const Args& a, int act_dtype, bool vec_ok, bool bwd) {
     z.width = a.G * a.N;
     units = a.vecs;
   }
-  // the backward's blocks are what an SM holds at its register use, the forward's many more
-  const int64_t blocks = SMS * (bwd ? (z.threads * z.chn * z.vec <= 2048 ? 4 : 2) : 16);
-  z.grid = std::max<int64_t>(1, std::min(units, blocks));
+  // The backward's blocks are what an SM holds at its register use (each keeps sums).  The
+  // forward's are 8 an SM, fewer where that makes their numbers of rounds equal (65536 x 768
+  // bf16: 79 us, 87 with a block for every 8 rows).
+  const int64_t blocks = SMS * (!bwd ? 8 : z.threads * z.chn * z.vec <= 2048 ? 4 : 2);
+  const int64_t rounds = std::max<int64_t>(1, (units + blocks - 1) / blocks);
+  z.grid = std::max<int64_t>(1, bwd ? std::min(units, blocks) : (units + rounds - 1) / rounds);
   if (bwd && !z.big && !z.tiny && z.team != SUB && a.G > 1)  // a multiple of G: a block keeps one group's weights
     z.grid = std::min<int64_t>(units, std::max<int64_t>(a.G, z.grid / a.G * a.G));
   z.parts = (int)(z.big ? std::min<int64_t>(BIG_PARTS, std::max<int64_t>(1, a.rows))
@@ -729,10 +746,11 @@ template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
 static cudaError_t go(const Args& a, const Plan& z, bool bwd, cudaStream_t s) {
   
   if (bwd) {
-      // 4 stages while the blocks that an SM's registers hold have room for them, else 2
+      // as many stages, up to 4, as the blocks that an SM's registers hold have room for
       const size_t stage = VEC > 1 ? (size_t)3 * CHN * z.threads * 16 : 0;
       const int stages = 4 * stage <= 50 << 10 ? 4 : 2;
-      const size_t sm = stages * stage + (TEAM == SUB || z.per_block > 1 ? (size_t)2 * z.width * sizeof(float) : 0);
+      const size_t sums = TEAM == SUB || z.per_block > 1 ? (size_t)z.per_block * 2 * z.width * sizeof(float) : 0;
+      const size_t sm = std::max(stages * stage, sums);
       cudaError_t e = allow_smem<bwd_kernel<TA, TEAM, LANES, VEC, CHN>>();
       if (e != cudaSuccess) return e;
       bwd_kernel<TA, TEAM, LANES, VEC, CHN><<<(unsigned)z.grid, z.threads, sm, s>>>(a, z.per_block, stages);
