@@ -14,7 +14,7 @@ import functools
 import torch
 
 from . import _lib as L
-from .scan import _WS, addr, empty_like, on_device, stream_of
+from .scan import _WS, addr, away, empty_like, stream_of
 
 
 class AtlasDecayParams(ctypes.Structure):
@@ -68,12 +68,12 @@ class _Plan:
         self.params = AtlasDecayParams(L.ATLAS_ABI_VERSION, B, T, H, D,
                                        L.ATLAS_BF16 if dtype == torch.bfloat16 else L.ATLAS_F32,
                                        D ** -0.5 if scale is None else scale, int(aligned), *strides)
-        self.ref = ctypes.byref(self.params)
+        self.lib, self.ref = _lib(), ctypes.byref(self.params)
         self.shape, self.dtype = tuple(shape), dtype
         self.B, self.state_shape = B, (B, H, D, D)
-        self.saved_bytes = self._size(_lib().atlas_decay_saved_bytes)
-        self.fwd_workspace_bytes = self._size(_lib().atlas_decay_fwd_workspace_bytes)
-        self.bwd_workspace_bytes = self._size(_lib().atlas_decay_bwd_workspace_bytes)
+        self.saved_bytes = self._size(self.lib.atlas_decay_saved_bytes)
+        self.fwd_workspace_bytes = self._size(self.lib.atlas_decay_fwd_workspace_bytes)
+        self.bwd_workspace_bytes = self._size(self.lib.atlas_decay_bwd_workspace_bytes)
 
     def _size(self, query):
         """A size query's answer; 0 is an error only when it left a message."""
@@ -115,13 +115,19 @@ def decay_attention_forward(q, k, v, log_decay, state=None, scale=None, need_sav
     if state is not None:
         _need(state, p.state_shape, "state", q)
         state = _aligned(state)
-    with on_device(dev):
-        y = empty_like(q)
-        out = torch.empty(p.state_shape, device=dev) if state is None else empty_like(state)
-        saved = torch.empty(p.saved_bytes, dtype=torch.uint8, device=dev) if need_saved else None
-        ws, wsb = (None, 0) if need_saved else (workspace or _WS).get(p.fwd_workspace_bytes, dev)
-        L.check(_lib().atlas_decay_fwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), addr(state),
-                                       y.data_ptr(), out.data_ptr(), addr(saved), addr(ws), wsb, stream_of(dev)))
+    if away(dev):
+        with torch.cuda.device(dev):
+            return decay_attention_forward(q, k, v, log_decay, state, scale, need_saved, workspace)
+    y = empty_like(q)
+    out = torch.empty(*p.state_shape, device=dev) if state is None else torch.empty_like(state)
+    if need_saved:
+        saved, ws, wsb = torch.empty(p.saved_bytes // 4, device=dev), None, 0
+    else:
+        saved, (ws, wsb) = None, (workspace or _WS).get(p.fwd_workspace_bytes, dev)
+    rc = p.lib.atlas_decay_fwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), addr(state),
+                               y.data_ptr(), out.data_ptr(), addr(saved), addr(ws), wsb, stream_of(dev))
+    if rc:
+        L.check(rc)
     return y, out, saved
 
 
@@ -137,13 +143,17 @@ def decay_attention_backward(q, k, v, log_decay, saved, dy, dstate=None, scale=N
         dstate = _aligned(dstate)
     if saved.numel() * saved.element_size() != p.saved_bytes or saved.get_device() != q.get_device():
         raise ValueError("saved: not what decay_attention_forward saved for these inputs")
-    with on_device(dev):
-        dq, dk, dv = empty_like(q), empty_like(q), empty_like(q)
-        dg, dstate_in = torch.empty(p.shape[2], device=dev), torch.empty(p.state_shape, device=dev)
-        ws, wsb = (workspace or _WS).get(p.bwd_workspace_bytes, dev)
-        L.check(_lib().atlas_decay_bwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
-                                       saved.data_ptr(), dy.data_ptr(), addr(dstate), dq.data_ptr(), dk.data_ptr(),
-                                       dv.data_ptr(), dg.data_ptr(), dstate_in.data_ptr(), addr(ws), wsb, stream_of(dev)))
+    if away(dev):
+        with torch.cuda.device(dev):
+            return decay_attention_backward(q, k, v, log_decay, saved, dy, dstate, scale, workspace)
+    dq, dk, dv = empty_like(q), empty_like(q), empty_like(q)
+    dg, dstate_in = torch.empty_like(log_decay), torch.empty(*p.state_shape, device=dev)
+    ws, wsb = (workspace or _WS).get(p.bwd_workspace_bytes, dev)
+    rc = p.lib.atlas_decay_bwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), saved.data_ptr(),
+                               dy.data_ptr(), addr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
+                               dstate_in.data_ptr(), addr(ws), wsb, stream_of(dev))
+    if rc:
+        L.check(rc)
     return dq, dk, dv, dg, dstate_in
 
 
@@ -158,7 +168,7 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None, out=
     p, q, k, v = _plan(q, k, v, log_decay, scale)
     dev = q.device
     n = p.B if slots is None else state.shape[0]
-    shape = (n,) + p.state_shape[1:]
+    shape = p.state_shape if n == p.B else (n,) + p.state_shape[1:]
     _need(state, shape, "state", q)
     if out is None:
         out = state
@@ -167,10 +177,14 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None, out=
     if slots is not None and (slots.dtype != torch.int32 or slots.shape != (p.B,) or not slots.is_contiguous()
                               or slots.get_device() != q.get_device()):
         raise ValueError(f"slots: expected contiguous int32 ({p.B},) on {dev}, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
-    with on_device(dev):
-        y = empty_like(q)
-        L.check(_lib().atlas_decay_step(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
-                                        state.data_ptr(), addr(slots), n, y.data_ptr(), out.data_ptr(), stream_of(dev)))
+    if away(dev):
+        with torch.cuda.device(dev):
+            return decay_attention_step(q, k, v, log_decay, state, slots, scale, out)
+    y = empty_like(q)
+    rc = p.lib.atlas_decay_step(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(),
+                                addr(slots), n, y.data_ptr(), out.data_ptr(), stream_of(dev))
+    if rc:
+        L.check(rc)
     return y, out
 
 

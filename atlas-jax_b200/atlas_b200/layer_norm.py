@@ -11,7 +11,7 @@ import functools
 import torch
 
 from . import _lib as L
-from .scan import _WS, addr, on_device, stream_of
+from .scan import _WS, addr, away, stream_of
 
 
 class AtlasNormParams(ctypes.Structure):
@@ -61,8 +61,8 @@ class _Plan:
         rows = shape.numel() // (G * N) if G * N else 0
         self.params = AtlasNormParams(L.ATLAS_ABI_VERSION, L.ATLAS_BF16 if dtype == torch.bfloat16 else L.ATLAS_F32,
                                       rows, G, N, eps, 0)
-        self.ref, self.vecs = ctypes.byref(self.params), rows * G
-        self.workspace_bytes = _lib().atlas_layernorm_workspace_bytes(self.ref)
+        self.lib, self.ref, self.vecs = _lib(), ctypes.byref(self.params), rows * G
+        self.workspace_bytes = self.lib.atlas_layernorm_workspace_bytes(self.ref)
         if self.workspace_bytes == 0:
             raise L.AtlasError(L.ATLAS_ERR_INVALID_ARGUMENT, L.load().atlas_last_error_string().decode())
 
@@ -90,14 +90,18 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None):
     p = _plan(x, weight, bias, eps)
     x = x.contiguous()
     dev = x.device
-    with on_device(dev):
-        y = torch.empty_like(x)
-        h = x
-        if residual is not None:
-            residual, h = _like(residual, x, "residual"), torch.empty_like(x)
-        stats = torch.empty((p.vecs, 2), device=dev)
-        L.check(_lib().atlas_layernorm_fwd(p.ref, x.data_ptr(), addr(residual), addr(weight), addr(bias), y.data_ptr(),
-                                           None if residual is None else h.data_ptr(), stats.data_ptr(), stream_of(dev)))
+    if away(dev):
+        with torch.cuda.device(dev):
+            return layer_norm_forward(x, weight, bias, eps, residual)
+    y, stats = torch.empty_like(x), torch.empty(p.vecs, 2, device=dev)
+    h, hp = x, None
+    if residual is not None:
+        residual, h = _like(residual, x, "residual"), torch.empty_like(x)
+        hp = h.data_ptr()
+    rc = p.lib.atlas_layernorm_fwd(p.ref, x.data_ptr(), addr(residual), addr(weight), addr(bias), y.data_ptr(), hp,
+                                   stats.data_ptr(), stream_of(dev))
+    if rc:
+        L.check(rc)
     return y, h, stats
 
 
@@ -118,16 +122,20 @@ def layer_norm_backward(dy, h, weight, stats, dh=None, need_params=True, shape=N
     if stats.dtype != torch.float32 or stats.shape != (p.vecs, 2) or not stats.is_contiguous() \
             or stats.get_device() != h.get_device():
         raise ValueError(f"stats: expected contiguous float32 {(p.vecs, 2)} on {dev}, got {stats.dtype} {tuple(stats.shape)}")
-    with on_device(dev):
-        dx = torch.empty_like(h)
-        dw = db = ws = None
-        wsb = 0
-        if need_params:
-            dw = torch.empty(p.param_shape, device=dev) if weight is None else torch.empty_like(weight)
-            db = torch.empty_like(dw)
-            ws, wsb = (workspace or _WS).get(p.workspace_bytes, dev)
-        L.check(_lib().atlas_layernorm_bwd(p.ref, dy.data_ptr(), h.data_ptr(), addr(weight), stats.data_ptr(), addr(dh),
-                                           dx.data_ptr(), addr(dw), addr(db), addr(ws), wsb, stream_of(dev)))
+    if away(dev):
+        with torch.cuda.device(dev):
+            return layer_norm_backward(dy, h, weight, stats, dh, need_params, shape, workspace)
+    dx = torch.empty_like(h)
+    dw = db = ws = None
+    wsb = 0
+    if need_params:
+        dw = torch.empty(*p.param_shape, device=dev) if weight is None else torch.empty_like(weight)
+        db = torch.empty_like(dw)
+        ws, wsb = (workspace or _WS).get(p.workspace_bytes, dev)
+    rc = p.lib.atlas_layernorm_bwd(p.ref, dy.data_ptr(), h.data_ptr(), addr(weight), stats.data_ptr(), addr(dh),
+                                   dx.data_ptr(), addr(dw), addr(db), addr(ws), wsb, stream_of(dev))
+    if rc:
+        L.check(rc)
     return dx, dw, db
 
 

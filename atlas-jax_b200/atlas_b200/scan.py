@@ -7,7 +7,6 @@ for the custom-VJP pair): ``scan_forward`` / ``scan_backward`` are the two halve
 of the custom VJP and ``AtlasScan`` glues them into autograd.
 """
 
-import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -56,12 +55,9 @@ def empty_like(x):
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
-def on_device(dev):
-    """Context in which ``dev`` is the current device."""
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-
-_HERE = contextlib.nullcontext()
+def away(dev):
+    """Whether ``dev`` is not the current device (launches then need ``torch.cuda.device``)."""
+    return torch.cuda.current_device() != dev.index
 
 
 def _check_act(x, name, dtype, shape):
