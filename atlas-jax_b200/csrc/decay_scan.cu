@@ -39,31 +39,34 @@ namespace atlas {
 namespace decay {
 namespace tcore {
 
-template <int DP>
+template <int DP, bool FWD>
 struct Cfg {
   static constexpr int NB = DP / 64;                    // boxes of a tile
   static constexpr int TILE = NB * BOX;                 // 64 tokens x DP channels
-  static constexpr int STAGES = DP == 64 ? 3 : 2;       // of q, k, v
-  static constexpr int DBL = DP == 64 ? 2 : 1;          // buffers of k', scores, S and the accumulators
-  static constexpr int KWARPS = DP == 64 ? 8 : 4;       // warps of the k' group
+  static constexpr int TILES = FWD ? 3 : 2;             // of a stage: (q,) k, v
+  static constexpr int STAGES = FWD ? (DP == 64 ? 3 : 2) : (DP == 64 ? 4 : 3);
+  static constexpr int DBL = FWD && DP == 128 ? 1 : 2;  // buffers of k', scores, S and the accumulators
+  static constexpr int KWARPS = FWD && DP == 128 ? 4 : 8;  // warps of the k' group
   static constexpr int SWARPS = DP == 64 ? 8 : 16;      // warps of the state group
-  static constexpr int NT = 32 * (KWARPS + 12 + SWARPS);
-  static constexpr int W_P = KWARPS, W_Y = W_P + 4, W_S = W_Y + 4, W_MMA = W_S + SWARPS;  // first warps of the groups (MMA: three)
+  static constexpr int MWARPS = FWD ? 3 : 1;            // warps that issue MMAs
+  static constexpr int W_P = KWARPS, W_Y = W_P + (FWD ? 4 : 0), W_S = W_Y + (FWD ? 4 : 0), W_MMA = W_S + SWARPS;  // first warps of the groups
+  static constexpr int NT = 32 * (W_MMA + MWARPS + 1);
   static constexpr int PT = C * C * 2;                  // a tile of scores
   static constexpr int ST = DP * DP * 2;                // one part of a state
-  static constexpr int OFF_KP = STAGES * 3 * TILE;
+  static constexpr int OFF_KP = STAGES * TILES * TILE;
   static constexpr int OFF_P = OFF_KP + DBL * 3 * TILE;
-  static constexpr int OFF_S = OFF_P + DBL * PT;
-  static constexpr int OFF_Y = OFF_S + DBL * 2 * ST;
-  static constexpr int OFF_CTL = OFF_Y + (DP == 64 ? 2 : 1) * BOX;
+  static constexpr int OFF_S = OFF_P + (FWD ? DBL * PT : 0);
+  static constexpr int OFF_Y = OFF_S + (FWD ? DBL * 2 * ST : 0);
+  static constexpr int OFF_CTL = OFF_Y + (FWD ? (DP == 64 ? 2 : 1) * BOX : 0);
   // TMEM columns
-  static constexpr uint32_t T_A = 0, T_DS = DBL * 64, T_QS = T_DS + DBL * DP, T_O = T_QS + DBL * DP;
-  static_assert(T_O + DBL * DP <= 512, "TMEM");
+  static constexpr uint32_t T_A = 0, T_DS = FWD ? DBL * 64 : 0, T_QS = T_DS + DBL * DP, T_O = T_QS + DBL * DP;
+  static constexpr uint32_t COLS = FWD ? 512 : DBL * DP;
+  static_assert(!FWD || T_O + DBL * DP <= 512, "TMEM");
 };
 
 struct Ctl {
   F2 w[2 * C];                       // w[C + lag] = (l^lag, l^(lag - 1)), clamped at exponent 0
-  uint64_t full[3], empty[3];        // stages
+  uint64_t full[4], empty[4];        // stages
   uint64_t a_full[2], a_free[2];     // A in TMEM
   uint64_t kp_full[2], kp_free[2];   // k' parts
   uint64_t ds_full[2], ds_free[2];   // dS in TMEM
@@ -74,8 +77,8 @@ struct Ctl {
   uint32_t tmem;
   volatile int bad;
 };
-template <int DP>
-constexpr size_t SEQ_SMEM = Cfg<DP>::OFF_CTL + sizeof(Ctl) + 1024;
+template <int DP, bool FWD>
+constexpr size_t SEQ_SMEM = Cfg<DP, FWD>::OFF_CTL + sizeof(Ctl) + 1024;
 
 struct SeqArgs {
   AtlasDecayParams p;
@@ -137,11 +140,11 @@ struct Walk {  // one CTA's blocks: first, first + step, ..., n of them
 };
 
 template <int DP, bool FWD>
-__global__ void __launch_bounds__(Cfg<DP>::NT, 1)
+__global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     seq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_x,
                const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_o, const SeqArgs a,
                bool reversed) {
-  using K = Cfg<DP>;
+  using K = Cfg<DP, FWD>;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   Ctl& ctl = *(Ctl*)(sm + K::OFF_CTL);
@@ -165,13 +168,13 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
   const float g = a.log_decay[z.h];
 
   if (w == K::W_MMA) {
-    tmem_alloc(&ctl.tmem, 512);
+    tmem_alloc(&ctl.tmem, K::COLS);
     tmem_relinquish();
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < K::STAGES; ++i) {
       mbar_init(&ctl.full[i], 1);
-      mbar_init(&ctl.empty[i], (FWD ? 3 : 1) + K::KWARPS);  // the issuing warps' last MMAs, and the warps that read k
+      mbar_init(&ctl.empty[i], K::MWARPS + K::KWARPS);  // the issuing warps' last MMAs, and the warps that read k
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.a_full[i], 1);
@@ -187,7 +190,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
       mbar_init(&ctl.s_full[i], K::SWARPS);
       mbar_init(&ctl.s_free[i], 1);
     }
-    mbar_init(&ctl.fin, FWD ? 3 : 1);
+    mbar_init(&ctl.fin, K::MWARPS);
     ctl.bad = 0;
     fence_mbar_init();
   }
@@ -212,7 +215,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
       if (i >= K::DBL && !wait(ctl, &ctl.kp_free[b], i / K::DBL - 1, a.status)) break;
       const float wr = reversed || L == C ? wfull : r < L ? powd(g, L - 1 - r) : 0.f;
       const F2 w2 = f2(wr, wr);
-      const uint8_t* x = sm + (st * 3 + 1) * K::TILE + r * 128;
+      const uint8_t* x = sm + (st * K::TILES + K::TILES - 2) * K::TILE + r * 128;
       uint8_t* kp = sm + K::OFF_KP + b * 3 * K::TILE + cm_off(r, 0, DP);
 #pragma unroll 1
       for (int jj = 0; jj < DP / 8 / KP; ++jj) {
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
         arrive(&ctl.empty[st]);
       }
     }
-  } else if (w < K::W_Y) {
+  } else if (FWD && w < K::W_Y) {
     // ---- scores ----
     if (FWD) {
       const int q = w & 3, r = lane >> 2, c2 = 2 * (lane & 3), t0 = 16 * q + r;
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
         }
       }
     }
-  } else if (w < K::W_S) {
+  } else if (FWD && w < K::W_S) {
     // ---- outputs ----
     if (FWD) {
       const int q = w & 3, r = lane >> 2, c2 = 2 * (lane & 3), t0 = 16 * q + r;
@@ -406,14 +409,14 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
       put_state(mid_state(a, z.chain, z.seg + 1));
     else if (a.out && z.seg == a.segs - 1)
       put_state(a.out + z.chain * DD);
-  } else if (w < K::W_MMA + 3) {
+  } else if (w < K::W_MMA + K::MWARPS) {
     // ---- MMAs ----
     // Issuing blocks while the tensor pipe is busy, and a wait costs its latency even when it
     // is over at once; with one warp for all of them the pipe idled through every wait.
     // Descriptors step through a tile by adding to their start address (bytes / 16).
     const uint32_t base = smem_u32(sm);
     const uint32_t tmu = __shfl_sync(0xffffffffu, tm, 0);
-    auto tile = [&](int i, int which) { return base + ((i % K::STAGES) * 3 + which) * K::TILE; };
+    auto tile = [&](int i, int which) { return base + ((i % K::STAGES + 1) * K::TILES - which) * K::TILE; };  // 1: v, 2: k, 3: q
     if (w == K::W_MMA) {  // dS = K'^T V
       const uint32_t id = idesc_bf16(DP, DP, true, true);
       for (int i = 0; i < z.n; ++i) {
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
               (i < K::DBL || wait(ctl, &ctl.ds_free[b], n - 1, a.status))))
           break;
         fence_after();
-        const uint64_t v = desc_tile_mn(tile(i, 2)), kp = desc_mnmajor(base + K::OFF_KP + b * 3 * K::TILE, DP);
+        const uint64_t v = desc_tile_mn(tile(i, 1)), kp = desc_mnmajor(base + K::OFF_KP + b * 3 * K::TILE, DP);
 #pragma unroll 1
         for (int p = 2; p >= 0; --p)  // small parts first: each step truncates to the accumulator's exponent
 #pragma unroll
@@ -436,7 +439,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
     } else if (FWD && w == K::W_MMA + 1) {  // A = Q K^T of the next block, O = P V
       const uint32_t id = idesc_bf16(64, 64, false, false), ido = idesc_bf16(64, DP, false, true);
       auto scores = [&](int i) {
-        const uint64_t q = desc_tile(tile(i, 0)), k = desc_tile(tile(i, 1));
+        const uint64_t q = desc_tile(tile(i, 3)), k = desc_tile(tile(i, 2));
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
           const uint64_t o = ((ks >> 2) * BOX + (ks & 3) * 32) / 16;
@@ -459,7 +462,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
         ok = wait(ctl, &ctl.p_full[b], n, a.status) && (i < K::DBL || wait(ctl, &ctl.o_free[b], n - 1, a.status));
         if (!ok) break;
         fence_after();
-        const uint64_t v = desc_tile_mn(tile(i, 2)), pt = desc_kmajor(base + K::OFF_P + b * K::PT, C);
+        const uint64_t v = desc_tile_mn(tile(i, 1)), pt = desc_kmajor(base + K::OFF_P + b * K::PT, C);
 #pragma unroll
         for (int ks = 0; ks < C / 16; ++ks)
           mma_kf16(tmu + K::T_O + b * DP, pt + ks * (256 / 16), v + ks * (2048 / 16), ido, ks > 0);
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
               (i < K::DBL || wait(ctl, &ctl.o_free[b], n - 1, a.status))))
           break;
         fence_after();
-        const uint64_t q = desc_tile(tile(i, 0)), S = desc_mnmajor(base + K::OFF_S + b * 2 * K::ST, DP);
+        const uint64_t q = desc_tile(tile(i, 3)), S = desc_mnmajor(base + K::OFF_S + b * 2 * K::ST, DP);
 #pragma unroll 1
         for (int p = 1; p >= 0; --p)
 #pragma unroll
@@ -498,12 +501,12 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
       const int st = i % K::STAGES, blk = z.first + i * z.step;
       if (i >= K::STAGES && !wait(ctl, &ctl.empty[st], i / K::STAGES - 1, a.status)) break;
       const int nbox = D > 64 ? 2 : 1;
-      mbar_expect_tx(&ctl.full[st], (uint32_t)((FWD ? 3 : 2) * nbox * BOX));
-      uint8_t* t = sm + st * 3 * K::TILE;
+      mbar_expect_tx(&ctl.full[st], (uint32_t)(K::TILES * nbox * BOX));
+      uint8_t* t = sm + (st + 1) * K::TILES * K::TILE;
       for (int hb = 0; hb < nbox; ++hb) {
-        if (FWD) tma_load(t + hb * BOX, &map_q, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
-        tma_load(t + K::TILE + hb * BOX, &map_x, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
-        tma_load(t + 2 * K::TILE + hb * BOX, &map_y, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
+        if (FWD) tma_load(t - 3 * K::TILE + hb * BOX, &map_q, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
+        tma_load(t - 2 * K::TILE + hb * BOX, &map_x, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
+        tma_load(t - K::TILE + hb * BOX, &map_y, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
       }
     }
     if (ctl.bad)  // let the copies land before the CTA goes
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(Cfg<DP>::NT, 1)
   }
   fence_before();
   __syncthreads();
-  if (w == K::W_MMA) tmem_dealloc(tm, 512);
+  if (w == K::W_MMA) tmem_dealloc(tm, K::COLS);
 }
 
 // ---------------------------------------------------------------------------
@@ -559,9 +562,9 @@ bool mappable(const AtlasDecayParams& p, const int64_t* s) {
 template <int DP, bool FWD>
 static cudaError_t launch(const CUtensorMap& q, const CUtensorMap& x, const CUtensorMap& y, const CUtensorMap& o,
                           const SeqArgs& a, bool reversed, cudaStream_t s) {
-  cudaError_t e = allow_smem<seq_kernel<DP, FWD>>(SEQ_SMEM<DP>);
+  cudaError_t e = allow_smem<seq_kernel<DP, FWD>>(SEQ_SMEM<DP, FWD>);
   if (e != cudaSuccess) return e;
-  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums)), Cfg<DP>::NT, SEQ_SMEM<DP>, s>>>(q, x, y, o, a, reversed);
+  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums)), Cfg<DP, FWD>::NT, SEQ_SMEM<DP, FWD>, s>>>(q, x, y, o, a, reversed);
   return cudaGetLastError();
 }
 
