@@ -13,7 +13,7 @@
 //
 //     8 (4) warps   k' split into three bf16 parts (float32 accuracy of the state)
 //     4 warps       scores: A from TMEM, decayed, masked, rounded to bf16
-//     4 warps       outputs: O and QS from TMEM, y through shared memory and a TMA store
+//     4 warps       outputs: O and QS from TMEM, y to memory, 64 bytes of a row at a time
 //     8 (16) warps  the state: dS from TMEM, S in registers, two bf16 parts of S for QS
 //     3 warps       issue the MMAs;  one warp issues the TMA loads of q, k, v
 //
@@ -56,8 +56,7 @@ struct Cfg {
   static constexpr int OFF_KP = STAGES * TILES * TILE;
   static constexpr int OFF_P = OFF_KP + DBL * 3 * TILE;
   static constexpr int OFF_S = OFF_P + (FWD ? DBL * PT : 0);
-  static constexpr int OFF_Y = OFF_S + (FWD ? DBL * 2 * ST : 0);
-  static constexpr int OFF_CTL = OFF_Y + (FWD ? (DP == 64 ? 2 : 1) * BOX : 0);
+  static constexpr int OFF_CTL = OFF_S + (FWD ? DBL * 2 * ST : 0);
   // TMEM columns
   static constexpr uint32_t T_A = 0, T_DS = FWD ? DBL * 64 : 0, T_QS = T_DS + DBL * DP, T_O = T_QS + DBL * DP;
   static constexpr uint32_t COLS = FWD ? 512 : DBL * DP;
@@ -90,6 +89,7 @@ struct SeqArgs {
   // segment s to the place of segment s + 1.
   float* mid;
   int64_t mid_pitch, mid_first, mid_step;
+  bf16* y;
   float* saves;    // state entering every block, in the order of the walk; or NULL
   int segs;        // segments of a sequence
   int seg_blocks;  // blocks of a segment
@@ -122,16 +122,17 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) arrive(bar);
 }
 
-// Barrier of the four output warps; whether all of them say yes.
-__device__ __forceinline__ bool group_all(bool yes) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\t"
-      "selp.b32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)yes)
-      : "memory");
-  return r != 0;
+// Lanes 4 n .. 4 n + 3: v[j] of lane c and v[c] of lane j change places.
+__device__ __forceinline__ void quad_transpose(uint32_t* v, int c) {
+#pragma unroll
+  for (int m = 1; m <= 2; m *= 2)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int j = m == 1 ? 2 * n : n;  // pair (j, j + m)
+      const uint32_t x = __shfl_xor_sync(0xffffffffu, c & m ? v[j] : v[j + m], m);
+      v[j] = c & m ? x : v[j];
+      v[j + m] = c & m ? v[j + m] : x;
+    }
 }
 
 struct Walk {  // one CTA's blocks: first, first + step, ..., n of them
@@ -142,7 +143,7 @@ struct Walk {  // one CTA's blocks: first, first + step, ..., n of them
 template <int DP, bool FWD>
 __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     seq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_x,
-               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_o, const SeqArgs a,
+               const __grid_constant__ CUtensorMap map_y, const SeqArgs a,
                bool reversed) {
   using K = Cfg<DP, FWD>;
   extern __shared__ uint8_t raw[];
@@ -272,58 +273,42 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
   } else if (FWD && w < K::W_S) {
     // ---- outputs ----
     if (FWD) {
-      const int q = w & 3, r = lane >> 2, c2 = 2 * (lane & 3), t0 = 16 * q + r;
+      const int q = w & 3, r = lane >> 2, cq = lane & 3, t0 = 16 * q + r;
       const float i0 = P.scale * powd(g, t0 + 1), i1 = P.scale * powd(g, t0 + 9);
-      const bool lead = threadIdx.x == K::W_Y * 32;
       const F2 i02 = f2(i0, i0), i12 = f2(i1, i1), sc2 = f2(P.scale, P.scale);
+      const int64_t row = (int64_t)P.H * D;
+      bf16* y0 = a.y + (((int64_t)z.b * P.T + t0) * P.H + z.h) * D + 8 * cq;
       for (int i = 0; i < z.n; ++i) {
-        const int b = i % K::DBL, blk = z.first + i * z.step;
-        bool ok = wait(ctl, &ctl.o_full[b], i / K::DBL, a.status);
+        const int b = i % K::DBL, blk = z.first + i * z.step, L = P.T - blk * C;
+        if (!wait(ctl, &ctl.o_full[b], i / K::DBL, a.status)) break;
         fence_after();
-#pragma unroll
-        for (int hb = 0; hb < K::NB; ++hb) {
-          // the staging buffer of the store before last (DP = 128: of the last) has been read
-          if (lead) {
-            if (DP == 64)
-              asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-            else
-              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          }
-          if (!group_all(ok)) {  // the same verdict in all four warps
-            ok = false;
-            break;
-          }
-          uint8_t* y = sm + K::OFF_Y + (DP == 64 ? (i & 1) * BOX : 0) + t0 * 128 + 2 * c2;
-          const uint32_t at = tm + ((uint32_t)(32 * q) << 16) + b * DP + 64 * hb;
+        const uint32_t at = tm + ((uint32_t)(32 * q) << 16) + b * DP;
 #pragma unroll 1
-          for (int hc = 0; hc < 2; ++hc) {  // 32 columns
-            float v[16], x[16];
-            tmem_frag32(at + K::T_O + 32 * hc, v);
-            tmem_frag32(at + K::T_QS + 32 * hc, x);
-            tmem_wait_ld();
-            if (hb == K::NB - 1 && hc == 1) {
-              fence_before();
-              warp_arrive(&ctl.o_free[b]);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const F2 e = fma2(i02, f2(x[4 * j], x[4 * j + 1]), sc2 * f2(v[4 * j], v[4 * j + 1]));
-              const F2 f = fma2(i12, f2(x[4 * j + 2], x[4 * j + 3]), sc2 * f2(v[4 * j + 2], v[4 * j + 3]));
-              uint8_t* d = y + (((4 * hc + j) ^ r) << 4);  // t0 % 8 = r
-              *(uint32_t*)d = bf2_pack(e);
-              *(uint32_t*)(d + 8 * 128) = bf2_pack(f);
-            }
+        for (int col = 0; col < DP; col += 32) {
+          float v[16], x[16];
+          tmem_frag32(at + K::T_O + col, v);
+          tmem_frag32(at + K::T_QS + col, x);
+          tmem_wait_ld();
+          if (col == DP - 32) {
+            fence_before();
+            warp_arrive(&ctl.o_free[b]);
           }
-          fence_async_smem();
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          if (lead) {
-            if (64 * hb < D) tma_store(&map_o, 64 * hb, z.h, blk * C, z.b, y - (t0 * 128 + 2 * c2));
-            bulk_commit();
+          uint32_t e[4], f[4];  // rows t0 and t0 + 8, columns 8 j + 2 cq and the next
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            e[j] = bf2_pack(fma2(i02, f2(x[4 * j], x[4 * j + 1]), sc2 * f2(v[4 * j], v[4 * j + 1])));
+            f[j] = bf2_pack(fma2(i12, f2(x[4 * j + 2], x[4 * j + 3]), sc2 * f2(v[4 * j + 2], v[4 * j + 3])));
+          }
+          // now columns 8 cq .. 8 cq + 7: 16 bytes a lane, 64 in a row for the four lanes of one
+          quad_transpose(e, cq);
+          quad_transpose(f, cq);
+          bf16* y = y0 + (int64_t)blk * C * row + col;
+          if (col + 8 * cq < D) {
+            if (t0 < L) *(uint4*)y = make_uint4(e[0], e[1], e[2], e[3]);
+            if (t0 + 8 < L) *(uint4*)(y + 8 * row) = make_uint4(f[0], f[1], f[2], f[3]);
           }
         }
-        if (!ok) break;
       }
-      if (lead) bulk_wait0();
     }
   } else if (w < K::W_MMA) {
     // ---- the state ----
@@ -560,11 +545,11 @@ bool mappable(const AtlasDecayParams& p, const int64_t* s) {
 }
 
 template <int DP, bool FWD>
-static cudaError_t launch(const CUtensorMap& q, const CUtensorMap& x, const CUtensorMap& y, const CUtensorMap& o,
-                          const SeqArgs& a, bool reversed, cudaStream_t s) {
+static cudaError_t launch(const CUtensorMap& q, const CUtensorMap& x, const CUtensorMap& y, const SeqArgs& a,
+                          bool reversed, cudaStream_t s) {
   cudaError_t e = allow_smem<seq_kernel<DP, FWD>>(SEQ_SMEM<DP, FWD>);
   if (e != cudaSuccess) return e;
-  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums)), Cfg<DP, FWD>::NT, SEQ_SMEM<DP, FWD>, s>>>(q, x, y, o, a, reversed);
+  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums)), Cfg<DP, FWD>::NT, SEQ_SMEM<DP, FWD>, s>>>(q, x, y, a, reversed);
   return cudaGetLastError();
 }
 
@@ -621,13 +606,12 @@ cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, flo
                        cudaStream_t s) {
   const AtlasDecayParams& p = a.p;
   const int64_t flat[3] = {(int64_t)p.T * p.H * p.D, (int64_t)p.H * p.D, p.D};
-  CUtensorMap mq{}, mx{}, my{}, mo{};
+  CUtensorMap mq{}, mx{}, my{};
   bool ok;
   if (bwd)
     ok = make_map(&mx, a.q, p, p.q_stride) && make_map(&my, a.dy, p, flat);
   else
-    ok = make_map(&mq, a.q, p, p.q_stride) && make_map(&mx, a.k, p, p.k_stride) && make_map(&my, a.v, p, p.v_stride) &&
-         make_map(&mo, a.y, p, flat);
+    ok = make_map(&mq, a.q, p, p.q_stride) && make_map(&mx, a.k, p, p.k_stride) && make_map(&my, a.v, p, p.v_stride);
   if (!ok) return cudaErrorInvalidValue;
   const Split z = split(p);
   const bool wide = p.D > 64;
@@ -636,6 +620,7 @@ cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, flo
   q.log_decay = a.log_decay;
   q.in = in;
   q.out = out;
+  q.y = (bf16*)a.y;
   q.saves = nullptr;
   q.segs = z.segs;
   q.seg_blocks = z.blocks;
@@ -653,7 +638,7 @@ cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, flo
   }
   if (z.segs > 1) {
     q.sums = 1;
-    cudaError_t e = wide ? launch<128, false>(mq, mx, my, mo, q, bwd, s) : launch<64, false>(mq, mx, my, mo, q, bwd, s);
+    cudaError_t e = wide ? launch<128, false>(mq, mx, my, q, bwd, s) : launch<64, false>(mq, mx, my, q, bwd, s);
     if (e != cudaSuccess) return e;
     const int full = z.blocks * C, last = p.T - (z.segs - 1) * full;
     const int64_t n = chains(p) * p.D * p.D / 4;
@@ -663,8 +648,8 @@ cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, flo
     q.sums = 0;
   }
   q.saves = saves;
-  if (bwd) return wide ? launch<128, false>(mq, mx, my, mo, q, true, s) : launch<64, false>(mq, mx, my, mo, q, true, s);
-  return wide ? launch<128, true>(mq, mx, my, mo, q, false, s) : launch<64, true>(mq, mx, my, mo, q, false, s);
+  if (bwd) return wide ? launch<128, false>(mq, mx, my, q, true, s) : launch<64, false>(mq, mx, my, q, true, s);
+  return wide ? launch<128, true>(mq, mx, my, q, false, s) : launch<64, true>(mq, mx, my, q, false, s);
 }
 
 }  // namespace tcore
