@@ -374,20 +374,22 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
       }
       if (!wait(ctl, &ctl.ds_full[b], n, a.status)) break;
       fence_after();
-      float v[4 * NJ];
-      if constexpr (DP == 64)
-        tmem_frag32(at + b * DP, v);
-      else
-        tmem_frag64(at + b * DP, v);
-      tmem_wait_ld();
-      fence_before();
-      warp_arrive(&ctl.ds_free[b]);
       const F2 h2 = f2(fbh, fbh), l2 = f2(fbl, fbl), c = f2(sc, sc);
 #pragma unroll
-      for (int j = 0; j < 2 * NJ; ++j) {
-        F2 x = f2(v[2 * j], v[2 * j + 1]);
-        if (!FWD) x = x * c;
-        S[j] = fma2(S[j], h2, fma2(S[j], l2, x));
+      for (int j = 0; j < 2 * NJ; j += 8) {  // 32 columns at a time: the registers of 1024 threads hold no more
+        float v[16];
+        tmem_frag32(at + b * DP + 4 * j, v);
+        tmem_wait_ld();
+        if (j == 2 * NJ - 8) {
+          fence_before();
+          warp_arrive(&ctl.ds_free[b]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          F2 x = f2(v[2 * k], v[2 * k + 1]);
+          if (!FWD) x = x * c;
+          S[j + k] = fma2(S[j + k], h2, fma2(S[j + k], l2, x));
+        }
       }
     }
     if (a.sums)
