@@ -32,7 +32,8 @@ def _lib():
     lib = L.load()
     if not _bound:
         pp = ctypes.POINTER(AtlasDecayParams)
-        for n in ("atlas_decay_saved_bytes", "atlas_decay_fwd_workspace_bytes", "atlas_decay_bwd_workspace_bytes"):
+        for n in ("atlas_decay_saved_bytes", "atlas_decay_fwd_workspace_bytes",
+                  "atlas_decay_saved_workspace_bytes", "atlas_decay_bwd_workspace_bytes"):
             getattr(lib, n).restype = ctypes.c_size_t
             getattr(lib, n).argtypes = [pp]
         lib.atlas_decay_fwd.restype = ctypes.c_int
@@ -73,6 +74,7 @@ class _Plan:
         self.B, self.state_shape = B, (B, H, D, D)
         self.saved_bytes = self._size(self.lib.atlas_decay_saved_bytes)
         self.fwd_workspace_bytes = self._size(self.lib.atlas_decay_fwd_workspace_bytes)
+        self.saved_workspace_bytes = self._size(self.lib.atlas_decay_saved_workspace_bytes)
         self.bwd_workspace_bytes = self._size(self.lib.atlas_decay_bwd_workspace_bytes)
 
     def _size(self, query):
@@ -120,10 +122,10 @@ def decay_attention_forward(q, k, v, log_decay, state=None, scale=None, need_sav
             return decay_attention_forward(q, k, v, log_decay, state, scale, need_saved, workspace)
     y = empty_like(q)
     out = torch.empty(*p.state_shape, device=dev) if state is None else torch.empty_like(state)
+    saved, need = None, p.fwd_workspace_bytes
     if need_saved:
-        saved, ws, wsb = torch.empty(p.saved_bytes // 4, device=dev), None, 0
-    else:
-        saved, (ws, wsb) = None, (workspace or _WS).get(p.fwd_workspace_bytes, dev)
+        saved, need = torch.empty(p.saved_bytes // 4, device=dev), p.saved_workspace_bytes
+    ws, wsb = (workspace or _WS).get(need, dev)
     rc = p.lib.atlas_decay_fwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), addr(state),
                                y.data_ptr(), out.data_ptr(), addr(saved), addr(ws), wsb, stream_of(dev))
     if rc:

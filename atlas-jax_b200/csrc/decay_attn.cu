@@ -654,9 +654,6 @@ static size_t state_bytes(const AtlasDecayParams& p) {
   return (size_t)chains(p) * chunks(p) * p.D * p.D * sizeof(float);
 }
 static int parts(const AtlasDecayParams& p) { return 2 * chunks(p) * (CH / TT); }  // of dlog_decay per chain
-static size_t ws_bytes(const AtlasDecayParams& p) {
-  return state_bytes(p) + (size_t)chains(p) * parts(p) * sizeof(float);
-}
 static int status_of(cudaError_t e) {
   return e == cudaSuccess ? ATLAS_OK : report_error(ATLAS_ERR_CUDA, cudaGetErrorString(e));
 }
@@ -668,8 +665,15 @@ static bool tensor_path(const AtlasDecayParams& p) {
   return p.act_dtype == ATLAS_BF16 && p.D % 8 == 0 && p.aligned16 && tcore::mappable(p, p.q_stride) &&
          tcore::mappable(p, p.k_stride) && tcore::mappable(p, p.v_stride);
 }
-// what the forward needs where it keeps no states
-static size_t fwd_bytes(const AtlasDecayParams& p) { return tensor_path(p) ? tcore::mid_bytes(p) : state_bytes(p); }
+// workspaces: the sums of a split walk (tensor path); the chunks' states, where they are not kept
+static size_t fwd_bytes(const AtlasDecayParams& p, bool saved) {
+  return tensor_path(p) ? tcore::sums_bytes(p) : saved ? 0 : state_bytes(p);
+}
+// the chunks' cotangent states, the sums of their walk, the parts of dlog_decay
+static size_t bwd_states(const AtlasDecayParams& p) { return state_bytes(p) + (tensor_path(p) ? tcore::sums_bytes(p) : 0); }
+static size_t bwd_bytes(const AtlasDecayParams& p) {
+  return bwd_states(p) + (size_t)chains(p) * parts(p) * sizeof(float);
+}
 // the pointers that a call promises to be 16-byte aligned
 template <class... T>
 static int check_aligned(const AtlasDecayParams& p, T... ptr) {
@@ -769,12 +773,17 @@ extern "C" size_t atlas_decay_saved_bytes(const AtlasDecayParams* p) {
 
 extern "C" size_t atlas_decay_fwd_workspace_bytes(const AtlasDecayParams* p) {
   if (check(p) != ATLAS_OK) return 0;
-  return fwd_bytes(*p);
+  return fwd_bytes(*p, false);
+}
+
+extern "C" size_t atlas_decay_saved_workspace_bytes(const AtlasDecayParams* p) {
+  if (check(p) != ATLAS_OK) return 0;
+  return fwd_bytes(*p, true);
 }
 
 extern "C" size_t atlas_decay_bwd_workspace_bytes(const AtlasDecayParams* p) {
   if (check(p) != ATLAS_OK) return 0;
-  return ws_bytes(*p);
+  return bwd_bytes(*p);
 }
 
 extern "C" int atlas_decay_fwd(const AtlasDecayParams* p, const void* q, const void* k, const void* v,
@@ -787,10 +796,11 @@ extern "C" int atlas_decay_fwd(const AtlasDecayParams* p, const void* q, const v
   if (!state_out || !log_decay) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
   if (p->T == 0) return status_of(pass_state(*p, state_in, state_out, s));
   if (!q || !k || !v || !y) return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
-  const size_t need = saved ? 0 : fwd_bytes(*p);
+  const size_t need = fwd_bytes(*p, saved != nullptr);
   if (need && (!workspace || workspace_bytes < need))
-    return report_error(ATLAS_ERR_WORKSPACE, "workspace smaller than atlas_decay_fwd_workspace_bytes()");
-  rc = check_aligned(*p, q, k, v, y, state_in, state_out, saved, saved ? nullptr : workspace);
+    return report_error(ATLAS_ERR_WORKSPACE, "workspace smaller than atlas_decay_fwd_workspace_bytes() (with saved: "
+                                             "atlas_decay_saved_workspace_bytes())");
+  rc = check_aligned(*p, q, k, v, y, state_in, state_out, saved, need ? workspace : nullptr);
   if (rc) return rc;
   Args a{};
   a.p = *p;
@@ -822,7 +832,7 @@ extern "C" int atlas_decay_bwd(const AtlasDecayParams* p, const void* q, const v
   }
   if (!q || !k || !v || !log_decay || !saved || !dy || !dq || !dk || !dv)
     return report_error(ATLAS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
-  if (!workspace || workspace_bytes < ws_bytes(*p))
+  if (!workspace || workspace_bytes < bwd_bytes(*p))
     return report_error(ATLAS_ERR_WORKSPACE, "workspace smaller than atlas_decay_bwd_workspace_bytes()");
   rc = check_aligned(*p, q, k, v, dy, dq, dk, dv, saved, dstate_out, dstate_in, workspace);
   if (rc) return rc;
@@ -833,11 +843,11 @@ extern "C" int atlas_decay_bwd(const AtlasDecayParams* p, const void* q, const v
   a.dq = dq, a.dk = dk, a.dv = dv;
   a.states = (float*)const_cast<void*>(saved);
   a.dstates = (float*)workspace;
-  a.dg_part = (float*)((uint8_t*)workspace + state_bytes(*p));
+  a.dg_part = (float*)((uint8_t*)workspace + bwd_states(*p));
   a.status = device_status_ptr();
   const bool tensor = tensor_path(*p);
   a.dg_parts = tensor ? chunks(*p) : 2 * ((p->T + TT - 1) / TT);
-  cudaError_t e = tensor ? tcore::launch_seq(a, true, dstate_out, dstate_in, a.dstates, nullptr, s)
+  cudaError_t e = tensor ? tcore::launch_seq(a, true, dstate_out, dstate_in, a.dstates, (float*)workspace + state_bytes(*p) / sizeof(float), s)
                          : plain_states(a, dstate_out, dstate_in, true, s);
   if (e == cudaSuccess) e = tensor ? tcore::launch_grads(a, s) : plain(a, GRADS, s);
   if (e == cudaSuccess && dlog_decay) {

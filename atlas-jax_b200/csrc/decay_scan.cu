@@ -22,8 +22,8 @@
 // taken from the last to the first, the cotangent states of the backward.
 //
 // A sequence is split into segments where there are fewer (batch, head) pairs than SMs: the
-// segments' sums first, then the recurrence over segments, then every segment from the
-// state that enters it.
+// segments' sums first, then every segment, from a state put together from the sums before
+// it.
 //
 // Layout: q, k, v, y tiles as TMA writes them (rows of 128 bytes, 128-byte swizzle, a box per
 // 64 channels); k', scores and S in the core-matrix layout of tc_ops.cuh.  All M = 64
@@ -50,13 +50,18 @@ struct Cfg {
   static constexpr int SWARPS = DP == 64 ? 8 : 16;      // warps of the state group
   static constexpr int MWARPS = FWD ? 3 : 1;            // warps that issue MMAs
   static constexpr int W_P = KWARPS, W_Y = W_P + (FWD ? 4 : 0), W_S = W_Y + (FWD ? 4 : 0), W_MMA = W_S + SWARPS;  // first warps of the groups
-  static constexpr int NT = 32 * (W_MMA + MWARPS + 1);
+  static constexpr int W_LOAD = W_MMA + MWARPS, NT = 32 * (W_LOAD + 1);
   static constexpr int PT = C * C * 2;                  // a tile of scores
   static constexpr int ST = DP * DP * 2;                // one part of a state
   static constexpr int OFF_KP = STAGES * TILES * TILE;
   static constexpr int OFF_P = OFF_KP + DBL * 3 * TILE;
   static constexpr int OFF_S = OFF_P + (FWD ? DBL * PT : 0);
   static constexpr int OFF_CTL = OFF_S + (FWD ? DBL * 2 * ST : 0);
+  // Whether a segment puts its entering state together itself.  At D = 128 that is 64 KB a segment before
+  // it, read at 2 to 3 us each (32 loads a thread with S in registers: few in flight), and join_kernel
+  // is faster: 4 x 1900 tokens x 6 heads 26.7 + 4.8 us against 38.7.  At D = 64 the launch costs more:
+  // 3 x 777 x 12 10.2 + 3.0 us against 10.4.
+  static constexpr bool JOIN = DP == 64;
   // TMEM columns
   static constexpr uint32_t T_A = 0, T_DS = FWD ? DBL * 64 : 0, T_QS = T_DS + DBL * DP, T_O = T_QS + DBL * DP;
   static constexpr uint32_t COLS = FWD ? 512 : DBL * DP;
@@ -84,20 +89,18 @@ struct SeqArgs {
   const float* log_decay;
   const float* in;  // (chains, D, D) entering the first segment of the walk, or NULL: zeros
   float* out;       // leaving the last one
-  // The states entering segments 1, 2, .. of the walk: segment s of a chain at
-  // (chain * mid_pitch + mid_first + s * mid_step) * D * D.  The sums' pass writes the sum of
-  // segment s to the place of segment s + 1.
-  float* mid;
-  int64_t mid_pitch, mid_first, mid_step;
+  // What enters segments 0 and 1 of every chain's walk and the sums of segments 1 .. segs - 2, written
+  // by the sums' pass.  Segment 0's is a copy, so that `out` may be `in`.
+  float* sums;
   bf16* y;
   float* saves;    // state entering every block, in the order of the walk; or NULL
   int segs;        // segments of a sequence
   int seg_blocks;  // blocks of a segment
-  int sums;        // the sums' pass: segments 0 .. segs - 2, each from zeros
+  int sums_pass;   // segments 0 .. segs - 2, all but the first from zeros, to `sums`
   int* status;
 };
-__device__ __forceinline__ float* mid_state(const SeqArgs& a, int64_t chain, int s) {
-  return a.mid + (chain * a.mid_pitch + a.mid_first + s * a.mid_step) * a.p.D * a.p.D;
+__device__ __forceinline__ float* sum_at(const SeqArgs& a, int64_t chain, int i) {
+  return a.sums + (chain * a.segs + i) * a.p.D * a.p.D;
 }
 
 // Waits for completion number n (from 0) of a barrier.  Bounded; a timeout anywhere in the
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
   const int w = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int D = P.D, nblk = (P.T + C - 1) / C;
   Walk z;
-  const int per_chain = a.segs - a.sums;
+  const int per_chain = a.segs - a.sums_pass;
   z.chain = blockIdx.x / per_chain;
   z.seg = (int)(blockIdx.x % per_chain);  // in the order of the walk
   z.b = (int)(z.chain / P.H);
@@ -166,13 +169,18 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     z.first = reversed ? hi - 1 : lo;
     z.step = reversed ? -1 : 1;
   }
-  const float g = a.log_decay[z.h];
-
-  if (w == K::W_MMA) {
-    tmem_alloc(&ctl.tmem, K::COLS);
-    tmem_relinquish();
-  }
-  if (threadIdx.x == 0) {
+  const int nbox = D > 64 ? 2 : 1;
+  auto load_block = [&](int i) {  // one thread
+    const int st = i % K::STAGES, blk = z.first + i * z.step;
+    mbar_expect_tx(&ctl.full[st], (uint32_t)(K::TILES * nbox * BOX));
+    uint8_t* t = sm + (st + 1) * K::TILES * K::TILE;
+    for (int hb = 0; hb < nbox; ++hb) {
+      if (FWD) tma_load(t - 3 * K::TILE + hb * BOX, &map_q, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
+      tma_load(t - 2 * K::TILE + hb * BOX, &map_x, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
+      tma_load(t - K::TILE + hb * BOX, &map_y, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
+    }
+  };
+  if (w == K::W_LOAD && lane == 0) {
     for (int i = 0; i < K::STAGES; ++i) {
       mbar_init(&ctl.full[i], 1);
       mbar_init(&ctl.empty[i], K::MWARPS + K::KWARPS);  // the issuing warps' last MMAs, and the warps that read k
@@ -194,7 +202,13 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     mbar_init(&ctl.fin, K::MWARPS);
     ctl.bad = 0;
     fence_mbar_init();
+    for (int i = 0; i < min(K::STAGES, z.n); ++i) load_block(i);  // on their way while the rest is set up
   }
+  if (w == K::W_MMA) {
+    tmem_alloc(&ctl.tmem, K::COLS);
+    tmem_relinquish();
+  }
+  const float g = a.log_decay[z.h];
   for (int u = threadIdx.x; u < 2 * C; u += K::NT) ctl.w[u] = f2(powd(g, max(u - C, 0)), powd(g, max(u - C - 1, 0)));
   if (FWD)  // score blocks above the diagonal are written here once and never again
     for (int u = threadIdx.x; u < K::DBL * K::PT / 16; u += K::NT) *(uint4*)(sm + K::OFF_P + u * 16) = make_uint4(0, 0, 0, 0);
@@ -323,16 +337,30 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     const int64_t DD = (int64_t)D * D;
     const bool in0 = d0 < D, in1 = d0 + 8 < D;
     {
-      const float* s = a.sums ? nullptr : z.seg > 0 ? mid_state(a, z.chain, z.seg) : a.in ? a.in + z.chain * DD : nullptr;
+      // S = f s + S for the state at s (or zeros); f as a float pair
+      auto add_state = [&](const float* s, double f, bool first) {
+        const float fh = (float)f, fl = (float)(f - (double)fh);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int e = e0 + 8 * j + c2;
-        float2 x = make_float2(0.f, 0.f), y = x;
-        if (s && e < D) {
-          if (in0) x = *(const float2*)(s + (int64_t)d0 * D + e);
-          if (in1) y = *(const float2*)(s + (int64_t)(d0 + 8) * D + e);
+        for (int j = 0; j < NJ; ++j) {
+          const int e = e0 + 8 * j + c2;
+          float2 x = make_float2(0.f, 0.f), y = x;
+          if (s && e < D) {
+            if (in0) x = *(const float2*)(s + (int64_t)d0 * D + e);
+            if (in1) y = *(const float2*)(s + (int64_t)(d0 + 8) * D + e);
+          }
+          const F2 h2 = f2(fh, fh), l2 = f2(fl, fl);
+          S[2 * j] = first ? f2(x.x, x.y) : fma2(S[2 * j], h2, fma2(S[2 * j], l2, f2(x.x, x.y)));
+          S[2 * j + 1] = first ? f2(y.x, y.y) : fma2(S[2 * j + 1], h2, fma2(S[2 * j + 1], l2, f2(y.x, y.y)));
         }
-        S[2 * j] = f2(x.x, x.y), S[2 * j + 1] = f2(y.x, y.y);
+      };
+      const float* in = a.in ? a.in + z.chain * DD : nullptr;
+      if (a.sums_pass || a.segs == 1) {
+        add_state(z.seg == 0 ? in : nullptr, 0., true);
+      } else if (z.seg == 0) {
+        add_state(in ? sum_at(a, z.chain, 0) : nullptr, 0., true);
+      } else {
+        const double f = exp((double)g * ((double)a.seg_blocks * C));
+        for (int j = K::JOIN ? 1 : z.seg; j <= z.seg; ++j) add_state(sum_at(a, z.chain, j), f, j == (K::JOIN ? 1 : z.seg));
       }
     }
     auto put_state = [&](float* out) {
@@ -345,6 +373,7 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
         }
       }
     };
+    if (a.sums_pass && z.seg == 0 && a.in) put_state(sum_at(a, z.chain, 0));
     // decay over a block as a float pair: its rounding would be multiplied in again every block
     const double fd = exp((double)g * C);
     const float fh = (float)fd, fl = (float)(fd - (double)fh), sc = reversed ? P.scale : 1.f;
@@ -392,8 +421,8 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
         }
       }
     }
-    if (a.sums)
-      put_state(mid_state(a, z.chain, z.seg + 1));
+    if (a.sums_pass)
+      put_state(sum_at(a, z.chain, z.seg + 1));
     else if (a.out && z.seg == a.segs - 1)
       put_state(a.out + z.chain * DD);
   } else if (w < K::W_MMA + K::MWARPS) {
@@ -483,18 +512,10 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     }
   } else if (lane == 0) {
     // ---- loads ----
-    int i = 0;
+    int i = min(K::STAGES, z.n);
     for (; i < z.n; ++i) {
-      const int st = i % K::STAGES, blk = z.first + i * z.step;
-      if (i >= K::STAGES && !wait(ctl, &ctl.empty[st], i / K::STAGES - 1, a.status)) break;
-      const int nbox = D > 64 ? 2 : 1;
-      mbar_expect_tx(&ctl.full[st], (uint32_t)(K::TILES * nbox * BOX));
-      uint8_t* t = sm + (st + 1) * K::TILES * K::TILE;
-      for (int hb = 0; hb < nbox; ++hb) {
-        if (FWD) tma_load(t - 3 * K::TILE + hb * BOX, &map_q, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
-        tma_load(t - 2 * K::TILE + hb * BOX, &map_x, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
-        tma_load(t - K::TILE + hb * BOX, &map_y, 64 * hb, z.h, blk * C, z.b, &ctl.full[st]);
-      }
+      if (!wait(ctl, &ctl.empty[i % K::STAGES], i / K::STAGES - 1, a.status)) break;
+      load_block(i);
     }
     if (ctl.bad)  // let the copies land before the CTA goes
       for (int k = max(0, i - K::STAGES); k < i; ++k)
@@ -551,13 +572,13 @@ static cudaError_t launch(const CUtensorMap& q, const CUtensorMap& x, const CUte
                           bool reversed, cudaStream_t s) {
   cudaError_t e = allow_smem<seq_kernel<DP, FWD>>(SEQ_SMEM<DP, FWD>);
   if (e != cudaSuccess) return e;
-  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums)), Cfg<DP, FWD>::NT, SEQ_SMEM<DP, FWD>, s>>>(q, x, y, a, reversed);
+  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums_pass)), Cfg<DP, FWD>::NT, SEQ_SMEM<DP, FWD>, s>>>(q, x, y, a, reversed);
   return cudaGetLastError();
 }
 
 // How many segments to cut a sequence into, and their blocks.  In block times: a CTA an SM,
-// rounds of them; a split adds the sums' pass, at about 0.5 of a full block's time, and two
-// launches (about 4 blocks' time).
+// rounds of them; a split adds the sums' pass, at about 0.5 of a full block's time, its
+// launch and the reading of its sums (about 4 blocks' time).
 struct Split {
   int segs, blocks;
 };
@@ -575,36 +596,34 @@ static Split split(const AtlasDecayParams& p) {
   return best;
 }
 
-// The states entering segments 1, 2, ..: S <- l^len S + sum, in place.  One thread per 4
-// elements of a chain's state; len: of segment 0, and of the others.
-__global__ void __launch_bounds__(256) mid_kernel(SeqArgs a, int len0, int len) {
+// What enters segments 2, 3, ..: S <- l^len S + sum, in place, len tokens each.  One thread per 4
+// elements of a chain's state.
+__global__ void __launch_bounds__(256) join_kernel(SeqArgs a) {
   const int per = a.p.D * a.p.D / 4;
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (u >= chains(a.p) * per) return;
   const int64_t chain = u / per;
-  const int e = (int)(u - chain * per) * 4;
-  const double g = (double)a.log_decay[chain % a.p.H], f = exp(g * len);
-  float4 S = a.in ? *(const float4*)(a.in + chain * per * 4 + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-  float4 x = *(const float4*)(mid_state(a, chain, 1) + e);
-  for (int s = 1; s < a.segs; ++s) {
-    float* m = mid_state(a, chain, s) + e;
-    const float4 y = s + 1 < a.segs ? *(const float4*)(mid_state(a, chain, s + 1) + e) : x;  // the next load early
-    const double fs = s == 1 ? exp(g * len0) : f;
-    const float fh = (float)fs, fl = (float)(fs - (double)fh);
+  float4* m = (float4*)sum_at(a, chain, 1) + (u - chain * per);
+  const double f = exp((double)a.log_decay[chain % a.p.H] * ((double)a.seg_blocks * C));
+  const float fh = (float)f, fl = (float)(f - (double)fh);
+  float4 S = m[0], x = m[per];
+  for (int s = 2; s < a.segs; ++s) {
+    const float4 y = s + 1 < a.segs ? m[(int64_t)s * per] : x;  // the next load early
     S.x = fmaf(S.x, fh, fmaf(S.x, fl, x.x));
     S.y = fmaf(S.y, fh, fmaf(S.y, fl, x.y));
     S.z = fmaf(S.z, fh, fmaf(S.z, fl, x.z));
     S.w = fmaf(S.w, fh, fmaf(S.w, fl, x.w));
-    *(float4*)m = S;
+    m[(int64_t)(s - 1) * per] = S;
     x = y;
   }
 }
 
-size_t mid_bytes(const AtlasDecayParams& p) {
-  return (size_t)chains(p) * (split(p).segs - 1) * p.D * p.D * sizeof(float);
+size_t sums_bytes(const AtlasDecayParams& p) {
+  const int segs = split(p).segs;
+  return segs > 1 ? (size_t)chains(p) * segs * p.D * p.D * sizeof(float) : 0;
 }
 
-cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, float* saves, float* mid,
+cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, float* saves, float* sums,
                        cudaStream_t s) {
   const AtlasDecayParams& p = a.p;
   const int64_t flat[3] = {(int64_t)p.T * p.H * p.D, (int64_t)p.H * p.D, p.D};
@@ -627,27 +646,18 @@ cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, flo
   q.segs = z.segs;
   q.seg_blocks = z.blocks;
   q.status = a.status;
-  if (saves) {  // a segment's entering state is that of its first block in the walk
-    q.mid = saves;
-    q.mid_pitch = chunks(p);
-    q.mid_first = bwd ? (int64_t)z.segs * z.blocks - 1 : 0;
-    q.mid_step = bwd ? -z.blocks : z.blocks;
-  } else {
-    q.mid = mid;
-    q.mid_pitch = z.segs - 1;
-    q.mid_first = -1;
-    q.mid_step = 1;
-  }
+  q.sums = sums;
   if (z.segs > 1) {
-    q.sums = 1;
+    q.sums_pass = 1;
     cudaError_t e = wide ? launch<128, false>(mq, mx, my, q, bwd, s) : launch<64, false>(mq, mx, my, q, bwd, s);
     if (e != cudaSuccess) return e;
-    const int full = z.blocks * C, last = p.T - (z.segs - 1) * full;
-    const int64_t n = chains(p) * p.D * p.D / 4;
-    mid_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(q, bwd ? last : full, full);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    q.sums = 0;
+    q.sums_pass = 0;
+    if (wide && z.segs > 2) {
+      const int64_t n = chains(p) * p.D * p.D / 4;
+      join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(q);
+      e = cudaGetLastError();
+      if (e != cudaSuccess) return e;
+    }
   }
   q.saves = saves;
   if (bwd) return wide ? launch<128, false>(mq, mx, my, q, true, s) : launch<64, false>(mq, mx, my, q, true, s);

@@ -61,9 +61,10 @@ typedef struct {
  * (0 on invalid params, with the message set, and for empty problems). */
 size_t atlas_decay_saved_bytes(const AtlasDecayParams* p);
 
-/* Bytes of workspace of a forward without `saved`, and of the backward (0 on invalid params,
+/* Bytes of workspace of a forward without `saved`, of one with it, and of the backward (0 on invalid params,
  * and where none is needed). */
 size_t atlas_decay_fwd_workspace_bytes(const AtlasDecayParams* p);
+size_t atlas_decay_saved_workspace_bytes(const AtlasDecayParams* p);
 size_t atlas_decay_bwd_workspace_bytes(const AtlasDecayParams* p);
 
 /* Forward.  state_in may be NULL (zeros); state_out = S after token T - 1 and may be the same

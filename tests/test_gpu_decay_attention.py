@@ -241,6 +241,25 @@ def test_backward_is_deterministic_and_streams_are_kept():
         assert torch.equal(x, z)
 
 
+@pytest.mark.parametrize("T,D,need_saved", [(700, 128, True), (700, 128, False), (1500, 64, False), (300, 24, True)])
+def test_state_in_its_own_place(T, D, need_saved):
+    """The state left may go to where the one entering came from, also where a sequence is split."""
+    from atlas_b200.decay_attention import _plan, decay_attention_forward
+    q, k, v, g, S, _, _ = _inputs(2, T, 3, D, BF, True, True, T)
+    y, out, saved = decay_attention_forward(q, k, v, g, S, 0.5, need_saved)
+    p, q, k, v = _plan(q, k, v, g, 0.5)
+    y2, S2 = torch.empty_like(y), S.clone()
+    saved2 = torch.empty_like(saved) if need_saved else None
+    n = p.saved_workspace_bytes if need_saved else p.fwd_workspace_bytes
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+    s = torch.cuda.current_stream().cuda_stream
+    assert 0 == p.lib.atlas_decay_fwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), S2.data_ptr(),
+                                      y2.data_ptr(), S2.data_ptr(), saved2.data_ptr() if need_saved else None,
+                                      ws.data_ptr(), n, s)
+    assert torch.equal(y, y2) and torch.equal(out, S2)
+    assert not need_saved or torch.equal(saved, saved2)
+
+
 def test_offsets_beyond_32_bits():
     """Sequences more than 2^31 elements apart in one buffer."""
     from atlas_b200.decay_attention import decay_attention_forward, decay_attention_step
