@@ -236,35 +236,38 @@ __global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd, bool vec) {
 }
 
 // acc (rows ty, ty + 16; the thread's columns) += w_r * sum_m A[r][m] M(m, column) over a D x D
-// matrix in global memory; transposed: M(m, c) = M[c][m].  `stage` is a free tile.
+// matrix in global memory; transposed: M(m, c) = M[c][m].  `stage`: two free tiles, SR rows.
 template <int DP>
 __device__ void times_state(float (*acc)[Tile<DP>::NC], const Tile<DP>& A, const float* M, bool transposed, int D,
-                            const float* w, Tile<DP>& stage) {
+                            const float* w, Tile<DP>* stage) {
   using L = Tile<DP>;
+  constexpr int SR = DP < 2 * TT ? DP : 2 * TT;
+  float(*st)[L::LD] = stage->x;  // the second tile follows the first
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   float part[2][L::NC];
 #pragma unroll
   for (int j = 0; j < L::NC; ++j) part[0][j] = part[1][j] = 0.f;
-  for (int m0 = 0; m0 < D; m0 += TT) {
-    __syncthreads();
+  for (int m0 = 0; m0 < D; m0 += SR) {
+    if (m0) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < TT * DP / 256; ++i) {
+    for (int i = 0; i < SR * DP / 256; ++i) {
       const int u = threadIdx.x + 256 * i;
       // consecutive threads along the contiguous axis of M
-      const int m = transposed ? u % TT : u / DP, c = transposed ? u / TT : u % DP;
+      const int m = transposed ? u % SR : u / DP, c = transposed ? u / SR : u % DP;
       float x = 0.f;
       if (m0 + m < D && c < D) x = transposed ? M[(int64_t)c * D + m0 + m] : M[(int64_t)(m0 + m) * D + c];
-      stage.x[m][c] = x;
+      st[m][c] = x;
     }
     __syncthreads();
-#pragma unroll
-    for (int m = 0; m < TT; m += 4) {  // rows of `stage` beyond D are 0
+    const int n = min(SR, (D - m0 + 3) & ~3);
+#pragma unroll 4
+    for (int m = 0; m < n; m += 4) {  // rows beyond D are 0
       const float4 a0 = *(const float4*)&A.x[ty][m0 + m], a1 = *(const float4*)&A.x[ty + 16][m0 + m];
       const float p0[4] = {a0.x, a0.y, a0.z, a0.w}, p1[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float x[L::NC];
-        row_cols(x, stage, m + k, tx);
+        row_cols(x, stage[(m + k) / TT], (m + k) % TT, tx);
 #pragma unroll
         for (int j = 0; j < L::NC; ++j) {
           part[0][j] = fmaf(p0[k], x[j], part[0][j]);
@@ -383,9 +386,9 @@ __global__ void __launch_bounds__(256) out_kernel(Args a, int tiles, bool vec) {
   float acc[2][L::NC];
 #pragma unroll
   for (int j = 0; j < L::NC; ++j) acc[0][j] = acc[1][j] = 0.f;
-  __syncthreads();
+  __syncthreads();  // pw
   const float w[2] = {pw[z.r0 + ty + 1], pw[z.r0 + ty + 17]};
-  times_state<DP>(acc, A, a.states + (z.chain * chunks(P) + z.c) * (int64_t)D * D, false, D, w, K);
+  times_state<DP>(acc, A, a.states + (z.chain * chunks(P) + z.c) * (int64_t)D * D, false, D, w, &K);
   for (int s0 = 0; s0 <= z.r0; s0 += TT) {
     __syncthreads();
     load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, vec);
@@ -406,128 +409,84 @@ __global__ void __launch_bounds__(256) out_kernel(Args a, int tiles, bool vec) {
   store_rows<TA, DP>(a.y, acc, P, z.b, z.h, z.tc + z.r0, tend, P.scale);
 }
 
-// dq of one tile of 32 tokens, and its part of dlog_decay (terms with q)
+// One gradient of one tile of 32 tokens: a product with S or R, and masked scores x with the other
+// tokens' rows:
+//
+//     out = w (X M) + sum over tiles of (weights o X W^T) U      dq: X = dy, M = S^T, W = v,  U = k
+//                                                                dk: X = v,  M = R^T, W = dy, U = q
+//                                                                dv: X = k,  M = R,   W = q,  U = dy
+//
+// Three CTAs a tile, each with one accumulator (dk and dv share no product, and a CTA that made both
+// was the launch's longest: 2 x 500 tokens x 8 heads of 48 45 us, now 38).  dq's and dk's also sum their terms of
+// dlog_decay, with Y = q and k.
+enum Grad { DK, DV, DQ };
 template <typename TA, int DP>
-__device__ void dq_tile(const Args& a, const TilePos& z, int part, bool vec, Tile<DP>* t, const float* pw) {
+__global__ void __launch_bounds__(256, DP == 128 ? 2 : 4) grads_kernel(Args a, int tiles, bool vec) {
   using L = Tile<DP>;
-  L &Q = t[0], &O = t[1], &K = t[2], &V = t[3];
+  extern __shared__ float sm[];
+  __shared__ float pw[CH + 1];
+  L *const t = (L*)sm, &X = t[0], &Y = t[1], &U = t[2], &W = t[3];
   float(*Pm)[LP] = (float(*)[LP])(t + 4);
   const AtlasDecayParams& P = a.p;
+  const TilePos z = tile_pos(P, blockIdx.x / 3, tiles);
+  const int kind = blockIdx.x % 3;
   const int D = P.D, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
-  load_rows<TA>(Q, view(a.q, P.q_stride), z.b, z.h, z.tc + z.r0, tend, D, vec);
-  load_rows<TA>(O, flat(a.dy, P), z.b, z.h, z.tc + z.r0, tend, D, vec);
+  const View q = view(a.q, P.q_stride), k = view(a.k, P.k_stride), v = view(a.v, P.v_stride), o = flat(a.dy, P);
+  const View xs = kind == DQ ? o : kind == DK ? v : k, us = kind == DQ ? k : kind == DK ? q : o,
+             ws = kind == DQ ? v : kind == DK ? o : q;
+  load_rows<TA>(X, xs, z.b, z.h, z.tc + z.r0, tend, D, vec);
+  if (kind != DV) load_rows<TA>(Y, kind == DQ ? q : k, z.b, z.h, z.tc + z.r0, tend, D, vec);
+  if (threadIdx.x <= CH) pw[threadIdx.x] = pow_decay(a.log_decay[z.h], threadIdx.x);
+  __syncthreads();
   float acc[2][L::NC], dg = 0.f;
 #pragma unroll
   for (int j = 0; j < L::NC; ++j) acc[0][j] = acc[1][j] = 0.f;
-  const float w[2] = {P.scale * pw[z.r0 + ty + 1], P.scale * pw[z.r0 + ty + 17]};
-  times_state<DP>(acc, O, a.states + (z.chain * chunks(P) + z.c) * (int64_t)D * D, true, D, w, K);
-  {  // columns from D on are 0 in Q
-    float q0[L::NC], q1[L::NC];
-    row_cols(q0, Q, ty, tx);
-    row_cols(q1, Q, ty + 16, tx);
-#pragma unroll
-    for (int j = 0; j < L::NC; ++j)
-      dg += (float)(z.r0 + ty + 1) * q0[j] * acc[0][j] + (float)(z.r0 + ty + 17) * q1[j] * acc[1][j];
-  }
-  for (int s0 = 0; s0 <= z.r0; s0 += TT) {
-    __syncthreads();
-    load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, vec);
-    load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + s0, tend, D, vec);
-    __syncthreads();
-    float p[2][2], x[2][2];
-    dots(p, Q, K);
-    dots(x, O, V);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int lag = z.r0 + ty + 16 * i - (s0 + tx + 16 * j);
-        const float da = lag >= 0 ? P.scale * pw[lag] * x[i][j] : 0.f;
-        if (lag > 0) dg += (float)lag * p[i][j] * da;
-        Pm[ty + 16 * i][tx + 16 * j] = da;
-      }
-    __syncthreads();
-    times_tile<DP>(acc, Pm, K);
-  }
-  store_rows<TA, DP>(a.dq, acc, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
-  dg = cta_sum(dg);
-  if (threadIdx.x == 0) a.dg_part[z.chain * a.dg_parts + part] = dg;
-}
-
-// dk and dv of one tile of 32 tokens, and the terms of dlog_decay with k, R and S
-template <typename TA, int DP>
-__device__ void dkv_tile(const Args& a, const TilePos& z, int part, bool vec, Tile<DP>* t, const float* pw) {
-  using L = Tile<DP>;
-  L &K = t[0], &V = t[1], &Q = t[2], &O = t[3];
-  float(*Pm)[LP] = (float(*)[LP])(t + 4);
-  float(*Am)[LP] = Pm + TT;
-  const AtlasDecayParams& P = a.p;
-  const int D = P.D, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
-  load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + z.r0, tend, D, vec);
-  load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + z.r0, tend, D, vec);
-  float dk[2][L::NC], dv[2][L::NC], dg = 0.f;
-#pragma unroll
-  for (int j = 0; j < L::NC; ++j) dk[0][j] = dk[1][j] = dv[0][j] = dv[1][j] = 0.f;
-  const int n0 = z.L - 1 - z.r0 - ty, n1 = n0 - 16;  // steps from the row to the chunk's end
-  const float w[2] = {n0 >= 0 ? pw[n0] : 0.f, n1 >= 0 ? pw[n1] : 0.f};
+  // steps from the rows to the chunk's start (dq) or end
+  const int n0 = kind == DQ ? z.r0 + ty + 1 : z.L - 1 - z.r0 - ty, n1 = kind == DQ ? n0 + 16 : n0 - 16;
+  const float s = kind == DQ ? P.scale : 1.f, w[2] = {n0 >= 0 ? s * pw[n0] : 0.f, n1 >= 0 ? s * pw[n1] : 0.f};
   const int64_t so = (z.chain * chunks(P) + z.c) * (int64_t)D * D;
   const float *R = a.dstates + so, *S = a.states + so;
-  times_state<DP>(dk, V, R, true, D, w, Q);
-  times_state<DP>(dv, K, R, false, D, w, Q);
-  {
-    float k0[L::NC], k1[L::NC];
-    row_cols(k0, K, ty, tx);
-    row_cols(k1, K, ty + 16, tx);
+  times_state<DP>(acc, X, kind == DQ ? S : R, kind != DV, D, w, &U);
+  if (kind != DV) {  // columns from D on are 0 in Y
+    float y0[L::NC], y1[L::NC];
+    row_cols(y0, Y, ty, tx);
+    row_cols(y1, Y, ty + 16, tx);
 #pragma unroll
     for (int j = 0; j < L::NC; ++j) {
-      if (n0 > 0) dg += (float)n0 * k0[j] * dk[0][j];
-      if (n1 > 0) dg += (float)n1 * k1[j] * dk[1][j];
+      if (n0 > 0) dg += (float)n0 * y0[j] * acc[0][j];
+      if (n1 > 0) dg += (float)n1 * y1[j] * acc[1][j];
     }
   }
-  if (z.r0 == 0) {  // once for each chunk
+  if (kind == DQ && z.r0 == 0) {  // once for each chunk, where the loop below is short
     float rs = 0.f;
+#pragma unroll 4
     for (int u = threadIdx.x; u < D * D; u += 256) rs = fmaf(R[u], S[u], rs);
     dg += (float)z.L * pw[z.L] * rs;
   }
-  for (int t0 = z.r0; t0 < z.L; t0 += TT) {
+  for (int s0 = kind == DQ ? 0 : z.r0; s0 < (kind == DQ ? z.r0 + 1 : z.L); s0 += TT) {
     __syncthreads();
-    load_rows<TA>(Q, view(a.q, P.q_stride), z.b, z.h, z.tc + t0, tend, D, vec);
-    load_rows<TA>(O, flat(a.dy, P), z.b, z.h, z.tc + t0, tend, D, vec);
+    load_rows<TA>(U, us, z.b, z.h, z.tc + s0, tend, D, vec);
+    load_rows<TA>(W, ws, z.b, z.h, z.tc + s0, tend, D, vec);
     __syncthreads();
-    float p[2][2], x[2][2];
-    dots(p, K, Q);
-    dots(x, V, O);
+    float x[2][2], p[2][2];
+    dots(x, X, W);
+    if (kind == DQ) dots(p, Y, U);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int lag = t0 + tx + 16 * j - (z.r0 + ty + 16 * i);
-        const float f = lag >= 0 ? P.scale * pw[lag] : 0.f;
-        Pm[ty + 16 * i][tx + 16 * j] = lag >= 0 ? f * p[i][j] : 0.f;
-        Am[ty + 16 * i][tx + 16 * j] = lag >= 0 ? f * x[i][j] : 0.f;
+        const int d = z.r0 + ty + 16 * i - (s0 + tx + 16 * j), lag = kind == DQ ? d : -d;
+        const float f = lag >= 0 ? P.scale * pw[lag] * x[i][j] : 0.f;
+        if (kind == DQ && lag > 0) dg += (float)lag * p[i][j] * f;
+        Pm[ty + 16 * i][tx + 16 * j] = f;
       }
     __syncthreads();
-    times_tile<DP>(dk, Am, Q);
-    times_tile<DP>(dv, Pm, O);
+    times_tile<DP>(acc, Pm, U);
   }
-  store_rows<TA, DP>(a.dk, dk, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
-  store_rows<TA, DP>(a.dv, dv, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
+  store_rows<TA, DP>(kind == DQ ? a.dq : kind == DK ? a.dk : a.dv, acc, P, z.b, z.h, z.tc + z.r0, tend, 1.f);
+  if (kind == DV) return;
   dg = cta_sum(dg);
-  if (threadIdx.x == 0) a.dg_part[z.chain * a.dg_parts + part] = dg;
-}
-
-// even CTAs take dk and dv of a tile (the longer work first), odd ones dq
-template <typename TA, int DP>
-__global__ void __launch_bounds__(256) grads_kernel(Args a, int tiles, bool vec) {
-  extern __shared__ float sm[];
-  __shared__ float pw[CH + 1];
-  const TilePos z = tile_pos(a.p, blockIdx.x >> 1, tiles);
-  if (threadIdx.x <= CH) pw[threadIdx.x] = pow_decay(a.log_decay[z.h], threadIdx.x);
-  __syncthreads();
-  if (blockIdx.x & 1)
-    dq_tile<TA, DP>(a, z, z.tile, vec, (Tile<DP>*)sm, pw);
-  else
-    dkv_tile<TA, DP>(a, z, tiles + z.tile, vec, (Tile<DP>*)sm, pw);
+  if (threadIdx.x == 0) a.dg_part[z.chain * a.dg_parts + (kind == DQ ? 0 : tiles) + z.tile] = dg;
 }
 
 // ---------------------------------------------------------------------------
@@ -642,9 +601,9 @@ static int check(const AtlasDecayParams* p) {
     if (s[0] < 0 || s[1] < 0 || s[2] < 0)
       return report_error(ATLAS_ERR_INVALID_ARGUMENT, "strides must not be negative");
   if (p->T > 1 << 30) return report_error(ATLAS_ERR_UNSUPPORTED, "decay attention: T must be at most 2^30");
-  // grids are one-dimensional: (batch, head, 32-token tile) and (batch, head, state element / 256)
+  // grids are one-dimensional: (batch, head, 32-token tile, gradient) and (batch, head, state element / 256)
   const int64_t n = chains(*p);
-  if (n * std::max(4 * chunks(*p), 64) >= (int64_t)1 << 31)
+  if (n * std::max(6 * chunks(*p), 64) >= (int64_t)1 << 31)
     return report_error(ATLAS_ERR_UNSUPPORTED, "decay attention: B * H * T is too large for one call");
   clear_error();
   return ATLAS_OK;
@@ -716,9 +675,9 @@ static cudaError_t plain_dp(const Args& a, Phase f, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     out_kernel<TA, DP><<<(unsigned)(chains(a.p) * tiles), 256, smem(3, 1), s>>>(a, tiles, vec);
   } else if (f == GRADS) {
-    const cudaError_t e = allow_smem<grads_kernel<TA, DP>>(smem(4, 2));
+    const cudaError_t e = allow_smem<grads_kernel<TA, DP>>(smem(4, 1));
     if (e != cudaSuccess) return e;
-    grads_kernel<TA, DP><<<(unsigned)(chains(a.p) * tiles * 2), 256, smem(4, 2), s>>>(a, tiles, vec);
+    grads_kernel<TA, DP><<<(unsigned)(chains(a.p) * tiles * 3), 256, smem(4, 1), s>>>(a, tiles, vec);
   } else {
     sums_kernel<TA, DP><<<(unsigned)(chains(a.p) * chunks(a.p)), 256, 0, s>>>(a, f == SUMS_BWD, vec);
   }
