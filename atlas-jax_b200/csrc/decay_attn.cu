@@ -45,6 +45,8 @@ template <int VEC>
 __global__ void __launch_bounds__(256) scan_kernel(Args a, const float* in, float* out, float* buf, bool bwd) {
   constexpr int UN = 8;
   const AtlasDecayParams& P = a.p;
+  let_next_start();
+  after_previous();
   const int nc = chunks(P), DD = P.D * P.D, per = DD / VEC;
   const int64_t total = chains(P) * per;
   const int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -94,6 +96,7 @@ __global__ void __launch_bounds__(256) dg_kernel(Args a, float* dg) {
   const AtlasDecayParams& P = a.p;
   const int h = blockIdx.x;
   const int64_t n = (int64_t)P.B * a.dg_parts;
+  after_previous();
   double acc = 0;
   for (int64_t i = threadIdx.x; i < n; i += 256) {
     const int64_t b = i / a.dg_parts, c = i - b * a.dg_parts;
@@ -187,6 +190,7 @@ __global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd, bool vec) {
   __shared__ L X, Y;
   __shared__ float w[CH];
   const AtlasDecayParams& P = a.p;
+  let_next_start();
   const int nc = chunks(P), D = P.D;
   const int64_t chain = blockIdx.x / nc;
   const int c = (int)(blockIdx.x % nc), b = (int)(chain / P.H), h = (int)(chain % P.H);
@@ -386,7 +390,8 @@ __global__ void __launch_bounds__(256) out_kernel(Args a, int tiles, bool vec) {
   float acc[2][L::NC];
 #pragma unroll
   for (int j = 0; j < L::NC; ++j) acc[0][j] = acc[1][j] = 0.f;
-  __syncthreads();  // pw
+  after_previous();  // the states
+  __syncthreads();   // pw
   const float w[2] = {pw[z.r0 + ty + 1], pw[z.r0 + ty + 17]};
   times_state<DP>(acc, A, a.states + (z.chain * chunks(P) + z.c) * (int64_t)D * D, false, D, w, &K);
   for (int s0 = 0; s0 <= z.r0; s0 += TT) {
@@ -437,6 +442,8 @@ __global__ void __launch_bounds__(256, DP == 128 ? 2 : 4) grads_kernel(Args a, i
   load_rows<TA>(X, xs, z.b, z.h, z.tc + z.r0, tend, D, vec);
   if (kind != DV) load_rows<TA>(Y, kind == DQ ? q : k, z.b, z.h, z.tc + z.r0, tend, D, vec);
   if (threadIdx.x <= CH) pw[threadIdx.x] = pow_decay(a.log_decay[z.h], threadIdx.x);
+  let_next_start();
+  after_previous();  // R
   __syncthreads();
   float acc[2][L::NC], dg = 0.f;
 #pragma unroll
@@ -647,11 +654,7 @@ static cudaError_t scan(const Args& a, const float* in, float* out, bool bwd, cu
   const bool v4 = a.p.D % 2 == 0 && aligned16(in) && aligned16(out) && aligned16(buf);  // D * D % 4 == 0
   const int64_t n = chains(a.p) * a.p.D * a.p.D / (v4 ? 4 : 1);
   const unsigned grid = (unsigned)((n + 255) / 256);
-  if (v4)
-    scan_kernel<4><<<grid, 256, 0, s>>>(a, in, out, buf, bwd);
-  else
-    scan_kernel<1><<<grid, 256, 0, s>>>(a, in, out, buf, bwd);
-  return cudaGetLastError();
+  return follow(v4 ? scan_kernel<4> : scan_kernel<1>, grid, 256, 0, s, a, in, out, buf, bwd);
 }
 
 // whether groups of four channels of every tensor can be loaded at once
@@ -673,11 +676,11 @@ static cudaError_t plain_dp(const Args& a, Phase f, cudaStream_t s) {
   if (f == OUT) {
     const cudaError_t e = allow_smem<out_kernel<TA, DP>>(smem(3, 1));
     if (e != cudaSuccess) return e;
-    out_kernel<TA, DP><<<(unsigned)(chains(a.p) * tiles), 256, smem(3, 1), s>>>(a, tiles, vec);
+    return follow(out_kernel<TA, DP>, (unsigned)(chains(a.p) * tiles), 256, smem(3, 1), s, a, tiles, vec);
   } else if (f == GRADS) {
     const cudaError_t e = allow_smem<grads_kernel<TA, DP>>(smem(4, 1));
     if (e != cudaSuccess) return e;
-    grads_kernel<TA, DP><<<(unsigned)(chains(a.p) * tiles * 3), 256, smem(4, 1), s>>>(a, tiles, vec);
+    return follow(grads_kernel<TA, DP>, (unsigned)(chains(a.p) * tiles * 3), 256, smem(4, 1), s, a, tiles, vec);
   } else {
     sums_kernel<TA, DP><<<(unsigned)(chains(a.p) * chunks(a.p)), 256, 0, s>>>(a, f == SUMS_BWD, vec);
   }
@@ -810,8 +813,7 @@ extern "C" int atlas_decay_bwd(const AtlasDecayParams* p, const void* q, const v
                          : plain_states(a, dstate_out, dstate_in, true, s);
   if (e == cudaSuccess) e = tensor ? tcore::launch_grads(a, s) : plain(a, GRADS, s);
   if (e == cudaSuccess && dlog_decay) {
-    dg_kernel<<<p->H, 256, 0, s>>>(a, dlog_decay);
-    e = cudaGetLastError();
+    e = follow(dg_kernel, p->H, 256, 0, s, a, dlog_decay);
   }
   return status_of(e);
 }

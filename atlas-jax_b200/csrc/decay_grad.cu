@@ -123,7 +123,6 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   F2 y0[4];
 #pragma unroll
   for (int i = 0; i < NU; ++i) load8(Sg, tid + NT * i, x[i]);
-  if (DP == 64) load8(Rg, tid, y0);
   if (tid == 0) {
     mbar_init(&ctl.loaded, 1);
     for (int i = 0; i < 5; ++i) mbar_init(&ctl.done[i], 1);
@@ -159,7 +158,9 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   }
   if (tid >= 64 && tid <= 64 + C) ctl.pw[tid - 64] = powd(g, tid - 64);
 
+  after_previous();  // R
   if constexpr (DP == 64) {
+    load8(Rg, tid, y0);
     dot8(x[0], y0);
     put_parts3(parts + tid * 16, G::ST, x[0]);
     put_parts3(parts + 3 * G::ST + tid * 16, G::ST, y0);
@@ -172,6 +173,7 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   }
   fence_async_smem();
   cta_sync();
+  let_next_start();  // (after the allocation of tensor memory)
   const uint32_t tm = ctl.tmem, tmu = __shfl_sync(0xffffffffu, tm, 0), at = tm + ((uint32_t)(32 * q) << 16);
   const uint64_t pd = desc_mnmajor(base + G::OFF_PARTS, DP), pk = desc_kmajor(base + G::OFF_PARTS, DP);
   constexpr uint64_t STEP_K = 256 / 16, STEP_MN = DP * 32 / 16, PART = G::ST / 16, TSTEP_MN = 2048 / 16;
@@ -376,8 +378,7 @@ template <int DP>
 static cudaError_t launch(const Maps& m, const Args& a, cudaStream_t s) {
   cudaError_t e = allow_smem<grads_kernel<DP>>(GRAD_SMEM<DP>);
   if (e != cudaSuccess) return e;
-  grads_kernel<DP><<<(unsigned)(chains(a.p) * chunks(a.p)), NT, GRAD_SMEM<DP>, s>>>(m, a);
-  return cudaGetLastError();
+  return follow(grads_kernel<DP>, (unsigned)(chains(a.p) * chunks(a.p)), NT, GRAD_SMEM<DP>, s, m, a);
 }
 
 cudaError_t launch_grads(const Args& a, cudaStream_t s) {

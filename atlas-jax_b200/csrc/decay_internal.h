@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "atlas_decay.h"
+#include "follow.cuh"
 #include "scan_internal.h"
 
 namespace atlas {

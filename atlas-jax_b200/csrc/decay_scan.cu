@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
   __syncthreads();
   fence_after();
   const uint32_t tm = ctl.tmem;
+  let_next_start();  // this CTA has its tensor memory: the next kernel cannot take it away
 
   if (w < K::KWARPS) {
     // ---- k' : thread (token row, every KP-th 16-byte group) ----
@@ -333,6 +334,7 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     const int d0 = DP == 64 ? 16 * q + r : 32 * q + 16 * hf + r;
     const uint32_t at = tm + K::T_DS + e0 + ((uint32_t)(32 * q + 16 * hf) << 16);
     constexpr int NJ = DP / 16;  // 8-column blocks of a warp
+    after_previous();            // (no other warp reads or writes what an earlier kernel of the call does)
     F2 S[2 * NJ];                // [2 j]: row d0, columns e0 + 8 j + c2 and the next; [2 j + 1]: row d0 + 8
     const int64_t DD = (int64_t)D * D;
     const bool in0 = d0 < D, in1 = d0 + 8 < D;
@@ -572,7 +574,10 @@ static cudaError_t launch(const CUtensorMap& q, const CUtensorMap& x, const CUte
                           bool reversed, cudaStream_t s) {
   cudaError_t e = allow_smem<seq_kernel<DP, FWD>>(SEQ_SMEM<DP, FWD>);
   if (e != cudaSuccess) return e;
-  seq_kernel<DP, FWD><<<(unsigned)(chains(a.p) * (a.segs - a.sums_pass)), Cfg<DP, FWD>::NT, SEQ_SMEM<DP, FWD>, s>>>(q, x, y, a, reversed);
+  const unsigned grid = (unsigned)(chains(a.p) * (a.segs - a.sums_pass));
+  if (a.segs > 1 && !a.sums_pass)
+    return follow(seq_kernel<DP, FWD>, grid, Cfg<DP, FWD>::NT, SEQ_SMEM<DP, FWD>, s, q, x, y, a, reversed);
+  seq_kernel<DP, FWD><<<grid, Cfg<DP, FWD>::NT, SEQ_SMEM<DP, FWD>, s>>>(q, x, y, a, reversed);
   return cudaGetLastError();
 }
 
@@ -601,6 +606,8 @@ static Split split(const AtlasDecayParams& p) {
 __global__ void __launch_bounds__(256) join_kernel(SeqArgs a) {
   const int per = a.p.D * a.p.D / 4;
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  let_next_start();
+  after_previous();
   if (u >= chains(a.p) * per) return;
   const int64_t chain = u / per;
   float4* m = (float4*)sum_at(a, chain, 1) + (u - chain * per);
@@ -654,8 +661,7 @@ cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, flo
     q.sums_pass = 0;
     if (wide && z.segs > 2) {
       const int64_t n = chains(p) * p.D * p.D / 4;
-      join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(q);
-      e = cudaGetLastError();
+      e = follow(join_kernel, (unsigned)((n + 255) / 256), 256, 0, s, q);
       if (e != cudaSuccess) return e;
     }
   }

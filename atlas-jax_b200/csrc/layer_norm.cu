@@ -25,6 +25,7 @@
 #include "atlas_norm.h"
 #include "common.cuh"
 #include "f32x2.cuh"
+#include "follow.cuh"
 #include "scan_internal.h"
 
 namespace atlas {
@@ -288,6 +289,7 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : T
   constexpr bool RING = VEC > 1;
   constexpr int NP = PAIRS<VEC>;
   typedef Pack<TA, VEC> Raw;
+  let_next_start();
   int turn = 0;
   const Place<TEAM, LANES> z(a, per_block);
   float* red = red_all[TEAM == MANY ? z.team : 0];
@@ -432,6 +434,7 @@ __global__ void __launch_bounds__(PCOL * PROW) param_kernel(Args a, int parts, f
   const int tx = threadIdx.x % PCOL, ty = threadIdx.x / PCOL, col = blockIdx.x * PCOL + tx, total = a.G * a.N;
   const int groups = total / a.width;
   float sw = 0.f, sb = 0.f;
+  after_previous();
   if (col < total) {
     const int grp = col / a.width, n = col % a.width;
 #pragma unroll 4
@@ -878,8 +881,7 @@ extern "C" int atlas_layernorm_bwd(const AtlasNormParams* p, const void* dy, con
   a.width = z.width;
   cudaError_t e = launch(a, *p, z, true, s);
   if (e == cudaSuccess && params) {
-    param_kernel<<<(unsigned)((p->G * p->N + PCOL - 1) / PCOL), PCOL * PROW, 0, s>>>(a, z.parts, dweight, dbias);
-    e = cudaGetLastError();
+    e = follow(param_kernel, (unsigned)((p->G * p->N + PCOL - 1) / PCOL), PCOL * PROW, 0, s, a, z.parts, dweight, dbias);
   }
   return status_of(e);
 }
