@@ -119,8 +119,7 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   };
   uint8_t* parts = sm + G::OFF_PARTS;
   constexpr int NU = DP * DP / 8 / NT;  // groups of 8 of a state a thread
-  F2 x[NU][4];
-  F2 y0[4];
+  F2 x[NU][4], y[NU][4];
 #pragma unroll
   for (int i = 0; i < NU; ++i) load8(Sg, tid + NT * i, x[i]);
   if (tid == 0) {
@@ -158,19 +157,16 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   }
   if (tid >= 64 && tid <= 64 + C) ctl.pw[tid - 64] = powd(g, tid - 64);
 
-  after_previous();  // R
-  if constexpr (DP == 64) {
-    load8(Rg, tid, y0);
-    dot8(x[0], y0);
-    put_parts3(parts + tid * 16, G::ST, x[0]);
-    put_parts3(parts + 3 * G::ST + tid * 16, G::ST, y0);
-  } else {
+  after_previous();  // R: loaded while S is split
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      F2 y[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
-      put_parts3(parts + (tid + NT * i) * 16, G::ST, y);
-    }
+  for (int i = 0; i < NU; ++i) load8(Rg, tid + NT * i, y[i]);
+#pragma unroll
+  for (int i = 0; i < NU; ++i) {
+    if (DP == 64) dot8(x[i], y[i]);
+    F2 t[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
+    put_parts3(parts + (tid + NT * i) * 16, G::ST, t);
   }
+  if (DP == 64) put_parts3(parts + 3 * G::ST + tid * 16, G::ST, y[0]);
   fence_async_smem();
   cta_sync();
   let_next_start();  // (after the allocation of tensor memory)
@@ -212,15 +208,9 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
     mma_commit(&ctl.done[1]);
   }
   __syncwarp();
-  if constexpr (DP != 64) {  // R, while the products with S run
+  if (DP != 64) {
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      F2 y[4];
-      load8(Rg, tid + NT * i, y);
-      dot8(x[i], y);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[i][j] = y[j];
-    }
+    for (int i = 0; i < NU; ++i) dot8(x[i], y[i]);
   }
   float dg = 0.f;
   // ---- scores ----
@@ -252,7 +242,7 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   if constexpr (DP != 64) {  // the parts of R in the place of S's
     wait_for(ctl, &ctl.done[1], a.status);
 #pragma unroll
-    for (int i = 0; i < NU; ++i) put_parts3(parts + (tid + NT * i) * 16, G::ST, x[i]);
+    for (int i = 0; i < NU; ++i) put_parts3(parts + (tid + NT * i) * 16, G::ST, y[i]);
   }
   fence_async_smem();
   cta_sync();

@@ -79,7 +79,9 @@ __device__ __forceinline__ uint64_t desc_tile_mn(uint32_t saddr) {
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-// Eight float32 values as three bf16 parts whose sum holds 24 bits, 16-byte groups `stride` apart.
+// Eight float32 values as three bf16 parts whose sum holds all 24 bits, 16-byte groups `stride`
+// apart.  The upper parts are cut off, not rounded: 8 bits each leave 8 for the last (and the
+// kernels run as fast as with rounding conversions).
 __device__ __forceinline__ void put_parts3(uint8_t* dst, uint32_t stride, F2* v) {
 #pragma unroll
   for (int p = 0; p < 3; ++p) {
@@ -87,7 +89,7 @@ __device__ __forceinline__ void put_parts3(uint8_t* dst, uint32_t stride, F2* v)
     uint32_t* h = (uint32_t*)&pk;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      h[j] = bf2_pack(v[j]);
+      h[j] = bf2_cut(v[j]);
       if (p < 2) v[j] = v[j] - bf2_unpack(h[j]);
     }
     *(uint4*)(dst + p * stride) = pk;

@@ -45,5 +45,10 @@ __device__ __forceinline__ uint32_t bf2_pack(F2 a) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x.y), "f"(x.x));
   return r;
 }
+// the upper halves of both: rounded toward zero
+__device__ __forceinline__ uint32_t bf2_cut(F2 a) {
+  const float2 x = f2_get(a);
+  return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+}
 
 }  // namespace atlas
