@@ -11,10 +11,10 @@
 // Only QS and the update of S depend on the block before, so the CTA is a pipeline of
 // groups that hand blocks on through mbarriers:
 //
-//     8 (4) warps   k' split into three bf16 parts (float32 accuracy of the state)
+//     4 warps       k' split into three bf16 parts (float32 accuracy of the state)
 //     4 warps       scores: A from TMEM, decayed, masked, rounded to bf16
 //     4 warps       outputs: O and QS from TMEM, y to memory, 64 bytes of a row at a time
-//     8 (16) warps  the state: dS from TMEM, S in registers, two bf16 parts of S for QS
+//     4 (16) warps  the state: dS from TMEM, S in registers, two bf16 parts of S for QS
 //     3 warps       issue the MMAs;  one warp issues the TMA loads of q, k, v
 //
 // The same kernel without q's side gives the states alone: the sums of a segment (first
@@ -46,8 +46,10 @@ struct Cfg {
   static constexpr int TILES = FWD ? 3 : 2;             // of a stage: (q,) k, v
   static constexpr int STAGES = FWD ? (DP == 64 ? 3 : 2) : (DP == 64 ? 4 : 3);
   static constexpr int DBL = FWD && DP == 128 ? 1 : 2;  // buffers of k', scores, S and the accumulators
-  static constexpr int KWARPS = FWD && DP == 128 ? 4 : 8;  // warps of the k' group
-  static constexpr int SWARPS = DP == 64 ? 8 : 16;      // warps of the state group
+  // Warps of the k' and of the state group.  Few, with more values each, where the registers allow: the
+  // schedulers are shared with the groups that wait (D = 64, 8 x 8192 tokens x 12 heads, 8 and 8: 164 us;
+  // 4 and 8: 156; 4 and 4: 150).  D = 128 with a state group of 8 spills.
+  static constexpr int KWARPS = FWD ? 4 : 8, SWARPS = DP == 64 ? 4 : 16;
   static constexpr int MWARPS = FWD ? 3 : 1;            // warps that issue MMAs
   static constexpr int W_P = KWARPS, W_Y = W_P + (FWD ? 4 : 0), W_S = W_Y + (FWD ? 4 : 0), W_MMA = W_S + SWARPS;  // first warps of the groups
   static constexpr int W_LOAD = W_MMA + MWARPS, NT = 32 * (W_LOAD + 1);
@@ -329,11 +331,11 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     // ---- the state ----
     // DP = 64: 16 rows in lanes 0-15 of the quadrant.  DP = 128: rows are lanes.  A warp has 16 rows and
     // half of the columns.
+    constexpr int NJ = DP == 64 ? 32 / K::SWARPS : 8;  // 8-column blocks of a warp
     const int sub = (w - K::W_S) >> 2, q = w & 3, r = lane >> 2, c2 = 2 * (lane & 3);
-    const int hf = DP == 64 ? 0 : sub & 1, e0 = (DP == 64 ? sub : sub >> 1) * (DP / 2);
+    const int hf = DP == 64 ? 0 : sub & 1, e0 = (DP == 64 ? sub : sub >> 1) * 8 * NJ;
     const int d0 = DP == 64 ? 16 * q + r : 32 * q + 16 * hf + r;
     const uint32_t at = tm + K::T_DS + e0 + ((uint32_t)(32 * q + 16 * hf) << 16);
-    constexpr int NJ = DP / 16;  // 8-column blocks of a warp
     after_previous();            // (no other warp reads or writes what an earlier kernel of the call does)
     F2 S[2 * NJ];                // [2 j]: row d0, columns e0 + 8 j + c2 and the next; [2 j + 1]: row d0 + 8
     const int64_t DD = (int64_t)D * D;
