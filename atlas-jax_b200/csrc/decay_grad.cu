@@ -12,8 +12,8 @@
 //
 // Blocks are independent: one CTA each.  q, k, v, dy arrive by TMA and leave as dq, dk, dv
 // through the same tiles; S and R are split into three bf16 parts (dlog_decay is a float32
-// output; dv needs two of R's).  All accumulators have M = 64 (decay_tc.cuh); warp w of
-// 16 reads lane quadrant w % 4 and the column quarter w / 4.
+// output; dv needs two of R's).  All accumulators have M = 64 (decay_tc.cuh); warp w
+// reads lane quadrant w % 4 and its half (D <= 64) or quarter w / 4 of the columns.
 //
 // D <= 64: 256 TMEM columns (dA K, P^T O, dA^T Q and K R take the places of A, B, O S^T and
 // V R^T), 97 KB of shared memory: two CTAs share an SM, and one's loads and float32 work
@@ -27,10 +27,11 @@ namespace atlas {
 namespace decay {
 namespace tcore {
 
-constexpr int NT = 512;
-
 template <int DP>
 struct GCfg {
+  // Threads, and warps of a TMEM lane quadrant, with 1 / HF of the columns each.  (D = 64 with 512: 16 x
+  // 4096 tokens x 8 heads 5 us longer; D = 128 with 256: 4 x 1900 x 6 2 us longer.)
+  static constexpr int NT = DP == 64 ? 256 : 512, HF = NT / 128;
   static constexpr int NB = DP / 64, TILE = NB * BOX, ST = DP * DP * 2, PT = C * C * 2;
   static constexpr int OFF_PARTS = 4 * TILE;
   static constexpr int OFF_P = OFF_PARTS + (DP == 64 ? 6 : 3) * ST;
@@ -43,7 +44,7 @@ struct GCfg {
 };
 struct GCtl {
   float pw[C + 1];
-  float red[NT / 32];
+  float red[16];  // a warp's part of dlog_decay
   uint64_t loaded, done[5];
   uint32_t tmem;
   volatile int bad;
@@ -80,14 +81,17 @@ template <int NV>
 __device__ __forceinline__ void frag(uint32_t addr, float* v) {
   if constexpr (NV == 8)
     tmem_frag16(addr, v);
-  else
+  else if constexpr (NV == 16)
     tmem_frag32(addr, v);
+  else
+    tmem_frag64(addr, v);
 }
 
 template <int DP>
-__global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __grid_constant__ Maps maps, const Args a) {
+__global__ void __launch_bounds__(GCfg<DP>::NT, DP == 64 ? 2 : 1) grads_kernel(const __grid_constant__ Maps maps, const Args a) {
   using G = GCfg<DP>;
-  constexpr int CW = DP / 4, NV = CW / 2;  // columns of a warp; values of a thread's fragment: 2 rows x CW / 4 columns
+  constexpr int NT = G::NT, CW = DP / G::HF, SC = C / G::HF;  // columns of a warp, of outputs and of scores
+  constexpr int NV = CW / 2;                                 // values of a thread's fragment: 2 rows x CW / 4 columns
   extern __shared__ uint8_t raw[];
   uint8_t* sm = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   GCtl& ctl = *(GCtl*)(sm + G::OFF_CTL);
@@ -166,7 +170,10 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
     F2 t[4] = {x[i][0], x[i][1], x[i][2], x[i][3]};
     put_parts3(parts + (tid + NT * i) * 16, G::ST, t);
   }
-  if (DP == 64) put_parts3(parts + 3 * G::ST + tid * 16, G::ST, y[0]);
+  if (DP == 64) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) put_parts3(parts + 3 * G::ST + (tid + NT * i) * 16, G::ST, y[i]);
+  }
   fence_async_smem();
   cta_sync();
   let_next_start();  // (after the allocation of tensor memory)
@@ -216,17 +223,17 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   // ---- scores ----
   wait_for(ctl, &ctl.done[0], a.status);
   {
-    float xa[8], xb[8];
-    tmem_frag16(at + G::T_A + 16 * hf, xa);
-    tmem_frag16(at + G::T_B + 16 * hf, xb);
+    float xa[SC / 2], xb[SC / 2];
+    frag<SC / 2>(at + G::T_A + SC * hf, xa);
+    frag<SC / 2>(at + G::T_B + SC * hf, xb);
     tmem_wait_ld();
     F2 gl = f2(0.f, 0.f);
-    uint8_t* pt = sm + G::OFF_P + cm_off(t0, 16 * hf + c2, C);
+    uint8_t* pt = sm + G::OFF_P + cm_off(t0, SC * hf + c2, C);
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < SC / 8; ++j)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int lag = t0 + 8 * k - (16 * hf + 8 * j + c2);  // of the pair's first column
+        const int lag = t0 + 8 * k - (SC * hf + 8 * j + c2);  // of the pair's first column
         const F2 M = f2(lag >= 0 ? ctl.pw[lag] : 0.f, lag >= 1 ? ctl.pw[lag - 1] : 0.f);
         // masked scores are dropped, not multiplied by 0
         const F2 A = f2(lag >= 0 ? xa[4 * j + 2 * k] : 0.f, lag >= 1 ? xa[4 * j + 2 * k + 1] : 0.f);
@@ -259,7 +266,7 @@ __global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) grads_kernel(const __gri
   }
   __syncwarp();
   // ---- the terms with S and R ----
-  F2 dq[NV / 2], dk[NV / 2];  // [2 j]: row t0, columns 8 j + c2 and the next of this quarter; [2 j + 1]: row t0 + 8
+  F2 dq[NV / 2], dk[NV / 2];  // [2 j]: row t0, columns 8 j + c2 and the next of this warp's; [2 j + 1]: row t0 + 8
   const float wo0 = t0 < L ? ctl.pw[L - 1 - t0] : 0.f, wo1 = t0 + 8 < L ? ctl.pw[L - 9 - t0] : 0.f;
   const F2 o0 = f2(wo0, wo0), o1 = f2(wo1, wo1);
   // rows t0 and t0 + 8 of a tile . a fragment
@@ -368,7 +375,7 @@ template <int DP>
 static cudaError_t launch(const Maps& m, const Args& a, cudaStream_t s) {
   cudaError_t e = allow_smem<grads_kernel<DP>>(GRAD_SMEM<DP>);
   if (e != cudaSuccess) return e;
-  return follow(grads_kernel<DP>, (unsigned)(chains(a.p) * chunks(a.p)), NT, GRAD_SMEM<DP>, s, m, a);
+  return follow(grads_kernel<DP>, (unsigned)(chains(a.p) * chunks(a.p)), GCfg<DP>::NT, GRAD_SMEM<DP>, s, m, a);
 }
 
 cudaError_t launch_grads(const Args& a, cudaStream_t s) {
