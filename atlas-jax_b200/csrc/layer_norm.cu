@@ -205,70 +205,125 @@ struct Place {
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
+// The vectors to come are copied into a ring in shared memory, `stages` - 1 of them ahead; every
+// thread copies the groups that it will work on itself, so the ring needs no barrier and holds no
+// registers.  Single channels (VEC = 1) are loaded directly.  Bound by memory: about 140 KB an SM are on
+// their way, and the weights stay in registers (read again for every row they were as many bytes as the
+// row, through an L1 that was then 72 % busy).  65536 x 768 bf16 with a residual: 65 us, 6.2 TB/s;
+// 79 us with direct loads and 32 warps an SM.
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
-__global__ void __launch_bounds__(TEAM == MANY ? 512 : 256) fwd_kernel(Args a, int per_block) {
+__global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : VEC * CHN <= 8 ? 4 : 2)
+    fwd_kernel(Args a, int per_block, int stages) {
+  extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float red_all[8][2 * 16];
+  constexpr bool RING = VEC > 1;
+  constexpr int NP = PAIRS<VEC>;
+  typedef Pack<TA, VEC> Raw;
   int turn = 0;
   const Place<TEAM, LANES> z(a, per_block);
   float* red = red_all[TEAM == MANY ? z.team : 0];
-  const TA *x = (const TA*)a.x, *res = (const TA*)a.res;
   const float inv = 1.f / (float)a.N;
-  for (int64_t v0 = z.first; !z.done(v0, a.vecs); v0 += z.stride) {
-    const bool on = v0 < a.vecs;
-    const int64_t base = v0 * a.N;
-    float f[CHN][VEC], s[1] = {0.f};
-#pragma unroll
-    for (int c = 0; c < CHN; ++c) {
-      const int n = (c * z.lanes + z.lane) * VEC;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[c][j] = 0.f;
-      if (on && n < a.N) load<TA, VEC>(f[c], x + base + n);
-    }
-    if (res) {
-#pragma unroll
-      for (int c = 0; c < CHN; ++c) {
-        const int n = (c * z.lanes + z.lane) * VEC;
-        if (on && n < a.N) {
-          float r[VEC];
-          load<TA, VEC>(r, res + base + n);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) f[c][j] = round_to<TA>(f[c][j] + r[j]);
-          store<TA, VEC>((TA*)a.h + base + n, f[c]);
-        }
-      }
-    }
+  const int n0 = z.lane * VEC, dn = z.lanes * VEC, left = a.N - n0;  // this thread's groups start at n0 + c * dn
+  const TA *x = (const TA*)a.x + n0, *res = a.res ? (const TA*)a.res + n0 : nullptr;
+  F2 w[CHN][NP], b[CHN][NP];
+  auto params = [&](int64_t g) {
 #pragma unroll
     for (int c = 0; c < CHN; ++c)
+      if (c * dn < left) {
+        const int64_t k = g * a.N + n0 + c * dn;
+        float u[2 * NP], v[2 * NP];
+        u[2 * NP - 1] = v[2 * NP - 1] = 0.f;
+        load_param<VEC>(u, a.w ? a.w + k : nullptr, 1.f);
+        load_param<VEC>(v, a.b ? a.b + k : nullptr, 0.f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s[0] += f[c][j];
-    team_sum<TEAM, LANES, 1>(s, red, turn, z.warps, 1 + z.team);
-    const float mean = s[0] * inv;
-    s[0] = 0.f;
+        for (int j = 0; j < NP; ++j) w[c][j] = f2(u[2 * j], u[2 * j + 1]), b[c][j] = f2(v[2 * j], v[2 * j + 1]);
+      }
+  };
+  const bool fixed = TEAM == SUB || a.G == 1;  // one group's weights in every round
+  if (fixed) params(TEAM == SUB ? z.first % a.G : 0);
+  Raw* ring = (Raw*)dyn + threadIdx.x;  // slot (stage, stream, c): 2 streams
+  const int pitch = blockDim.x;
+  auto fetch = [&](int64_t v, int st) {
+    if constexpr (RING) {
+      if (v < a.vecs) {
+        const int64_t o = v * a.N;
+        Raw* r = ring + st * 2 * CHN * pitch;
+#pragma unroll
+        for (int c = 0; c < CHN; ++c)
+          if (c * dn < left) {
+            copy16(r + c * pitch, x + o + c * dn);
+            if (res) copy16(r + (CHN + c) * pitch, res + o + c * dn);
+          }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  int at = 0;  // stage of the current vector
+  for (int i = 0; i < 3; ++i) fetch(i < stages - 1 ? z.first + i * z.stride : a.vecs, i);  // 3 groups always
+  for (int64_t v0 = z.first; !z.done(v0, a.vecs); v0 += z.stride) {
+    const bool on = v0 < a.vecs;
+    const int64_t o = v0 * a.N;
+    if (!fixed) params(v0 % a.G);
+    if constexpr (RING) {
+      // the group of this vector is the (stages - 1)-th newest
+      if (stages == 4)
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    const Raw* slot = ring + at * 2 * CHN * pitch;
+    F2 f[CHN][NP], s2 = f2(0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < CHN; ++c) {
-      const int n = (c * z.lanes + z.lane) * VEC;
+      if (on && c * dn < left) {
+        unpack2<TA, VEC>(f[c], RING ? slot[c * pitch] : *(const Raw*)(x + o + c * dn));
+        if (res) {
+          F2 r[NP];
+          unpack2<TA, VEC>(r, RING ? slot[(CHN + c) * pitch] : *(const Raw*)(res + o + c * dn));
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        f[c][j] -= mean;
-        if (n < a.N) s[0] = fmaf(f[c][j], f[c][j], s[0]);
+          for (int j = 0; j < NP; ++j) {
+            f[c][j] = f[c][j] + r[j];
+            if (sizeof(TA) == 2) f[c][j] = bf2_unpack(bf2_pack(f[c][j]));  // the stream's type: what h holds
+          }
+          store2<TA, VEC>((TA*)a.h + o + n0 + c * dn, f[c]);
+        }
+#pragma unroll
+        for (int j = 0; j < NP; ++j) s2 = s2 + f[c][j];
       }
     }
+    if constexpr (RING) {  // into the slot of the vector before
+      const int to = at == 0 ? stages - 1 : at - 1;
+      fetch(v0 + (stages - 1) * z.stride, to);
+      at = at + 1 == stages ? 0 : at + 1;
+    }
+    float2 t = f2_get(s2);
+    float s[1] = {t.x + t.y};
+    team_sum<TEAM, LANES, 1>(s, red, turn, z.warps, 1 + z.team);
+    const float mean = s[0] * inv;
+    const F2 nmean = f2(-mean, VEC == 1 ? 0.f : -mean);
+    s2 = f2(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < CHN; ++c)
+      if (on && c * dn < left) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          f[c][j] = f[c][j] + nmean;
+          s2 = fma2(f[c][j], f[c][j], s2);
+        }
+      }
+    t = f2_get(s2);
+    s[0] = t.x + t.y;
     team_sum<TEAM, LANES, 1>(s, red, turn, z.warps, 1 + z.team);
     const float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps));
     if (on && z.lane == 0 && a.stats) *(float2*)(a.stats + 2 * v0) = make_float2(mean, rstd);
-    const int g = a.G == 1 ? 0 : (int)(v0 % a.G);
+    const F2 r2 = f2(rstd, rstd);
 #pragma unroll
-    for (int c = 0; c < CHN; ++c) {
-      const int n = (c * z.lanes + z.lane) * VEC;
-      if (on && n < a.N) {
-        float w[VEC], b[VEC];
-        load_param<VEC>(w, a.w ? a.w + (int64_t)g * a.N + n : nullptr, 1.f);
-        load_param<VEC>(b, a.b ? a.b + (int64_t)g * a.N + n : nullptr, 0.f);
+    for (int c = 0; c < CHN; ++c)
+      if (on && c * dn < left) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[c][j] = fmaf(f[c][j] * rstd, w[j], b[j]);
-        store<TA, VEC>((TA*)a.y + base + n, f[c]);
+        for (int j = 0; j < NP; ++j) f[c][j] = fma2(f[c][j] * r2, w[c][j], b[c][j]);
+        store2<TA, VEC>((TA*)a.y + o + n0 + c * dn, f[c]);
       }
-    }
   }
 }
 
@@ -277,10 +332,8 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256) fwd_kernel(Args a, i
 // ---------------------------------------------------------------------------
 // With z = (h - mean) rstd and u = dy w:  dx = rstd (u - mean(u) - z mean(u z)) + dh,
 // dw += dy z, db += dy.
-// The vectors to come are copied into a ring in shared memory, `stages` - 1 of them ahead;
-// every thread copies the groups that it will work on itself, so the ring needs no barrier
-// and holds no registers (a register prefetch spilled, which made every copy wait for its
-// load: 325 us at 65536 x 768 bf16 with dh).  Single channels (VEC = 1) are loaded directly.
+// A ring as in the forward (a register prefetch spilled, which made every copy wait for its
+// load: 325 us at 65536 x 768 bf16 with dh; the ring 82).
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
 __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : TEAM == SUB ? 4 : VEC * CHN <= 8 ? 3 : 2)
     bwd_kernel(Args a, int per_block, int stages) {
@@ -709,10 +762,9 @@ static Plan plan(const Args& a, int act_dtype, bool vec_ok, bool bwd) {
     z.width = a.G * a.N;
     units = a.vecs;
   }
-  // The backward's blocks are what an SM holds at its register use (each keeps sums).  The
-  // forward's are 8 an SM, fewer where that makes their numbers of rounds equal (65536 x 768
-  // bf16: 79 us, 87 with a block for every 8 rows).
-  const int64_t blocks = SMS * (!bwd ? 8 : z.threads * z.chn * z.vec <= 2048 ? 4 : 2);
+  // Blocks are what an SM holds at its register use (each keeps sums, or weights); the forward's
+  // fewer where that makes their numbers of rounds equal.
+  const int64_t blocks = SMS * (!bwd && (z.big || z.tiny) ? 8 : z.threads * z.chn * z.vec <= 2048 ? 4 : 2);
   const int64_t rounds = std::max<int64_t>(1, (units + blocks - 1) / blocks);
   z.grid = std::max<int64_t>(1, bwd ? std::min(units, blocks) : (units + rounds - 1) / rounds);
   if (bwd && !z.big && !z.tiny && z.team != SUB && a.G > 1)  // a multiple of G: a block keeps one group's weights
@@ -747,18 +799,20 @@ static cudaError_t allow_smem() {
 }
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
 static cudaError_t go(const Args& a, const Plan& z, bool bwd, cudaStream_t s) {
-  
+  // as many stages, up to 4, as the blocks that an SM's registers hold have room for
+  const int stage = VEC > 1 ? (bwd ? 3 : 2) * CHN * z.threads * 16 : 0;
+  const int room = (bwd || VEC * CHN <= 8 ? 50 : z.threads <= 256 ? 100 : 200) << 10;
+  const int stages = 4 * stage <= room ? 4 : 2;
   if (bwd) {
-      // as many stages, up to 4, as the blocks that an SM's registers hold have room for
-      const size_t stage = VEC > 1 ? (size_t)3 * CHN * z.threads * 16 : 0;
-      const int stages = 4 * stage <= 50 << 10 ? 4 : 2;
-      const size_t sums = TEAM == SUB || z.per_block > 1 ? (size_t)z.per_block * 2 * z.width * sizeof(float) : 0;
-      const size_t sm = std::max(stages * stage, sums);
-      cudaError_t e = allow_smem<bwd_kernel<TA, TEAM, LANES, VEC, CHN>>();
-      if (e != cudaSuccess) return e;
-      bwd_kernel<TA, TEAM, LANES, VEC, CHN><<<(unsigned)z.grid, z.threads, sm, s>>>(a, z.per_block, stages);
+    const size_t sums = TEAM == SUB || z.per_block > 1 ? (size_t)z.per_block * 2 * z.width * sizeof(float) : 0;
+    const size_t sm = std::max((size_t)(stages * stage), sums);
+    cudaError_t e = allow_smem<bwd_kernel<TA, TEAM, LANES, VEC, CHN>>();
+    if (e != cudaSuccess) return e;
+    bwd_kernel<TA, TEAM, LANES, VEC, CHN><<<(unsigned)z.grid, z.threads, sm, s>>>(a, z.per_block, stages);
   } else {
-    fwd_kernel<TA, TEAM, LANES, VEC, CHN><<<(unsigned)z.grid, z.threads, 0, s>>>(a, z.per_block);
+    cudaError_t e = allow_smem<fwd_kernel<TA, TEAM, LANES, VEC, CHN>>();
+    if (e != cudaSuccess) return e;
+    fwd_kernel<TA, TEAM, LANES, VEC, CHN><<<(unsigned)z.grid, z.threads, stages * stage, s>>>(a, z.per_block, stages);
   }
   return cudaGetLastError();
 }
