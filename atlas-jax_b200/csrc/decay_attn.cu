@@ -201,6 +201,7 @@ __device__ __forceinline__ void mult4(float (*acc)[Tile<DP>::NC], const float* A
 }
 
 // per-chunk sums of weight * X^T Y (forward: k, v, l^(L-1-s); bwd: q, scale dy, l^(t+1)).
+// 2 x 500 tokens x 8 heads of 48: 6.6 us, the latency of two loads and a chunk's products.
 // Thread (ty, tx): rows NR ty + i and its columns.
 template <typename TA, int DP>
 __global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd, bool vec) {
@@ -367,7 +368,8 @@ __device__ __forceinline__ TilePos tile_pos(const AtlasDecayParams& P, int64_t i
   return t;
 }
 
-// y of one tile of 32 tokens
+// y of one tile of 32 tokens.  2 x 500 tokens x 8 heads of 48: 13 us, the latency of three or four
+// loads one after the other and their products.
 template <typename TA, int DP>
 __global__ void __launch_bounds__(NTH) out_kernel(Args a, int tiles, bool vec) {
   using L = Tile<DP>;
@@ -508,7 +510,8 @@ __global__ void __launch_bounds__(NTH, DP == 128 ? 3 : 6) grads_kernel(Args a, i
 // group cg) keeps rows rg, rg + RG, ... of VEC consecutive columns in registers from the
 // first token to the last; y's sum over rows goes through shared memory.  Bound by the state's
 // bytes where there are many sequences: SL = 64 then moves four 16-byte groups a thread
-// (DP = 64), 32 twice as many CTAs for few sequences.
+// (DP = 64), 32 twice as many CTAs for few sequences.  256 sequences x 12 heads of 64: 18 us, 5.6 TB/s
+// (27 us with SL = 32); one sequence: 2.4 us, most of it the launch.
 template <typename TA, int DP, int SL, int VEC>
 __global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, const int32_t* slots, int32_t n_slots,
                                                    float* out) {

@@ -333,7 +333,9 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : V
 // With z = (h - mean) rstd and u = dy w:  dx = rstd (u - mean(u) - z mean(u z)) + dh,
 // dw += dy z, db += dy.
 // A ring as in the forward (a register prefetch spilled, which made every copy wait for its
-// load: 325 us at 65536 x 768 bf16 with dh; the ring 82).
+// load: 325 us at 65536 x 768 bf16 with dh; the ring 82, 4.9 TB/s).  The sums of the weights' gradients
+// take the registers that the forward has for the weights, and leave 16 warps an SM; they and a ring of
+// two stages (there are three streams) keep it from the forward's bandwidth.
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
 __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : TEAM == SUB ? 4 : VEC * CHN <= 8 ? 3 : 2)
     bwd_kernel(Args a, int per_block, int stages) {

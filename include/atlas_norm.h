@@ -15,9 +15,9 @@
  * bias, dweight, dbias (G, N) float32; stats (rows, G, 2) float32, 8-byte aligned: mean
  * and rstd (up to 8 channels: rstd as two floats whose sum it is).
  * Arithmetic is float32 (float64 for vectors of up to 8 channels, whose gradients cancel);
- * outputs in act_dtype are rounded once.  The variance is the mean of
- * the squared differences from the mean (two passes over registers), so a large mean costs
- * no digits.  The parameter gradients are summed in a fixed order (no atomics).
+ * outputs in act_dtype are rounded once.  The variance is the mean of the squared differences
+ * from the mean (two passes over registers), so a large mean costs no digits.  The parameter
+ * gradients are summed in a fixed order (no atomics).
  *
  * Conventions (status codes, thread-local error string, stream as void*, caller-owned
  * device buffers) are those of atlas_scan.h.
