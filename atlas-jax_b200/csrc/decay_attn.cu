@@ -115,12 +115,12 @@ __global__ void __launch_bounds__(256) dg_kernel(Args a, float* dg) {
 // ---------------------------------------------------------------------------
 // float32 CUDA-core kernels (any D <= 128, strides and alignment; float32 activations)
 // ---------------------------------------------------------------------------
-// Token tiles of TT = 32 rows in shared memory, D zero-padded to DP.  128 threads as 8 x 16: thread
-// (ty, tx) owns rows ty + 8 i, i < RT, of a tile's product and NJ groups of VW consecutive
-// columns.  It reads its operands as 16-byte groups (rows along the summed axis, columns along the
-// output): 8 of them for 64 multiply-adds (two rows a thread: 6 for 32).
-constexpr int TT = 32, NTH = 128, RT = TT / 8;
-constexpr int LP = TT + 4;  // row pitch of a tile of scores: 16-byte aligned rows, no wider than a tile's
+// 256 threads as 16 x 16 over token tiles of TT = 32 rows in shared memory, D zero-padded to
+// DP.  Thread (ty, tx) owns rows ty and ty + 16 of a tile's product and NJ groups of VW
+// consecutive columns; it reads its operands as 16-byte groups (rows along the summed axis,
+// columns along the output), so a multiply-add costs a quarter of a shared-memory load or less.
+constexpr int TT = 32;
+constexpr int LP = TT + 4;  // row pitch of a tile of scores: 16-byte aligned rows
 
 template <int DP>
 struct Tile {
@@ -141,12 +141,12 @@ __device__ __forceinline__ View flat(const void* p, const AtlasDecayParams& P) {
 
 // rows [t0, t0 + TT) of head (b, h) into a tile; rows from t_end on and columns from D on are
 // 0.  vec: groups of four channels can be loaded at once.
-template <typename TA, int NT, int DP>
+template <typename TA, int DP>
 __device__ void load_rows(Tile<DP>& tile, const View& x, int b, int h, int t0, int t_end, int D, bool vec) {
   const TA* base = (const TA*)x.p + b * x.sb + h * x.sh;
 #pragma unroll
-  for (int i = 0; i < TT * DP / 4 / NT; ++i) {
-    const int u = threadIdx.x + NT * i, r = u / (DP / 4), c = 4 * (u % (DP / 4)), t = t0 + r;
+  for (int i = 0; i < TT * DP / 4 / 256; ++i) {
+    const int u = threadIdx.x + 256 * i, r = u / (DP / 4), c = 4 * (u % (DP / 4)), t = t0 + r;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (t < t_end && c < D) {
       const TA* p = base + (int64_t)t * x.st + c;
@@ -168,35 +168,16 @@ __device__ void load_rows(Tile<DP>& tile, const View& x, int b, int h, int t0, i
     *(float4*)&tile.x[r][c] = *(const float4*)v;
   }
 }
-// columns tx owns, of a row
+// columns tx owns, of row r
 template <int DP>
-__device__ __forceinline__ void row_cols(float* v, const float* row, int tx) {
+__device__ __forceinline__ void row_cols(float* v, const Tile<DP>& t, int r, int tx) {
   using L = Tile<DP>;
 #pragma unroll
   for (int j = 0; j < L::NJ; ++j) {
     if constexpr (L::VW == 4)
-      *(float4*)(v + 4 * j) = *(const float4*)(row + L::col(tx, j));
+      *(float4*)(v + 4 * j) = *(const float4*)&t.x[r][L::col(tx, j)];
     else
-      *(float2*)v = *(const float2*)(row + L::col(tx, j));
-  }
-}
-
-// acc += A (rows of pitch `pitch`, four columns) B (four rows)
-template <int DP>
-__device__ __forceinline__ void mult4(float (*acc)[Tile<DP>::NC], const float* A, int pitch, const float (*B)[Tile<DP>::LD]) {
-  using L = Tile<DP>;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float a[RT][4];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) *(float4*)a[i] = *(const float4*)(A + (ty + 8 * i) * pitch);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float x[L::NC];
-    row_cols<DP>(x, B[k], tx);
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < L::NC; ++j) acc[i][j] = fmaf(a[i][k], x[j], acc[i][j]);
+      *(float2*)v = *(const float2*)&t.x[r][L::col(tx, j)];
   }
 }
 
@@ -229,8 +210,8 @@ __global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd, bool vec) {
     for (int j = 0; j < L::NC; ++j) acc[i][j] = 0.f;
   for (int s0 = 0; s0 < len; s0 += TT) {
     __syncthreads();
-    load_rows<TA, 256>(X, xv, b, h, tc + s0, tc + len, D, vec);
-    load_rows<TA, 256>(Y, yv, b, h, tc + s0, tc + len, D, vec);
+    load_rows<TA>(X, xv, b, h, tc + s0, tc + len, D, vec);
+    load_rows<TA>(Y, yv, b, h, tc + s0, tc + len, D, vec);
     __syncthreads();
 #pragma unroll 4
     for (int r = 0; r < TT; ++r) {  // rows beyond the chunk are 0
@@ -242,7 +223,7 @@ __global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd, bool vec) {
         xr[i] = wr * t.x;
         xr[i + 1] = wr * t.y;
       }
-      row_cols<DP>(yr, Y.x[r], tx);
+      row_cols(yr, Y, r, tx);
 #pragma unroll
       for (int i = 0; i < NR; ++i)
 #pragma unroll
@@ -259,24 +240,23 @@ __global__ void __launch_bounds__(256) sums_kernel(Args a, bool bwd, bool vec) {
     }
 }
 
-// acc (the thread's rows and columns) += w_row * sum_m A[row][m] M(m, column) over a D x D matrix
-// in global memory; transposed: M(m, c) = M[c][m].  `stage`: two free tiles, SR rows.
+// acc (rows ty, ty + 16; the thread's columns) += w_r * sum_m A[r][m] M(m, column) over a D x D
+// matrix in global memory; transposed: M(m, c) = M[c][m].  `stage`: two free tiles, SR rows.
 template <int DP>
 __device__ void times_state(float (*acc)[Tile<DP>::NC], const Tile<DP>& A, const float* M, bool transposed, int D,
                             const float* w, Tile<DP>* stage) {
   using L = Tile<DP>;
   constexpr int SR = DP < 2 * TT ? DP : 2 * TT;
   float(*st)[L::LD] = stage->x;  // the second tile follows the first
-  float part[RT][L::NC];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float part[2][L::NC];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < L::NC; ++j) part[i][j] = 0.f;
+  for (int j = 0; j < L::NC; ++j) part[0][j] = part[1][j] = 0.f;
   for (int m0 = 0; m0 < D; m0 += SR) {
     if (m0) __syncthreads();
-#pragma unroll 16
-    for (int i = 0; i < SR * DP / NTH; ++i) {
-      const int u = threadIdx.x + NTH * i;
+#pragma unroll
+    for (int i = 0; i < SR * DP / 256; ++i) {
+      const int u = threadIdx.x + 256 * i;
       // consecutive threads along the contiguous axis of M
       const int m = transposed ? u % SR : u / DP, c = transposed ? u / SR : u % DP;
       float x = 0.f;
@@ -284,41 +264,68 @@ __device__ void times_state(float (*acc)[Tile<DP>::NC], const Tile<DP>& A, const
       st[m][c] = x;
     }
     __syncthreads();
-    const int n = min(SR, (D - m0 + 3) & ~3);  // rows beyond D are 0
-#pragma unroll 2
-    for (int m = 0; m < n; m += 4) mult4<DP>(part, &A.x[0][m0 + m], L::LD, st + m);
+    const int n = min(SR, (D - m0 + 3) & ~3);
+#pragma unroll 4
+    for (int m = 0; m < n; m += 4) {  // rows beyond D are 0
+      const float4 a0 = *(const float4*)&A.x[ty][m0 + m], a1 = *(const float4*)&A.x[ty + 16][m0 + m];
+      const float p0[4] = {a0.x, a0.y, a0.z, a0.w}, p1[4] = {a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float x[L::NC];
+        row_cols(x, stage[(m + k) / TT], (m + k) % TT, tx);
+#pragma unroll
+        for (int j = 0; j < L::NC; ++j) {
+          part[0][j] = fmaf(p0[k], x[j], part[0][j]);
+          part[1][j] = fmaf(p1[k], x[j], part[1][j]);
+        }
+      }
+    }
   }
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < L::NC; ++j) acc[i][j] = fmaf(w[i], part[i][j], acc[i][j]);
+  for (int j = 0; j < L::NC; ++j) {
+    acc[0][j] = fmaf(w[0], part[0][j], acc[0][j]);
+    acc[1][j] = fmaf(w[1], part[1][j], acc[1][j]);
+  }
 }
 
 __device__ __forceinline__ float dot4(float4 x, float4 y, float s) {
   return fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s))));
 }
-// (row ty + 8 i) . (row tx + 16 j) of two tiles
+// (row ty + 16 i) . (row tx + 16 j) for i, j < 2, of two tiles
 template <int DP>
 __device__ __forceinline__ void dots(float (*p)[2], const Tile<DP>& A, const Tile<DP>& B) {
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < RT; ++i) p[i][0] = p[i][1] = 0.f;
-#pragma unroll 4
+  p[0][0] = p[0][1] = p[1][0] = p[1][1] = 0.f;
+#pragma unroll 8
   for (int m = 0; m < DP; m += 4) {
+    const float4 a0 = *(const float4*)&A.x[ty][m], a1 = *(const float4*)&A.x[ty + 16][m];
     const float4 b0 = *(const float4*)&B.x[tx][m], b1 = *(const float4*)&B.x[tx + 16][m];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const float4 x = *(const float4*)&A.x[ty + 8 * i][m];
-      p[i][0] = dot4(x, b0, p[i][0]);
-      p[i][1] = dot4(x, b1, p[i][1]);
-    }
+    p[0][0] = dot4(a0, b0, p[0][0]);
+    p[0][1] = dot4(a0, b1, p[0][1]);
+    p[1][0] = dot4(a1, b0, p[1][0]);
+    p[1][1] = dot4(a1, b1, p[1][1]);
   }
 }
 // acc += Pm (32 x 32) B
 template <int DP>
 __device__ __forceinline__ void times_tile(float (*acc)[Tile<DP>::NC], const float (*Pm)[LP], const Tile<DP>& B) {
-#pragma unroll 2
-  for (int m = 0; m < TT; m += 4) mult4<DP>(acc, &Pm[0][m], LP, B.x + m);
+  using L = Tile<DP>;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int m = 0; m < TT; m += 4) {
+    const float4 a0 = *(const float4*)&Pm[ty][m], a1 = *(const float4*)&Pm[ty + 16][m];
+    const float p0[4] = {a0.x, a0.y, a0.z, a0.w}, p1[4] = {a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float x[L::NC];
+      row_cols(x, B, m + k, tx);
+#pragma unroll
+      for (int j = 0; j < L::NC; ++j) {
+        acc[0][j] = fmaf(p0[k], x[j], acc[0][j]);
+        acc[1][j] = fmaf(p1[k], x[j], acc[1][j]);
+      }
+    }
+  }
 }
 template <typename TA, int DP>
 __device__ void store_rows(void* x, const float (*acc)[Tile<DP>::NC], const AtlasDecayParams& P, int b, int h, int t0,
@@ -326,8 +333,8 @@ __device__ void store_rows(void* x, const float (*acc)[Tile<DP>::NC], const Atla
   using L = Tile<DP>;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int t = t0 + ty + 8 * i;
+  for (int i = 0; i < 2; ++i) {
+    const int t = t0 + ty + 16 * i;
     if (t >= t_end) continue;
     TA* row = (TA*)x + (((int64_t)b * P.T + t) * P.H + h) * P.D;
 #pragma unroll
@@ -339,7 +346,7 @@ __device__ void store_rows(void* x, const float (*acc)[Tile<DP>::NC], const Atla
 }
 
 __device__ __forceinline__ float cta_sum(float v) {  // every thread gets the sum
-  __shared__ float red[NTH / 32];
+  __shared__ float red[8];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
@@ -347,7 +354,7 @@ __device__ __forceinline__ float cta_sum(float v) {  // every thread gets the su
   __syncthreads();
   float s = 0;
 #pragma unroll
-  for (int i = 0; i < NTH / 32; ++i) s += red[i];
+  for (int i = 0; i < 8; ++i) s += red[i];
   return s;
 }
 
@@ -371,41 +378,37 @@ __device__ __forceinline__ TilePos tile_pos(const AtlasDecayParams& P, int64_t i
 // y of one tile of 32 tokens.  2 x 500 tokens x 8 heads of 48: 13 us, the latency of three or four
 // loads one after the other and their products.
 template <typename TA, int DP>
-__global__ void __launch_bounds__(NTH) out_kernel(Args a, int tiles, bool vec) {
+__global__ void __launch_bounds__(256) out_kernel(Args a, int tiles, bool vec) {
   using L = Tile<DP>;
   extern __shared__ float sm[];
   L &A = *(L*)sm, &K = *(&A + 1), &V = *(&A + 2);
-  float(*Pm)[LP] = (float(*)[LP])&K;  // K's place, when the scores are done
+  float(*Pm)[LP] = (float(*)[LP])(&A + 3);
   __shared__ float pw[CH + 1];
   const AtlasDecayParams& P = a.p;
   const TilePos z = tile_pos(P, blockIdx.x, tiles);
   const int D = P.D, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, tend = z.tc + z.L;
-  if (threadIdx.x <= CH) pw[threadIdx.x] = pow_decay(a.log_decay[z.h], threadIdx.x);  // CH < NTH
-  load_rows<TA, NTH>(A, view(a.q, P.q_stride), z.b, z.h, z.tc + z.r0, tend, D, vec);
-  float acc[RT][L::NC], w[RT];
+  if (threadIdx.x <= CH) pw[threadIdx.x] = pow_decay(a.log_decay[z.h], threadIdx.x);
+  load_rows<TA>(A, view(a.q, P.q_stride), z.b, z.h, z.tc + z.r0, tend, D, vec);
+  float acc[2][L::NC];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < L::NC; ++j) acc[i][j] = 0.f;
+  for (int j = 0; j < L::NC; ++j) acc[0][j] = acc[1][j] = 0.f;
   after_previous();  // the states
   __syncthreads();   // pw
-#pragma unroll
-  for (int i = 0; i < RT; ++i) w[i] = pw[z.r0 + ty + 8 * i + 1];
+  const float w[2] = {pw[z.r0 + ty + 1], pw[z.r0 + ty + 17]};
   times_state<DP>(acc, A, a.states + (z.chain * chunks(P) + z.c) * (int64_t)D * D, false, D, w, &K);
   for (int s0 = 0; s0 <= z.r0; s0 += TT) {
     __syncthreads();
-    load_rows<TA, NTH>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, vec);
-    load_rows<TA, NTH>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + s0, tend, D, vec);
+    load_rows<TA>(K, view(a.k, P.k_stride), z.b, z.h, z.tc + s0, tend, D, vec);
+    load_rows<TA>(V, view(a.v, P.v_stride), z.b, z.h, z.tc + s0, tend, D, vec);
     __syncthreads();
-    float p[RT][2];
+    float p[2][2];
     dots(p, A, K);
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int lag = z.r0 + ty + 8 * i - (s0 + tx + 16 * j);
-        Pm[ty + 8 * i][tx + 16 * j] = lag >= 0 ? p[i][j] * pw[lag] : 0.f;
+        const int lag = z.r0 + ty + 16 * i - (s0 + tx + 16 * j);
+        Pm[ty + 16 * i][tx + 16 * j] = lag >= 0 ? p[i][j] * pw[lag] : 0.f;
       }
     __syncthreads();
     times_tile<DP>(acc, Pm, V);
@@ -421,18 +424,19 @@ __global__ void __launch_bounds__(NTH) out_kernel(Args a, int tiles, bool vec) {
 //                                                                dv: X = k,  M = R,   W = q,  U = dy
 //
 // Three CTAs a tile, each with one accumulator; dk and dv share no product, and a CTA that made both
-// was the launch's longest (2 x 500 tokens x 8 heads of 48: 45 us, with three 38).  With the scores in
-// W's place six CTAs share an SM, and those 768 run at once: 32 us.  About half of its issue slots are
-// multiply-adds (8 us of them); the rest of the time is the latency of four dependent loads.  dq's and
-// dk's CTAs also sum their terms of dlog_decay, with Y = q and k.
+// was the launch's longest (2 x 500 tokens x 8 heads of 48: 45 us, with three 38).  8 us of that are
+// multiply-adds at the full rate, about half of its issue slots; the rest is the latency of four loads, one
+// after the other, with five CTAs an SM.  (128 threads of four rows, six CTAs an SM: 32 us with all
+// data in L2, but 8 us longer where it comes from memory.)  dq's and dk's CTAs also sum their terms of
+// dlog_decay, with Y = q and k.
 enum Grad { DK, DV, DQ };
 template <typename TA, int DP>
-__global__ void __launch_bounds__(NTH, DP == 128 ? 3 : 6) grads_kernel(Args a, int tiles, bool vec) {
+__global__ void __launch_bounds__(256, DP == 128 ? 2 : 4) grads_kernel(Args a, int tiles, bool vec) {
   using L = Tile<DP>;
   extern __shared__ float sm[];
   __shared__ float pw[CH + 1];
   L *const t = (L*)sm, &X = t[0], &Y = t[1], &U = t[2], &W = t[3];
-  float(*Pm)[LP] = (float(*)[LP])&W;  // W's place, when the scores are done
+  float(*Pm)[LP] = (float(*)[LP])(t + 4);
   const AtlasDecayParams& P = a.p;
   const TilePos z = tile_pos(P, blockIdx.x / 3, tiles);
   const int kind = blockIdx.x % 3;
@@ -440,58 +444,53 @@ __global__ void __launch_bounds__(NTH, DP == 128 ? 3 : 6) grads_kernel(Args a, i
   const View q = view(a.q, P.q_stride), k = view(a.k, P.k_stride), v = view(a.v, P.v_stride), o = flat(a.dy, P);
   const View xs = kind == DQ ? o : kind == DK ? v : k, us = kind == DQ ? k : kind == DK ? q : o,
              ws = kind == DQ ? v : kind == DK ? o : q;
-  load_rows<TA, NTH>(X, xs, z.b, z.h, z.tc + z.r0, tend, D, vec);
-  if (kind != DV) load_rows<TA, NTH>(Y, kind == DQ ? q : k, z.b, z.h, z.tc + z.r0, tend, D, vec);
+  load_rows<TA>(X, xs, z.b, z.h, z.tc + z.r0, tend, D, vec);
+  if (kind != DV) load_rows<TA>(Y, kind == DQ ? q : k, z.b, z.h, z.tc + z.r0, tend, D, vec);
   if (threadIdx.x <= CH) pw[threadIdx.x] = pow_decay(a.log_decay[z.h], threadIdx.x);
   let_next_start();
   after_previous();  // R
   __syncthreads();
-  float acc[RT][L::NC], w[RT], dg = 0.f;
-  int n[RT];  // steps from the rows to the chunk's start (dq) or end
+  float acc[2][L::NC], dg = 0.f;
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-#pragma unroll
-    for (int j = 0; j < L::NC; ++j) acc[i][j] = 0.f;
-    const int r = z.r0 + ty + 8 * i;
-    n[i] = kind == DQ ? r + 1 : z.L - 1 - r;
-    w[i] = n[i] >= 0 ? (kind == DQ ? P.scale : 1.f) * pw[n[i]] : 0.f;
-  }
+  for (int j = 0; j < L::NC; ++j) acc[0][j] = acc[1][j] = 0.f;
+  // steps from the rows to the chunk's start (dq) or end
+  const int n0 = kind == DQ ? z.r0 + ty + 1 : z.L - 1 - z.r0 - ty, n1 = kind == DQ ? n0 + 16 : n0 - 16;
+  const float s = kind == DQ ? P.scale : 1.f, w[2] = {n0 >= 0 ? s * pw[n0] : 0.f, n1 >= 0 ? s * pw[n1] : 0.f};
   const int64_t so = (z.chain * chunks(P) + z.c) * (int64_t)D * D;
   const float *R = a.dstates + so, *S = a.states + so;
   times_state<DP>(acc, X, kind == DQ ? S : R, kind != DV, D, w, &U);
   if (kind != DV) {  // columns from D on are 0 in Y
+    float y0[L::NC], y1[L::NC];
+    row_cols(y0, Y, ty, tx);
+    row_cols(y1, Y, ty + 16, tx);
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      float y[L::NC], s = 0.f;
-      row_cols<DP>(y, Y.x[ty + 8 * i], tx);
-#pragma unroll
-      for (int j = 0; j < L::NC; ++j) s = fmaf(y[j], acc[i][j], s);
-      if (n[i] > 0) dg = fmaf((float)n[i], s, dg);
+    for (int j = 0; j < L::NC; ++j) {
+      if (n0 > 0) dg += (float)n0 * y0[j] * acc[0][j];
+      if (n1 > 0) dg += (float)n1 * y1[j] * acc[1][j];
     }
   }
   if (kind == DQ && z.r0 == 0) {  // once for each chunk, where the loop below is short
     float rs = 0.f;
 #pragma unroll 4
-    for (int u = threadIdx.x; u < D * D; u += NTH) rs = fmaf(R[u], S[u], rs);
+    for (int u = threadIdx.x; u < D * D; u += 256) rs = fmaf(R[u], S[u], rs);
     dg += (float)z.L * pw[z.L] * rs;
   }
   for (int s0 = kind == DQ ? 0 : z.r0; s0 < (kind == DQ ? z.r0 + 1 : z.L); s0 += TT) {
     __syncthreads();
-    load_rows<TA, NTH>(U, us, z.b, z.h, z.tc + s0, tend, D, vec);
-    load_rows<TA, NTH>(W, ws, z.b, z.h, z.tc + s0, tend, D, vec);
+    load_rows<TA>(U, us, z.b, z.h, z.tc + s0, tend, D, vec);
+    load_rows<TA>(W, ws, z.b, z.h, z.tc + s0, tend, D, vec);
     __syncthreads();
-    float x[RT][2], p[RT][2];
+    float x[2][2], p[2][2];
     dots(x, X, W);
     if (kind == DQ) dots(p, Y, U);
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int d = z.r0 + ty + 8 * i - (s0 + tx + 16 * j), lag = kind == DQ ? d : -d;
+        const int d = z.r0 + ty + 16 * i - (s0 + tx + 16 * j), lag = kind == DQ ? d : -d;
         const float f = lag >= 0 ? P.scale * pw[lag] * x[i][j] : 0.f;
         if (kind == DQ && lag > 0) dg += (float)lag * p[i][j] * f;
-        Pm[ty + 8 * i][tx + 16 * j] = f;
+        Pm[ty + 16 * i][tx + 16 * j] = f;
       }
     __syncthreads();
     times_tile<DP>(acc, Pm, U);
@@ -679,15 +678,15 @@ template <typename TA, int DP>
 static cudaError_t plain_dp(const Args& a, Phase f, cudaStream_t s) {
   const int tiles = (a.p.T + TT - 1) / TT;
   const bool vec = vec4(a);
-  const auto smem = [](int n) { return n * sizeof(Tile<DP>); };
+  const auto smem = [](int n, int squares) { return n * sizeof(Tile<DP>) + (size_t)squares * TT * LP * sizeof(float); };
   if (f == OUT) {
-    const cudaError_t e = allow_smem<out_kernel<TA, DP>>(smem(3));
+    const cudaError_t e = allow_smem<out_kernel<TA, DP>>(smem(3, 1));
     if (e != cudaSuccess) return e;
-    return follow(out_kernel<TA, DP>, (unsigned)(chains(a.p) * tiles), NTH, smem(3), s, a, tiles, vec);
+    return follow(out_kernel<TA, DP>, (unsigned)(chains(a.p) * tiles), 256, smem(3, 1), s, a, tiles, vec);
   } else if (f == GRADS) {
-    const cudaError_t e = allow_smem<grads_kernel<TA, DP>>(smem(4));
+    const cudaError_t e = allow_smem<grads_kernel<TA, DP>>(smem(4, 1));
     if (e != cudaSuccess) return e;
-    return follow(grads_kernel<TA, DP>, (unsigned)(chains(a.p) * tiles * 3), NTH, smem(4), s, a, tiles, vec);
+    return follow(grads_kernel<TA, DP>, (unsigned)(chains(a.p) * tiles * 3), 256, smem(4, 1), s, a, tiles, vec);
   } else {
     sums_kernel<TA, DP><<<(unsigned)(chains(a.p) * chunks(a.p)), 256, 0, s>>>(a, f == SUMS_BWD, vec);
   }
