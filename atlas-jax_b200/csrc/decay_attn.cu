@@ -639,10 +639,10 @@ static bool tensor_path(const AtlasDecayParams& p) {
 }
 // workspaces: the sums of a split walk (tensor path); the chunks' states, where they are not kept
 static size_t fwd_bytes(const AtlasDecayParams& p, bool saved) {
-  return tensor_path(p) ? tcore::sums_bytes(p) : saved ? 0 : state_bytes(p);
+  return tensor_path(p) ? tcore::sums_bytes(p, false) : saved ? 0 : state_bytes(p);
 }
 // the chunks' cotangent states, the sums of their walk, the parts of dlog_decay
-static size_t bwd_states(const AtlasDecayParams& p) { return state_bytes(p) + (tensor_path(p) ? tcore::sums_bytes(p) : 0); }
+static size_t bwd_states(const AtlasDecayParams& p) { return state_bytes(p) + (tensor_path(p) ? tcore::sums_bytes(p, true) : 0); }
 static size_t bwd_bytes(const AtlasDecayParams& p) {
   return bwd_states(p) + (size_t)chains(p) * parts(p) * sizeof(float);
 }

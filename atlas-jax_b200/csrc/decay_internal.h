@@ -49,7 +49,7 @@ bool mappable(const AtlasDecayParams& p, const int64_t* strides);  // whether TM
 // The walk along the sequences (decay_scan.cu): forward y and states, or (bwd) the cotangent
 // states.  saves: (chains, chunks, D, D), the state entering every chunk in the order of the
 // walk, or NULL.  sums: sums_bytes() of scratch.
-size_t sums_bytes(const AtlasDecayParams& p);
+size_t sums_bytes(const AtlasDecayParams& p, bool bwd);
 cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, float* saves, float* sums,
                        cudaStream_t s);
 // dq, dk, dv and the parts of dlog_decay, chunk by chunk, from a.states and a.dstates (decay_grad.cu)

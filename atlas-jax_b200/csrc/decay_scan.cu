@@ -66,11 +66,6 @@ struct Cfg {
   static constexpr int OFF_P = OFF_KP + DBL * 3 * TILE;
   static constexpr int OFF_S = OFF_P + (FWD ? DBL * PT : 0);
   static constexpr int OFF_CTL = OFF_S + (FWD ? DBL * 2 * ST : 0);
-  // Whether a segment puts its entering state together itself.  At D = 128 that is 64 KB a segment before
-  // it, read at 2 to 3 us each (32 loads a thread with S in registers: few in flight), and join_kernel
-  // is faster: 4 x 1900 tokens x 6 heads 26.7 + 4.8 us against 38.7.  At D = 64 the launch costs more:
-  // 3 x 777 x 12 10.2 + 3.0 us against 10.4.
-  static constexpr bool JOIN = DP == 64;
   // TMEM columns
   static constexpr uint32_t T_A = 0, T_DS = FWD ? DBL * 64 : 0, T_QS = T_DS + DBL * DP, T_O = T_QS + DBL * DP;
   static constexpr uint32_t COLS = FWD ? 512 : DBL * DP;
@@ -105,6 +100,7 @@ struct SeqArgs {
   float* saves;    // state entering every block, in the order of the walk; or NULL
   int segs;        // segments of a sequence
   int seg_blocks;  // blocks of a segment
+  int joined;      // join_kernel has made the sums the states that enter their segments
   int sums_pass;   // segments 0 .. segs - 2, all but the first from zeros, to `sums`
   int* status;
 };
@@ -371,7 +367,8 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
         add_state(in ? sum_at(a, z.chain, 0) : nullptr, 0., true);
       } else {
         const double f = exp((double)g * ((double)a.seg_blocks * C));
-        for (int j = K::JOIN ? 1 : z.seg; j <= z.seg; ++j) add_state(sum_at(a, z.chain, j), f, j == (K::JOIN ? 1 : z.seg));
+        const int j0 = a.joined ? z.seg : 1;
+        for (int j = j0; j <= z.seg; ++j) add_state(sum_at(a, z.chain, j), f, j == j0);
       }
     }
     auto put_state = [&](float* out) {
@@ -590,29 +587,40 @@ static cudaError_t launch(const CUtensorMap& q, const CUtensorMap& x, const CUte
   return cudaGetLastError();
 }
 
-// How many segments to cut a sequence into, and their blocks.  In block times: a CTA an SM,
-// rounds of them; a split adds the sums' pass, at about 0.5 of a full block's time, its
-// launch and the reading of its sums (about 4 blocks' time).
+// Whether the sums are joined by a kernel of their own, and not by the segments' CTAs, which read them one
+// after the other at about 0.7 us (D = 64) or 2.5 us (D = 128, with few registers left for loads) each.
+// 4 x 1900 tokens x 6 heads of 128, six segments: 26.7 + 4.8 us against 38.7; 3 x 777 x 12 heads of 64, four:
+// 10.2 + 3.0 us against 10.4; 32768 x 2 heads of 64, 64 segments, the whole forward: 37 us against 116.
+static bool join_first(const AtlasDecayParams& p, int segs) { return segs > (p.D > 64 ? 2 : 4); }
+
+// How many segments to cut a sequence into, and their blocks: the least time by what was measured (us).
+// A CTA an SM, in rounds; a round is a CTA's start and end, and its blocks.
 struct Split {
   int segs, blocks;
 };
-static Split split(const AtlasDecayParams& p) {
+static Split split(const AtlasDecayParams& p, bool bwd) {
+  const bool wide = p.D > 64;
+  const double start = wide ? 9 : 5, start_sum = wide ? 7.5 : 3;  // (the sums' end runs beside the next start)
+  const double sum = wide ? 1.3 : 0.9, full = wide ? (bwd ? 1.9 : 3.1) : bwd ? 0.9 : 1.15;  // a block
   const int nblk = (p.T + C - 1) / C;
   const int64_t n = chains(p), sms = 148;
+  auto rounds = [&](int64_t ctas) { return (double)((ctas + sms - 1) / sms); };
   Split best{1, nblk};
-  double cost = (double)((n + sms - 1) / sms) * nblk;
+  double cost = rounds(n) * (start + nblk * full);
   for (int k = 2; k <= 64 && k <= nblk; ++k) {
     const int len = (nblk + k - 1) / k, segs = (nblk + len - 1) / len;
     if (segs != k) continue;
-    const double c = (double)((n * k + sms - 1) / sms) * len + 0.5 * (double)((n * (k - 1) + sms - 1) / sms) * len + 4;
+    const double c = rounds(n * k) * (start + len * full) + rounds(n * (k - 1)) * (start_sum + len * sum) +
+                     (join_first(p, k) ? 4 + 0.1 * k : 0.7 * (k - 2));
     if (c < 0.95 * cost) cost = c, best = Split{k, len};
   }
   return best;
 }
 
 // What enters segments 2, 3, ..: S <- l^len S + sum, in place, len tokens each.  One thread per 4
-// elements of a chain's state.
+// elements of a chain's state; the loads of UN segments are in flight together.
 __global__ void __launch_bounds__(256) join_kernel(SeqArgs a) {
+  constexpr int UN = 8;
   const int per = a.p.D * a.p.D / 4;
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
   let_next_start();
@@ -622,20 +630,26 @@ __global__ void __launch_bounds__(256) join_kernel(SeqArgs a) {
   float4* m = (float4*)sum_at(a, chain, 1) + (u - chain * per);
   const double f = exp((double)a.log_decay[chain % a.p.H] * ((double)a.seg_blocks * C));
   const float fh = (float)f, fl = (float)(f - (double)fh);
-  float4 S = m[0], x = m[per];
-  for (int s = 2; s < a.segs; ++s) {
-    const float4 y = s + 1 < a.segs ? m[(int64_t)s * per] : x;  // the next load early
-    S.x = fmaf(S.x, fh, fmaf(S.x, fl, x.x));
-    S.y = fmaf(S.y, fh, fmaf(S.y, fl, x.y));
-    S.z = fmaf(S.z, fh, fmaf(S.z, fl, x.z));
-    S.w = fmaf(S.w, fh, fmaf(S.w, fl, x.w));
-    m[(int64_t)(s - 1) * per] = S;
-    x = y;
+  float4 S = m[0];
+  for (int s0 = 1; s0 < a.segs - 1; s0 += UN) {
+    float4 x[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i)
+      if (s0 + i < a.segs - 1) x[i] = m[(int64_t)(s0 + i) * per];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      if (s0 + i >= a.segs - 1) break;
+      S.x = fmaf(S.x, fh, fmaf(S.x, fl, x[i].x));
+      S.y = fmaf(S.y, fh, fmaf(S.y, fl, x[i].y));
+      S.z = fmaf(S.z, fh, fmaf(S.z, fl, x[i].z));
+      S.w = fmaf(S.w, fh, fmaf(S.w, fl, x[i].w));
+      m[(int64_t)(s0 + i) * per] = S;
+    }
   }
 }
 
-size_t sums_bytes(const AtlasDecayParams& p) {
-  const int segs = split(p).segs;
+size_t sums_bytes(const AtlasDecayParams& p, bool bwd) {
+  const int segs = split(p, bwd).segs;
   return segs > 1 ? (size_t)chains(p) * segs * p.D * p.D * sizeof(float) : 0;
 }
 
@@ -650,7 +664,7 @@ cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, flo
   else
     ok = make_map(&mq, a.q, p, p.q_stride) && make_map(&mx, a.k, p, p.k_stride) && make_map(&my, a.v, p, p.v_stride);
   if (!ok) return cudaErrorInvalidValue;
-  const Split z = split(p);
+  const Split z = split(p, bwd);
   const bool wide = p.D > 64;
   SeqArgs q{};
   q.p = p;
@@ -668,7 +682,8 @@ cudaError_t launch_seq(const Args& a, bool bwd, const float* in, float* out, flo
     cudaError_t e = wide ? launch<128, false>(mq, mx, my, q, bwd, s) : launch<64, false>(mq, mx, my, q, bwd, s);
     if (e != cudaSuccess) return e;
     q.sums_pass = 0;
-    if (wide && z.segs > 2) {
+    if (join_first(p, z.segs)) {
+      q.joined = 1;
       const int64_t n = chains(p) * p.D * p.D / 4;
       e = follow(join_kernel, (unsigned)((n + 255) / 256), 256, 0, s, q);
       if (e != cudaSuccess) return e;

@@ -73,6 +73,12 @@ def test_forward_backward(B, T, H, D, dtype):
     _check(B, T, H, D, dtype)
 
 
+@pytest.mark.parametrize("B,T,H,D", [(1, 4133, 1, 64), (1, 1100, 2, 128), (1, 600, 3, 40), (2, 321, 5, 72)])
+def test_many_segments(B, T, H, D):
+    """Few heads: sequences cut into many segments, the last one short."""
+    _check(B, T, H, D, BF)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("fused,state", [(False, False), (False, True), (True, False)])
 def test_without_state_and_unfused(dtype, fused, state):
