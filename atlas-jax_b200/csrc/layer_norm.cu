@@ -122,6 +122,41 @@ __device__ __forceinline__ void copy16(void* slot, const void* g) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slot)), "l"(g)
                : "memory");
 }
+enum Team { SUB, ONE, MANY };  // MANY: WARPS teams of more than one warp
+
+// n elements from element o on of a tensor of `total`, at any alignment, into a slot of shared memory: the
+// aligned 16-byte pieces that hold them, copied by the lanes of a team (which have to meet before they
+// read).  Pieces reach into the neighbouring vectors, but not beyond the tensor: at its ends
+// single elements.  The vector starts at offset span_shift() of the slot.
+template <typename TA>
+__device__ __forceinline__ int span_shift(const TA* t, int64_t o) {
+  return (int)((uintptr_t)(t + o) & 15) / (int)sizeof(TA);
+}
+template <typename TA>
+__device__ __forceinline__ void copy_span(uint8_t* slot, const TA* t, int64_t o, int n, int64_t total, int lane,
+                                          int lanes) {
+  const uintptr_t lo = (uintptr_t)(t + o), hi = (uintptr_t)(t + o + n), a0 = lo & ~(uintptr_t)15;
+  for (uintptr_t a = a0 + 16 * lane; a < hi; a += 16 * lanes) {
+    uint8_t* d = slot + (a - a0);
+    if (a >= (uintptr_t)t && a + 16 <= (uintptr_t)(t + total)) {
+      copy16(d, (const void*)a);
+    } else {
+      for (int j = 0; j < 16 / (int)sizeof(TA); ++j) {
+        const uintptr_t e = a + j * sizeof(TA);
+        if (e >= lo && e < hi) ((TA*)d)[j] = *(const TA*)e;
+      }
+    }
+  }
+}
+static __host__ __device__ __forceinline__ int span_bytes(int n, int size) { return (n * size + 30) / 16 * 16; }
+// the lanes of a team meet
+template <Team TEAM>
+__device__ __forceinline__ void team_sync(int warps, int barrier) {
+  if constexpr (TEAM == MANY)
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
+  else
+    __syncwarp();
+}
 template <typename TA>
 __device__ __forceinline__ float round_to(float x) {
   TA t[1];
@@ -142,8 +177,6 @@ __device__ __forceinline__ void load_param(float* f, const float* p, float missi
     for (int j = 0; j < VEC; ++j) f[j] = p[j];
   }
 }
-
-enum Team { SUB, ONE, MANY };  // MANY: WARPS teams of more than one warp
 
 // Sums of K values over a team; every lane gets them.  MANY: `red` holds 2 x 16 x K floats of
 // the team, used alternately so that one barrier per call is enough.
@@ -207,7 +240,9 @@ struct Place {
 // ---------------------------------------------------------------------------
 // The vectors to come are copied into a ring in shared memory, `stages` - 1 of them ahead; every
 // thread copies the groups that it will work on itself, so the ring needs no barrier and holds no
-// registers.  Single channels (VEC = 1) are loaded directly.  Bound by memory: about 140 KB an SM are on
+// registers.  Where rows are not aligned (VEC = 1) a team copies the aligned span that holds its vector,
+// meets, and each lane picks its channels (5099 x 2533 bf16, training: 165 us, 294 with direct
+// loads of single channels).  Bound by memory: about 140 KB an SM are on
 // their way, and the weights stay in registers (read again for every row they were as many bytes as the
 // row, through an L1 that was then 72 % busy).  65536 x 768 bf16 with a residual: 65 us, 6.2 TB/s;
 // 79 us with direct loads and 32 warps an SM.
@@ -216,7 +251,7 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : V
     fwd_kernel(Args a, int per_block, int stages) {
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float red_all[8][2 * 16];
-  constexpr bool RING = VEC > 1;
+  constexpr bool OWN = VEC > 1;  // a thread copies what it uses; otherwise the team copies a span
   constexpr int NP = PAIRS<VEC>;
   typedef Pack<TA, VEC> Raw;
   int turn = 0;
@@ -242,11 +277,12 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : V
   const bool fixed = TEAM == SUB || a.G == 1;  // one group's weights in every round
   if (fixed) params(TEAM == SUB ? z.first % a.G : 0);
   Raw* ring = (Raw*)dyn + threadIdx.x;  // slot (stage, stream, c): 2 streams
-  const int pitch = blockDim.x;
+  const int pitch = blockDim.x, bytes = span_bytes(a.N, sizeof(TA));
+  uint8_t* spans = dyn + (size_t)z.team * stages * 2 * bytes;  // slot (stage, stream) of the team
   auto fetch = [&](int64_t v, int st) {
-    if constexpr (RING) {
-      if (v < a.vecs) {
-        const int64_t o = v * a.N;
+    if (v < a.vecs) {
+      const int64_t o = v * a.N;
+      if constexpr (OWN) {
         Raw* r = ring + st * 2 * CHN * pitch;
 #pragma unroll
         for (int c = 0; c < CHN; ++c)
@@ -254,9 +290,12 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : V
             copy16(r + c * pitch, x + o + c * dn);
             if (res) copy16(r + (CHN + c) * pitch, res + o + c * dn);
           }
+      } else {
+        copy_span(spans + st * 2 * bytes, (const TA*)a.x, o, a.N, a.vecs * a.N, z.lane, z.lanes);
+        if (res) copy_span(spans + (st * 2 + 1) * bytes, (const TA*)a.res, o, a.N, a.vecs * a.N, z.lane, z.lanes);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   int at = 0;  // stage of the current vector
   for (int i = 0; i < 3; ++i) fetch(i < stages - 1 ? z.first + i * z.stride : a.vecs, i);  // 3 groups always
@@ -264,22 +303,25 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : V
     const bool on = v0 < a.vecs;
     const int64_t o = v0 * a.N;
     if (!fixed) params(v0 % a.G);
-    if constexpr (RING) {
-      // the group of this vector is the (stages - 1)-th newest
-      if (stages == 4)
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-    }
-    const Raw* slot = ring + at * 2 * CHN * pitch;
+    // the group of this vector is the (stages - 1)-th newest
+    if (stages == 4)
+      asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!OWN) team_sync<TEAM>(z.warps, 1 + z.team);
+    const Raw* slot = OWN ? ring + at * 2 * CHN * pitch
+                          : (const Raw*)(spans + at * 2 * bytes) + span_shift((const TA*)a.x, o) + n0;
+    const Raw* slot_r = OWN ? slot + CHN * pitch
+                            : (const Raw*)(spans + (at * 2 + 1) * bytes) + span_shift((const TA*)a.res, o) + n0;
+    const int step = OWN ? pitch : dn;
     F2 f[CHN][NP], s2 = f2(0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < CHN; ++c) {
       if (on && c * dn < left) {
-        unpack2<TA, VEC>(f[c], RING ? slot[c * pitch] : *(const Raw*)(x + o + c * dn));
+        unpack2<TA, VEC>(f[c], slot[c * step]);
         if (res) {
           F2 r[NP];
-          unpack2<TA, VEC>(r, RING ? slot[(CHN + c) * pitch] : *(const Raw*)(res + o + c * dn));
+          unpack2<TA, VEC>(r, slot_r[c * step]);
 #pragma unroll
           for (int j = 0; j < NP; ++j) {
             f[c][j] = f[c][j] + r[j];
@@ -291,7 +333,7 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : V
         for (int j = 0; j < NP; ++j) s2 = s2 + f[c][j];
       }
     }
-    if constexpr (RING) {  // into the slot of the vector before
+    {  // into the slot of the vector before
       const int to = at == 0 ? stages - 1 : at - 1;
       fetch(v0 + (stages - 1) * z.stride, to);
       at = at + 1 == stages ? 0 : at + 1;
@@ -341,7 +383,7 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : T
     bwd_kernel(Args a, int per_block, int stages) {
   extern __shared__ __align__(16) uint8_t dyn[];  // the ring; after it the teams' sums, 2 x width each
   __shared__ float red_all[8][2 * 16 * 2];
-  constexpr bool RING = VEC > 1;
+  constexpr bool OWN = VEC > 1;  // as in the forward
   constexpr int NP = PAIRS<VEC>;
   typedef Pack<TA, VEC> Raw;
   let_next_start();
@@ -359,11 +401,12 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : T
 #pragma unroll
     for (int j = 0; j < NP; ++j) dw[c][j] = db[c][j] = f2(0.f, 0.f);
   Raw* ring = (Raw*)dyn + threadIdx.x;  // slot (stage, stream, c): 3 streams
-  const int pitch = blockDim.x;
+  const int pitch = blockDim.x, bytes = span_bytes(a.N, sizeof(TA));
+  uint8_t* spans = dyn + (size_t)z.team * stages * 3 * bytes;  // slot (stage, stream) of the team
   auto fetch = [&](int64_t v, int st) {
-    if constexpr (RING) {
-      if (v < a.vecs) {
-        const int64_t o = v * a.N;
+    if (v < a.vecs) {
+      const int64_t o = v * a.N;
+      if constexpr (OWN) {
         Raw* r = ring + st * 3 * CHN * pitch;
 #pragma unroll
         for (int c = 0; c < CHN; ++c)
@@ -372,37 +415,45 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : T
             copy16(r + (CHN + c) * pitch, dy + o + c * dn);
             if (dh) copy16(r + (2 * CHN + c) * pitch, dh + o + c * dn);
           }
+      } else {
+        uint8_t* r = spans + st * 3 * bytes;
+        copy_span(r, (const TA*)a.h, o, a.N, a.vecs * a.N, z.lane, z.lanes);
+        copy_span(r + bytes, (const TA*)a.dy, o, a.N, a.vecs * a.N, z.lane, z.lanes);
+        if (dh) copy_span(r + 2 * bytes, (const TA*)a.dh, o, a.N, a.vecs * a.N, z.lane, z.lanes);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   int at = 0;  // stage of the current vector
+  auto span = [&](int st, int k, const void* t, int64_t o) {  // this thread's first channel in stream k of a stage
+    return (const Raw*)(spans + (st * 3 + k) * bytes) + span_shift((const TA*)t, o) + n0;
+  };
   for (int i = 0; i < 3; ++i) fetch(i < stages - 1 ? z.first + i * z.stride : a.vecs, i);  // 3 groups always
   float2 nst = z.first < a.vecs ? *(const float2*)(a.cstats + 2 * z.first) : make_float2(0.f, 0.f);
   for (int64_t v0 = z.first; !z.done(v0, a.vecs); v0 += z.stride) {
     const bool on = v0 < a.vecs;
     const float2 st = nst;
     if (v0 + z.stride < a.vecs) nst = *(const float2*)(a.cstats + 2 * (v0 + z.stride));
-    if constexpr (RING) {
-      // the group of this vector is the (stages - 1)-th newest
-      if (stages == 4)
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-    }
+    // the group of this vector is the (stages - 1)-th newest
+    if (stages == 4)
+      asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!OWN) team_sync<TEAM>(z.warps, 1 + z.team);
     F2 f[CHN][NP], d[CHN][NP], s0 = f2(0.f, 0.f), s1 = f2(0.f, 0.f);
     const F2 nmean = f2(-st.x, -st.x), rstd = f2(st.y, st.y);
-    const Raw* slot = ring + at * 3 * CHN * pitch;
+    const int cur = at;
+    const Raw* slot = ring + cur * 3 * CHN * pitch;
     const int64_t o = v0 * a.N;
 #pragma unroll
     for (int c = 0; c < CHN; ++c) {
       if (on && n0 + c * dn < a.N) {
-        if constexpr (RING) {
+        if constexpr (OWN) {
           unpack2<TA, VEC>(f[c], slot[c * pitch]);
           unpack2<TA, VEC>(d[c], slot[(CHN + c) * pitch]);
         } else {
-          unpack2<TA, VEC>(f[c], *(const Raw*)(h + o + c * dn));
-          unpack2<TA, VEC>(d[c], *(const Raw*)(dy + o + c * dn));
+          unpack2<TA, VEC>(f[c], span(cur, 0, a.h, o)[c * dn]);
+          unpack2<TA, VEC>(d[c], span(cur, 1, a.dy, o)[c * dn]);
         }
         float w[2 * NP];
         w[2 * NP - 1] = 0.f;
@@ -418,7 +469,7 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : T
         }
       }
     }
-    if constexpr (RING) {  // into the slot of the vector before
+    {  // into the slot of the vector before
       const int to = at == 0 ? stages - 1 : at - 1;
       fetch(v0 + (stages - 1) * z.stride, to);
       at = at + 1 == stages ? 0 : at + 1;
@@ -434,10 +485,10 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : T
 #pragma unroll
         for (int j = 0; j < NP; ++j) d[c][j] = fma2(rstd, d[c][j], fma2(f[c][j], c2, c1));
         if (dh) {
-          if constexpr (RING)
+          if constexpr (OWN)
             unpack2<TA, VEC>(f[c], slot[(2 * CHN + c) * pitch]);
           else
-            unpack2<TA, VEC>(f[c], *(const Raw*)(dh + o + c * dn));
+            unpack2<TA, VEC>(f[c], span(cur, 2, a.dh, o)[c * dn]);
 #pragma unroll
           for (int j = 0; j < NP; ++j) d[c][j] = d[c][j] + f[c][j];
         }
@@ -448,7 +499,7 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : T
   if (!a.part) return;
   float* pw = a.part + (int64_t)blockIdx.x * 2 * a.width;
   // the teams of the block side by side, where the ring was, then added up in order
-  if (RING) asm volatile("cp.async.wait_all;" ::: "memory");
+  asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
   const bool alone = TEAM != SUB && per_block == 1;  // one team: straight to its partial row
   float* aw = alone ? pw : (float*)dyn + z.team * 2 * a.width;
@@ -802,8 +853,8 @@ static cudaError_t allow_smem() {
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
 static cudaError_t go(const Args& a, const Plan& z, bool bwd, cudaStream_t s) {
   // as many stages, up to 4, as the blocks that an SM's registers hold have room for
-  const int stage = VEC > 1 ? (bwd ? 3 : 2) * CHN * z.threads * 16 : 0;
-  const int room = (bwd || VEC * CHN <= 8 ? 50 : z.threads <= 256 ? 100 : 200) << 10;
+  const int stage = (bwd ? 3 : 2) * (VEC > 1 ? CHN * z.threads * 16 : z.per_block * span_bytes(a.N, sizeof(TA)));
+  const int room = (VEC == 1 && z.threads > 256 ? 200 : bwd || VEC * CHN <= 8 ? 50 : z.threads <= 256 ? 100 : 200) << 10;
   const int stages = 4 * stage <= room ? 4 : 2;
   if (bwd) {
     const size_t sums = TEAM == SUB || z.per_block > 1 ? (size_t)z.per_block * 2 * z.width * sizeof(float) : 0;

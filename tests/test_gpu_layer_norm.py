@@ -65,6 +65,15 @@ def test_forward_backward(shape, wshape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("shape,wshape", [((20011, 33), (33,)), ((6007, 261), (261,)), ((9001, 3, 17), (3, 17)), ((2411, 1031), (1031,))])
+def test_many_odd_rows(shape, wshape, dtype):
+    """Rows at every alignment, more of them than the vectors that a team holds at once."""
+    x, res, w, b, dy, dh = _make(shape, wshape, dtype)
+    _check(x, res, w, b, dy, dh)
+    _check(x, None, w, b, dy, dh)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_missing_parameters(dtype):
     x, res, w, b, dy, dh = _make((20, 4, 64), (4, 64), dtype)
     _check(x, None, None, None, dy, dh)
