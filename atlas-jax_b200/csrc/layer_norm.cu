@@ -241,7 +241,7 @@ struct Place {
 // The vectors to come are copied into a ring in shared memory, `stages` - 1 of them ahead; every
 // thread copies the groups that it will work on itself, so the ring needs no barrier and holds no
 // registers.  Where rows are not aligned (VEC = 1) a team copies the aligned span that holds its vector,
-// meets, and each lane picks its channels (5099 x 2533 bf16, training: 165 us, 294 with direct
+// meets, and each lane picks its channels (5099 x 2533 bf16, training: 160 us, 294 with direct
 // loads of single channels).  Bound by memory: about 140 KB an SM are on
 // their way, and the weights stay in registers (read again for every row they were as many bytes as the
 // row, through an L1 that was then 72 % busy).  65536 x 768 bf16 with a residual: 65 us, 6.2 TB/s;
@@ -799,7 +799,7 @@ static Plan plan(const Args& a, int act_dtype, bool vec_ok, bool bwd) {
     z.width = a.G * a.N;
     units = (a.rows + z.per_block - 1) / z.per_block;
   } else if (groups <= 512 * most) {
-    const int per_lane = z.vec == 8 ? 3 : 4;
+    const int per_lane = z.vec == 8 ? 3 : z.vec == 4 ? 4 : 8;  // (single channels, 4 a lane: 20000 x 787 234 us, 8: 180)
     const int warps = std::min(16, (groups + 32 * per_lane - 1) / (32 * per_lane));
     z.team = warps == 1 ? ONE : MANY;
     z.chn = (groups + 32 * warps - 1) / (32 * warps);
