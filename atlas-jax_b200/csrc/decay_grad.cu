@@ -85,12 +85,11 @@ __device__ __forceinline__ void mma_steps(uint32_t d, uint64_t A, uint64_t sa, u
 }
 template <int NV>
 __device__ __forceinline__ void frag(uint32_t addr, float* v) {
+  static_assert(NV == 8 || NV == 16, "fragments of 16 or 32 columns");
   if constexpr (NV == 8)
     tmem_frag16(addr, v);
-  else if constexpr (NV == 16)
-    tmem_frag32(addr, v);
   else
-    tmem_frag64(addr, v);
+    tmem_frag32(addr, v);
 }
 
 template <int DP>

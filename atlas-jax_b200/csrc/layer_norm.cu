@@ -51,38 +51,6 @@ template <typename TA, int VEC>
 struct alignas(sizeof(TA) * VEC) Pack {
   TA v[VEC];
 };
-template <typename TA, int VEC>
-__device__ __forceinline__ void unpack(float* f, const Pack<TA, VEC>& k) {
-  if constexpr (sizeof(TA) == 2 && VEC > 1) {
-    const __nv_bfloat162* h = (const __nv_bfloat162*)&k;
-#pragma unroll
-    for (int j = 0; j < VEC / 2; ++j) {
-      const float2 t = __bfloat1622float2(h[j]);
-      f[2 * j] = t.x;
-      f[2 * j + 1] = t.y;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = ld_act(k.v, (size_t)j);
-  }
-}
-template <typename TA, int VEC>
-__device__ __forceinline__ void load(float* f, const TA* p) {
-  unpack<TA, VEC>(f, *(const Pack<TA, VEC>*)p);
-}
-template <typename TA, int VEC>
-__device__ __forceinline__ void store(TA* p, const float* f) {
-  Pack<TA, VEC> k;
-  if constexpr (sizeof(TA) == 2 && VEC > 1) {
-    __nv_bfloat162* h = (__nv_bfloat162*)&k;
-#pragma unroll
-    for (int j = 0; j < VEC / 2; ++j) h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) st_act(k.v, (size_t)j, f[j]);
-  }
-  *(Pack<TA, VEC>*)p = k;
-}
 // A group as pairs (the backward is as near to the issue limit as to the memory's); a single
 // channel is a pair with a zero.
 template <int VEC>

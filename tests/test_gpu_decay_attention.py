@@ -266,6 +266,32 @@ def test_state_in_its_own_place(T, D, need_saved):
     assert not need_saved or torch.equal(saved, saved2)
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 48)])
+def test_in_a_graph(dtype, D):
+    """Captured and replayed on new inputs in the same buffers: the chained kernels keep their order."""
+    from atlas_b200.decay_attention import decay_attention_backward, decay_attention_forward
+    ins = _inputs(1, 900, 3, D, dtype, False, True, 1)
+    q, k, v, g, S, dy, dS = ins
+
+    def call():
+        y, out, saved = decay_attention_forward(q, k, v, g, S, 0.4)
+        return (y, out) + decay_attention_backward(q, k, v, g, saved, dy, dS, 0.4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = call()
+    for seed in (2, 3):
+        for t, u in zip(ins, _inputs(1, 900, 3, D, dtype, False, True, seed)):
+            t.copy_(u)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, r in zip(got, call()):
+            assert torch.equal(x, r)
+
+
 def test_offsets_beyond_32_bits():
     """Sequences more than 2^31 elements apart in one buffer."""
     from atlas_b200.decay_attention import decay_attention_forward, decay_attention_step
