@@ -209,8 +209,8 @@ struct Place {
 // The vectors to come are copied into a ring in shared memory, `stages` - 1 of them ahead; every
 // thread copies the groups that it will work on itself, so the ring needs no barrier and holds no
 // registers.  Where rows are not aligned (VEC = 1) a team copies the aligned span that holds its vector,
-// meets, and each lane picks its channels (5099 x 2533 bf16, training: 160 us, 294 with direct
-// loads of single channels).  Bound by memory: about 140 KB an SM are on
+// meets, and each lane picks its channels (51739 x 183 bf16: 38 us, 99 with direct loads
+// of single channels).  Bound by memory: about 140 KB an SM are on
 // their way, and the weights stay in registers (read again for every row they were as many bytes as the
 // row, through an L1 that was then 72 % busy).  65536 x 768 bf16 with a residual: 65 us, 6.2 TB/s;
 // 79 us with direct loads and 32 warps an SM.
@@ -576,6 +576,14 @@ __global__ void __launch_bounds__(512) big_fwd_kernel(Args a) {
   }
 }
 
+// Loads of BU elements 512 apart are in flight together (the compiler cannot move them over the stores):
+// 9000 x 4099 bf16 with dh 237 -> 141 us.
+constexpr int BU = 4;
+template <typename TA>
+__device__ __forceinline__ void load_apart(float* f, const TA* p, int n0, int n) {
+#pragma unroll
+  for (int i = 0; i < BU; ++i) f[i] = n0 + 512 * i < n ? ld_act(p, (size_t)(n0 + 512 * i)) : 0.f;
+}
 // dx; the weight gradients are summed by columns in big_param_kernel, which runs first (dx
 // may be the buffer of dy)
 template <typename TA>
@@ -586,19 +594,34 @@ __global__ void __launch_bounds__(512) big_bwd_kernel(Args a) {
   for (int64_t v = blockIdx.x; v < a.vecs; v += gridDim.x) {
     const TA *h = (const TA*)a.h + v * a.N, *dy = (const TA*)a.dy + v * a.N;
     const TA* dh = a.dh ? (const TA*)a.dh + v * a.N : nullptr;
-    const float* w = a.w ? a.w + (v % a.G) * (int64_t)a.N : nullptr;
+    const float* wg = a.w ? a.w + (v % a.G) * (int64_t)a.N : nullptr;
     const float2 st = *(const float2*)(a.cstats + 2 * v);
     float s[2] = {0.f, 0.f};
-    for (int n = threadIdx.x; n < a.N; n += 512) {
-      const float u = ld_act(dy, (size_t)n) * (w ? w[n] : 1.f);
-      s[0] += u;
-      s[1] = fmaf(u, (ld_act(h, (size_t)n) - st.x) * st.y, s[1]);
+    for (int n0 = threadIdx.x; n0 < a.N; n0 += 512 * BU) {
+      float f[BU], d[BU], w[BU];
+      load_apart<TA>(f, h, n0, a.N);
+      load_apart<TA>(d, dy, n0, a.N);
+      if (wg) load_apart<float>(w, wg, n0, a.N);
+#pragma unroll
+      for (int i = 0; i < BU; ++i) {
+        const float u = wg ? d[i] * w[i] : d[i];  // 0 beyond the vector
+        s[0] += u;
+        s[1] = fmaf(u, (f[i] - st.x) * st.y, s[1]);
+      }
     }
     team_sum<MANY, 32, 2>(s, red, turn, 16, 1);
-    for (int n = threadIdx.x; n < a.N; n += 512) {
-      const float u = ld_act(dy, (size_t)n) * (w ? w[n] : 1.f), zz = (ld_act(h, (size_t)n) - st.x) * st.y;
-      const float d = st.y * (u - s[0] * inv - zz * (s[1] * inv));
-      st_act((TA*)a.dx + v * a.N, (size_t)n, d + (dh ? ld_act(dh, (size_t)n) : 0.f));
+    for (int n0 = threadIdx.x; n0 < a.N; n0 += 512 * BU) {
+      float f[BU], d[BU], w[BU], e[BU];
+      load_apart<TA>(f, h, n0, a.N);
+      load_apart<TA>(d, dy, n0, a.N);
+      if (wg) load_apart<float>(w, wg, n0, a.N);
+      if (dh) load_apart<TA>(e, dh, n0, a.N);
+#pragma unroll
+      for (int i = 0; i < BU; ++i) {
+        const float u = wg ? d[i] * w[i] : d[i], zz = (f[i] - st.x) * st.y;
+        const float g = st.y * (u - s[0] * inv - zz * (s[1] * inv));
+        if (n0 + 512 * i < a.N) st_act((TA*)a.dx + v * a.N, (size_t)(n0 + 512 * i), dh ? g + e[i] : g);
+      }
     }
   }
 }
@@ -610,6 +633,7 @@ __global__ void __launch_bounds__(256) big_param_kernel(Args a) {
   if (col >= total) return;
   const int g = (int)(col / a.N);
   float sw = 0.f, sb = 0.f;
+#pragma unroll 4
   for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
     const float2 st = *(const float2*)(a.cstats + 2 * (r * a.G + g));
     const float d = ld_act((const TA*)a.dy + r * total, (size_t)col);
@@ -745,6 +769,8 @@ struct Plan {
   int vec, lanes, chn, threads, per_block, width, parts;
   int64_t grid;
 };
+// single channels: BIG from here on (bf16 training, WARPS and BIG: 14000 x 1301 237 and 312 us, 9000 x 2051 310 and 241)
+constexpr int SINGLES = 1600;
 static Plan plan(const Args& a, int act_dtype, bool vec_ok, bool bwd) {
   Plan z{};
   const int full = act_dtype == ATLAS_BF16 ? 8 : 4;
@@ -766,7 +792,7 @@ static Plan plan(const Args& a, int act_dtype, bool vec_ok, bool bwd) {
     z.threads = (z.per_block * a.G * groups + 31) / 32 * 32;
     z.width = a.G * a.N;
     units = (a.rows + z.per_block - 1) / z.per_block;
-  } else if (groups <= 512 * most) {
+  } else if (groups <= (z.vec == 1 ? SINGLES : 512 * most)) {
     const int per_lane = z.vec == 8 ? 3 : z.vec == 4 ? 4 : 8;  // (single channels, 4 a lane: 20000 x 787 234 us, 8: 180)
     const int warps = std::min(16, (groups + 32 * per_lane - 1) / (32 * per_lane));
     z.team = warps == 1 ? ONE : MANY;
