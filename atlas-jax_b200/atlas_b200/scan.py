@@ -60,6 +60,13 @@ def away(dev):
     return torch.cuda.current_device() != dev.index
 
 
+def _capturing(dev):
+    if away(dev):
+        with torch.cuda.device(dev):
+            return torch.cuda.is_current_stream_capturing()
+    return torch.cuda.is_current_stream_capturing()
+
+
 def _check_act(x, name, dtype, shape):
     if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous() or not x.is_cuda:
         raise ValueError(f"{name}: expected contiguous CUDA {dtype} {shape}, got {x.dtype} {tuple(x.shape)}")
@@ -70,7 +77,9 @@ class Workspace:
 
     One buffer per (device, current stream): calls issued on different streams or
     devices never share scratch, and a buffer is only regrown by calls ordered on
-    the stream that used it."""
+    the stream that used it.  A call that is being captured into a CUDA graph gets scratch of its
+    own from the graph's memory: the graph replays with that address, on any stream, after the
+    buffer of its capturing stream may have been regrown and freed."""
 
     def __init__(self):
         self.bufs = {}
@@ -78,6 +87,8 @@ class Workspace:
     def get(self, nbytes, device):
         if nbytes == 0:
             return None, 0
+        if _capturing(device):
+            return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
         key = (device, stream_of(device))
         buf = self.bufs.get(key)
         if buf is None or buf.numel() < nbytes:

@@ -1,0 +1,64 @@
+"""Decay attention and layer norm as programs call them: captured in graphs, under other default
+types, far from the tests' usual sizes.  Against float64 (tests/decay_ref.py) or against the same
+call made eagerly."""
+import pytest
+import torch
+
+import decay_ref as R
+from test_gpu_decay_attention import _inputs
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _train(ins):
+    from atlas_b200.decay_attention import decay_attention_backward, decay_attention_forward
+    q, k, v, g, S, dy, dS = ins
+    y, out, saved = decay_attention_forward(q, k, v, g, S, 0.4)
+    return (y, out) + decay_attention_backward(q, k, v, g, saved, dy, dS, 0.4)
+
+
+def _norm(x, w, dy):
+    from atlas_b200.layer_norm import layer_norm_backward, layer_norm_forward
+    y, h, stats = layer_norm_forward(x, w, w)
+    return (y,) + layer_norm_backward(dy, h, w, stats)
+
+
+def _captured(call, stream):
+    with torch.cuda.stream(stream):
+        call()  # (eager scratch of this stream, smaller than the calls that come after the capture)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = call()
+    return graph, out
+
+
+def test_graphs_outlive_the_scratch_of_their_stream():
+    """After a capture a larger eager call on the capturing stream, then tensors that may take over any
+    memory that was freed: a replay writes none of them, and two graphs replayed on two
+    streams give what each gives alone."""
+    ins = _inputs(1, 900, 3, 64, BF, False, True, 1)
+    big = _inputs(4, 3000, 6, 64, BF, False, True, 2)
+    x, dy = (torch.randn(5000, 768, device="cuda").to(BF) for _ in range(2))
+    w = torch.randn(768, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g1, out1 = _captured(lambda: _train(ins), side)
+    g2, out2 = _captured(lambda: _norm(x, w, dy), side)
+    with torch.cuda.stream(side):
+        _train(big)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        guard = [torch.full((1 << 20,), 3, dtype=torch.uint8, device="cuda") for _ in range(96)]
+    torch.cuda.synchronize()
+    want1, want2 = _train(ins), _norm(x, w, dy)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for g, s in zip((g1, g2), streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for got, want in ((out1, want1), (out2, want2)):
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+        assert all(bool((t == 3).all()) for t in guard)
