@@ -121,10 +121,10 @@ def decay_attention_forward(q, k, v, log_decay, state=None, scale=None, need_sav
         with torch.cuda.device(dev):
             return decay_attention_forward(q, k, v, log_decay, state, scale, need_saved, workspace)
     y = empty_like(q)
-    out = torch.empty(*p.state_shape, device=dev) if state is None else torch.empty_like(state)
+    out = torch.empty(*p.state_shape, dtype=torch.float32, device=dev) if state is None else torch.empty_like(state)
     saved, need = None, p.fwd_workspace_bytes
     if need_saved:
-        saved, need = torch.empty(p.saved_bytes // 4, device=dev), p.saved_workspace_bytes
+        saved, need = torch.empty(p.saved_bytes // 4, dtype=torch.float32, device=dev), p.saved_workspace_bytes
     ws, wsb = (workspace or _WS).get(need, dev)
     rc = p.lib.atlas_decay_fwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), addr(state),
                                y.data_ptr(), out.data_ptr(), addr(saved), addr(ws), wsb, stream_of(dev))
@@ -149,7 +149,7 @@ def decay_attention_backward(q, k, v, log_decay, saved, dy, dstate=None, scale=N
         with torch.cuda.device(dev):
             return decay_attention_backward(q, k, v, log_decay, saved, dy, dstate, scale, workspace)
     dq, dk, dv = empty_like(q), empty_like(q), empty_like(q)
-    dg, dstate_in = torch.empty_like(log_decay), torch.empty(*p.state_shape, device=dev)
+    dg, dstate_in = torch.empty_like(log_decay), torch.empty(*p.state_shape, dtype=torch.float32, device=dev)
     ws, wsb = (workspace or _WS).get(p.bwd_workspace_bytes, dev)
     rc = p.lib.atlas_decay_bwd(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), saved.data_ptr(),
                                dy.data_ptr(), addr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),

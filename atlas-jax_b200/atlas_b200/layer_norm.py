@@ -93,7 +93,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None):
     if away(dev):
         with torch.cuda.device(dev):
             return layer_norm_forward(x, weight, bias, eps, residual)
-    y, stats = torch.empty_like(x), torch.empty(p.vecs, 2, device=dev)
+    y, stats = torch.empty_like(x), torch.empty(p.vecs, 2, dtype=torch.float32, device=dev)
     h, hp = x, None
     if residual is not None:
         residual, h = _like(residual, x, "residual"), torch.empty_like(x)
@@ -129,7 +129,7 @@ def layer_norm_backward(dy, h, weight, stats, dh=None, need_params=True, shape=N
     dw = db = ws = None
     wsb = 0
     if need_params:
-        dw = torch.empty(*p.param_shape, device=dev) if weight is None else torch.empty_like(weight)
+        dw = torch.empty(*p.param_shape, dtype=torch.float32, device=dev) if weight is None else torch.empty_like(weight)
         db = torch.empty_like(dw)
         ws, wsb = (workspace or _WS).get(p.workspace_bytes, dev)
     rc = p.lib.atlas_layernorm_bwd(p.ref, dy.data_ptr(), h.data_ptr(), addr(weight), stats.data_ptr(), addr(dh),

@@ -11,9 +11,26 @@ from atlas_b200 import scan
 
 @pytest.fixture
 def host(monkeypatch):
-    """No device: one stream, which captures while ``host.capturing`` is set."""
+    """No device: CPU tensors count as device 0's, launches are noted in ``host.calls``, and the
+    one stream captures while ``host.capturing`` is set."""
     from atlas_b200 import decay_attention, layer_norm
-    h = types.SimpleNamespace(capturing=False)
+    h = types.SimpleNamespace(capturing=False, calls=[])
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: h.calls.append((name, a)) or 0
+
+    def planned(module):
+        real = module._Plan
+
+        def plan(*keys):
+            dev0 = [k if not isinstance(k, tuple) else tuple(0 if type(i) is int and i < 0 else i for i in k) for k in keys]
+            p = real(*dev0)
+            p.lib = Library()
+            return p
+        monkeypatch.setattr(module, "_plans", plan)
+    planned(decay_attention)
+    planned(layer_norm)
     for m in (scan, decay_attention, layer_norm):
         monkeypatch.setattr(m, "away", lambda dev: False)
         monkeypatch.setattr(m, "stream_of", lambda dev: 7)
@@ -36,3 +53,32 @@ def test_captured_scratch_is_the_graphs_own(host):
     assert ws.get(80, dev)[0] is eager
     larger, n = ws.get(200, dev)
     assert n >= 200 and larger is not eager and ws.get(200, dev)[0] is larger
+
+
+def _decay_inputs(B=2, T=70, H=3, D=16, dtype=torch.bfloat16):
+    q, k, v = (torch.zeros(B, T, H, D, dtype=dtype) for _ in range(3))
+    return q, k, v, torch.zeros(H, dtype=torch.float32)
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_buffers_are_float32_under_any_default_type(host, default):
+    """The kernels write float32 states, statistics and parameter gradients whatever type torch makes
+    by default: half as many bytes would be written past their end."""
+    from atlas_b200.decay_attention import decay_attention_backward, decay_attention_forward
+    from atlas_b200.layer_norm import layer_norm_backward, layer_norm_forward
+    torch.set_default_dtype(default)
+    try:
+        q, k, v, g = _decay_inputs()
+        y, out, saved = decay_attention_forward(q, k, v, g)
+        assert out.dtype == torch.float32 and out.shape == (2, 3, 16, 16)
+        assert saved.numel() * saved.element_size() == 2 * 3 * 2 * 16 * 16 * 4  # two chunks of 64 tokens
+        dq, dk, dv, dg, dS = decay_attention_backward(q, k, v, g, saved, y)
+        assert dg.dtype == torch.float32 and dS.dtype == torch.float32 and dS.shape == out.shape
+        x = torch.zeros(5, 4, 16, dtype=torch.bfloat16)
+        y, h, stats = layer_norm_forward(x)
+        assert stats.dtype == torch.float32 and stats.shape == (20, 2)
+        dx, dw, db = layer_norm_backward(y, h, None, stats)
+        assert dw.dtype == torch.float32 and db.dtype == torch.float32 and dw.shape == (16,)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert [n for n, _ in host.calls] == ["atlas_decay_fwd", "atlas_decay_bwd", "atlas_layernorm_fwd", "atlas_layernorm_bwd"]
