@@ -96,9 +96,9 @@ def prologue_forward(geo, proj, conv_w, conv_b, poly, gate_bias):
     _need(gate_bias, torch.float32, (geo.n_gates - int(geo.has_retrieve), H), "gate_bias")
     p = geo.params(dt)
     q, k, v = (torch.empty(B, T, H, D, dtype=dt, device=dev) for _ in range(3))
-    g = [torch.empty(B, T, H, device=dev) for _ in range(3)]
-    g.append(torch.empty(B, T, H, device=dev) if geo.has_gamma else None)
-    g.append(torch.empty(B, T, H, device=dev) if geo.has_retrieve else None)
+    g = [torch.empty(B, T, H, dtype=torch.float32, device=dev) for _ in range(3)]
+    g.append(torch.empty(B, T, H, dtype=torch.float32, device=dev) if geo.has_gamma else None)
+    g.append(torch.empty(B, T, H, dtype=torch.float32, device=dev) if geo.has_retrieve else None)
     L.check(lib.atlas_layer_prologue_fwd(ctypes.byref(p), _ptr(proj), _ptr(conv_w), _ptr(conv_b), _ptr(poly),
                                          _ptr(gate_bias), _ptr(q), _ptr(k), _ptr(v), *[_ptr(x) for x in g],
                                          _stream(dev)))

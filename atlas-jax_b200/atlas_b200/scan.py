@@ -129,8 +129,8 @@ def _forward(lib, q, k, v, alpha, eta, theta, gamma, state, cfg, need_saved, wor
             _check_act(x, n, torch.float32, (B, T, H))
     p = _params(cfg, B, T, H, D, E, q.dtype)
     y = torch.empty_like(q)
-    out = (torch.empty(B, H, D, E, device=dev), torch.empty(B, H, E, D, device=dev),
-           torch.empty(B, H, D, E, device=dev), torch.empty(B, H, E, D, device=dev))
+    out = (torch.empty(B, H, D, E, dtype=torch.float32, device=dev), torch.empty(B, H, E, D, dtype=torch.float32, device=dev),
+           torch.empty(B, H, D, E, dtype=torch.float32, device=dev), torch.empty(B, H, E, D, dtype=torch.float32, device=dev))
     nsave = lib.atlas_scan_saved_bytes(ctypes.byref(p)) if need_saved else 0
     if need_saved and nsave == 0:
         raise L.AtlasError(L.ATLAS_ERR_INVALID_ARGUMENT, lib.atlas_last_error_string().decode())
@@ -153,9 +153,9 @@ def scan_backward(q, k, v, alpha, eta, theta, gamma, saved, dy, dstate=None, cfg
     p = _params(cfg, B, T, H, D, E, q.dtype)
     _check_act(dy, "dy", q.dtype, (B, T, H, D))
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    g = [torch.empty(B, T, H, device=dev) for _ in range(4)]
-    dst = (torch.empty(B, H, D, E, device=dev), torch.empty(B, H, E, D, device=dev),
-           torch.empty(B, H, D, E, device=dev), torch.empty(B, H, E, D, device=dev))
+    g = [torch.empty(B, T, H, dtype=torch.float32, device=dev) for _ in range(4)]
+    dst = (torch.empty(B, H, D, E, dtype=torch.float32, device=dev), torch.empty(B, H, E, D, dtype=torch.float32, device=dev),
+           torch.empty(B, H, D, E, dtype=torch.float32, device=dev), torch.empty(B, H, E, D, dtype=torch.float32, device=dev))
     dso = [None] * 4 if dstate is None else [None if s is None else s.contiguous() for s in dstate]
     ws, wsb = (workspace or _WS).get(lib.atlas_scan_workspace_bytes(ctypes.byref(p)), dev)
     L.check(lib.atlas_scan_bwd(ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(alpha), _ptr(eta), _ptr(theta),
@@ -182,7 +182,7 @@ def linear_scan_forward(q, k, v, alpha, eta, theta, gamma=None, state=None, cfg=
             _check_act(x, n, torch.float32, (B, T, H))
     p = _params(cfg, B, T, H, D, D, q.dtype)
     y = torch.empty_like(q)
-    out = (torch.empty(B, H, D, D, device=dev), torch.empty(B, H, D, D, device=dev))
+    out = (torch.empty(B, H, D, D, dtype=torch.float32, device=dev), torch.empty(B, H, D, D, dtype=torch.float32, device=dev))
     need = lib.atlas_linear_scan_workspace_bytes(ctypes.byref(p))
     if need == 0:
         raise L.AtlasError(L.ATLAS_ERR_UNSUPPORTED, lib.atlas_last_error_string().decode())
@@ -203,8 +203,8 @@ def linear_scan_backward(q, k, v, alpha, eta, theta, gamma, state, dy, dstate=No
     dev = q.device
     p = _params(cfg, B, T, H, D, D, q.dtype)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    g = [torch.empty(B, T, H, device=dev) for _ in range(4)]
-    dst = (torch.empty(B, H, D, D, device=dev), torch.empty(B, H, D, D, device=dev))
+    g = [torch.empty(B, T, H, dtype=torch.float32, device=dev) for _ in range(4)]
+    dst = (torch.empty(B, H, D, D, dtype=torch.float32, device=dev), torch.empty(B, H, D, D, dtype=torch.float32, device=dev))
     st = [None, None] if state is None else [s.contiguous() for s in state]
     dso = [None, None] if dstate is None else [None if s is None else s.contiguous() for s in dstate]
     need = lib.atlas_linear_scan_workspace_bytes(ctypes.byref(p))

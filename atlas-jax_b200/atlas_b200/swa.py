@@ -50,7 +50,7 @@ def swa_forward(q, k, v, window, rope=True):
     B, T, H, D = q.shape
     p = _params(q, window, rope)
     o = torch.empty_like(q)
-    lse = torch.empty(B, H, T, device=q.device)
+    lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device)
     ws = torch.empty(lib.atlas_swa_workspace_bytes(ctypes.byref(p)), dtype=torch.uint8, device=q.device)
     L.check(lib.atlas_swa_fwd(ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(ws), ws.numel(),
                               _stream(q.device)))

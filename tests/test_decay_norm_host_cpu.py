@@ -1,6 +1,9 @@
 """CPU checks of the Python side of decay attention and layer norm, with the library and the
 device queries replaced: what buffers a call makes, which calls it refuses, and what autograd
 is told."""
+import ast
+import glob
+import os
 import types
 
 import pytest
@@ -82,3 +85,16 @@ def test_buffers_are_float32_under_any_default_type(host, default):
     finally:
         torch.set_default_dtype(torch.float32)
     assert [n for n, _ in host.calls] == ["atlas_decay_fwd", "atlas_decay_bwd", "atlas_layernorm_fwd", "atlas_layernorm_bwd"]
+
+
+def test_every_device_buffer_names_its_type():
+    """A buffer that the library fills never takes torch's default type, in any of the package's calls."""
+    bare = []
+    for path in glob.glob(os.path.join(os.path.dirname(scan.__file__), "*.py")):
+        for n in ast.walk(ast.parse(open(path).read())):
+            if isinstance(n, ast.Call) and isinstance(n.func, ast.Attribute) and n.func.attr in ("empty", "zeros", "full") \
+                    and isinstance(n.func.value, ast.Name) and n.func.value.id == "torch":
+                names = {k.arg for k in n.keywords}
+                if "device" in names and "dtype" not in names:
+                    bare.append(f"{os.path.basename(path)}:{n.lineno}")
+    assert not bare
