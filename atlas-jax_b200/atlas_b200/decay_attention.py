@@ -14,7 +14,7 @@ import functools
 import torch
 
 from . import _lib as L
-from .scan import _WS, addr, away, empty_like, stream_of
+from .scan import _WS, addr, away, empty_like, first_derivatives, stream_of
 
 
 class AtlasDecayParams(ctypes.Structure):
@@ -204,6 +204,7 @@ class DecayAttention(torch.autograd.Function):
         return y, out
 
     @staticmethod
+    @first_derivatives
     def backward(ctx, dy, dstate):
         q, k, v, log_decay, saved = ctx.saved_tensors
         dy = torch.zeros_like(q) if dy is None else dy.to(q.dtype)
@@ -213,5 +214,6 @@ class DecayAttention(torch.autograd.Function):
 
 
 def decay_attention(q, k, v, log_decay, state=None, scale=None):
-    """Differentiable decay attention: returns (y, state after the last token)."""
+    """Differentiable decay attention: returns (y, state after the last token).  First
+    derivatives only: differentiating a gradient again raises."""
     return DecayAttention.apply(q, k, v, log_decay, state, scale)

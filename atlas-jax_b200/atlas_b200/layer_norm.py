@@ -11,7 +11,7 @@ import functools
 import torch
 
 from . import _lib as L
-from .scan import _WS, addr, away, stream_of
+from .scan import _WS, addr, away, first_derivatives, stream_of
 
 
 class AtlasNormParams(ctypes.Structure):
@@ -149,6 +149,7 @@ class LayerNorm(torch.autograd.Function):
         return (y, h) if residual is not None else y
 
     @staticmethod
+    @first_derivatives
     def backward(ctx, dy, dh=None):
         h, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -160,5 +161,6 @@ class LayerNorm(torch.autograd.Function):
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
-    """Differentiable layer norm of x, or with ``residual`` (y, h) of h = x + residual."""
+    """Differentiable layer norm of x, or with ``residual`` (y, h) of h = x + residual.  First
+    derivatives only: differentiating a gradient again raises."""
     return LayerNorm.apply(x, weight, bias, eps, residual)

@@ -8,6 +8,7 @@ of the custom VJP and ``AtlasScan`` glues them into autograd.
 """
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -238,6 +239,35 @@ def polar_express(X, steps=5, eps_in_sqrt=1e-12, precision=L.ATLAS_PREC_EXACT):
     L.check(lib.atlas_polar_express_batched(_ptr(X), _ptr(Y), batch, rows, cols, steps, eps_in_sqrt, precision,
                                             _ptr(ws), wsb, _stream(X.device)))
     return Y
+
+
+class _FirstDerivatives(torch.autograd.Function):
+    """The identity, whose backward raises."""
+
+    @staticmethod
+    def forward(ctx, *x):
+        return tuple(t.view_as(t) for t in x)
+
+    @staticmethod
+    def backward(ctx, *dx):
+        raise RuntimeError("this operator has first derivatives only: its gradients cannot be differentiated")
+
+
+def first_derivatives(backward):
+    """For the backward of an autograd Function that runs kernels: under create_graph its
+    gradients are tensors that raise when they are differentiated.  (torch's once_differentiable
+    does so only where the incoming cotangents require a gradient; what the gradients owe to the
+    saved inputs it would drop.)"""
+    @functools.wraps(backward)
+    def run(ctx, *dy):
+        with torch.no_grad():
+            grads = backward(ctx, *dy)
+        if not torch.is_grad_enabled():
+            return grads
+        grads = grads if isinstance(grads, tuple) else (grads,)
+        kept = iter(_FirstDerivatives.apply(*[g.detach().requires_grad_(True) for g in grads if g is not None]))
+        return tuple(None if g is None else next(kept) for g in grads)
+    return run
 
 
 class AtlasScan(torch.autograd.Function):

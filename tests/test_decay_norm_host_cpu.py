@@ -98,3 +98,30 @@ def test_every_device_buffer_names_its_type():
                 if "device" in names and "dtype" not in names:
                     bare.append(f"{os.path.basename(path)}:{n.lineno}")
     assert not bare
+
+
+def _second_derivative(y, x):
+    """Differentiates a first derivative of y by x again."""
+    g, = torch.autograd.grad(y.float().sum(), x, create_graph=True)
+    (y.float().sum() + g.float().square().sum()).backward()
+
+
+def test_second_derivatives_are_refused(host):
+    """The backward kernels are no graph that autograd could differentiate: a penalty on a
+    gradient raises and is not dropped without a word."""
+    from atlas_b200.decay_attention import decay_attention
+    from atlas_b200.layer_norm import layer_norm
+    q, k, v, g = _decay_inputs()
+    q.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        _second_derivative(decay_attention(q, k, v, g)[0], q)
+    x, r = (torch.zeros(5, 4, 16, requires_grad=True) for _ in range(2))
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        _second_derivative(layer_norm(x), x)
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        _second_derivative(layer_norm(x, residual=r)[1], r)
+    # first derivatives are as before, with create_graph too
+    assert torch.autograd.grad(layer_norm(x).sum(), x, create_graph=True)[0].shape == x.shape
+    y, h = layer_norm(x, residual=r)
+    (y.sum() + h.sum()).backward()
+    assert x.grad.shape == r.grad.shape == x.shape and not x.grad.requires_grad
