@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib as L
-from .scan import _ptr, _stream
+from .scan import _ptr, _stream, first_derivatives
 
 
 class AtlasLayerParams(ctypes.Structure):
@@ -132,6 +132,7 @@ class Prologue(torch.autograd.Function):
         return (q, k, v) + tuple(g)
 
     @staticmethod
+    @first_derivatives
     def backward(ctx, dq, dk, dv, da, de, dt, dg, dr):
         proj, conv_w, conv_b, poly, gate_bias = ctx.saved_tensors
         dproj, dcw, dcb, dpoly, dgb = prologue_backward(ctx.geo, proj, conv_w, conv_b, poly, gate_bias, dq, dk, dv,
@@ -158,6 +159,7 @@ class RetrieveGate(torch.autograd.Function):
         return yg
 
     @staticmethod
+    @first_derivatives
     def backward(ctx, dyg):
         y, r = ctx.saved_tensors
         lib = _lib()

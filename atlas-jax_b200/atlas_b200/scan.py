@@ -286,6 +286,7 @@ class AtlasScan(torch.autograd.Function):
         return (y,) + tuple(out)
 
     @staticmethod
+    @first_derivatives
     def backward(ctx, dy, dW1, dW2, dS1, dS2):
         q, k, v, alpha, eta, theta, gamma, saved = ctx.saved_tensors
         dq, dk, dv, da, de, dt, dg, dst = scan_backward(q, k, v, alpha, eta, theta, gamma, saved,

@@ -10,7 +10,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .scan import _ptr, _stream
+from .scan import _ptr, _stream, first_derivatives
 
 
 class AtlasSwaParams(ctypes.Structure):
@@ -77,6 +77,7 @@ class SwaFunction(torch.autograd.Function):
         return o
 
     @staticmethod
+    @first_derivatives
     def backward(ctx, do):
         q, k, v, o, lse = ctx.saved_tensors
         dq, dk, dv = swa_backward(q, k, v, o, lse, do.to(torch.bfloat16), ctx.window, ctx.rope)

@@ -125,3 +125,12 @@ def test_second_derivatives_are_refused(host):
     y, h = layer_norm(x, residual=r)
     (y.sum() + h.sum()).backward()
     assert x.grad.shape == r.grad.shape == x.shape and not x.grad.requires_grad
+
+
+def test_every_kernel_backward_has_first_derivatives_only():
+    """The same for the package's other autograd Functions: their backward is wrapped."""
+    from atlas_b200 import decay_attention, layer_io, layer_norm, swa
+    functions = {f for m in (scan, decay_attention, layer_io, layer_norm, swa) for f in vars(m).values()
+                 if isinstance(f, type) and issubclass(f, torch.autograd.Function) and f is not scan._FirstDerivatives}
+    assert len(functions) == 6
+    assert [f.__name__ for f in functions if not hasattr(f.backward, "__wrapped__")] == []
