@@ -12,6 +12,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from .scan import _WS, addr, away, empty_like, first_derivatives, stream_of
@@ -187,6 +188,7 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None, out=
                                 addr(slots), n, y.data_ptr(), out.data_ptr(), stream_of(dev))
     if rc:
         L.check(rc)
+    increment_version(out)  # written behind autograd's back
     return y, out
 
 

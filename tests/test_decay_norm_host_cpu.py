@@ -134,3 +134,21 @@ def test_every_kernel_backward_has_first_derivatives_only():
                  if isinstance(f, type) and issubclass(f, torch.autograd.Function) and f is not scan._FirstDerivatives}
     assert len(functions) == 6
     assert [f.__name__ for f in functions if not hasattr(f.backward, "__wrapped__")] == []
+
+
+def test_the_step_tells_autograd_what_it_writes(host):
+    """A state that autograd has saved for a backward is not overwritten unnoticed."""
+    from atlas_b200.decay_attention import decay_attention_step
+    q, k, v, g = _decay_inputs(T=1)
+    w = torch.ones((), requires_grad=True)
+    for other in (False, True):
+        state = torch.zeros(2, 3, 16, 16)
+        out = torch.zeros_like(state) if other else state
+        loss = (w * out).sum()
+        versions = state._version, out._version
+        decay_attention_step(q, k, v, g, state, out=out if other else None)
+        assert out._version > versions[1] and (not other or state._version == versions[0])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        decay_attention_step(q, k, v, g, torch.zeros(2, 3, 16, 16))
