@@ -167,7 +167,11 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None, out=
     int32 a pool (n, H, D, D) in which sequence b uses row slots[b] (every running
     sequence a row of its own; a slot outside the pool marks an idle sequence, whose y is
     0).  The new states are written to ``out`` (a buffer like ``state``; default: in place).
+    There is no backward: inputs that require gradients are for torch.no_grad().
     Returns (y, out)."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or state.requires_grad or (out is not None and out.requires_grad)):
+        raise ValueError("decay_attention_step has no backward: call it under torch.no_grad(), or use decay_attention")
     p, q, k, v = _plan(q, k, v, log_decay, scale)
     dev = q.device
     n = p.B if slots is None else state.shape[0]

@@ -152,3 +152,22 @@ def test_the_step_tells_autograd_what_it_writes(host):
             loss.backward()
     with torch.inference_mode():
         decay_attention_step(q, k, v, g, torch.zeros(2, 3, 16, 16))
+
+
+def test_the_step_refuses_to_drop_gradients(host):
+    """The step has no backward: inputs that want gradients are refused where gradients are recorded, and
+    taken under no_grad."""
+    from atlas_b200.decay_attention import decay_attention_step
+    for i in range(8):
+        if i in (5, 6):  # slots, scale
+            continue
+        ins = [*_decay_inputs(T=1), torch.zeros(2, 3, 16, 16), None, 1.0, torch.zeros(2, 3, 16, 16)]
+        ins[i].requires_grad_(True)
+        with pytest.raises(ValueError, match="no_grad"):
+            decay_attention_step(*ins)
+        assert not host.calls
+        with torch.no_grad():
+            decay_attention_step(*ins)
+        assert len(host.calls) == 1
+        host.calls.clear()
+    decay_attention_step(*_decay_inputs(T=1), torch.zeros(2, 3, 16, 16))
