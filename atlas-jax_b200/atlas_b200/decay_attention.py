@@ -62,10 +62,11 @@ class _Plan:
         B, T, H, D = shape
         if g[0] != (H,) or g[2] != torch.float32 or g[3] != dev or (g[1] != (1,) and H > 1):
             raise ValueError(f"log_decay: expected contiguous CUDA float32 {(H,)}, got {g[2]} {tuple(g[0])}")
-        # contiguous channels; bf16 on the tensor cores also has no broadcast (stride 0) axes
+        # contiguous channels; bf16 on the tensor cores also has no broadcast (stride 0) axes.  Strides of
+        # empty tensors say nothing, and contiguous() keeps them.
         fast = dtype == torch.bfloat16 and D % 8 == 0
-        self.packed = all((x[1][3] == 1 or D == 1) and not (fast and any(s == 0 and n > 1 for s, n in zip(x[1], shape)))
-                          for x in (q, k, v))
+        self.packed = 0 in shape or all(
+            (x[1][3] == 1 or D == 1) and not (fast and any(s == 0 and n > 1 for s, n in zip(x[1], shape))) for x in (q, k, v))
         strides = [(ctypes.c_int64 * 3)(*x[1][:3]) for x in (q, k, v)]
         self.params = AtlasDecayParams(L.ATLAS_ABI_VERSION, B, T, H, D,
                                        L.ATLAS_BF16 if dtype == torch.bfloat16 else L.ATLAS_F32,

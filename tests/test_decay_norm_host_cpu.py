@@ -171,3 +171,20 @@ def test_the_step_refuses_to_drop_gradients(host):
         assert len(host.calls) == 1
         host.calls.clear()
     decay_attention_step(*_decay_inputs(T=1), torch.zeros(2, 3, 16, 16))
+
+
+def test_empty_views(host):
+    """An empty tensor's strides say nothing (contiguous() keeps them): empty batches and sequences in any
+    layout, and broadcast, are valid calls."""
+    from atlas_b200.decay_attention import decay_attention_backward, decay_attention_forward, decay_attention_step
+    g = torch.zeros(4)
+    transposed = torch.empty(2, 16, 4, 0, dtype=torch.bfloat16).permute(0, 3, 2, 1)
+    assert transposed.shape == (2, 0, 4, 16) and transposed.stride(3) != 1
+    broadcast = torch.zeros(2, 1, 1, 16, dtype=torch.bfloat16).expand(2, 1, 4, 16)[:, :0]
+    nobody = torch.empty(16, 5, 4, 0).permute(3, 1, 2, 0)
+    for q in (transposed, broadcast, nobody, nobody.bfloat16()):
+        B = q.shape[0]
+        y, out, saved = decay_attention_forward(q, q, q, g)
+        assert y.shape == q.shape and out.shape == (B, 4, 16, 16) and saved.numel() == 0
+        assert decay_attention_backward(q, q, q, g, saved, y)[0].shape == q.shape
+        assert decay_attention_step(q, q, q, g, out)[0].shape == q.shape
