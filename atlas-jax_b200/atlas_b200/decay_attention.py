@@ -92,6 +92,7 @@ _plans = functools.lru_cache(maxsize=512)(_Plan)
 
 def _plan(q, k, v, log_decay, scale):
     """Checks the inputs; returns their plan and q, k, v with contiguous channels."""
+    scale = None if scale is None else float(scale)  # (a tensor would be a key by its identity)
     aligned = (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 == 0
     p = _plans(*[(x.shape, x.stride(), x.dtype, x.get_device()) for x in (q, k, v, log_decay)], scale, aligned)
     if not p.packed:

@@ -75,7 +75,7 @@ def _key(w):
 
 
 def _plan(x, weight, bias, eps):
-    return _plans((x.shape, x.dtype, x.get_device()), _key(weight), _key(bias), eps)
+    return _plans((x.shape, x.dtype, x.get_device()), _key(weight), _key(bias), float(eps))  # (a tensor: its value)
 
 
 def _like(x, ref, name):

@@ -188,3 +188,29 @@ def test_empty_views(host):
         assert y.shape == q.shape and out.shape == (B, 4, 16, 16) and saved.numel() == 0
         assert decay_attention_backward(q, q, q, g, saved, y)[0].shape == q.shape
         assert decay_attention_step(q, q, q, g, out)[0].shape == q.shape
+
+
+def test_numbers_given_as_tensors_are_read_at_every_call(host):
+    """A scale or eps held in a tensor is its value now, not what it was when a plan was made for that tensor."""
+    import functools
+
+    from atlas_b200 import decay_attention as D
+    from atlas_b200 import layer_norm as N
+    seen = []
+
+    @functools.lru_cache
+    def plans(*keys):
+        seen.append(keys)
+        return made(*keys)
+    for module, call in ((D, lambda t: D.decay_attention_forward(*_decay_inputs(), scale=t)),
+                         (N, lambda t: N.layer_norm_forward(torch.zeros(3, 16), eps=t))):
+        made, module._plans = module._plans, plans
+        seen.clear()
+        t = torch.tensor(0.5)
+        call(t)
+        t.fill_(0.25)
+        call(t)
+        call(0.25)
+        module._plans = made
+        numbers = [[k for k in keys if isinstance(k, float)] for keys in seen]
+        assert numbers == [[0.5], [0.25]], module
