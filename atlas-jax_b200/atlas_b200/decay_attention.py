@@ -60,6 +60,8 @@ class _Plan:
             if x[0] != shape or x[2] != dtype or x[3] != dev or dev < 0:
                 raise ValueError(f"{n}: expected CUDA {dtype} {tuple(shape)} on the device of q, got {x[2]} {tuple(x[0])}")
         B, T, H, D = shape
+        if max(shape) >= 1 << 31:  # (a c_int32 field would keep the lower half)
+            raise L.AtlasError(L.ATLAS_ERR_UNSUPPORTED, f"decay attention: sizes must be below 2^31, got {tuple(shape)}")
         if g[0] != (H,) or g[2] != torch.float32 or g[3] != dev or (g[1] != (1,) and H > 1):
             raise ValueError(f"log_decay: expected contiguous CUDA float32 {(H,)}, got {g[2]} {tuple(g[0])}")
         # contiguous channels; bf16 on the tensor cores also has no broadcast (stride 0) axes.  Strides of
@@ -177,6 +179,8 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None, out=
     p, q, k, v = _plan(q, k, v, log_decay, scale)
     dev = q.device
     n = p.B if slots is None else state.shape[0]
+    if n >= 1 << 31:
+        raise ValueError(f"state: expected fewer than 2^31 rows, got {n}")
     shape = p.state_shape if n == p.B else (n,) + p.state_shape[1:]
     _need(state, shape, "state", q)
     if out is None:

@@ -58,6 +58,8 @@ class _Plan:
                 raise ValueError(f"{n}: expected contiguous float32 {p} on the device of x, got {w[1]} {tuple(w[0])}")
         self.param_shape = p or (shape[-1],)
         G, N = (1, shape[-1]) if len(self.param_shape) == 1 else self.param_shape
+        if G >= 1 << 31 or N >= 1 << 31:  # (a c_int32 field would keep the lower half)
+            raise L.AtlasError(L.ATLAS_ERR_UNSUPPORTED, f"layer norm: G * N must be at most 2^20, got {G} * {N}")
         rows = shape.numel() // (G * N) if G * N else 0
         self.params = AtlasNormParams(L.ATLAS_ABI_VERSION, L.ATLAS_BF16 if dtype == torch.bfloat16 else L.ATLAS_F32,
                                       rows, G, N, eps, 0)

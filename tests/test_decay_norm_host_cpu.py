@@ -214,3 +214,23 @@ def test_numbers_given_as_tensors_are_read_at_every_call(host):
         module._plans = made
         numbers = [[k for k in keys if isinstance(k, float)] for keys in seen]
         assert numbers == [[0.5], [0.25]], module
+
+
+def test_sizes_beyond_32_bits_are_refused(host, monkeypatch):
+    """The C parameters hold sizes in 32 bits: larger ones raise and are not cut down."""
+    from atlas_b200 import decay_attention as D
+    from atlas_b200 import layer_norm as N
+    from atlas_b200 import AtlasError
+    big, bf = (1 << 32) + 1, torch.bfloat16
+    for shape in ((big, 1, 1, 1), (1, big, 1, 1), (1, 1, big, 1), (1, 1, 1, big), (1 << 31, 1, 1, 1)):
+        x = torch.empty(1, dtype=bf).expand(shape)
+        with pytest.raises((ValueError, AtlasError)):
+            D.decay_attention_forward(x, x, x, torch.zeros(1).expand(shape[2]))
+    with pytest.raises(AtlasError):
+        N.layer_norm_forward(torch.empty(1, dtype=bf).expand(big))
+    q, k, v, g = _decay_inputs(T=1, H=1, D=1)
+    pool = torch.empty(1).expand(big, 1, 1, 1)
+    monkeypatch.setattr(D, "_need", lambda *a: None)  # (this one is not contiguous)
+    with pytest.raises(ValueError):
+        D.decay_attention_step(q, k, v, g, pool, torch.zeros(2, dtype=torch.int32))
+    assert not host.calls
