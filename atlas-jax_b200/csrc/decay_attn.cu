@@ -615,8 +615,7 @@ static int check(const AtlasDecayParams* p) {
       return report_error(ATLAS_ERR_INVALID_ARGUMENT, "strides must not be negative");
   if (p->T > 1 << 30) return report_error(ATLAS_ERR_UNSUPPORTED, "decay attention: T must be at most 2^30");
   // grids are one-dimensional: (batch, head, 32-token tile, gradient) and (batch, head, state element / 256)
-  const int64_t n = chains(*p);
-  if (n * std::max(6 * chunks(*p), 64) >= (int64_t)1 << 31)
+  if (chains(*p) > INT32_MAX / std::max(6 * chunks(*p), 64))  // (a product of the three could pass 2^63)
     return report_error(ATLAS_ERR_UNSUPPORTED, "decay attention: B * H * T is too large for one call");
   clear_error();
   return ATLAS_OK;

@@ -234,3 +234,16 @@ def test_sizes_beyond_32_bits_are_refused(host, monkeypatch):
     with pytest.raises(ValueError):
         D.decay_attention_step(q, k, v, g, pool, torch.zeros(2, dtype=torch.int32))
     assert not host.calls
+
+
+def test_products_of_sizes_do_not_wrap():
+    """B * H * T near and beyond 2^63 is too large a problem, not a small one."""
+    import ctypes
+
+    from atlas_b200 import _lib as L
+    from atlas_b200.decay_attention import AtlasDecayParams, _lib
+    lib, s = _lib(), (ctypes.c_int64 * 3)(0, 0, 0)
+    for B, T, H in ((1 << 29, 1, 1 << 29), ((1 << 31) - 1, 1 << 30, (1 << 31) - 1), (1 << 30, 0, 1 << 30), (1 << 30, 1 << 30, 1 << 5)):
+        p = ctypes.byref(AtlasDecayParams(L.ATLAS_ABI_VERSION, B, T, H, 1, L.ATLAS_F32, 1.0, 0, s, s, s))
+        assert lib.atlas_decay_saved_bytes(p) == 0 and b"too large" in lib.atlas_last_error_string(), (B, T, H)
+        assert lib.atlas_decay_step(p, *[None] * 6, 0, *[None] * 3) == L.ATLAS_ERR_UNSUPPORTED
