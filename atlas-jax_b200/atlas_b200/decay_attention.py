@@ -148,7 +148,8 @@ def decay_attention_backward(q, k, v, log_decay, saved, dy, dstate=None, scale=N
     if dstate is not None:
         _need(dstate, p.state_shape, "dstate", q)
         dstate = _aligned(dstate)
-    if saved.numel() * saved.element_size() != p.saved_bytes or saved.get_device() != q.get_device():
+    if saved.numel() * saved.element_size() != p.saved_bytes or not saved.is_contiguous() \
+            or saved.get_device() != q.get_device():
         raise ValueError("saved: not what decay_attention_forward saved for these inputs")
     if away(dev):
         with torch.cuda.device(dev):

@@ -247,3 +247,16 @@ def test_products_of_sizes_do_not_wrap():
         p = ctypes.byref(AtlasDecayParams(L.ATLAS_ABI_VERSION, B, T, H, 1, L.ATLAS_F32, 1.0, 0, s, s, s))
         assert lib.atlas_decay_saved_bytes(p) == 0 and b"too large" in lib.atlas_last_error_string(), (B, T, H)
         assert lib.atlas_decay_step(p, *[None] * 6, 0, *[None] * 3) == L.ATLAS_ERR_UNSUPPORTED
+
+
+def test_saved_states_have_to_be_contiguous(host):
+    """The backward reads as many bytes as were saved from the buffer's start on."""
+    from atlas_b200.decay_attention import decay_attention_backward, decay_attention_forward
+    q, k, v, g = _decay_inputs()
+    y, _, saved = decay_attention_forward(q, k, v, g)
+    every_other = torch.empty(2 * saved.numel())[::2]
+    with pytest.raises(ValueError, match="saved"):
+        decay_attention_backward(q, k, v, g, every_other, y)
+    with pytest.raises(ValueError, match="saved"):
+        decay_attention_backward(q, k, v, g, saved[:1].expand(saved.numel()), y)
+    decay_attention_backward(q, k, v, g, saved, y)
