@@ -72,7 +72,7 @@ class _Plan:
         strides = [(ctypes.c_int64 * 3)(*x[1][:3]) for x in (q, k, v)]
         self.params = AtlasDecayParams(L.ATLAS_ABI_VERSION, B, T, H, D,
                                        L.ATLAS_BF16 if dtype == torch.bfloat16 else L.ATLAS_F32,
-                                       D ** -0.5 if scale is None else scale, int(aligned), *strides)
+                                       max(D, 1) ** -0.5 if scale is None else scale, int(aligned), *strides)
         self.lib, self.ref = _lib(), ctypes.byref(self.params)
         self.shape, self.dtype = tuple(shape), dtype
         self.B, self.state_shape = B, (B, H, D, D)

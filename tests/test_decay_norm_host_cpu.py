@@ -260,3 +260,10 @@ def test_saved_states_have_to_be_contiguous(host):
     with pytest.raises(ValueError, match="saved"):
         decay_attention_backward(q, k, v, g, saved[:1].expand(saved.numel()), y)
     decay_attention_backward(q, k, v, g, saved, y)
+
+
+def test_head_size_zero_is_refused_like_other_sizes(host):
+    from atlas_b200 import AtlasError
+    from atlas_b200.decay_attention import decay_attention_forward
+    with pytest.raises(AtlasError, match="positive"):
+        decay_attention_forward(*_decay_inputs(D=0))
