@@ -507,7 +507,9 @@ __global__ void __launch_bounds__(256, DP == 128 ? 2 : 4) grads_kernel(Args a, i
 // One CTA per (sequence, head, slice of SL value columns): the columns of the state are
 // independent, so a slice needs no exchange with the others.  Thread (row group rg, column
 // group cg) keeps rows rg, rg + RG, ... of VEC consecutive columns in registers from the
-// first token to the last; y's sum over rows goes through shared memory.  Bound by the state's
+// first token to the last; y's sum over rows goes through shared memory.  The decay is applied as a
+// float pair, as along a sequence: rounded to one float32 its error would be multiplied in again at
+// every token, for as long as the state is kept (1 - 2^-10: up to 1.4e-4 of the state).  Bound by the state's
 // bytes where there are many sequences: SL = 64 then moves four 16-byte groups a thread
 // (DP = 64), 32 twice as many CTAs for few sequences.  256 sequences x 12 heads of 64: 18 us, 5.6 TB/s
 // (27 us with SL = 32); one sequence: 2.4 us, most of it the launch.
@@ -517,6 +519,7 @@ __global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, cons
   constexpr int CG = SL / VEC, RG = 256 / CG, NR = DP / RG;  // column groups, row groups, rows a thread
   static_assert(CG <= 32 && NR >= 1, "a warp holds whole rows of a slice");
   __shared__ float red[8][SL + 1], qs[DP], ks[DP];
+  __shared__ float2 decay;
   const AtlasDecayParams& P = a.p;
   const int D = P.D, slices = (D + SL - 1) / SL;
   const int chain = blockIdx.x / slices, sl = blockIdx.x % slices, b = chain / P.H, h = chain % P.H;
@@ -531,7 +534,11 @@ __global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, cons
     return;
   }
   const int64_t off = ((int64_t)row * P.H + h) * D * D + rg * D + e0;
-  const float l = pow_decay(a.log_decay[h], 1);
+  if (threadIdx.x == 255) {
+    const double l = exp((double)a.log_decay[h]);
+    const float lh = (float)l;
+    decay = make_float2(lh, (float)(l - (double)lh));
+  }
   const TA* q = (const TA*)a.q + b * P.q_stride[0] + h * P.q_stride[2];
   const TA* k = (const TA*)a.k + b * P.k_stride[0] + h * P.k_stride[2];
   const TA* v = (const TA*)a.v + b * P.v_stride[0] + h * P.v_stride[2];
@@ -560,12 +567,13 @@ __global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, cons
       acc[j] = 0.f;
     }
     __syncthreads();
+    const float lh = decay.x, ll = decay.y;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {  // rows from D on: k = q = 0
       const float kd = ks[rg + i * RG], qd = qs[rg + i * RG];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        S[i][j] = fmaf(l, S[i][j], kd * vv[j]);
+        S[i][j] = fmaf(lh, S[i][j], fmaf(ll, S[i][j], kd * vv[j]));
         acc[j] = fmaf(qd, S[i][j], acc[j]);
       }
     }

@@ -62,3 +62,21 @@ def test_graphs_outlive_the_scratch_of_their_stream():
             for a, b in zip(got, want):
                 assert torch.equal(a, b)
         assert all(bool((t == 3).all()) for t in guard)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_long_generation_keeps_the_states_accuracy(dtype):
+    """4096 single tokens at decays of 1 - 2^-9 .. 1 - 2^-12.  An update rounds the state once, at
+    most 2^-24 of it and at random; some 2^11 of them are remembered: sqrt(2^11) 2^-24 = 2.7e-6 at most,
+    below the 4e-6 that the prompt's states are held to.  A decay rounded to float32 adds up to 2^12 2^-25."""
+    from atlas_b200.decay_attention import decay_attention_step
+    T, H, D = 4096, 4, 64
+    e = torch.tensor([9.0, 10.0, 11.0, 12.0], dtype=torch.float64)
+    q, k, v, g, S, _, _ = _inputs(1, T, H, D, dtype, True, True, 4, torch.log1p(-torch.exp2(-e)).float())
+    ref, kd, vd = S.double(), k.double(), v.double()
+    lam = torch.exp(g.double())[None, :, None, None]
+    for t in range(T):
+        decay_attention_step(q[:, t:t + 1], k[:, t:t + 1], v[:, t:t + 1], g, S)
+        ref = lam * ref + kd[:, t, :, :, None] * vd[:, t, :, None, :]
+    for h in range(H):
+        assert R.rel(S[:, h], ref[:, h]) < 4e-6, h
