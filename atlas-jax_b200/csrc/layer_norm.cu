@@ -2,7 +2,8 @@
 //
 // Bound by memory: forward and backward each read every input element once and write every
 // output element once; a vector stays in registers between the statistics and the output.
-// The variance is summed from (h - mean)^2 over those registers.
+// The variance is summed from (h - mean)^2 over those registers; a mean far above the deviation is
+// corrected once (far() below).
 //
 // A team of lanes owns a vector; lane i holds CHN groups of VEC consecutive channels (16
 // bytes where the rows allow it), group j at (j * lanes + i) * VEC.  Teams:
@@ -171,6 +172,20 @@ __device__ __forceinline__ void team_sum(float* v, float* red, int& turn, int wa
   }
 }
 
+// The rounding of a float32 mean is some 2^-23 of it: beyond FAR deviations it would show in y, and the
+// forward then sums h - mean once more (the differences are exact there) and takes off what the mean
+// missed.  Other vectors keep their results and pay for a comparison (20000 x 787 bf16 with a residual, forward: 83 -> 87 us;
+// other sizes nothing; summed for every vector 91, and 3 to 8 % at other sizes).
+constexpr float FAR = 4.f;
+__device__ __forceinline__ bool far(float mean, float rstd) {  // alike in a warp, and in a team
+  return __any_sync(0xffffffffu, fabsf(mean) * rstd > FAR);
+}
+// `missed`: mean of h - mean; var: mean of its square.  1 / deviation about the mean itself.
+__device__ __forceinline__ float far_rstd(float missed, float var, float eps) {
+  const float v = fmaf(-missed, missed, var);
+  return 1.f / sqrtf((v < 0.f ? 0.f : v) + eps);  // (below 0: rounding, where all channels are equal)
+}
+
 // Where this thread's team works: its vectors are first, first + stride, ... and lane /
 // lanes place it in the team.  SUB: the position inside a row is fixed, rows advance.
 // WARPS: `per_block` teams of a block take consecutive vectors.
@@ -324,8 +339,35 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : V
     t = f2_get(s2);
     s[0] = t.x + t.y;
     team_sum<TEAM, LANES, 1>(s, red, turn, z.warps, 1 + z.team);
-    const float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps));
-    if (on && z.lane == 0 && a.stats) *(float2*)(a.stats + 2 * v0) = make_float2(mean, rstd);
+    float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps)), missed = 0.f;
+    if (far(mean, rstd)) {
+      const float var = s[0] * inv;
+      if constexpr (OWN) {
+        s2 = f2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < CHN; ++c)
+          if (on && c * dn < left) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) s2 = s2 + f[c][j];
+          }
+        t = f2_get(s2);
+        s[0] = t.x + t.y;
+      } else {  // from memory (this thread wrote h): fewer registers
+        const TA* hv = (res ? (const TA*)a.h + n0 : x) + o;
+        s[0] = 0.f;
+#pragma unroll 1
+        for (int n = 0; on && n < left; n += dn) s[0] += ld_act(hv, (size_t)n) - mean;
+      }
+      team_sum<TEAM, LANES, 1>(s, red, turn, z.warps, 1 + z.team);
+      missed = s[0] * inv;
+      rstd = far_rstd(missed, var, a.eps);
+      const F2 m2 = f2(-missed, VEC == 1 ? 0.f : -missed);
+#pragma unroll
+      for (int c = 0; c < CHN; ++c)
+#pragma unroll
+        for (int j = 0; j < NP; ++j) f[c][j] = f[c][j] + m2;
+    }
+    if (on && z.lane == 0 && a.stats) *(float2*)(a.stats + 2 * v0) = make_float2(mean + missed, rstd);
     const F2 r2 = f2(rstd, rstd);
 #pragma unroll
     for (int c = 0; c < CHN; ++c)
@@ -567,11 +609,19 @@ __global__ void __launch_bounds__(512) big_fwd_kernel(Args a) {
       s[0] = fmaf(f, f, s[0]);
     }
     team_sum<MANY, 32, 1>(s, red, turn, 16, 1);
-    const float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps));
-    if (threadIdx.x == 0 && a.stats) *(float2*)(a.stats + 2 * v) = make_float2(mean, rstd);
+    float rstd = 1.f / sqrtf(fmaf(s[0], inv, a.eps)), missed = 0.f;
+    if (far(mean, rstd)) {
+      const float var = s[0] * inv;
+      s[0] = 0.f;
+      for (int n = threadIdx.x; n < a.N; n += 512) s[0] += ld_act(h, (size_t)n) - mean;
+      team_sum<MANY, 32, 1>(s, red, turn, 16, 1);
+      missed = s[0] * inv;
+      rstd = far_rstd(missed, var, a.eps);
+    }
+    if (threadIdx.x == 0 && a.stats) *(float2*)(a.stats + 2 * v) = make_float2(mean + missed, rstd);
     for (int n = threadIdx.x; n < a.N; n += 512) {
       const float w = a.w ? a.w[(int64_t)g * a.N + n] : 1.f, b = a.b ? a.b[(int64_t)g * a.N + n] : 0.f;
-      st_act((TA*)a.y + v * a.N, (size_t)n, fmaf((ld_act(h, (size_t)n) - mean) * rstd, w, b));
+      st_act((TA*)a.y + v * a.N, (size_t)n, fmaf((ld_act(h, (size_t)n) - mean - missed) * rstd, w, b));
     }
   }
 }

@@ -16,8 +16,10 @@
  * and rstd (up to 8 channels: rstd as two floats whose sum it is).
  * Arithmetic is float32 (float64 for vectors of up to 8 channels, whose gradients cancel);
  * outputs in act_dtype are rounded once.  The variance is the mean of the squared differences
- * from the mean (two passes over registers), so a large mean costs no digits.  The parameter
- * gradients are summed in a fixed order (no atomics).
+ * from the mean (two passes over registers).  Where the mean is above four deviations the forward
+ * sums the differences once more and corrects it, so a large mean costs y no digits; stats hold it
+ * rounded to float32 (2^-24 of it), which the backward's (h - mean) rstd then contains.  The
+ * parameter gradients are summed in a fixed order (no atomics).
  *
  * Conventions (status codes, thread-local error string, stream as void*, caller-owned
  * device buffers) are those of atlas_scan.h.

@@ -80,3 +80,20 @@ def test_a_long_generation_keeps_the_states_accuracy(dtype):
         ref = lam * ref + kd[:, t, :, :, None] * vd[:, t, :, None, :]
     for h in range(H):
         assert R.rel(S[:, h], ref[:, h]) < 4e-6, h
+
+
+@pytest.mark.parametrize("shape", [(40, 768), (9, 12, 64), (21, 787), (5, 8192), (3, 5069), (3, 20000), (2, 262144), (30, 8)])
+def test_a_large_mean_costs_the_output_no_digits(shape):
+    """Float32 vectors with a mean a thousand and ten thousand times the deviation: differences from a
+    float32 near the mean are exact, and what that float32 misses of the mean is summed with them, so y
+    is held to the bound of other float32 outputs (2e-6), long vectors' too."""
+    from atlas_b200.layer_norm import layer_norm_forward
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w, b = (torch.randn(shape[1:], device="cuda", generator=g) for _ in range(2))
+    for mean in (1e3, -1e4):
+        x = mean + torch.randn(shape, device="cuda", generator=g)
+        y, _, st = layer_norm_forward(x, w, b)
+        xd = x.cpu().double()
+        assert R.rel(y, R.layer_norm(xd, w.cpu().double(), b.cpu().double(), 1e-5)) < 2e-6, mean
+        if shape[-1] > 8:  # the mean is kept in float32
+            assert (st[:, 0].cpu().double() - xd.mean(-1).reshape(-1)).abs().max() < 2 ** -23 * abs(mean) * 1.05
