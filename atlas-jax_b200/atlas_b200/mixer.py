@@ -7,7 +7,11 @@ puts next to an Atlas memory layer or a sliding-window attention layer.
 ``delta`` is the output of the block before, so the residual add of the stream rides in
 the norm.  Training and prompts take whole sequences (``forward``); generation advances a
 pool of states by one token per running sequence (``step``).  The norms and the attention
-run in libatlas_scan.so, the two projections are plain GEMMs."""
+run in libatlas_scan.so, the two projections are plain GEMMs.
+
+For bf16 activations cast the projections (``to_qkv``, ``to_out``), not the block: the decay
+logits and the norms' weights are used in float32, and a logit rounded to bf16 moves a
+decay of 1 - 2^-10 by up to 2 % of its distance from 1."""
 
 import torch
 import torch.nn as nn
