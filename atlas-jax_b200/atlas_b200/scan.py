@@ -88,9 +88,10 @@ class Workspace:
     def get(self, nbytes, device):
         if nbytes == 0:
             return None, 0
-        if _capturing(device):
+        stream = stream_of(device)
+        if stream and _capturing(device):  # (0, the default stream, cannot be captured)
             return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
-        key = (device, stream_of(device))
+        key = (device, stream)
         buf = self.bufs.get(key)
         if buf is None or buf.numel() < nbytes:
             buf = self.bufs[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
