@@ -58,7 +58,7 @@ def empty_like(x):
 
 def away(dev):
     """Whether ``dev`` is not the current device (launches then need ``torch.cuda.device``)."""
-    return torch.cuda.current_device() != dev.index
+    return torch._C._cuda_getDevice() != dev.index  # (CUDA is up: dev has tensors)
 
 
 def _capturing(dev):
