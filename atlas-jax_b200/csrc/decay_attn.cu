@@ -511,8 +511,10 @@ __global__ void __launch_bounds__(256, DP == 128 ? 2 : 4) grads_kernel(Args a, i
 // float pair, as along a sequence: rounded to one float32 its error would be multiplied in again at
 // every token, for as long as the state is kept (2.1e-5 of the state after 4096 at 1 - 2^-9).  Bound by the state's
 // bytes where there are many sequences: SL = 64 then moves four 16-byte groups a thread
-// (DP = 64), 32 twice as many CTAs for few sequences.  256 sequences x 12 heads of 64: 18 us, 5.6 TB/s
-// (27 us with SL = 32); one sequence: 2.4 us, most of it the launch.
+// (DP = 64), 32 twice as many CTAs for few sequences (256 x 12 heads of 64: 27 us with SL = 32).
+// 256 sequences x 12 heads of 64: 21 us, 4.8 TB/s; one sequence: 2.5 us, most of it the launch.  Several
+// tokens wait for their q, k and v one after the other: 128 sequences x 4 heads of 128 in float32, two
+// tokens 18 us, five 26 (floor 11).
 template <typename TA, int DP, int SL, int VEC>
 __global__ void __launch_bounds__(256) step_kernel(Args a, const float* in, const int32_t* slots, int32_t n_slots,
                                                    float* out) {

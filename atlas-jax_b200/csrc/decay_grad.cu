@@ -12,8 +12,11 @@
 //
 // Blocks are independent: one CTA each.  q, k, v, dy arrive by TMA and leave as dq, dk, dv
 // through the same tiles (straight from registers: no faster); S and R are split into three bf16 parts
-// (dlog_decay is a float32 output; dv needs two of R's).  All accumulators have M = 64 (decay_tc.cuh); warp w
-// reads lane quadrant w % 4 and its half (D <= 64) or quarter w / 4 of the columns.
+// (dlog_decay is a float32 output; K R reads two of R's, 16 bits, since dv rounds to bf16's 8).  P and dA
+// are rounded to bf16 as operands of dq, dk and dv, whose relative error goes from the 1.66e-3 of
+// their own rounding to 1.8e-3; dlog_decay takes A and dA from before that rounding.  All accumulators
+// have M = 64 (decay_tc.cuh); warp w reads lane quadrant w % 4 and its half (D <= 64) or quarter w / 4 of the
+// columns.
 //
 // D <= 64: 256 TMEM columns (dA K, P^T O, dA^T Q and K R take the places of A, B, O S^T and
 // V R^T), 97 KB of shared memory: two CTAs share an SM, and one's loads and float32 work
@@ -22,7 +25,7 @@
 //
 // What bounds it: the latency of one block's steps (loads, splits, five groups of MMAs, stores: about
 // 13,000 cycles at D = 64, 22,000 at D = 128) with two blocks or one in flight an SM; the tensor pipe is
-// busy for a fifth of the time, the schedulers for 40 %.  Measured: 16 x 4096 tokens x 8 heads of 64 about
+// busy for a fifth of the time, the schedulers for 29 % (D = 64) and 23 %.  Measured: 16 x 4096 tokens x 8 heads of 64 about
 // 200 us (88 KB a block: 3.6 TB/s); 4 x 1900 x 6 heads of 128 67 us.  A CTA an SM that walks over the blocks, the next
 // one's tiles on their way (D = 64) or its state in registers (D = 128), took as long.
 #include <algorithm>

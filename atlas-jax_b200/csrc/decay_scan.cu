@@ -25,11 +25,12 @@
 // segments' sums first, then every segment, from a state put together from the sums before
 // it.
 //
-// What bounds it: the schedulers.  A block is about 5,300 warp instructions at D = 64 (four schedulers:
-// 1,340 of the 2,200 cycles that it takes) and 15,000 at D = 128 (3,770 of 5,900); the tensor pipe is
-// busy for 37 % and 20 %.  Measured: 8 x 8192 tokens x 12 heads of 64 150 us (96 CTAs, one a chain:
-// 2.7 TB/s); 65536 x 16 heads of 128, in nine segments, 144 us of sums and 351 us of outputs; the
-// cotangent states of 16 x 4096 x 8 heads of 64 58 us (4.6 TB/s).  A prefetch of the blocks to come into
+// What bounds it: the latency of a block's two chains, S -> parts -> QS -> y and k' -> dS -> S, each step
+// of which waits for the group before.  No unit is full: a block is about 5,300 warp instructions at
+// D = 64, 1,340 of the 2,200 cycles that it takes on each of four schedulers (61 %), and 15,000 at D = 128,
+// 3,770 of 5,900 (64 %); the tensor pipe is busy for 37 % and 20 %.  Measured: 8 x 8192 tokens x 12 heads
+// of 64 149 us (96 CTAs, one a chain: 2.7 TB/s); 65536 x 16 heads of 128, in nine segments, 494 us, 144 of
+// them sums; the cotangent states of 16 x 4096 x 8 heads of 64 58 us (4.6 TB/s).  A prefetch of the blocks to come into
 // L2 and a fourth stage change nothing; O and QS handed on in halves of 64 columns (D = 128) cost 12 %.
 //
 // Layout: q, k, v tiles as TMA writes them (rows of 128 bytes, 128-byte swizzle, a box per
@@ -254,6 +255,8 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     }
   } else if (FWD && w < K::W_Y) {
     // ---- scores ----
+    // Rounded to bf16, as P V's operand: y's relative error goes from the 1.66e-3 of its own rounding to
+    // 1.8e-3.  (A second part would be as many MMAs again and a tile more, for digits that y's type drops.)
     if (FWD) {
       const int q = w & 3, r = lane >> 2, c2 = 2 * (lane & 3), t0 = 16 * q + r;
       uint8_t* prow = sm + K::OFF_P + cm_off(t0, c2, C);
@@ -388,7 +391,7 @@ __global__ void __launch_bounds__(Cfg<DP, FWD>::NT, 1)
     for (int i = 0; i < z.n; ++i) {
       const int blk = z.first + i * z.step, b = i % K::DBL, n = i / K::DBL;
       if (a.saves) put_state(a.saves + (z.chain * nblk + blk) * DD);
-      if (FWD) {
+      if (FWD) {  // two parts for QS: 16 bits of S, an error of 2^-17 where y rounds by 2^-9 (S itself stays float32)
         if (i >= K::DBL && !wait(ctl, &ctl.s_free[b], n - 1, a.status)) break;
         uint8_t* s = sm + K::OFF_S + b * 2 * K::ST + cm_off(d0, e0 + c2, DP);
 #pragma unroll

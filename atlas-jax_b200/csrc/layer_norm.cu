@@ -224,11 +224,12 @@ struct Place {
 // The vectors to come are copied into a ring in shared memory, `stages` - 1 of them ahead; every
 // thread copies the groups that it will work on itself, so the ring needs no barrier and holds no
 // registers.  Where rows are not aligned (VEC = 1) a team copies the aligned span that holds its vector,
-// meets, and each lane picks its channels (51739 x 183 bf16: 38 us, 99 with direct loads
+// meets, and each lane picks its channels (51739 x 183 bf16: 35 us, 99 with direct loads
 // of single channels).  Bound by memory: about 140 KB an SM are on
-// their way, and the weights stay in registers (read again for every row they were as many bytes as the
-// row, through an L1 that was then 72 % busy).  65536 x 768 bf16 with a residual: 65 us, 6.2 TB/s;
-// 79 us with direct loads and 32 warps an SM.
+// their way with a residual (half of it without: the residual's slots then stay empty), and the weights stay
+// in registers (read again for every row they were as many bytes as the row, through an L1 that was then
+// 72 % busy).  65536 x 768 bf16 with a residual: 77 us, 5.2 TB/s, 14 us less than with direct loads and 32
+// warps an SM.
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
 __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : VEC * CHN <= 8 ? 4 : 2)
     fwd_kernel(Args a, int per_block, int stages) {
@@ -385,9 +386,10 @@ __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : V
 // With z = (h - mean) rstd and u = dy w:  dx = rstd (u - mean(u) - z mean(u z)) + dh,
 // dw += dy z, db += dy.
 // A ring as in the forward (a register prefetch spilled, which made every copy wait for its
-// load: 325 us at 65536 x 768 bf16 with dh; the ring 82, 4.9 TB/s).  The sums of the weights' gradients
-// take the registers that the forward has for the weights, and leave 16 warps an SM; they and a ring of
-// two stages (there are three streams) keep it from the forward's bandwidth.
+// load: 325 us at 65536 x 768 bf16 with dh; the ring 79, 5.1 TB/s, and 4 for the sum of the partial rows).  The
+// sums of the weights' gradients take the registers that the forward has for the weights, and leave 16
+// warps an SM.  Three groups of 8 bf16 with their sums are more than 128 registers: 80 (one warp a
+// vector) and 136 bytes (more) of each thread's are kept in local memory and read again.
 template <typename TA, Team TEAM, int LANES, int VEC, int CHN>
 __global__ void __launch_bounds__(TEAM == MANY ? 512 : 256, TEAM == MANY ? 1 : TEAM == SUB ? 4 : VEC * CHN <= 8 ? 3 : 2)
     bwd_kernel(Args a, int per_block, int stages) {
@@ -627,7 +629,7 @@ __global__ void __launch_bounds__(512) big_fwd_kernel(Args a) {
 }
 
 // Loads of BU elements 512 apart are in flight together (the compiler cannot move them over the stores):
-// 9000 x 4099 bf16 with dh 237 -> 141 us.
+// 9000 x 4099 bf16 with dh 237 -> 144 us.
 constexpr int BU = 4;
 template <typename TA>
 __device__ __forceinline__ void load_apart(float* f, const TA* p, int n0, int n) {
@@ -811,15 +813,16 @@ static int status_of(cudaError_t e) {
 // How a problem runs.  VEC: channels per load.  SUB for vectors of 4 to 32 aligned groups, a
 // power of two, where the row of G vectors fits a block; TINY for up to 8 channels; WARPS
 // while a thread holds at most 3 groups of 8 bf16, 4 groups of 4 float32 or 8 single
-// channels (what the backward keeps in 128 registers); else BIG.  As few warps as hold the
-// vector: the shuffles and address arithmetic of a vector are paid once for each warp.
+// channels (what the backward keeps in 128 registers, but for 80 to 136 bytes at 3 groups of
+// bf16; single channels of one warp spill more, in 64 and 80 registers); else BIG.  As few warps as hold
+// the vector: the shuffles and address arithmetic of a vector are paid once for each warp.
 struct Plan {
   bool big, tiny;
   Team team;
   int vec, lanes, chn, threads, per_block, width, parts;
   int64_t grid;
 };
-// single channels: BIG from here on (bf16 training, WARPS and BIG: 14000 x 1301 237 and 312 us, 9000 x 2051 310 and 241)
+// single channels: BIG from here on (bf16 training, WARPS and BIG: 14000 x 1301 240 and 312 us, 9000 x 2051 310 and 235)
 constexpr int SINGLES = 1600;
 static Plan plan(const Args& a, int act_dtype, bool vec_ok, bool bwd) {
   Plan z{};
@@ -843,7 +846,7 @@ static Plan plan(const Args& a, int act_dtype, bool vec_ok, bool bwd) {
     z.width = a.G * a.N;
     units = (a.rows + z.per_block - 1) / z.per_block;
   } else if (groups <= (z.vec == 1 ? SINGLES : 512 * most)) {
-    const int per_lane = z.vec == 8 ? 3 : z.vec == 4 ? 4 : 8;  // (single channels, 4 a lane: 20000 x 787 234 us, 8: 180)
+    const int per_lane = z.vec == 8 ? 3 : z.vec == 4 ? 4 : 8;  // (single channels, 4 a lane: 20000 x 787 234 us, 8: 189)
     const int warps = std::min(16, (groups + 32 * per_lane - 1) / (32 * per_lane));
     z.team = warps == 1 ? ONE : MANY;
     z.chn = (groups + 32 * warps - 1) / (32 * warps);

@@ -23,12 +23,15 @@
  *
  * Arithmetic: sums, decays and states are float32.  bf16 activations with D a multiple of
  * 8 and 16-byte aligned rows run on the tcgen05 tensor cores; other calls run in float32
- * on the CUDA cores.  On the tensor cores the decayed scores of a chunk are rounded to bf16
- * before their product with v (the outputs are bf16 too); what reaches float32 outputs
- * (states, dlog_decay) is kept to float32 accuracy by splitting float32 operands into three
- * bf16 parts.
+ * on the CUDA cores.  On the tensor cores what reaches float32 outputs (states, dlog_decay) is
+ * kept to float32 accuracy by splitting float32 operands into three bf16 parts; for the bf16
+ * outputs operands are rounded to fewer bits: the decayed scores of a chunk to bf16 (q k^T
+ * before its products with v and dy, dy v^T before its products with k and q), the state in
+ * q S and the cotangent state in k R (for dv) to two bf16 parts, 16 bits.  The relative error of y, dq,
+ * dk and dv is then about 1.8e-3, where the one rounding to bf16 alone leaves 1.66e-3; the rounded
+ * scores make nearly all of the difference.
  * Causality holds for finite inputs; an infinity or NaN in v or k of a token reaches the
- * outputs of its own 64-token chunk as well as those after it.
+ * outputs of its own 64-token chunk as well as those after it, an infinity mostly as NaN.
  *
  * Conventions (status codes, thread-local error string, stream as void*, caller-owned
  * device buffers) are those of atlas_scan.h.
@@ -82,7 +85,8 @@ int atlas_decay_bwd(const AtlasDecayParams* p, const void* q, const void* k, con
                     size_t workspace_bytes, void* stream);
 
 /* The recurrent form: token by token from state_in to state_out (which may be the same
- * buffer).  slots NULL: the states are (B, H, D, D) and sequence b uses row b.  Otherwise
+ * buffer).  The decay is applied as a float pair, so that states kept over thousands of tokens stay
+ * as near to float64 as those of atlas_decay_fwd.  slots NULL: the states are (B, H, D, D) and sequence b uses row b.  Otherwise
  * they are pools of n_slots rows (n_slots, H, D, D) and sequence b uses row slots[b] (int32);
  * the running sequences' slots differ from one another, and a slot outside [0, n_slots)
  * marks an idle sequence: its y is 0 and no state is touched.  Rows that no sequence names
