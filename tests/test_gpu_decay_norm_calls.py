@@ -138,7 +138,7 @@ def test_step_of_many_sequences(D, T, dtype):
 
 
 @pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (BF, 40), (F32, 48), (F32, 128)])
-@pytest.mark.parametrize("B,T,H", [(20, 200, 8), (50, 67, 6)])
+@pytest.mark.parametrize("B,T,H", [(30, 200, 6), (50, 67, 6)])
 def test_more_chains_than_sms(B, T, H, dtype, D):
     """Forward and backward with a CTA for each whole sequence, more of them than run at once.
     Tolerances as in test_gpu_decay_attention.py."""
